@@ -476,6 +476,141 @@ int tmopt_prefill_check_positions(const int64_t* q_positions,
                                   const int64_t* kv_positions, int64_t T,
                                   int32_t* reject, tmopt_stream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* Differential attention                                                   */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Attention by the difference of two softmax maps. Query heads 2h and 2h + 1
+ * are the two maps of head pair h; stored heads 2g and 2g + 1, g = h / (HQ /
+ * HKV), hold their keys, and the two value rows side by side the pair's
+ * 256-wide values:
+ *   O_h = softmax(scale q_2h K_2g^T) V_g
+ *         - lam_h softmax(scale q_2h+1 K_2g+1^T) V_g
+ *   out_h = O_h / sqrt(mean(O_h^2) + norm_eps) * norm_weight * out_scale
+ * (norm_weight NULL: out_h = O_h * out_scale). The caches and pools are those
+ * of the other entry points; HKV is even, HQ a multiple of it.
+ * lam:          fp32, one value per pair (lam_stride 1) or one for all
+ *               (lam_stride 0).
+ * norm_weight:  fp32 [256], 16-byte aligned; norm_eps > 0 with it.
+ * Sums, maxima, the difference and the norm are fp32; probabilities are
+ * rounded to bf16 for their product with the values, outputs once.
+ */
+
+/*
+ * One new token per request over the paged cache. q [B, HQ, D], block_table,
+ * table_wrap, ctx_lens, window, scale, min_pages and num_workgroups as in
+ * tmopt_attn_decode_paged, pages and keys without an entry included (they are
+ * absent). out [B, HQ / 2, 2 D] bf16 (a request without a key: zeros), lse
+ * [B, HQ] fp32 natural-log sum-exp of each map or NULL. workspace:
+ * tmopt_attn_decode_diff_workspace_size bytes, 16-byte aligned, without
+ * initialisation. B <= 8192.
+ */
+size_t tmopt_attn_decode_diff_workspace_size(int B, int HQ, int HKV, int D,
+                                             int num_workgroups);
+int tmopt_attn_decode_diff(const void* q, const void* k_pool,
+                           const void* v_pool, const int32_t* block_table,
+                           int64_t bt_stride, int table_wrap,
+                           const int32_t* ctx_lens, int B, int HQ, int HKV,
+                           int D, int page_size, int64_t num_pages, int window,
+                           float scale, const float* lam, int lam_stride,
+                           const float* norm_weight, float norm_eps,
+                           float out_scale, int min_pages, int num_workgroups,
+                           void* out, float* lse, void* workspace,
+                           size_t workspace_bytes, tmopt_stream_t stream);
+
+/*
+ * Varlen causal (optionally windowed) form. q [total, HQ, D] with element
+ * strides, D contiguous; cu_seqlens_q, prior_lens, max_seqlen_q, window, scale
+ * and reject as in tmopt_attn_prefill_varlen. Keys:
+ *   block_table == NULL: k, v [total, HKV, D], the runs' own rows packed by
+ *         cu_seqlens_q (strides % 8, D contiguous); prior_lens NULL;
+ *   block_table != NULL, k == v == NULL: every key from k_pool / v_pool
+ *         [num_pages, page_size, HKV, D] through block_table [num_seqs,
+ *         bt_stride], the runs' own rows already written. Pages past the row
+ *         width or outside the pool read as zeros.
+ * out: [total, HQ / 2, 2 D] with element strides (% 8, 16-byte aligned), the
+ * 2 D contiguous; lse fp32 [HQ, total] rows of lse_stride_head elements, or
+ * NULL. Rows past the last run are left as they were.
+ * workspace: scratch of tmopt_attn_prefill_diff_workspace_size bytes, 16-byte
+ * aligned, without initialisation; NULL: the keys of a block of queries are
+ * not split over work-groups.
+ */
+size_t tmopt_attn_prefill_diff_workspace_size(int num_seqs, int max_seqlen_q,
+                                              int HQ, int HKV,
+                                              int64_t bt_stride, int window);
+int tmopt_attn_prefill_diff(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k,
+    int64_t k_stride_tok, int64_t k_stride_head, const void* v,
+    int64_t v_stride_tok, int64_t v_stride_head, const int32_t* cu_seqlens_q,
+    const int32_t* prior_lens, int num_seqs, int max_seqlen_q,
+    const void* k_pool, const void* v_pool, const int32_t* block_table,
+    int64_t bt_stride, int page_size, int64_t num_pages, int HQ, int HKV,
+    int D, int window, float scale, const float* lam, int lam_stride,
+    const float* norm_weight, float norm_eps, float out_scale, void* out,
+    int64_t o_stride_tok, int64_t o_stride_head, float* lse,
+    int64_t lse_stride_head, const int32_t* reject, void* workspace, size_t workspace_bytes,
+    tmopt_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* Page plan of a serving step                                              */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * What the entry points above take of a step, made on the device from its
+ * requests' lengths. page_table [table_rows, table_width] int32 is the cache's
+ * own table: row slots[i] backs request i, its first ceil(ctx_lens[i] / 16)
+ * entries name the pages the request holds. new_lens[i] tokens come to it in
+ * this step (0: none), and the pages they need are taken off the stack
+ * free_pages[0 .. free_count) (from its top, in request order) into the row.
+ * A negative slot is padding: a request without tokens or pages.
+ * Written:
+ *   block_table  [B, width]: row i of the step, the request's pages up to
+ *                ceil((ctx + new) / 16), then -1
+ *   seq_lens     [B]: ctx + new (may be ctx_lens)
+ *   cu_seqlens   [B + 1]: exclusive sums of new
+ *   slot_mapping [max_tokens] int64: pool row of each new token, -1 past the
+ *                last (and where the row names no page)
+ *   positions    [max_tokens] int64: its position, 0 past the last
+ *   free_count_out [1]: what is left of the stack (may be free_count)
+ *   reject       [1]: 0, or 1 if the step cannot be: a slot outside the table
+ *                or named twice, a negative length, a request past 16 *
+ *                min(table_width, width) tokens, more than max_tokens in all,
+ *                or more pages than are free. A rejected step takes no page
+ *                and has no tokens: block_table and slot_mapping are -1,
+ *                cu_seqlens and positions 0, seq_lens the contexts.
+ * No other outputs may overlap inputs or each other. B <= 8192 (0: no
+ * request), table_rows <= 262144, max_tokens, width and table_width <= 2^24.
+ */
+int tmopt_plan_pages(int32_t* page_table, int64_t table_rows,
+                     int64_t table_width, const int64_t* slots,
+                     const int32_t* ctx_lens, const int32_t* new_lens, int B,
+                     const int32_t* free_pages, int64_t free_capacity,
+                     const int32_t* free_count, int64_t max_tokens,
+                     int64_t width, int32_t* block_table, int32_t* seq_lens,
+                     int32_t* cu_seqlens, int64_t* slot_mapping,
+                     int64_t* positions, int32_t* free_count_out,
+                     int32_t* reject, tmopt_stream_t stream);
+
+/*
+ * Pushes the ceil(lens[i] / 16) pages of table row slots[i] onto the stack
+ * free_pages (capacity free_capacity), request by request in page order, and
+ * writes its new height (free_count_out may be free_count). Negative slots are
+ * skipped; the rows keep their entries. reject = 1, and nothing else happens,
+ * for a slot outside the table or named twice, a length that is negative or
+ * past the row, or a stack that would overflow. workspace:
+ * tmopt_release_pages_workspace_size bytes, 16-byte aligned. Limits as in
+ * tmopt_plan_pages.
+ */
+size_t tmopt_release_pages_workspace_size(int B);
+int tmopt_release_pages(const int32_t* page_table, int64_t table_rows,
+                        int64_t table_width, const int64_t* slots,
+                        const int32_t* lens, int B, int32_t* free_pages,
+                        int64_t free_capacity, const int32_t* free_count,
+                        int32_t* free_count_out, int32_t* reject,
+                        void* workspace, size_t workspace_bytes,
+                        tmopt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,6 +8,9 @@ lib/libtmopt_attn.so), reached from PyTorch-ROCm through ctypes:
             decode_paged / decode_ring (split-KV + LSE combine),
             decode_paged_noalloc, prefill_varlen (MFMA),
             prefill_check_positions.
+  diff      differential attention: decode_diff_paged, prefill_diff_varlen.
+  pages     the page plan of a step from its requests' lengths: plan_pages,
+            release_pages.
   compat    the reference's call signatures (attn_swa, attn_global,
             attn_prefill_fused) over the native kernels.
   graph     hipGraph capture of the decode step and of the adapters with
@@ -29,6 +32,9 @@ from .attn import (HEAD_DIM, PAGE_SIZE, decode_default_workgroups,
 from .compat import (attn_global, attn_prefill_chunk_global,
                      attn_prefill_chunk_swa, attn_prefill_fused, attn_swa,
                      prefill_chunk_state)
+from .diff import (decode_diff_paged, decode_diff_workspace,
+                   prefill_diff_varlen)
+from .pages import PagePlan, plan_pages, release_pages
 
 __all__ = [
     "TmoptError", "TmoptLibraryMissing", "version", "HEAD_DIM", "PAGE_SIZE",
@@ -41,4 +47,6 @@ __all__ = [
     "prefill_varlen", "attn_swa", "attn_global", "attn_prefill_fused",
     "attn_prefill_chunk_swa", "attn_prefill_chunk_global",
     "prefill_chunk_state",
+    "decode_diff_paged", "decode_diff_workspace", "prefill_diff_varlen",
+    "PagePlan", "plan_pages", "release_pages",
 ]

@@ -18,7 +18,8 @@ LIB = os.path.join(LIB_DIR, "libtmopt_attn.so")
 ARCH = os.environ.get("TMOPT_ARCH", "gfx950")
 
 SOURCES = ["capi.hip", "kv_write.hip", "decode.hip", "prefill.hip",
-           "prefill_split.hip"]
+           "prefill_split.hip", "decode_diff.hip", "prefill_diff.hip",
+           "page_plan.hip"]
 
 FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-fPIC", "-std=c++17",
