@@ -77,6 +77,19 @@ __device__ __forceinline__ float lane_pair(float x, int dist, bool want_max) {
   return want_max ? fmaxf(a, b) : a + b;
 }
 
+// Inclusive sum over the wave by DPP (VALU, no LDS round trips): within each
+// 16-lane row by shifts of 1, 2, 4, 8, then row 0's total into row 1 and row
+// 2's into row 3, then rows 0-1's total into rows 2-3.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);   // shr 1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);   // shr 2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);   // shr 4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);   // shr 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // bcast 15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // bcast 31
+  return x;
+}
+
 // View of read-only global memory through the constant address space: a
 // wave-uniform load through it becomes a scalar (s_load) fetch that waits on
 // lgkmcnt, so it never drains the wave's in-flight vector loads. Only for

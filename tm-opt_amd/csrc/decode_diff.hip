@@ -1,9 +1,43 @@
-// Differential attention of one new token per request over the paged cache.
-// One work-group per (request, head pair).
-#include "diff_row.h"
+// Differential attention of one new token per request over the paged cache,
+// split over the cache's length and joined, for gfx950 (see diff.h for the
+// formula).
+//
+// HBM bound: every visible token's K and V rows are read once (1 KB per pair of
+// stored heads), for up to eight head pairs at a time.
+//
+//  * Both maps of up to eight head pairs are the 16 columns of one MFMA tile:
+//    column c is map c >> 3 of pair c & 7. S^T = K.Q^T of a 16-token page is
+//    taken with both key heads (v_mfma_f32_16x16x32_bf16), and each lane keeps
+//    the product of its column's own one. The values are shared: O^T = V^T.P^T
+//    (v_mfma_f32_16x16x16_bf16) multiplies the page's 256-wide values by all
+//    columns at once. A plain attention kernel run once per map would read K
+//    once and V twice.
+//  * Pages of all requests are laid end to end and dealt out in equal
+//    contiguous ranges, one per wave and pair of stored heads, so that a launch
+//    streams the same bytes everywhere whatever the lengths, and its grid does
+//    not depend on them (a captured call stays valid). A piece of a request
+//    that one range does not hold whole leaves a normalised fp32 result of both
+//    maps with their LSE; decode_diff_merge joins the pieces in order, then
+//    takes the difference and the norm. No atomics: repeated calls are bitwise
+//    equal.
+//  * One page is a wave's step: 16 KB (two K and two V slices of 16 tokens)
+//    straight into LDS (buffer_load ... lds), two steps ahead. The resource of
+//    a load is the page's rows that hold visible keys; other rows read as zeros
+//    and cost no traffic, so every step issues the same loads and the waits
+//    count exactly.
+//  * Page ids of a range are fetched before the walk into LDS.
+#include "diff.h"
 
 namespace tmopt {
 namespace {
+
+constexpr int kRowB = 256;                 // one token's slice of a stored head
+constexpr int kSliceB = kPage * kRowB;     // a page's slice: 4 KB
+constexpr int kStageB = 4 * kSliceB;       // K, K', V, V' of a page
+constexpr int kWaveLds = 2 * kStageB + 16 * kRowB;   // two stages, query rows
+constexpr int kWaves = 4;
+constexpr int kMaxB = 8192;                // prefix table lives in LDS
+constexpr int kIds = 4000;                 // page ids kept in LDS, all ranges
 
 struct DecodeDiffArgs {
   const __bf16* q;
@@ -11,36 +45,614 @@ struct DecodeDiffArgs {
   const __bf16* vpool;
   const int32_t* bt;
   int64_t bt_stride;
+  int bt_width;      // entries a row may be read at: min(bt_stride, 2^31-1)
   int table_wrap;
   const int32_t* ctx_lens;
-  int HQ, HKV;
-  int64_t num_pages;
+  int B, HQ;
+  int HKV;           // stored heads of a pool row
+  int rep;           // head pairs per scheduled pair of stored heads (1..8)
+  int kv_div;        // scheduled pairs per stored one
+  int per_wg;        // pairs of stored heads per work-group (1, 2 or 4)
+  int num_pages;     // clamped to INT32_MAX: page ids are int32
   int window;
-  float scale;
+  float scale_log2;
+  int min_pages;
   DiffWeights w;
   __bf16* out;
   float* lse;
+  float* part_o;     // [B + ranges, HQ, 256] fp32
+  float* part_lse;   // [B + ranges, HQ]
+  int* geo;          // [B + 2]: pages per range, then the page prefix
+  int ids_off;       // LDS byte offset of the page ids
 };
 
-__global__ __launch_bounds__(256) void decode_diff_kernel(DecodeDiffArgs a) {
-  const int h = blockIdx.x, b = blockIdx.y;
-  const int n = max(0, a.ctx_lens[b]);
-  const int lo = a.window > 0 && n > a.window ? n - a.window : 0;
-  const int64_t row_e = (int64_t)a.HKV * kD;
-  const int32_t* const row = a.bt + b * a.bt_stride;
-  auto rows = [&](int pos, int64_t& kr, int64_t& vr) {
-    int lp = pos / kPage;
-    if (a.table_wrap > 0) lp %= a.table_wrap;
-    if (lp >= a.bt_stride) return;
-    const int pg = row[lp];
-    if (pg < 0 || pg >= a.num_pages) return;
-    kr = vr = ((int64_t)pg * kPage + pos % kPage) * row_e;
+__device__ __forceinline__ int vis_lo(int n, int window) {
+  return (window > 0 && n > window) ? n - window : 0;
+}
+// pages of a request of n tokens that hold a visible key
+__device__ __forceinline__ int vis_pages(int n, int window) {
+  if (n <= 0) return 0;
+  return (int)(((uint32_t)n + kPage - 1) / kPage) - vis_lo(n, window) / kPage;
+}
+
+__device__ __forceinline__ int page_id(const DecodeDiffArgs& a, int b, int lp) {
+  const int idx = a.table_wrap > 0 ? lp % a.table_wrap : lp;
+  // a logical page past the row's width has no entry: its keys are absent
+  if ((unsigned)idx >= (unsigned)a.bt_width) return -1;
+  const int v = as_const(a.bt)[(int64_t)b * a.bt_stride + idx];
+  return (unsigned)v < (unsigned)a.num_pages ? v : -1;
+}
+
+// The arguments in the argument segment, read again where they are needed
+// rarely (the pointer is opaque to the compiler), so that they hold no
+// registers over the walk.
+typedef const __attribute__((address_space(4))) DecodeDiffArgs* ArgsPtr;
+__device__ __forceinline__ ArgsPtr rare_args() {
+  auto p = (ArgsPtr)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
+
+// One page of the flattened page stream (wave-uniform).
+struct Step {
+  int b;       // request (-1: past the end of the range)
+  int n;       // its context length
+  int pg;      // logical page
+  int flags;
+};
+enum : int {
+  kFirst = 1,   // first step of this piece: the query rows come with it
+  kLast = 2,    // last step of this piece
+  kFull = 4,    // the page is there and all its tokens are visible
+  kThere = 8,   // the page is there
+  kWhole = 16,  // the piece is the whole request
+};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// value of the lane eight columns on (within 16-lane rows): the other map's
+__device__ __forceinline__ float other_map(float x) {
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128,
+                                         0xF, 0xF, false));   // row_ror 8
+}
+
+// One work-group per CU by its LDS, one wave per SIMD.
+__global__ __launch_bounds__(64 * kWaves)
+__attribute__((amdgpu_waves_per_eu(2, 2)))
+void decode_diff_kernel(DecodeDiffArgs a) {
+  extern __shared__ __align__(16) char smem[];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15;  // MFMA row / column index
+  const int g = lane >> 4;  // MFMA k-group
+  const int ranges = kWaves / a.per_wg;            // of this work-group
+  const int v = w / a.per_wg;
+  const int range = blockIdx.x * ranges + v;
+  const int R = gridDim.x * ranges;
+  const int pair = blockIdx.y * a.per_wg + w % a.per_wg;
+  int* pref = reinterpret_cast<int*>(smem);  // [B + 1]
+  int* wsum = pref + a.B + 1;                // [4]
+  int* nlen = wsum + kWaves;                 // [B]
+  const int ids_cap = kIds / ranges;
+  int* ids = reinterpret_cast<int*>(smem + a.ids_off) + v * (ids_cap + 2);
+
+  // ---- 1. prefix sums of visible pages: pref[b] = first page of request b --
+  {
+    int carry = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64 * kWaves) {
+      const int b = b0 + threadIdx.x;
+      const int nb = b < a.B ? as_const(a.ctx_lens)[b] : 0;
+      if (b < a.B) nlen[b] = nb;
+      const int x = wave_scan(vis_pages(nb, a.window));
+      if (lane == 63) wsum[w] = x;
+      __syncthreads();
+      int before = carry;
+      for (int j = 0; j < w; ++j) before += wsum[j];
+      if (b < a.B) pref[b + 1] = before + x;
+      for (int j = 0; j < kWaves; ++j) carry += wsum[j];
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) pref[0] = 0;
+    __syncthreads();
+  }
+  const int U = __builtin_amdgcn_readfirstlane(pref[a.B]);
+  const int C = max((U + R - 1) / R, a.min_pages);
+  // publish the split geometry for the merge
+  if (blockIdx.x == 0 && blockIdx.y == 0) {
+    for (int i = threadIdx.x; i <= a.B; i += 64 * kWaves)
+      a.geo[1 + i] = pref[i];
+    if (threadIdx.x == 0) a.geo[0] = C;
+  }
+  const int u0 = (int)min((int64_t)range * C, (int64_t)U);
+  const int u1 = (int)min((int64_t)u0 + C, (int64_t)U);
+  const int rep = a.rep;
+  const int col_h = r & 7;                        // head pair of the column
+  const bool col_ok = col_h < rep;
+  const int hq = 2 * (pair * rep + col_h) + (r >> 3);   // query head
+
+  // ---- 2. requests with no visible key: output 0, LSE -inf ---------------
+  for (int b = range; b < a.B; b += R) {
+    if (pref[b + 1] != pref[b] || !col_ok) continue;
+    __bf16* o = a.out + ((int64_t)b * (a.HQ / 2) + pair * rep + col_h) * kDV +
+                (r >> 3) * kD;
+#pragma unroll
+    for (int blk = 0; blk < 8; ++blk)
+      *reinterpret_cast<u32x2*>(o + 16 * blk + 4 * g) = u32x2{0, 0};
+    if (a.lse && g == 0) a.lse[(int64_t)b * a.HQ + hq] = -INFINITY;
+  }
+
+  // ---- 3. the page stream of [u0, u1) -------------------------------------
+  auto seq_of = [&](int u) {   // first request with pref[b + 1] > u
+    int lo = 0, hi = a.B - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (pref[mid + 1] > u) hi = mid; else lo = mid + 1;
+    }
+    return lo;
   };
-  const __bf16* const q = a.q + ((int64_t)b * a.HQ + 2 * h) * kD;
-  float* const lse = a.lse ? a.lse + (int64_t)b * a.HQ + 2 * h : nullptr;
-  diff_row<true>(q, q + kD, a.kpool, kD, a.vpool, kD, rows, h / (a.HQ / a.HKV), lo,
-           n, a.scale, a.w, h, false,
-           a.out + ((int64_t)b * (a.HQ / 2) + h) * kDV, lse, lse + 1);
+  const int nids = min(u1 - u0, ids_cap);
+  for (int i = threadIdx.x - 64 * a.per_wg * v; i < nids; i += 64 * a.per_wg) {
+    const int b = seq_of(u0 + i);
+    ids[i] = page_id(a, b, vis_lo(nlen[b], a.window) / kPage +
+                               (u0 + i - pref[b]));
+  }
+  int cb = __builtin_amdgcn_readfirstlane(seq_of(u0));
+  int seq_start = __builtin_amdgcn_readfirstlane(pref[cb]);
+  int cur_n = __builtin_amdgcn_readfirstlane(nlen[cb]);
+  int seq_end = seq_start + vis_pages(cur_n, a.window);
+  int pg_of = vis_lo(cur_n, a.window) / kPage - seq_start;   // page of unit u
+  int cu = u0;
+  int last_b = -1;  // request of the previous step handed out
+  __syncthreads();  // the ids are there; every wave is done with the tables
+  if (u0 >= u1) return;
+  uint32_t ids_at =
+      (uint32_t)(uintptr_t)((__attribute__((address_space(3))) int*)ids);
+  const uint32_t ids_end = ids_at + 4 * ids_cap;
+  int id0 = (int)lds_ld32(ids_at);
+  // The next step, and the page it reads (-1: none).
+  auto next_step = [&](Step& st, int& phys) __attribute__((always_inline)) {
+    st.b = -1;
+    st.n = st.pg = st.flags = 0;
+    phys = -1;
+    if (cu >= u1) return;
+    if (seq_end <= cu) {   // the next request that has a page
+      const ArgsPtr ra = rare_args();
+      do {
+        ++cb;
+        seq_start = seq_end;
+        cur_n = as_const(ra->ctx_lens)[cb];
+        seq_end = seq_start + vis_pages(cur_n, a.window);
+      } while (seq_end <= cu);
+      pg_of = vis_lo(cur_n, a.window) / kPage - seq_start;
+    }
+    st.b = cb;
+    st.n = cur_n;
+    st.pg = cu + pg_of;
+    phys = __builtin_amdgcn_readfirstlane(id0);
+    if (ids_at >= ids_end) phys = page_id(a, cb, st.pg);
+    ++cu;
+    ids_at = min(ids_at + 4, ids_end);
+    id0 = (int)lds_ld32(ids_at);
+    const int past = st.n - (st.pg + 1) * kPage;   // tokens after the page
+    const bool full = phys >= 0 && past >= 0 &&
+                      (a.window <= 0 || past + kPage <= a.window);
+    st.flags = (cb != last_b ? kFirst : 0) |
+               (cu == min(seq_end, u1) ? kLast : 0) | (full ? kFull : 0) |
+               (phys >= 0 ? kThere : 0) |
+               (seq_start >= u0 && seq_end <= u1 ? kWhole : 0);
+    last_b = cb;
+  };
+
+  const int row_bytes = a.HKV * kRowB;
+  const int kvs = 2 * (pair / a.kv_div);   // the first of the stored heads
+  // Tiles in LDS: 16 token rows of 256 B per slice. K row x keeps 16-byte chunk
+  // c at slot c ^ x, V row x keeps 32-byte unit u at slot u ^ (x & 7):
+  // conflict-free for the K fragment reads (16 rows, one chunk) and for the
+  // transposed V reads (8 rows, one unit, per 32 lanes). They arrive by direct
+  // loads, 4 rows per instruction: lane l fills row l >> 4, physical slot
+  // l & 15, and fetches the chunk that belongs there.
+  const int wtok = lane >> 4, wslot = lane & 15;
+  int koff[2][4], voff[2][4];   // byte offsets in a page of rows 4i + wtok, less
+                                // the 1024 i of the instructions' own offsets
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int x = 4 * i + wtok;
+      const int base = x * row_bytes + (kvs + m) * kRowB - 1024 * i;
+      koff[m][i] = base + 16 * (wslot ^ x);
+      voff[m][i] = base + 32 * ((wslot >> 1) ^ (x & 7)) + 16 * (wslot & 1);
+    }
+  const uint32_t lds_w =
+      (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)smem) +
+      w * kWaveLds;
+  const uint32_t lds_q = lds_w + 2 * kStageB;
+  // K fragment (m, kk) of lane (r, g): row r, chunk 4kk + g (queries alike: row
+  // = column)
+  const uint32_t kr0 = lds_w + r * kRowB + 16 * (g ^ r);
+  // transposed V reads: rows 4g + (s >> 2), unit blk, dims 4 (s & 3)
+  const int x0 = 4 * g + (wslot >> 2);
+  const uint32_t vr0 = lds_w + 2 * kSliceB + x0 * kRowB + 32 * (x0 & 7) +
+                       8 * (wslot & 3);
+
+  // ---- direct loads of one step: 8 for K, then 8 for V --------------------
+  auto page_dma = [&](const __bf16* pool, const Step& st, int phys,
+                      uint32_t dst, const int (&off)[2][4])
+      __attribute__((always_inline)) {
+    const int past = st.n - st.pg * kPage;   // tokens from the page's first on
+    const int r_lo = a.window > 0 ? max(0, past - a.window) : 0;
+    const int r_hi = min(kPage, past);
+    const uint64_t base = (uint64_t)(uint32_t)max(phys, 0) *
+                              (uint32_t)(kPage * row_bytes) +
+                          (uint32_t)(r_lo * row_bytes);
+    const i32x4 rs =
+        make_rsrc(reinterpret_cast<const char*>(pool) + base,
+                  phys >= 0 ? (uint32_t)((r_hi - r_lo) * row_bytes) : 0u);
+    if (r_lo > 0) {   // the window's first page
+      const int d = r_lo * row_bytes;
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+        dma4_nt<false>(rs, dst + m * kSliceB, off[m][0] - d,
+                       off[m][1] + 1024 - d, off[m][2] + 2048 - d,
+                       off[m][3] + 3072 - d);
+    } else {
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+        dma4_nt<true>(rs, dst + m * kSliceB, off[m][0], off[m][1], off[m][2],
+                      off[m][3]);
+    }
+  };
+  auto issue_k = [&](const Step& st, int phys, int stage)
+      __attribute__((always_inline)) {
+    page_dma(a.kpool, st, phys, lds_w + stage * kStageB, koff);
+  };
+  auto issue_v = [&](const Step& st, int phys, int stage)
+      __attribute__((always_inline)) {
+    page_dma(a.vpool, st, phys, lds_w + stage * kStageB + 2 * kSliceB, voff);
+  };
+  // the 16 query rows of a piece, row c = column c's (columns without a head:
+  // past the resource, zeros)
+  auto issue_q = [&](int b) __attribute__((always_inline)) {
+    const i32x4 rs =
+        make_rsrc(a.q + ((int64_t)b * a.HQ + (int64_t)2 * pair * rep) * kD,
+                  (uint32_t)(2 * rep * kRowB));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int x = 4 * i + wtok;
+      dma(rs, lds_q + 1024 * i,
+          (2 * (x & 7) + (x >> 3)) * kRowB + 16 * (wslot ^ x));
+    }
+  };
+  // this wave's LDS reads are complete: what they read may be overwritten
+  auto lds_done = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));   // lgkmcnt 0
+    asm volatile("" ::: "memory");
+  };
+
+  // ---- per-piece state ----------------------------------------------------
+  f32x4 o_acc[16];
+#pragma unroll
+  for (int blk = 0; blk < 16; ++blk) o_acc[blk] = f32x4{0, 0, 0, 0};
+  float m_run = -INFINITY;
+  float l_part = 0.0f;
+  bf16x8 qf[4];   // query fragments
+
+  // End of a piece: the result of a whole request (difference and norm
+  // included), or both maps' normalised partials for the merge.
+  auto finish_piece = [&](const Step& st) {
+    const int b = st.b;
+    const float l_tot = lane_pair(lane_pair(l_part, 16, false), 32, false);
+    const float inv = l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
+    const float lse_nat =
+        l_tot > 0.0f ? (m_run + fast_log2(l_tot)) * kLn2 : -INFINITY;
+    const ArgsPtr ra = rare_args();
+    const int HQ = ra->HQ;
+    if (st.flags & kWhole) {
+      const int h = pair * rep + min(col_h, rep - 1);
+      const float lam = ra->w.lam[(int64_t)h * ra->w.lam_stride];
+      float ss = 0.0f;
+#pragma unroll
+      for (int blk = 0; blk < 16; ++blk)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = o_acc[blk][i] * inv;
+          const float d = x - lam * other_map(x);   // (columns of map 0)
+          o_acc[blk][i] = d;
+          ss += d * d;
+        }
+      float f = ra->w.out_scale;
+      const float* const wt = ra->w.weight;
+      if (wt != nullptr) {
+        ss = lane_pair(lane_pair(ss, 16, false), 32, false);
+        f *= __builtin_amdgcn_rsqf(ss * (1.0f / kDV) + ra->w.eps);
+      }
+      if (col_ok && r < 8) {
+        __bf16* const o = ra->out + ((int64_t)b * (HQ / 2) + h) * kDV + 4 * g;
+#pragma unroll
+        for (int blk = 0; blk < 16; ++blk) {
+          f32x4 x = o_acc[blk] * f;
+          if (wt != nullptr)
+            x *= *reinterpret_cast<const f32x4*>(wt + 16 * blk + 4 * g);
+          *reinterpret_cast<u32x2*>(o + 16 * blk) =
+              u32x2{pack_bf16x2_rn(x[0], x[1]), pack_bf16x2_rn(x[2], x[3])};
+        }
+      }
+      float* const lse = ra->lse;
+      if (lse != nullptr && col_ok && g == 0)
+        lse[(int64_t)b * HQ + hq] = lse_nat;
+    } else if (col_ok) {
+      // slot b + range is unique: ranges and requests are both in order
+      const int64_t slot = (int64_t)(b + range) * HQ + hq;
+      float* const o = ra->part_o + slot * kDV + 4 * g;
+#pragma unroll
+      for (int blk = 0; blk < 16; ++blk)
+        *reinterpret_cast<f32x4*>(o + 16 * blk) = o_acc[blk] * inv;
+      if (g == 0) ra->part_lse[slot] = lse_nat;
+    }
+#pragma unroll
+    for (int blk = 0; blk < 16; ++blk) o_acc[blk] = f32x4{0, 0, 0, 0};
+    m_run = -INFINITY;
+    l_part = 0.0f;
+  };
+
+  // ---- 4. software-pipelined walk ------------------------------------------
+  // Step s sits in stage s & 1. Its fragments are read into registers first,
+  // each half of the stage then makes room for step s + 2 at once: two steps
+  // (32 KB per wave) are in flight while one is computed. Queries: those of the
+  // next step, if it starts a piece, go out at the top of this one.
+  constexpr int kNK = 8, kNS = 16;   // loads of a step's K, and of a step
+  Step cur, nx, nn;
+  int phys;
+  next_step(cur, phys);
+  issue_q(cur.b);
+  issue_k(cur, phys, 0);
+  issue_v(cur, phys, 0);
+  next_step(nx, phys);
+  issue_k(nx, phys, 1);
+  issue_v(nx, phys, 1);
+  auto read_q = [&]() __attribute__((always_inline)) {
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+      qf[kk] = lds_ld128((kr0 ^ (64u * kk)) + 2 * kStageB);
+    lds_done();
+  };
+  wait_vm<2 * kNS>();
+  read_q();
+  cur.flags &= ~kFirst;
+  for (;;) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t so = k * kStageB;
+      if (cur.flags & kFirst) {
+        wait_vm<kNS>();
+        read_q();
+      }
+      if (nx.flags & kFirst) issue_q(nx.b);
+      // ---- K fragments -----------------------------------------------------
+      wait_vm<kNK + kNS>();   // after K(s), in flight: V(s) and step s + 1
+      asm volatile("" ::: "memory");
+      bf16x8 kf[2][4];
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+          kf[m][kk] = lds_ld128((kr0 ^ (64u * kk)) + so + m * kSliceB);
+      next_step(nn, phys);
+      lds_done();
+      // ---- S^T = K.Q^T with both key heads -----------------------------------
+      f32x4 sc[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+          sc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[m][kk], qf[kk],
+                                                          sc[m], 0, 0, 0);
+      issue_k(nn, phys, k);
+      // ---- V^T fragments -------------------------------------------------------
+      // A operand (dims 16 blk + r, tokens 4g..4g+3) by one transposed read:
+      // source lane s of each 16-lane group names token 4g + (s >> 2) and dims
+      // 16 blk + 4 (s & 3)..+3
+      wait_vm<kNS + kNK>();   // after V(s): step s + 1 and K(s + 2)
+      asm volatile("" ::: "memory");
+      bf16x4 vf[16];
+#pragma unroll
+      for (int blk = 0; blk < 16; ++blk)
+        vf[blk] = lds_tr16((vr0 ^ (32u * (blk & 7))) + so +
+                           (blk >> 3) * kSliceB);
+      __builtin_amdgcn_sched_barrier(0);   // (or the reads sink to their uses)
+      // ---- mask, running max -----------------------------------------------
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        x[i] = (r < 8 ? sc[0][i] : sc[1][i]) * a.scale_log2;
+      if (!(cur.flags & kFull)) {
+        const int lo = vis_lo(cur.n, a.window);
+        const bool there = cur.flags & kThere;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int kpos = cur.pg * kPage + 4 * g + i;
+          x[i] = there && kpos >= lo && kpos < cur.n ? x[i] : -INFINITY;
+        }
+      }
+      float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+      mx = lane_pair(lane_pair(mx, 16, true), 32, true);
+      const bool move = mx > m_run;
+      if (__builtin_amdgcn_ballot_w64(move)) {
+        const float m_new = move ? mx : m_run;
+        const float alpha = move ? fast_exp2(m_run - m_new) : 1.0f;
+        m_run = m_new;
+        l_part *= alpha;
+#pragma unroll
+        for (int blk = 0; blk < 16; ++blk) o_acc[blk] = o_acc[blk] * alpha;
+      }
+      const float m_use = m_run == -INFINITY ? 0.0f : m_run;
+      // ---- probabilities: fp32 sum, bf16 operand -----------------------------
+      // B-operand element i  <->  token 4g + i
+      float p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = fast_exp2(x[i] - m_use);
+      l_part += (p[0] + p[1]) + (p[2] + p[3]);
+      const s16x4 pf = __builtin_bit_cast(
+          s16x4, u32x2{pack_bf16x2_rn(p[0], p[1]), pack_bf16x2_rn(p[2], p[3])});
+      // ---- O^T += V^T.P^T ------------------------------------------------------
+      lds_done();
+#pragma unroll
+      for (int blk = 0; blk < 16; ++blk)
+        o_acc[blk] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
+            __builtin_bit_cast(s16x4, vf[blk]), pf, o_acc[blk], 0, 0, 0);
+      issue_v(nn, phys, k);
+      if (cur.flags & kLast) finish_piece(cur);
+      cur = nx;
+      nx = nn;
+      if (cur.b < 0) {
+        wait_vm<0>();   // no direct load outlives the wave
+        return;
+      }
+    }
+  }
+}
+
+// Join the pieces of every request that several ranges shared, in a fixed
+// order: grid (B, HQ / 2 / H), H head pairs per work-group, for each S groups
+// of two waves, one per map (4 dims per lane). Group s takes pieces s, s + S,
+// ..., eight loads in flight at a time; the groups' results then merge through
+// LDS in order, and the first group takes the difference and the norm.
+template <int H, int S>
+__global__ __launch_bounds__(128 * H * S) void decode_diff_merge(
+    DecodeDiffArgs a) {
+  const int b = blockIdx.x;
+  const int C = as_const(a.geo)[0];
+  const int s0 = as_const(a.geo)[1 + b];
+  const int s1 = as_const(a.geo)[2 + b];
+  if (s1 <= s0) return;                  // no visible key: written already
+  const int first = s0 / C;
+  const int np = (s1 - 1) / C - first + 1;
+  if (np <= 1) return;                   // one piece: written in place
+  __shared__ float part[H * S][2][6][64];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m = w & 1, grp = w >> 1, sub = grp % S;
+  const int h = blockIdx.y * H + grp / S;
+  const bool hok = h < a.HQ / 2;
+  const int d0 = 4 * lane;
+  const int64_t slot0 =
+      (int64_t)(b + first) * a.HQ + 2 * (hok ? h : 0) + m;
+  float mx = -INFINITY, sum = 0.0f;
+  f32x4 acc = f32x4{0, 0, 0, 0};
+  auto add = [&](float l, float w1, f32x4 o) {   // a piece (LSE l, weight w1)
+    const float m_new = fmaxf(mx, l);
+    const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+    const float keep = fast_exp2((mx - m_use) * kLog2e);
+    const float wt = fast_exp2((l - m_use) * kLog2e);
+    sum = sum * keep + wt * w1;
+    acc = acc * keep + o * wt;
+    mx = m_new;
+  };
+  constexpr int kBatch = 8;
+  for (int k = sub; k < np; k += kBatch * S) {
+    float l[kBatch];
+    f32x4 o[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const bool in = k + j * S < np;
+      const int64_t slot = slot0 + (int64_t)(in ? k + j * S : 0) * a.HQ;
+      l[j] = in ? a.part_lse[slot] : -INFINITY;
+      o[j] = *reinterpret_cast<const f32x4*>(a.part_o + slot * kDV + d0);
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)     // (0 x infinity: weight 0 won't do)
+      add(l[j], 1.0f, k + j * S < np ? o[j] : f32x4{0, 0, 0, 0});
+  }
+  auto put = [&]() {
+    part[grp][m][0][lane] = mx;
+    part[grp][m][1][lane] = sum;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[grp][m][2 + i][lane] = acc[i];
+  };
+  if (S > 1) {
+    if (sub > 0) put();
+    __syncthreads();
+    if (sub == 0)
+      for (int j = 1; j < min(np, S); ++j) {
+        f32x4 o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = part[grp + j][m][2 + i][lane];
+        add(part[grp + j][m][0][lane], part[grp + j][m][1][lane], o);
+      }
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  acc = acc * inv;
+  if (sub == 0 && hok && a.lse && lane == 0)
+    a.lse[(int64_t)b * a.HQ + 2 * h + m] =
+        sum > 0.0f ? mx + fast_log2(sum) * kLn2 : -INFINITY;
+  // the second map goes to the first one's wave
+  if (sub == 0 && m == 1) put();
+  __syncthreads();
+  if (sub > 0 || m > 0 || !hok) return;
+  const float lam = a.w.lam[(int64_t)h * a.w.lam_stride];
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    acc[i] -= lam * part[grp][1][2 + i][lane];
+    ss += acc[i] * acc[i];
+  }
+  acc = acc * a.w.out_scale;
+  if (a.w.weight) {
+    for (int x = 1; x < 64; x <<= 1) ss += __shfl_xor(ss, x);
+    acc = acc * __builtin_amdgcn_rsqf(ss * (1.0f / kDV) + a.w.eps) *
+          *reinterpret_cast<const f32x4*>(a.w.weight + d0);
+  }
+  *reinterpret_cast<u32x2*>(a.out + ((int64_t)b * (a.HQ / 2) + h) * kDV + d0) =
+      u32x2{pack_bf16x2_rn(acc[0], acc[1]), pack_bf16x2_rn(acc[2], acc[3])};
+}
+
+// The merge's shape, from the pieces of an average request.
+void launch_merge(const DecodeDiffArgs& a, int R, hipStream_t st) {
+  const int np = 1 + R / a.B, H = a.HQ / 2;
+  if (np <= 8 || H > 65535)
+    hipLaunchKernelGGL((decode_diff_merge<4, 1>), dim3(a.B, (H + 3) / 4),
+                       dim3(512), 0, st, a);
+  else
+    hipLaunchKernelGGL((decode_diff_merge<1, 8>), dim3(a.B, H), dim3(1024), 0,
+                       st, a);
+}
+
+// Head pairs per scheduled pair of stored heads: the whole ratio up to 8 (two
+// maps each fill the 16 MFMA columns), else its largest divisor up to 8, the
+// stored pair then scheduled several times (each reading its pages once).
+int group_of(int ratio) {
+  int rep = ratio;
+  while (rep > 8 || ratio % rep != 0) --rep;
+  return rep;
+}
+
+struct Shape {
+  int rep, pairs, per_wg, G, R;   // R: ranges of the launch
+};
+// Three work-groups per four CUs, as the plain decode; four waves each, which
+// take 4, 2 or 1 pairs of stored heads and 1, 2 or 4 ranges.
+Shape shape_of(int HQ, int HKV, int num_workgroups) {
+  Shape s;
+  s.rep = group_of(HQ / HKV);
+  s.pairs = HQ / 2 / s.rep;
+  s.per_wg = s.pairs % 4 == 0 ? 4 : s.pairs % 2 == 0 ? 2 : 1;
+  const int ny = s.pairs / s.per_wg;
+  s.G = num_workgroups > 0 ? num_workgroups : 3 * device_cus() / (4 * ny);
+  if (s.G < 1) s.G = 1;
+  s.R = s.G * (kWaves / s.per_wg);
+  return s;
+}
+
+size_t ws_layout(int B, int HQ, int R, size_t* off_lse, size_t* off_geo) {
+  const size_t slots = (size_t)B + R;
+  const size_t o_bytes = slots * HQ * kDV * sizeof(float);
+  const size_t l_bytes = (slots * HQ * sizeof(float) + 255) & ~(size_t)255;
+  const size_t g_bytes = (((size_t)B + 2) * sizeof(int) + 255) & ~(size_t)255;
+  if (off_lse) *off_lse = o_bytes;
+  if (off_geo) *off_geo = o_bytes + l_bytes;
+  return o_bytes + l_bytes + g_bytes;
 }
 
 }  // namespace
@@ -52,8 +664,9 @@ extern "C" size_t tmopt_attn_decode_diff_workspace_size(int B, int HQ, int HKV,
                                                         int D,
                                                         int num_workgroups) {
   (void)D;
-  (void)num_workgroups;
-  return B > 0 && HQ > 0 && HKV > 0 ? 16 : 0;
+  if (B <= 0 || HQ <= 0 || HKV <= 0 || HKV % 2 != 0 || HQ % HKV != 0) return 0;
+  return ws_layout(B, HQ, shape_of(HQ, HKV, num_workgroups).R, nullptr,
+                   nullptr);
 }
 
 extern "C" int tmopt_attn_decode_diff(
@@ -67,8 +680,8 @@ extern "C" int tmopt_attn_decode_diff(
   clear_error();
   if (B == 0) return TMOPT_OK;
   TMOPT_REQUIRE(B > 0, TMOPT_EINVAL, "decode_diff: B=%d", B);
-  TMOPT_REQUIRE(B <= 8192, TMOPT_EUNSUPPORTED, "decode_diff: B=%d above 8192",
-                B);
+  TMOPT_REQUIRE(B <= kMaxB, TMOPT_EUNSUPPORTED, "decode_diff: B=%d above %d",
+                B, kMaxB);
   TMOPT_REQUIRE(q && k_pool && v_pool && out && block_table && ctx_lens,
                 TMOPT_EINVAL, "decode_diff: null tensor pointer");
   const int rc = check_diff("decode_diff", HQ, HKV, D, window, scale, lam,
@@ -94,8 +707,13 @@ extern "C" int tmopt_attn_decode_diff(
   TMOPT_REQUIRE(((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool |
                  (uintptr_t)out) % 16 == 0,
                 TMOPT_EINVAL, "decode_diff: tensors must be 16-byte aligned");
-  const size_t need = tmopt_attn_decode_diff_workspace_size(B, HQ, HKV, D,
-                                                            num_workgroups);
+  const Shape s = shape_of(HQ, HKV, num_workgroups);
+  const int ny = s.pairs / s.per_wg;
+  TMOPT_REQUIRE(ny <= 65535, TMOPT_EUNSUPPORTED,
+                "decode_diff: %d pairs of stored heads exceed the grid",
+                s.pairs);
+  size_t off_lse = 0, off_geo = 0;
+  const size_t need = ws_layout(B, HQ, s.R, &off_lse, &off_geo);
   TMOPT_REQUIRE(workspace && workspace_bytes >= need &&
                     (uintptr_t)workspace % 16 == 0,
                 TMOPT_EWORKSPACE,
@@ -107,17 +725,35 @@ extern "C" int tmopt_attn_decode_diff(
   a.vpool = (const __bf16*)v_pool;
   a.bt = block_table;
   a.bt_stride = bt_stride;
+  a.bt_width = bt_stride > 0x7fffffff ? 0x7fffffff : (int)bt_stride;
   a.table_wrap = table_wrap;
   a.ctx_lens = ctx_lens;
+  a.B = B;
   a.HQ = HQ;
   a.HKV = HKV;
-  a.num_pages = num_pages;
+  a.rep = s.rep;
+  a.kv_div = HQ / HKV / s.rep;
+  a.per_wg = s.per_wg;
+  a.num_pages = num_pages > 0x7fffffff ? 0x7fffffff : (int)num_pages;
   a.window = window;
-  a.scale = scale;
+  a.scale_log2 = scale * kLog2e;
+  a.min_pages = min_pages;
   a.w = DiffWeights{lam, lam_stride, norm_weight, norm_eps, out_scale};
   a.out = (__bf16*)out;
   a.lse = lse;
-  hipLaunchKernelGGL(decode_diff_kernel, dim3(HQ / 2, B), dim3(256), 0,
-                     (hipStream_t)stream, a);
-  return check_launch("decode_diff");
+  a.part_o = (float*)workspace;
+  a.part_lse = (float*)((char*)workspace + off_lse);
+  a.geo = (int*)((char*)workspace + off_geo);
+  const size_t tab =
+      ((2 * (size_t)B + 1 + kWaves) * sizeof(int) + 15) & ~(size_t)15;
+  const size_t tiles = (size_t)kWaves * kWaveLds;
+  a.ids_off = (int)(tab > tiles ? tab : tiles);
+  const size_t lds = a.ids_off + (kIds + 2 * kWaves) * sizeof(int);
+  hipStream_t st = (hipStream_t)stream;
+  hipLaunchKernelGGL(decode_diff_kernel, dim3(s.G, ny), dim3(64 * kWaves), lds,
+                     st, a);
+  const int rc2 = check_launch("decode_diff");
+  if (rc2) return rc2;
+  launch_merge(a, s.R, st);
+  return check_launch("decode_diff_merge");
 }

@@ -55,18 +55,6 @@ __device__ __forceinline__ int pages_of(int n) {
   return (int)(((uint32_t)n + kPage - 1) / kPage);
 }
 
-// inclusive sum over the wave (as the decode's scan: row shifts, then the row
-// totals carried over)
-__device__ __forceinline__ int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
-  return x;
-}
-
 // last index i in [0, n) with s[i] <= x (s ascending, s[0] = 0 <= x)
 template <class P>
 __device__ __forceinline__ int run_of(P s, int n, int x) {
