@@ -1,24 +1,68 @@
-// Varlen causal differential attention. One work-group per (query, head pair).
-#include "diff_row.h"
+// Varlen causal (optionally windowed) differential attention on bf16 MFMA,
+// gfx950 (see diff.h for the formula).
+//
+// Matrix bound: per visible (query, key) pair and map 128 products for the
+// score and 256 for the values.
+//
+//  * A work-group owns (run, pair of stored heads, block of 128 / REP queries)
+//    for REP head pairs: 128 rows of each map, over the same tiles of 32 keys
+//    (K, K' and the 256-wide V: 32 KB) in LDS. Wave w has map w >> 2 of row
+//    block w & 3 (32 rows), so waves w and w + 4, which share a SIMD, are the
+//    two maps of the same rows. O^T of 32 rows x 256 dims takes 128 registers,
+//    which leaves two waves per SIMD room for 32-key tiles, not for 64-key
+//    ones.
+//  * S^T = K.Q^T (v_mfma_f32_32x32x16_bf16, keys on M, queries on N) leaves one
+//    query per lane; P^T is then the B operand of O^T = V^T.P^T as it is.
+//  * Tiles go from global memory straight into LDS (buffer_load ... lds), rows
+//    of 256 B, K chunks of 16 B swizzled by row & 15, V blocks of 64 B by row &
+//    3: neither the K fragments (16-byte reads) nor the V^T fragments (two
+//    transposed reads) conflict. Four stages, tiles issued three ahead.
+//  * Ping-pong: the two waves of a SIMD alternate, half a tile apart, between
+//    an MFMA phase (P.V of tile t and the scores of tile t + 1: 24 MFMAs) and
+//    the softmax of a tile.
+//  * The maps meet in LDS at the end: each wave gives its partner half of its
+//    normalised O and takes the difference and the norm of the other half.
+//  * Work items are dealt to the XCDs heaviest first (prefill_sched.h).
+#include <type_traits>
+
+#include "diff.h"
+#include "prefill_sched.h"
 
 namespace tmopt {
 namespace {
 
+constexpr int kBN = 32;                   // keys per tile
+constexpr int kRowB = 256;                // one key's slice of a stored head
+constexpr int kSliceB = kBN * kRowB;      // 8 KB
+constexpr int kStage = 4 * kSliceB;       // K, K', V, V'
+constexpr int kNStage = 4;
+constexpr int kLds = kNStage * kStage + 8 * 128;   // and the norms' sums
+constexpr float kLazy = 8.0f;             // lazy-rescale threshold (log2)
+constexpr int kRing = 4;                  // fragments read kRing - 1 ahead
+// a buffer offset past every resource this kernel builds (their ranges are
+// checked below 2^31 - 16 on the host): the load returns zeros
+constexpr int kOob = 0x7ffffff0;
+
 struct PrefillDiffArgs {
   const __bf16* q;
   int64_t q_st, q_sh;
-  const __bf16* k;
+  const __bf16* k;         // packed rows, or the pool
   int64_t k_st, k_sh;
   const __bf16* v;
   int64_t v_st, v_sh;
   const int32_t* cu;
   const int32_t* prior;
-  const int32_t* bt;     // NULL: packed k / v
+  const int32_t* bt;
   int64_t bt_stride;
-  int64_t num_pages;
-  int HQ, HKV, S;
+  int bt_width;      // entries a row may be read at: min(bt_stride, 2^31-1)
+  int num_pages;
+  int HQ;
+  int HKV;           // pairs of stored heads as scheduled
+  int kv_div;        // scheduled pairs per stored one
+  int S;
+  int nqb_max;       // query blocks of the longest run
   int window;
-  float scale;
+  float scale_log2;
   DiffWeights w;
   __bf16* out;
   int64_t o_st, o_sh;
@@ -27,30 +71,429 @@ struct PrefillDiffArgs {
   const int32_t* reject;
 };
 
-__global__ __launch_bounds__(256) void prefill_diff_kernel(PrefillDiffArgs a) {
-  const int h = blockIdx.x, j = blockIdx.y, s = blockIdx.z;
-  const int t0 = a.cu[s], len = a.cu[s + 1] - t0;
-  if (j >= len) return;
-  const int pos = (a.prior ? a.prior[s] : 0) + j;
-  const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-  const int32_t* const row = a.bt ? a.bt + s * a.bt_stride : nullptr;
-  auto rows = [&](int p, int64_t& kr, int64_t& vr) {
-    if (!row) {
-      kr = (int64_t)(t0 + p) * a.k_st;
-      vr = (int64_t)(t0 + p) * a.v_st;
-      return;
+template <int REP, bool PAGED>
+__global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
+  constexpr int BQ = 128 / REP;   // queries per work-group
+  constexpr int QSUB = BQ / 32;   // 32-query sub-blocks per head pair
+  extern __shared__ __align__(16) char smem[];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31;
+  const int h2 = lane >> 5;       // lane half
+  const Work wk = schedule(a, BQ, lane, blockIdx.x);
+  if (wk.seq < 0) return;
+  const int t0 = wk.t0, len = wk.len, prior = wk.prior;
+  const int q0 = wk.qb * BQ;
+  const int nk = prior + len;                 // keys of this run
+  const int pos_lo = prior + q0;              // first query position
+  const int pos_hi = pos_lo + min(BQ, len - q0) - 1;   // last valid one
+  // first key any query of the block may see; tiles start at a multiple of the
+  // tile width
+  const int kwin = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0;
+  const int k_lo = (kwin / kBN) * kBN;
+  const int ntiles = (pos_hi + 1 - k_lo + kBN - 1) / kBN;
+
+  // ---- this wave's row block: map, head pair and 32-query sub-block ------
+  const int map = w >> 2;
+  const int hp = wk.kvh * REP + (w & 3) / QSUB;
+  const int row0 = q0 + 32 * ((w & 3) % QSUB);
+  const int qi = row0 + l32;                  // this lane's query (column)
+  const bool qok = qi < len;
+  const int qpos = prior + qi;
+  const int kvs = 2 * (wk.kvh / a.kv_div);    // the first stored head
+
+  // ---- tile loads ----------------------------------------------------------
+  // Wave w moves key rows 4w..4w+3 of each of the four slices, one 1 KB
+  // instruction each: lane l fills row l >> 4, physical 16-byte slot l & 15,
+  // and fetches the logical chunk that belongs there.
+  const int grp = lane >> 4, slot = lane & 15;
+  const int krow = 4 * w + grp;
+  const int kchunk = slot ^ (krow & 15);
+  const int vchunk = ((((slot >> 2) ^ grp) & 3) << 2) | (slot & 3);
+  const uint32_t lds0 =
+      (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)smem);
+  const int kst_b = (int)(a.k_st * 2), vst_b = (int)(a.v_st * 2);
+  const int ksh_b = (int)(a.k_sh * 2), vsh_b = (int)(a.v_sh * 2);
+  // packed: one resource per slice, from the run's first row (rows past the run
+  // lie outside it); paged: one per page, lane offsets from the page's rows
+  i32x4 rk[2], rv[2];
+  int klane, vlane;
+  [[maybe_unused]] const int32_t __attribute__((address_space(4)))* trow =
+      PAGED ? as_const(a.bt) + (int64_t)wk.seq * a.bt_stride : nullptr;
+  if constexpr (PAGED) {
+    klane = grp * kst_b + kvs * kRowB + 16 * kchunk;
+    vlane = grp * vst_b + kvs * kRowB + 16 * vchunk;
+  } else {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      rk[m] = make_rsrc(a.k + (int64_t)t0 * a.k_st + (kvs + m) * a.k_sh,
+                        (uint32_t)(((int64_t)(len - 1) * a.k_st + kD) * 2));
+      rv[m] = make_rsrc(a.v + (int64_t)t0 * a.v_st + (kvs + m) * a.v_sh,
+                        (uint32_t)(((int64_t)(len - 1) * a.v_st + kD) * 2));
     }
-    if (p / kPage >= a.bt_stride) return;
-    const int pg = row[p / kPage];
-    if (pg < 0 || pg >= a.num_pages) return;
-    kr = vr = ((int64_t)pg * kPage + p % kPage) * a.k_st;
+    klane = grp * kst_b + 16 * kchunk;
+    vlane = grp * vst_b + 16 * vchunk;
+  }
+  // tile t (index from k_lo) into LDS stage st: 4 instructions per wave. live
+  // == false issues the same ones fetching nothing: the loops issue a tile
+  // every iteration, past the last one too, so that the count of loads in
+  // flight is the same on every path and the waits are exact.
+  auto issue_tile = [&](int t, int st, bool live = true)
+      __attribute__((always_inline)) {
+    const int key0 = k_lo + t * kBN + 4 * w;   // first of the wave's rows
+    const uint32_t dst = lds0 + st * kStage + 4 * w * kRowB;
+    if constexpr (PAGED) {
+      // The resource covers the page's rows in [kwin, nk): others, and pages
+      // without an entry, read as zeros and are never fetched.
+      const int lp = key0 >> 4;
+      const int pg = live && (unsigned)lp < (unsigned)a.bt_width ? trow[lp] : -1;
+      const int r_lo = min(kPage, max(0, kwin - kPage * lp));
+      const int r_hi = min(kPage, max(0, nk - kPage * lp));
+      const bool valid = (unsigned)pg < (unsigned)a.num_pages && r_hi > r_lo;
+      const uint32_t nrec = valid ? (uint32_t)((r_hi - r_lo) * kst_b) : 0u;
+      const int64_t ofs =
+          valid ? ((int64_t)pg * kPage + r_lo) * kst_b : 0;
+      const int roff = ((key0 & (kPage - 1)) - r_lo) * kst_b;
+      const i32x4 pk =
+          make_rsrc(reinterpret_cast<const char*>(a.k) + ofs, nrec);
+      const i32x4 pv =
+          make_rsrc(reinterpret_cast<const char*>(a.v) + ofs, nrec);
+      dma(pk, dst, klane + roff);
+      dma(pk, dst + kSliceB, klane + roff + kRowB);
+      dma(pv, dst + 2 * kSliceB, vlane + roff);
+      dma(pv, dst + 3 * kSliceB, vlane + roff + kRowB);
+    } else {
+      const int ko = live ? klane + key0 * kst_b : kOob;
+      const int vo = live ? vlane + key0 * vst_b : kOob;
+      dma(rk[0], dst, ko);
+      dma(rk[1], dst + kSliceB, ko);
+      dma(rv[0], dst + 2 * kSliceB, vo);
+      dma(rv[1], dst + 3 * kSliceB, vo);
+    }
   };
-  const __bf16* const q = a.q + (int64_t)(t0 + j) * a.q_st + 2 * h * a.q_sh;
-  const bool rejected = a.reject && *a.reject != 0;
-  float* const lse = a.lse ? a.lse + 2 * h * a.lse_sh + t0 + j : nullptr;
-  diff_row<false>(q, q + a.q_sh, a.k, a.k_sh, a.v, a.v_sh, rows, h / (a.HQ / a.HKV),
-           lo, rejected ? lo : pos + 1, a.scale, a.w, h, rejected,
-           a.out + (int64_t)(t0 + j) * a.o_st + h * a.o_sh, lse, lse + a.lse_sh);
+
+  // ---- LDS fragment addresses -------------------------------------------
+  // K fragment kk of lane (l32, h2): row l32, logical chunk 2 kk + h2 -> slot
+  // (2 kk + h2) ^ (l32 & 15).
+  const uint32_t ka0 = (uint32_t)(map * kSliceB + l32 * kRowB +
+                                  16 * (h2 ^ (l32 & 15)));
+  // V^T fragment (db, kk) by two transposed reads: within each 16-lane group,
+  // source lane s names key kbase + (s >> 2), dims 4 (s & 3)..+3 of a 16-dim
+  // half; lane i of the group then holds dim dbase + i of keys kbase..kbase+3.
+  // kbase = 16 kk + 4 h2 (+8 for the second read), dbase = 32 db + 16 (l32 >>
+  // 4): the order of this lane's probabilities.
+  const int s16 = lane & 15;
+  const uint32_t va0 = (uint32_t)(2 * kSliceB + (4 * h2 + (s16 >> 2)) * kRowB +
+                                  64 * (s16 >> 2) + 32 * ((lane >> 4) & 1) +
+                                  8 * (s16 & 3));
+  auto kfrag = [&](uint32_t sb, int kk) -> bf16x8 {
+    return lds_ld128((sb + ka0) ^ (32u * kk));
+  };
+  auto vfrag = [&](uint32_t sb, int db, int kk) -> bf16x8 {
+    const uint32_t p = ((sb + va0) ^ (64u * (db & 3))) + (db >> 2) * kSliceB +
+                       16 * kk * kRowB;
+    const bf16x4 lo = lds_tr16(p);
+    const bf16x4 hi = lds_tr16(p + 8 * kRowB);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+
+  bf16x8 qf[8];   // B operand of S^T (column = query, k = dims)
+  f32x16 o_acc[8];
+#pragma unroll
+  for (int db = 0; db < 8; ++db) o_acc[db] = f32x16{};
+  float m_run = -INFINITY;
+  float l_part = 0.0f;
+  f32x16 sc;       // scores of the tile after the one being multiplied
+  bf16x8 pf[2];    // probabilities of the tile being multiplied
+
+  // Softmax of the scores of the tile at kt: P^T fragments, running maximum and
+  // sum, O^T rescaled when the maximum moved. The maximum only moves when the
+  // tile's exceeds it by more than 2^kLazy, so that O^T is rescaled on few
+  // tiles; O / l and the LSE are exact for any reference point. Element j of
+  // the scores holds key kt + 4 h2 + 8 (j >> 2) + (j & 3). `hook` runs first.
+  auto softmax_phase = [&](int kt, bool first, auto&& hook)
+      __attribute__((always_inline)) {
+    // a tile every valid query of the block sees whole (columns past the run
+    // end hold zero queries and are never stored)
+    const bool full = (kt + kBN - 1 <= pos_lo) && (kt + kBN <= nk) &&
+                      (a.window == 0 || pos_hi - kt < a.window);
+    hook();
+    if (!full) {
+      const int base = kt + 4 * h2;
+      const int hi = qok ? min(qpos, nk - 1) - base : -1;
+      const int lo = a.window > 0 ? qpos - a.window - base : -1;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int c = 8 * (j >> 2) + (j & 3);
+        sc[j] = (c <= hi && c > lo) ? sc[j] : -INFINITY;
+      }
+    }
+    const float sl2 = a.scale_log2;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) mx = fmaxf(fmaxf(mx, sc[j]), sc[j + 1]);
+    mx = lane_pair(mx, 32, true);
+    const float m_cand = mx * sl2;
+    const bool move = m_cand > m_run + kLazy;
+    const float m_new = move ? m_cand : m_run;
+    const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+    const float alpha = move ? fast_exp2(m_run - m_use) : 1.0f;
+    m_run = m_new;
+    float psum = 0.0f;
+    uint32_t pw[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float p0 = fast_exp2(__builtin_fmaf(sc[2 * q], sl2, -m_use));
+      const float p1 = fast_exp2(__builtin_fmaf(sc[2 * q + 1], sl2, -m_use));
+      psum += p0 + p1;
+      pw[q] = pack_bf16x2_rn(p0, p1);
+    }
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+      pf[kk] = __builtin_bit_cast(
+          bf16x8, u32x4{pw[4 * kk], pw[4 * kk + 1], pw[4 * kk + 2],
+                        pw[4 * kk + 3]});
+    l_part = l_part * alpha + psum;
+    // (in place, each product tied to its accumulator register: a plain
+    // multiply under the branch costs a second copy of O^T)
+    if (!first && __builtin_amdgcn_ballot_w64(move)) {
+#pragma unroll
+      for (int db = 0; db < 8; ++db)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          float x = o_acc[db][j];
+          asm volatile("v_mul_f32 %0, %1, %0" : "+v"(x) : "v"(alpha));
+          o_acc[db][j] = x;
+        }
+    }
+  };
+
+  // MFMA phase of tile t: O^T += V^T.P^T for tile t, with the scores of tile
+  // t + 1 after every second MFMA, fragments read kRing - 1 MFMAs ahead.
+  auto mfma_phase = [&](int t, auto with_s_c) __attribute__((always_inline)) {
+    constexpr bool with_s = decltype(with_s_c)::value;
+    // this wave's MFMAs first; the softmax wave fills the issue slots between
+    __builtin_amdgcn_s_setprio(1);
+    const uint32_t vb = lds0 + (t & 3) * kStage;
+    const uint32_t kb = lds0 + ((t + 1) & 3) * kStage;
+    constexpr int R = kRing, RK = 3;
+    bf16x8 vf[R], kf[RK];
+#pragma unroll
+    for (int i = 0; i < R - 1; ++i) vf[i] = vfrag(vb, i & 7, i >> 3);
+    if (with_s) {
+#pragma unroll
+      for (int i = 0; i < RK - 1; ++i) kf[i] = kfrag(kb, i);
+    }
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+      const int x = n + R - 1;
+      if (x < 16) vf[x % R] = vfrag(vb, x & 7, x >> 3);
+      o_acc[n & 7] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+          vf[n % R], pf[n >> 3], o_acc[n & 7], 0, 0, 0);
+      if (with_s && (n & 1)) {
+        const int kk = n >> 1, y = kk + RK - 1;
+        if (y < 8) kf[y % RK] = kfrag(kb, y);
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            kf[kk % RK], qf[kk], kk == 0 ? f32x16{} : sc, 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+  };
+  auto first_scores = [&] {
+    sc = f32x16{};
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk)
+      sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfrag(lds0, kk), qf[kk], sc,
+                                                   0, 0, 0);
+  };
+
+  const bool rejected = a.reject != nullptr && as_const(a.reject)[0] != 0;
+  if (!rejected) {
+    // Slot 2t: group 0 multiplies tile t, group 1 does the softmax of tile t;
+    // slot 2t + 1: group 0 the softmax of tile t + 1, group 1 multiplies tile
+    // t. Tile t + 3 goes out at the start of slot 2t into the stage of tile t -
+    // 1 (last read in slot 2t - 1) and must be in LDS before slot 2t + 4; each
+    // wave waits for its own part at the end of every odd slot, before the
+    // barrier that publishes it. The queries come first, through stages 2 and 3
+    // (8 KB per wave; rows past the run end arrive as zeros).
+    const uint32_t qlds = lds0 + 2 * kStage + (uint32_t)w * (32 * kRowB);
+    {
+      const int64_t span = ((int64_t)(len - row0 - 1) * a.q_st + kD) * 2;
+      const i32x4 rq = make_rsrc(a.q + (int64_t)(t0 + row0) * a.q_st +
+                                     (int64_t)(2 * hp + map) * a.q_sh,
+                                 row0 < len ? (uint32_t)span : 0u);
+      const int qst_b = (int)(a.q_st * 2);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + grp;
+        dma(rq, qlds + i * 1024, r * qst_b + 16 * (slot ^ (r & 15)));
+      }
+    }
+    issue_tile(0, 0);
+    if (ntiles > 1) issue_tile(1, 1);
+    wait_vm<0>();
+    __syncthreads();
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      u32x4 x = __builtin_bit_cast(
+          u32x4,
+          lds_ld128(qlds + l32 * kRowB + 16 * ((2 * kk + h2) ^ (l32 & 15))));
+      if (!qok) x = u32x4{0, 0, 0, 0};
+      qf[kk] = __builtin_bit_cast(bf16x8, x);
+    }
+    __syncthreads();
+    if (ntiles > 2) issue_tile(2, 2);
+    auto odd_end = [&](int n) {
+      if (n == 4) wait_vm<4>();
+      else wait_vm<0>();
+      __syncthreads();
+    };
+    // (the first and last tiles are peeled off the loops, so that these hold
+    // one variant of the MFMA phase and O^T keeps one set of registers)
+    constexpr std::true_type kWithS{};
+    constexpr std::false_type kNoS{};
+    auto none = [] {};
+    if (map == 0) {
+      first_scores();
+      softmax_phase(k_lo, true, none);
+      for (int t = 0; t + 1 < ntiles; ++t) {
+        issue_tile(t + 3, (t + 3) & 3, t + 3 < ntiles);
+        mfma_phase(t, kWithS);
+        softmax_phase(k_lo + (t + 1) * kBN, false, none);
+        odd_end(4);
+      }
+      mfma_phase(ntiles - 1, kNoS);
+      odd_end(0);   // everything, before the outputs go through LDS
+    } else {
+      issue_tile(3, 3, 3 < ntiles);
+      first_scores();
+      softmax_phase(k_lo, true, none);
+      if (ntiles > 1) mfma_phase(0, kWithS);
+      else mfma_phase(0, kNoS);
+      odd_end(ntiles > 1 ? 4 : 0);
+      for (int t = 1; t + 1 < ntiles; ++t) {
+        softmax_phase(k_lo + t * kBN, false, [&] {
+          issue_tile(t + 3, (t + 3) & 3, t + 3 < ntiles);
+        });
+        mfma_phase(t, kWithS);
+        odd_end(4);
+      }
+      if (ntiles > 1) {
+        const int t = ntiles - 1;
+        softmax_phase(k_lo + t * kBN, false, none);
+        mfma_phase(t, kNoS);
+        odd_end(0);
+      }
+    }
+  }
+
+  // ---- the maps meet: normalise, difference, norm, store -------------------
+  const float l_tot = lane_pair(l_part, 32, false);
+  const float inv = rejected ? __builtin_nanf("") :
+                    l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
+  if (a.lse && h2 == 0 && qok)
+    a.lse[(2 * hp + map) * a.lse_sh + t0 + qi] =
+        rejected ? __builtin_nanf("") :
+        l_tot > 0.0f ? (m_run + fast_log2(l_tot)) * kLn2 : -INFINITY;
+  const float lam = a.w.lam[(int64_t)hp * a.w.lam_stride];
+  // dims 128 map .. +127 are this wave's; the others go to its partner, lane by
+  // lane (16 bytes each: 1 KB per store)
+  const uint32_t mine = lds0 + (uint32_t)w * 16384 + 16 * lane;
+  const uint32_t theirs = lds0 + (uint32_t)(w ^ 4) * 16384 + 16 * lane;
+  f32x16 d[4];
+#pragma unroll
+  for (int db = 0; db < 4; ++db) {
+    const f32x16 give = map == 0 ? o_acc[4 + db] : o_acc[db];
+    d[db] = (map == 0 ? o_acc[db] : o_acc[4 + db]) * inv;
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4)
+      lds_st128(mine + (4 * db + g4) * 1024,
+                __builtin_bit_cast(
+                    u32x4, f32x4{give[4 * g4] * inv, give[4 * g4 + 1] * inv,
+                                 give[4 * g4 + 2] * inv,
+                                 give[4 * g4 + 3] * inv}));
+  }
+  __syncthreads();
+  float ss = 0.0f;
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4) {
+      const f32x4 y = __builtin_bit_cast(
+          f32x4, lds_ld128(theirs + (4 * db + g4) * 1024));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float& x = reinterpret_cast<float*>(&d[db])[4 * g4 + i];
+        x = map == 0 ? x - lam * y[i] : y[i] - lam * x;
+        ss += x * x;
+      }
+    }
+  float f = a.w.out_scale;
+  const uint32_t sums = lds0 + kNStage * kStage;
+  if (a.w.weight) {
+    ss = lane_pair(ss, 32, false);
+    if (h2 == 0)
+      *(__attribute__((address_space(3))) float*)(uintptr_t)(sums + 128 * w +
+                                                             4 * l32) = ss;
+  }
+  __syncthreads();   // (and both halves of the exchange have been read)
+  if (a.w.weight) {
+    ss += __builtin_bit_cast(float, lds_ld32(sums + 128 * (w ^ 4) + 4 * l32));
+    f *= __builtin_amdgcn_rsqf(ss * (1.0f / kDV) + a.w.eps);
+  }
+  // Through LDS, so that the stores are whole rows: 32 queries x 128 dims,
+  // query-major (256-byte rows, 16-byte chunks swizzled by row & 15), then 4
+  // complete rows per store instruction.
+  const uint32_t ob = lds0 + (uint32_t)w * 16384;
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4) {
+      f32x4 x = f32x4{d[db][4 * g4], d[db][4 * g4 + 1], d[db][4 * g4 + 2],
+                      d[db][4 * g4 + 3]} * f;
+      if (a.w.weight)
+        x *= *reinterpret_cast<const f32x4*>(a.w.weight + 128 * map + 32 * db +
+                                             8 * g4 + 4 * h2);
+      const int c = 4 * db + g4;    // 16-byte chunk: dims 8c .. 8c+7
+      lds_st64(ob + l32 * kRowB + 16 * (c ^ (l32 & 15)) + 8 * h2,
+               u32x2{pack_bf16x2_rn(x[0], x[1]), pack_bf16x2_rn(x[2], x[3])});
+    }
+  wave_lds_sync();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + grp;
+    const u32x4 x = __builtin_bit_cast(
+        u32x4, lds_ld128(ob + r * kRowB + 16 * (slot ^ (r & 15))));
+    if (row0 + r < len)
+      *reinterpret_cast<u32x4*>(a.out + (int64_t)(t0 + row0 + r) * a.o_st +
+                                (int64_t)hp * a.o_sh + 128 * map + 8 * slot) =
+          x;
+  }
+}
+
+// Work-groups of a launch: scheduled pairs * items of each, rounded up to whole
+// XCD rounds.
+int64_t launch_wgs(int pairs, int BQ, int S, int max_seqlen) {
+  const int64_t items = (int64_t)S * ((max_seqlen + BQ - 1) / BQ);
+  if (pairs <= 8 && 8 % pairs == 0)
+    return 8 * ((items + 8 / pairs - 1) / (8 / pairs));
+  return pairs * items;
+}
+
+// Head pairs per work-group: the largest of 4, 2, 1 dividing HQ / HKV; a larger
+// ratio runs as several scheduled pairs per stored one.
+int group_of(int ratio) { return ratio % 4 == 0 ? 4 : ratio % 2 == 0 ? 2 : 1; }
+
+template <int REP>
+void launch(const PrefillDiffArgs& a, int64_t n, hipStream_t st) {
+  if (a.bt)
+    hipLaunchKernelGGL((prefill_diff_kernel<REP, true>), dim3((unsigned)n),
+                       dim3(512), kLds, st, a);
+  else
+    hipLaunchKernelGGL((prefill_diff_kernel<REP, false>), dim3((unsigned)n),
+                       dim3(512), kLds, st, a);
 }
 
 }  // namespace
@@ -137,6 +580,11 @@ extern "C" int tmopt_attn_prefill_diff(
                 TMOPT_EWORKSPACE,
                 "prefill_diff: workspace %zu bytes < %zu needed (or unaligned)",
                 workspace_bytes, need);
+  const int rep = group_of(HQ / HKV), pairs = HQ / 2 / rep, BQ = 128 / rep;
+  const int64_t n = launch_wgs(pairs, BQ, num_seqs, max_seqlen_q);
+  TMOPT_REQUIRE(n < 0x7fffffff, TMOPT_EUNSUPPORTED,
+                "prefill_diff: %lld work-groups exceed the grid limit",
+                (long long)n);
   PrefillDiffArgs a;
   a.q = (const __bf16*)q;
   a.q_st = q_stride_tok;
@@ -151,12 +599,15 @@ extern "C" int tmopt_attn_prefill_diff(
   a.prior = prior_lens;
   a.bt = block_table;
   a.bt_stride = bt_stride;
-  a.num_pages = num_pages;
+  a.bt_width = bt_stride > 0x7fffffff ? 0x7fffffff : (int)bt_stride;
+  a.num_pages = num_pages > 0x7fffffff ? 0x7fffffff : (int)num_pages;
   a.HQ = HQ;
-  a.HKV = HKV;
+  a.HKV = pairs;
+  a.kv_div = HQ / HKV / rep;
   a.S = num_seqs;
+  a.nqb_max = (max_seqlen_q + BQ - 1) / BQ;
   a.window = window;
-  a.scale = scale;
+  a.scale_log2 = scale * kLog2e;
   a.w = DiffWeights{lam, lam_stride, norm_weight, norm_eps, out_scale};
   a.out = (__bf16*)out;
   a.o_st = o_stride_tok;
@@ -164,9 +615,9 @@ extern "C" int tmopt_attn_prefill_diff(
   a.lse = lse;
   a.lse_sh = lse_stride_head;
   a.reject = reject;
-  TMOPT_REQUIRE(max_seqlen_q <= 65535, TMOPT_EUNSUPPORTED,
-                "prefill_diff: max_seqlen_q=%d", max_seqlen_q);
-  hipLaunchKernelGGL(prefill_diff_kernel, dim3(HQ / 2, max_seqlen_q, num_seqs),
-                     dim3(256), 0, (hipStream_t)stream, a);
+  const hipStream_t st = (hipStream_t)stream;
+  if (rep == 4) launch<4>(a, n, st);
+  else if (rep == 2) launch<2>(a, n, st);
+  else launch<1>(a, n, st);
   return check_launch("prefill_diff");
 }
