@@ -13,13 +13,17 @@
 //    columns at once. A plain attention kernel run once per map would read K
 //    once and V twice.
 //  * Pages of all requests are laid end to end and dealt out in equal
-//    contiguous ranges, one per wave and pair of stored heads, so that a launch
-//    streams the same bytes everywhere whatever the lengths, and its grid does
-//    not depend on them (a captured call stays valid). A piece of a request
-//    that one range does not hold whole leaves a normalised fp32 result of both
-//    maps with their LSE; decode_diff_merge joins the pieces in order, then
-//    takes the difference and the norm. No atomics: repeated calls are bitwise
-//    equal.
+//    contiguous ranges, so that a launch streams the same bytes everywhere
+//    whatever the lengths, and its grid does not depend on them (a captured
+//    call stays valid). A piece of a request that one range does not hold whole
+//    leaves a normalised fp32 result of both maps with their LSE;
+//    decode_diff_merge joins the pieces in order, then takes the difference and
+//    the norm. No atomics: repeated calls are bitwise equal.
+//  * A range belongs to two waves where there are fewer than four pairs of
+//    stored heads: the first walks its first half forward, the second its
+//    second half backward, so that the request in the middle is the last of
+//    both, and they join it in LDS. A 256-wide fp32 row per map and piece is
+//    what the split costs, twice that of plain attention.
 //  * One page is a wave's step: 16 KB (two K and two V slices of 16 tokens)
 //    straight into LDS (buffer_load ... lds), two steps ahead. The resource of
 //    a load is the page's rows that hold visible keys; other rows read as zeros
@@ -60,8 +64,8 @@ struct DecodeDiffArgs {
   DiffWeights w;
   __bf16* out;
   float* lse;
-  float* part_o;     // [B + ranges, HQ, 256] fp32
-  float* part_lse;   // [B + ranges, HQ]
+  float* part_o;     // [B + R, HQ, 256] fp32, R ranges
+  float* part_lse;   // [B + R, HQ]
   int* geo;          // [B + 2]: pages per range, then the page prefix
   int ids_off;       // LDS byte offset of the page ids
 };
@@ -106,6 +110,7 @@ enum : int {
   kFull = 4,    // the page is there and all its tokens are visible
   kThere = 8,   // the page is there
   kWhole = 16,  // the piece is the whole request
+  kCross = 32,  // the two waves of the range share the piece
 };
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -126,15 +131,18 @@ void decode_diff_kernel(DecodeDiffArgs a) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15;  // MFMA row / column index
   const int g = lane >> 4;  // MFMA k-group
-  const int ranges = kWaves / a.per_wg;            // of this work-group
+  // waves of one pair of stored heads, and how many of them share a range
+  const int subs = kWaves / a.per_wg;
+  const int halves = min(subs, 2);
   const int v = w / a.per_wg;
-  const int range = blockIdx.x * ranges + v;
-  const int R = gridDim.x * ranges;
+  const int half = v & (halves - 1);
+  const int range = blockIdx.x * (subs / halves) + v / halves;
+  const int R = gridDim.x * (subs / halves);
   const int pair = blockIdx.y * a.per_wg + w % a.per_wg;
   int* pref = reinterpret_cast<int*>(smem);  // [B + 1]
   int* wsum = pref + a.B + 1;                // [4]
   int* nlen = wsum + kWaves;                 // [B]
-  const int ids_cap = kIds / ranges;
+  const int ids_cap = kIds / subs;
   int* ids = reinterpret_cast<int*>(smem + a.ids_off) + v * (ids_cap + 2);
 
   // ---- 1. prefix sums of visible pages: pref[b] = first page of request b --
@@ -164,15 +172,20 @@ void decode_diff_kernel(DecodeDiffArgs a) {
       a.geo[1 + i] = pref[i];
     if (threadIdx.x == 0) a.geo[0] = C;
   }
-  const int u0 = (int)min((int64_t)range * C, (int64_t)U);
-  const int u1 = (int)min((int64_t)u0 + C, (int64_t)U);
+  // the range [r0, r1), and this wave's pages of it: [u0, u1), backward in the
+  // second half
+  const int r0 = (int)min((int64_t)range * C, (int64_t)U);
+  const int r1 = (int)min((int64_t)r0 + C, (int64_t)U);
+  const int mid = halves > 1 ? r0 + (r1 - r0 + 1) / 2 : r1;
+  const int u0 = half == 0 ? r0 : mid, u1 = half == 0 ? mid : r1;
+  const bool back = half != 0;
   const int rep = a.rep;
   const int col_h = r & 7;                        // head pair of the column
   const bool col_ok = col_h < rep;
   const int hq = 2 * (pair * rep + col_h) + (r >> 3);   // query head
 
   // ---- 2. requests with no visible key: output 0, LSE -inf ---------------
-  for (int b = range; b < a.B; b += R) {
+  for (int b = range; b < a.B && half == 0; b += R) {
     if (pref[b + 1] != pref[b] || !col_ok) continue;
     __bf16* o = a.out + ((int64_t)b * (a.HQ / 2) + pair * rep + col_h) * kDV +
                 (r >> 3) * kD;
@@ -197,50 +210,51 @@ void decode_diff_kernel(DecodeDiffArgs a) {
     ids[i] = page_id(a, b, vis_lo(nlen[b], a.window) / kPage +
                                (u0 + i - pref[b]));
   }
-  int cb = __builtin_amdgcn_readfirstlane(seq_of(u0));
+  int cu = back ? u1 - 1 : u0;   // the next page to hand out
+  int left = u1 - u0;
+  int cb = __builtin_amdgcn_readfirstlane(seq_of(max(cu, 0)));
   int seq_start = __builtin_amdgcn_readfirstlane(pref[cb]);
   int cur_n = __builtin_amdgcn_readfirstlane(nlen[cb]);
   int seq_end = seq_start + vis_pages(cur_n, a.window);
   int pg_of = vis_lo(cur_n, a.window) / kPage - seq_start;   // page of unit u
-  int cu = u0;
   int last_b = -1;  // request of the previous step handed out
   __syncthreads();  // the ids are there; every wave is done with the tables
-  if (u0 >= u1) return;
-  uint32_t ids_at =
+  const uint32_t ids0 =
       (uint32_t)(uintptr_t)((__attribute__((address_space(3))) int*)ids);
-  const uint32_t ids_end = ids_at + 4 * ids_cap;
-  int id0 = (int)lds_ld32(ids_at);
+  int id0 = (int)lds_ld32(ids0 + 4 * min(max(cu - u0, 0), ids_cap));
   // The next step, and the page it reads (-1: none).
   auto next_step = [&](Step& st, int& phys) __attribute__((always_inline)) {
     st.b = -1;
     st.n = st.pg = st.flags = 0;
     phys = -1;
-    if (cu >= u1) return;
-    if (seq_end <= cu) {   // the next request that has a page
+    if (left <= 0) return;
+    if (cu >= seq_end || cu < seq_start) {   // the next request with a page
       const ArgsPtr ra = rare_args();
       do {
-        ++cb;
-        seq_start = seq_end;
+        cb += back ? -1 : 1;
         cur_n = as_const(ra->ctx_lens)[cb];
-        seq_end = seq_start + vis_pages(cur_n, a.window);
-      } while (seq_end <= cu);
+        const int n = vis_pages(cur_n, a.window);
+        seq_start = back ? seq_start - n : seq_end;
+        seq_end = seq_start + n;
+      } while (cu >= seq_end || cu < seq_start);
       pg_of = vis_lo(cur_n, a.window) / kPage - seq_start;
     }
     st.b = cb;
     st.n = cur_n;
     st.pg = cu + pg_of;
     phys = __builtin_amdgcn_readfirstlane(id0);
-    if (ids_at >= ids_end) phys = page_id(a, cb, st.pg);
-    ++cu;
-    ids_at = min(ids_at + 4, ids_end);
-    id0 = (int)lds_ld32(ids_at);
+    if (cu - u0 >= ids_cap) phys = page_id(a, cb, st.pg);
+    const bool last = cu == (back ? max(seq_start, u0) : min(seq_end, u1) - 1);
+    cu += back ? -1 : 1;
+    --left;
+    id0 = (int)lds_ld32(ids0 + 4 * min(max(cu - u0, 0), ids_cap));
     const int past = st.n - (st.pg + 1) * kPage;   // tokens after the page
     const bool full = phys >= 0 && past >= 0 &&
                       (a.window <= 0 || past + kPage <= a.window);
-    st.flags = (cb != last_b ? kFirst : 0) |
-               (cu == min(seq_end, u1) ? kLast : 0) | (full ? kFull : 0) |
-               (phys >= 0 ? kThere : 0) |
-               (seq_start >= u0 && seq_end <= u1 ? kWhole : 0);
+    st.flags = (cb != last_b ? kFirst : 0) | (last ? kLast : 0) |
+               (full ? kFull : 0) | (phys >= 0 ? kThere : 0) |
+               (seq_start >= r0 && seq_end <= r1 ? kWhole : 0) |
+               (mid < r1 && seq_start < mid && seq_end > mid ? kCross : 0);
     last_b = cb;
   };
 
@@ -340,15 +354,14 @@ void decode_diff_kernel(DecodeDiffArgs a) {
 
   // End of a piece: the result of a whole request (difference and norm
   // included), or both maps' normalised partials for the merge.
-  auto finish_piece = [&](const Step& st) {
-    const int b = st.b;
+  auto finish_piece = [&](int b, int flags) {
     const float l_tot = lane_pair(lane_pair(l_part, 16, false), 32, false);
     const float inv = l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
     const float lse_nat =
         l_tot > 0.0f ? (m_run + fast_log2(l_tot)) * kLn2 : -INFINITY;
     const ArgsPtr ra = rare_args();
     const int HQ = ra->HQ;
-    if (st.flags & kWhole) {
+    if (flags & kWhole) {
       const int h = pair * rep + min(col_h, rep - 1);
       const float lam = ra->w.lam[(int64_t)h * ra->w.lam_stride];
       float ss = 0.0f;
@@ -404,8 +417,9 @@ void decode_diff_kernel(DecodeDiffArgs a) {
   constexpr int kNK = 8, kNS = 16;   // loads of a step's K, and of a step
   Step cur, nx, nn;
   int phys;
+  int end_b = -1, end_flags = 0;   // the piece that both waves share
   next_step(cur, phys);
-  issue_q(cur.b);
+  issue_q(max(cur.b, 0));
   issue_k(cur, phys, 0);
   issue_v(cur, phys, 0);
   next_step(nx, phys);
@@ -421,9 +435,10 @@ void decode_diff_kernel(DecodeDiffArgs a) {
   wait_vm<2 * kNS>();
   read_q();
   cur.flags &= ~kFirst;
-  for (;;) {
+  while (cur.b >= 0) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
+      if (k == 1 && cur.b < 0) break;
       const uint32_t so = k * kStageB;
       if (cur.flags & kFirst) {
         wait_vm<kNS>();
@@ -503,15 +518,47 @@ void decode_diff_kernel(DecodeDiffArgs a) {
         o_acc[blk] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
             __builtin_bit_cast(s16x4, vf[blk]), pf, o_acc[blk], 0, 0, 0);
       issue_v(nn, phys, k);
-      if (cur.flags & kLast) finish_piece(cur);
+      if (cur.flags & kLast) {
+        if (cur.flags & kCross) {   // (no step comes after it)
+          end_b = cur.b;
+          end_flags = cur.flags;
+        } else {
+          finish_piece(cur.b, cur.flags);
+        }
+      }
       cur = nx;
       nx = nn;
-      if (cur.b < 0) {
-        wait_vm<0>();   // no direct load outlives the wave
-        return;
-      }
     }
   }
+  wait_vm<0>();   // no direct load outlives the wave, or lands on what follows
+  asm volatile("" ::: "memory");
+
+  // ---- 5. the request in the middle of the range ---------------------------
+  // (it has a page in both halves or in neither: all waves know; the second
+  // wave's results go through its own stages)
+  if (halves == 1) return;
+  const uint32_t at = lds_w + (half == 0 ? a.per_wg * kWaveLds : 0) + 16 * lane;
+  if (half != 0 && end_b >= 0) {
+#pragma unroll
+    for (int blk = 0; blk < 16; ++blk)
+      lds_st128(at + 1024 * blk, __builtin_bit_cast(u32x4, o_acc[blk]));
+    lds_st64(at + 16384, u32x2{__builtin_bit_cast(uint32_t, m_run),
+                               __builtin_bit_cast(uint32_t, l_part)});
+  }
+  __syncthreads();
+  if (half != 0 || end_b < 0) return;
+  const float m1 = __builtin_bit_cast(float, lds_ld32(at + 16384));
+  const float l1 = __builtin_bit_cast(float, lds_ld32(at + 16388));
+  const float m_new = fmaxf(m_run, m1);
+  const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+  const float f0 = fast_exp2(m_run - m_use), f1 = fast_exp2(m1 - m_use);
+  l_part = l_part * f0 + l1 * f1;
+  m_run = m_new;
+#pragma unroll
+  for (int blk = 0; blk < 16; ++blk)
+    o_acc[blk] = o_acc[blk] * f0 +
+                 __builtin_bit_cast(f32x4, lds_ld128(at + 1024 * blk)) * f1;
+  finish_piece(end_b, end_flags);
 }
 
 // Join the pieces of every request that several ranges shared, in a fixed
@@ -632,7 +679,7 @@ struct Shape {
   int rep, pairs, per_wg, G, R;   // R: ranges of the launch
 };
 // Three work-groups per four CUs, as the plain decode; four waves each, which
-// take 4, 2 or 1 pairs of stored heads and 1, 2 or 4 ranges.
+// take 4, 2 or 1 pairs of stored heads of 1, 1 or 2 ranges.
 Shape shape_of(int HQ, int HKV, int num_workgroups) {
   Shape s;
   s.rep = group_of(HQ / HKV);
@@ -641,7 +688,8 @@ Shape shape_of(int HQ, int HKV, int num_workgroups) {
   const int ny = s.pairs / s.per_wg;
   s.G = num_workgroups > 0 ? num_workgroups : 3 * device_cus() / (4 * ny);
   if (s.G < 1) s.G = 1;
-  s.R = s.G * (kWaves / s.per_wg);
+  const int subs = kWaves / s.per_wg;
+  s.R = s.G * (subs > 1 ? subs / 2 : 1);
   return s;
 }
 
