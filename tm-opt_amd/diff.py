@@ -26,7 +26,7 @@ from .attn import HEAD_DIM, PAGE_SIZE, _check_rows, _ptr, _stream
 def _call(dev, name, *args):
     """A launch on the current stream of dev, with dev the current device (the
     library sizes its grids by that device's compute units)."""
-    if dev.type == "cuda" and dev.index != torch.cuda.current_device():
+    if dev.type == "cuda" and dev.index != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return _lib.call(name, *args, _stream(dev))
     return _lib.call(name, *args, _stream(dev))

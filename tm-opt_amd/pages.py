@@ -13,8 +13,6 @@ from typing import NamedTuple
 
 import torch
 
-from . import _lib
-from .attn import _ptr
 from .diff import _call
 
 
@@ -29,20 +27,19 @@ class PagePlan(NamedTuple):
     reject: torch.Tensor         # [1] int32: 0, or 1 for a step that cannot be
 
 
-def _state(page_table, slots, lens, free_pages, free_count):
-    dev = page_table.device
+def _check_state(dev, page_table, free_pages, free_count):
     assert page_table.dtype == torch.int32 and page_table.dim() == 2
     assert page_table.is_contiguous()
-    B = slots.shape[0]
-    for t, d, name in ((slots, torch.int64, "slots"),
-                       (lens, torch.int32, "lens")):
-        assert t.dtype == d and t.shape == (B,), (name, t.dtype, t.shape)
-        assert t.is_contiguous() and t.device == dev, name
     assert free_pages.dtype == torch.int32 and free_pages.dim() == 1
     assert free_pages.is_contiguous() and free_pages.device == dev
     assert free_count.dtype == torch.int32 and free_count.numel() == 1
     assert free_count.device == dev
-    return dev, B
+
+
+def _check_index(t, dtype, n, dev):
+    assert t.dtype == dtype and t.dim() == 1 and t.numel() == n, \
+        (t.dtype, tuple(t.shape), dtype, n)
+    assert t.is_contiguous() and t.device == dev
 
 
 def plan_pages(page_table, slots, ctx_lens, new_lens, free_pages, free_count,
@@ -66,36 +63,40 @@ def plan_pages(page_table, slots, ctx_lens, new_lens, free_pages, free_count,
     tokens: block table and slot mapping -1, cu_seqlens and positions 0,
     seq_lens the contexts. prefill_varlen and prefill_diff_varlen take reject
     as it is."""
-    dev, B = _state(page_table, slots, ctx_lens, free_pages, free_count)
+    dev, B, T = page_table.device, slots.numel(), int(max_tokens)
+    _check_state(dev, page_table, free_pages, free_count)
+    _check_index(slots, torch.int64, B, dev)
+    _check_index(ctx_lens, torch.int32, B, dev)
+    _check_index(new_lens, torch.int32, B, dev)
     S, W = page_table.shape
-    assert new_lens.dtype == torch.int32 and new_lens.shape == (B,)
-    assert new_lens.is_contiguous() and new_lens.device == dev
-    T = int(max_tokens)
     width = W if width is None else int(width)
     if out is None:
-        a = -(-B * width // 4) * 4       # 16-byte steps for what follows
-        buf = torch.empty(a + 2 * B + 3, dtype=torch.int32, device=dev)
-        rest = buf[a:]
-        tok = torch.empty((2, T), dtype=torch.int64, device=dev)
-        out = PagePlan(buf[:B * width].view(B, width), rest[:B],
-                       rest[B:2 * B + 1], tok[0], tok[1],
-                       rest[2 * B + 1:2 * B + 2], rest[2 * B + 2:])
+        # two allocations, cut (a slice costs as much as an allocation)
+        pad = -B * width % 4             # 16-byte steps for what follows
+        buf = torch.empty(B * (width + 2) + pad + 3, dtype=torch.int32,
+                          device=dev)
+        block, _, seq, cu, count, reject = buf.split_with_sizes(
+            (B * width, pad, B, B + 1, 1, 1))
+        slot_mapping, positions = torch.empty(
+            2 * T, dtype=torch.int64, device=dev).split_with_sizes((T, T))
+        out = PagePlan(block.view(B, width), seq, cu, slot_mapping, positions,
+                       count, reject)
     else:
-        for t, d, shape in ((out.block_table, torch.int32, (B, width)),
-                            (out.seq_lens, torch.int32, (B,)),
-                            (out.cu_seqlens, torch.int32, (B + 1,)),
-                            (out.slot_mapping, torch.int64, (T,)),
-                            (out.positions, torch.int64, (T,)),
-                            (out.free_count, torch.int32, (1,)),
-                            (out.reject, torch.int32, (1,))):
-            assert t.dtype == d and t.shape == shape, (t.dtype, t.shape, shape)
-            assert t.is_contiguous() and t.device == dev
-    _call(dev, "tmopt_plan_pages", page_table.data_ptr(), S, W, _ptr(slots),
-          _ptr(ctx_lens), _ptr(new_lens), B, free_pages.data_ptr(),
-          free_pages.shape[0], free_count.data_ptr(), T, width,
-          _ptr(out.block_table), _ptr(out.seq_lens), _ptr(out.cu_seqlens),
-          _ptr(out.slot_mapping), _ptr(out.positions), _ptr(out.free_count),
-          _ptr(out.reject))
+        block, seq, cu, slot_mapping, positions, count, reject = out
+        assert block.dtype == torch.int32 and block.shape == (B, width)
+        assert block.is_contiguous() and block.device == dev
+        _check_index(seq, torch.int32, B, dev)
+        _check_index(cu, torch.int32, B + 1, dev)
+        _check_index(slot_mapping, torch.int64, T, dev)
+        _check_index(positions, torch.int64, T, dev)
+        _check_index(count, torch.int32, 1, dev)
+        _check_index(reject, torch.int32, 1, dev)
+    _call(dev, "tmopt_plan_pages", page_table.data_ptr(), S, W,
+          slots.data_ptr(), ctx_lens.data_ptr(), new_lens.data_ptr(), B,
+          free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), T,
+          width, block.data_ptr(), seq.data_ptr(), cu.data_ptr(),
+          slot_mapping.data_ptr(), positions.data_ptr(), count.data_ptr(),
+          reject.data_ptr())
     return out
 
 
@@ -108,19 +109,23 @@ def release_pages(page_table, slots, lens, free_pages, free_count, out=None):
     named twice, a length that is negative or past the row, or a stack that
     would overflow. out: that pair to write into; its free_count may be
     free_count. The rows keep their entries; release a request once."""
-    dev, B = _state(page_table, slots, lens, free_pages, free_count)
+    dev, B = page_table.device, slots.numel()
+    _check_state(dev, page_table, free_pages, free_count)
+    _check_index(slots, torch.int64, B, dev)
+    _check_index(lens, torch.int32, B, dev)
+    S, W = page_table.shape
+    # the pair and the scratch in one allocation (16-byte steps)
+    n = -(-B // 4) * 4
+    ws, count, reject = torch.empty(n + 2, dtype=torch.int32,
+                                    device=dev).split_with_sizes((n, 1, 1))
     if out is None:
-        n = torch.empty(2, dtype=torch.int32, device=dev)
-        out = n[:1], n[1:]
+        out = count, reject
     else:
-        for t in out:
-            assert t.dtype == torch.int32 and t.shape == (1,)
-            assert t.device == dev
-    n = int(_lib.load().tmopt_release_pages_workspace_size(B))
-    ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
-    _call(dev, "tmopt_release_pages", page_table.data_ptr(),
-          page_table.shape[0], page_table.shape[1], _ptr(slots), _ptr(lens),
-          B, free_pages.data_ptr(), free_pages.shape[0],
-          free_count.data_ptr(), _ptr(out[0]), _ptr(out[1]), ws.data_ptr(),
-          ws.numel())
+        count, reject = out
+        _check_index(count, torch.int32, 1, dev)
+        _check_index(reject, torch.int32, 1, dev)
+    _call(dev, "tmopt_release_pages", page_table.data_ptr(), S, W,
+          slots.data_ptr(), lens.data_ptr(), B, free_pages.data_ptr(),
+          free_pages.numel(), free_count.data_ptr(), count.data_ptr(),
+          reject.data_ptr(), ws.data_ptr(), 4 * n)
     return out
