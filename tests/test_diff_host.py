@@ -73,6 +73,14 @@ def test_prefill_refusals(tm):
     for kw in (dict(D=64), dict(pool, ps=32), dict(n=1 << 18),
                dict(n=1 << 17, qt=128, kt=1 << 14)):
         assert call(**kw) == e.TMOPT_EUNSUPPORTED, kw
+    need = size(2, 64, 32, 4, 500, 0)
+    assert 0 < need <= 256 * 3 * 258 * 1024
+    for kw in (dict(ws=ctypes.c_void_p(8), nbytes=need),
+               dict(ws=P, nbytes=need - 1)):
+        assert call(**dict(pool, bts=500, **kw)) == e.TMOPT_EWORKSPACE, kw
+    # without a block table only the run's own length counts
+    assert size(1, 200, 32, 4, 0, 0) == 0 < size(1, 4000, 4, 2, 0, 0)
+    assert size(1, 4000, 4, 2, 0, 100) == 0
 
 
 def test_plan_refusals(tm):

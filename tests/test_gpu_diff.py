@@ -312,6 +312,8 @@ def test_prefill_chunk_after_long_context(tm, dev, n, prior):
     a, la = _prefill(tm, q, None, None, cu, w, **args)
     b, lb = _prefill(tm, q, None, None, cu, w, **args)
     assert torch.equal(a, b) and torch.equal(la, lb)
+    for most in (n + prior, 1):           # (a bound that is too low: one launch)
+        _prefill(tm, q, None, None, cu, w, call=dict(max_context=most), **args)
 
 
 def test_prefill_strides_and_outputs(tm, dev):

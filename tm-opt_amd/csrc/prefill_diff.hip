@@ -69,9 +69,81 @@ struct PrefillDiffArgs {
   float* lse;
   int64_t lse_sh;
   const int32_t* reject;
+  // split keys (see pieces_of): nsplit > 1 levels of n_base work-groups
+  int nsplit, n_base;
+  int cus;
+  float* part_o;     // [nsplit * n_base][8 waves][32][64 lanes][4] fp32
+  float* part_lse;   // [nsplit * n_base][8 waves][32 rows]
+  int* part_n;       // [n_base] pieces of each item (0: no such item)
 };
 
-template <int REP, bool PAGED>
+// First key a work item reads (a multiple of the tile width at or below the
+// first key a query of the block may see) and its tiles from there.
+struct Tiles {
+  int k_lo, n;
+};
+__device__ __forceinline__ Tiles item_tiles(const PrefillDiffArgs& a, int BQ,
+                                            int prior, int len, int qb) {
+  const int q0 = qb * BQ;
+  const int lo = a.window > 0 ? max(0, prior + q0 - a.window + 1) : 0;
+  const int k_lo = (lo / kBN) * kBN;
+  return Tiles{k_lo, (prior + min(len, q0 + BQ) - k_lo + kBN - 1) / kBN};
+}
+
+// Split keys: a launch of few items, or of few more than there are compute
+// units, leaves units idle while its longest items run. It cuts each item's
+// tiles into pieces, one work-group each (level s of the grid holds piece s of
+// every item); a piece leaves its normalised fp32 results with their LSE (up to
+// 257 KB), and prefill_diff_merge joins them in order and takes the difference
+// and the norm. The longest item gets the n pieces that the estimate below says
+// are quickest, others their share. The estimate, in us: items are taken as
+// evenly spread between `low` and `most` tiles, heaviest first, one work-group
+// per compute unit; a tile takes 1.05 on up to half the units and 1.4 on all
+// (power: 2.1 against 1.6 GHz); pieces cost 5 for their start and the merge,
+// and 0.115 each for what they write and the merge reads.
+constexpr int kMinPiece = 4;   // tiles
+__device__ __forceinline__ int pieces_of(const PrefillDiffArgs& a, int BQ,
+                                         int lane, int tiles) {
+  int sum = 0, most = 0, items = 0;
+  for (int s = lane; s < a.S; s += 64) {
+    const int len = a.cu[s + 1] - a.cu[s];
+    const int nb = (len + BQ - 1) / BQ;
+    const int prior = a.prior != nullptr ? a.prior[s] : 0;
+    if (nb > 0) {
+      const int t0 = item_tiles(a, BQ, prior, len, 0).n;
+      const int t1 = item_tiles(a, BQ, prior, len, nb - 1).n;
+      sum += nb * (t0 + t1) / 2;
+      most = max(most, max(t0, t1));
+      items += nb;
+    }
+  }
+  for (int x = 1; x < 64; x <<= 1) most = max(most, __shfl_xor(most, x));
+  most = __builtin_amdgcn_readfirstlane(most);
+  const int count = __builtin_amdgcn_readfirstlane(wave_sum(items));
+  if (most <= 0 || count <= 0) return 1;
+  const float mean =
+      (float)__builtin_amdgcn_readfirstlane(wave_sum(sum)) / count;
+  const float low = fmaxf(0.0f, 2.0f * mean - most);
+  const float all = (float)count * a.HKV;
+  float best = 0.0f;
+  int n = 1;
+  for (int x = 1; x <= a.nsplit; ++x) {
+    const float load = all * x / a.cus;
+    const float len = (low * fmaxf(1.0f, ceilf(load - 0.02f)) +
+                       (most - low) * fmaxf(1.0f, 0.5f * load)) / x;
+    const float us =
+        len * (0.7f + 0.7f * fminf(fmaxf(load, 0.5f), 1.0f)) +
+        (x > 1 ? 5.0f + 0.115f * x * all : 0.0f);
+    if (x == 1 || us < best) {
+      best = us;
+      n = x;
+    }
+  }
+  n = min(min(n, tiles / kMinPiece), (int)((float)n * tiles / most + 0.5f));
+  return __builtin_amdgcn_readfirstlane(max(1, n));
+}
+
+template <int REP, bool PAGED, bool SPLIT>
 __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
   constexpr int BQ = 128 / REP;   // queries per work-group
   constexpr int QSUB = BQ / 32;   // 32-query sub-blocks per head pair
@@ -81,18 +153,31 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31;
   const int h2 = lane >> 5;       // lane half
-  const Work wk = schedule(a, BQ, lane, blockIdx.x);
-  if (wk.seq < 0) return;
+  const int level = SPLIT ? (int)blockIdx.x / a.n_base : 0;
+  const int item = (int)blockIdx.x - level * a.n_base;
+  const Work wk = schedule(a, BQ, lane, item);
+  if (wk.seq < 0) {
+    if (SPLIT && level == 0 && tid == 0) a.part_n[item] = 0;
+    return;
+  }
   const int t0 = wk.t0, len = wk.len, prior = wk.prior;
   const int q0 = wk.qb * BQ;
   const int nk = prior + len;                 // keys of this run
   const int pos_lo = prior + q0;              // first query position
   const int pos_hi = pos_lo + min(BQ, len - q0) - 1;   // last valid one
-  // first key any query of the block may see; tiles start at a multiple of the
-  // tile width
+  // first key any query of the block may see
   const int kwin = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0;
-  const int k_lo = (kwin / kBN) * kBN;
-  const int ntiles = (pos_hi + 1 - k_lo + kBN - 1) / kBN;
+  const Tiles tl = item_tiles(a, BQ, prior, len, wk.qb);
+  int k_lo = tl.k_lo, ntiles = tl.n;
+  int np = 1;
+  if constexpr (SPLIT) {
+    np = pieces_of(a, BQ, lane, tl.n);
+    if (level == 0 && tid == 0) a.part_n[item] = np;
+    if (level >= np) return;
+    const int b0 = (int)((int64_t)tl.n * level / np);
+    k_lo += b0 * kBN;
+    ntiles = (int)((int64_t)tl.n * (level + 1) / np) - b0;
+  }
 
   // ---- this wave's row block: map, head pair and 32-query sub-block ------
   const int map = w >> 2;
@@ -393,6 +478,25 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
   const float l_tot = lane_pair(l_part, 32, false);
   const float inv = rejected ? __builtin_nanf("") :
                     l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
+  if (SPLIT && np > 1) {
+    // lane-major partial: every store writes 1 KB (of rows past the run,
+    // nothing)
+    const int64_t pw = (int64_t)blockIdx.x * 8 + w;
+    float* const po = a.part_o + (pw * 32 * 64 + lane) * 4;
+    if (qok)
+#pragma unroll
+    for (int db = 0; db < 8; ++db)
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4)
+        *reinterpret_cast<f32x4*>(po + (4 * db + g4) * 256) =
+            f32x4{o_acc[db][4 * g4] * inv, o_acc[db][4 * g4 + 1] * inv,
+                  o_acc[db][4 * g4 + 2] * inv, o_acc[db][4 * g4 + 3] * inv};
+    if (h2 == 0)
+      a.part_lse[pw * 32 + l32] =
+          rejected ? __builtin_nanf("") :
+          l_tot > 0.0f ? (m_run + fast_log2(l_tot)) * kLn2 : -INFINITY;
+    return;
+  }
   if (a.lse && h2 == 0 && qok)
     a.lse[(2 * hp + map) * a.lse_sh + t0 + qi] =
         rejected ? __builtin_nanf("") :
@@ -473,27 +577,164 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
   }
 }
 
-// Work-groups of a launch: scheduled pairs * items of each, rounded up to whole
-// XCD rounds.
-int64_t launch_wgs(int pairs, int BQ, int S, int max_seqlen) {
-  const int64_t items = (int64_t)S * ((max_seqlen + BQ - 1) / BQ);
+// Join the pieces of the items that were split: grid (n_base, 16), a work-group
+// per 8 query rows of both maps. Thread t has row t & 7 and dims 8 (t >> 3) ..
+// +7 of both, so the difference is its own and the norm one sum over threads;
+// four pieces' loads in flight at a time, joined in piece order.
+template <int REP>
+__global__ __launch_bounds__(256) void prefill_diff_merge(PrefillDiffArgs a) {
+  constexpr int BQ = 128 / REP, QSUB = BQ / 32;
+  __shared__ float sums[4][8];
+  const int np = min(as_const(a.part_n)[blockIdx.x], a.nsplit);
+  if (np <= 1) return;                        // no item, or written in place
+  const int lane = threadIdx.x & 63;
+  const int w = threadIdx.x >> 6;
+  const Work wk = schedule(a, BQ, lane, blockIdx.x);
+  const int rb = blockIdx.y >> 2;             // 32-row block of the item
+  const int l32 = 8 * (blockIdx.y & 3) + (threadIdx.x & 7);
+  const int c = threadIdx.x >> 3;             // 8-dim chunk
+  const int row0 = wk.qb * BQ + 32 * (rb % QSUB) + 8 * (blockIdx.y & 3);
+  if (row0 >= wk.len) return;
+  const int qi = row0 + (threadIdx.x & 7);
+  const int hp = wk.kvh * REP + rb / QSUB;
+  float m[2] = {-INFINITY, -INFINITY}, sum[2] = {0, 0};
+  f32x4 acc[2][2] = {};
+  constexpr int kBatch = 4;
+  for (int s0 = 0; s0 < np; s0 += kBatch) {
+    float l[kBatch][2];
+    f32x4 o[kBatch][2][2];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int64_t slot =
+          (int64_t)min(s0 + j, np - 1) * a.n_base + blockIdx.x;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int64_t pw = slot * 8 + 4 * i + rb;
+        l[j][i] = a.part_lse[pw * 32 + l32];
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          o[j][i][x] = *reinterpret_cast<const f32x4*>(
+              a.part_o + ((pw * 32 + c) * 64 + 32 * x + l32) * 4);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (s0 + j >= np) break;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float m_new = fmaxf(m[i], l[j][i]);
+        const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+        const float keep = fast_exp2((m[i] - m_use) * kLog2e);
+        const float wt = fast_exp2((l[j][i] - m_use) * kLog2e);
+        sum[i] = sum[i] * keep + wt;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          acc[i][x] = acc[i][x] * keep + o[j][i][x] * wt;
+        m[i] = m_new;
+      }
+    }
+  }
+  // (a rejected launch's pieces are NaN, and so are their sums)
+  const bool rejected = a.reject != nullptr && as_const(a.reject)[0] != 0;
+  const bool qok = qi < wk.len;
+  if (a.lse && c < 2 && qok)
+    a.lse[(2 * hp + c) * a.lse_sh + wk.t0 + qi] =
+        rejected ? __builtin_nanf("") :
+        sum[c] > 0.0f ? m[c] + fast_log2(sum[c]) * kLn2 : -INFINITY;
+  const float inv0 = sum[0] > 0.0f ? 1.0f / sum[0] : 0.0f;
+  const float inv1 = sum[1] > 0.0f ? 1.0f / sum[1] : 0.0f;
+  const float lam = a.w.lam[(int64_t)hp * a.w.lam_stride];
+  float ss = 0.0f;
+  f32x4 d[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    d[x] = acc[0][x] * inv0 - acc[1][x] * (lam * inv1);
+    if (rejected) d[x] = d[x] + __builtin_nanf("");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ss += d[x][i] * d[x][i];
+  }
+  float f = a.w.out_scale;
+  if (a.w.weight) {
+    ss += __shfl_xor(ss, 8);
+    ss = lane_pair(lane_pair(ss, 16, false), 32, false);
+    if (lane < 8) sums[w][lane] = ss;
+    __syncthreads();
+    const int q = threadIdx.x & 7;
+    ss = (sums[0][q] + sums[1][q]) + (sums[2][q] + sums[3][q]);
+    f *= __builtin_amdgcn_rsqf(ss * (1.0f / kDV) + a.w.eps);
+  }
+  u32x4 y;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    f32x4 z = d[x] * f;
+    if (a.w.weight)
+      z *= *reinterpret_cast<const f32x4*>(a.w.weight + 8 * c + 4 * x);
+    y[2 * x] = pack_bf16x2_rn(z[0], z[1]);
+    y[2 * x + 1] = pack_bf16x2_rn(z[2], z[3]);
+  }
+  if (qok)
+    *reinterpret_cast<u32x4*>(a.out + (int64_t)(wk.t0 + qi) * a.o_st +
+                              (int64_t)hp * a.o_sh + 8 * c) = y;
+}
+
+// Work-groups of one level: scheduled pairs * items of each, rounded up to
+// whole XCD rounds.
+int64_t level_wgs(int pairs, int BQ, int64_t S, int max_seqlen) {
+  const int64_t items = S * ((max_seqlen + BQ - 1) / BQ);
   if (pairs <= 8 && 8 % pairs == 0)
     return 8 * ((items + 8 / pairs - 1) / (8 / pairs));
   return pairs * items;
+}
+
+// Levels of a launch (1: keys are not split), from what the host knows: the
+// longest run, and the row width of a block table or the window as bounds of
+// its keys. Up to half the compute units' worth of items, as many pieces as
+// there are units; up to one and a half, two or three pieces an item even out
+// the rounds; larger grids fill the chip by themselves. The device decides from
+// the lengths.
+int split_levels(int64_t n_base, int BQ, int max_seqlen, int64_t bt_stride,
+                 int window) {
+  const int64_t cus = device_cus();
+  int64_t keys = bt_stride > 0 ? bt_stride * kPage : max_seqlen;
+  if (window > 0 && keys > (int64_t)window + BQ + kBN)
+    keys = (int64_t)window + BQ + kBN;
+  const int64_t tiles = (keys + kBN - 1) / kBN;
+  int64_t n = (2 * n_base <= cus ? cus : 3 * cus) / n_base;
+  if (n > 64) n = 64;
+  // a piece costs kPieceUs, so the tiles it saves must be worth that
+  if (n > tiles / 8) n = tiles / 8;
+  return n < 2 || tiles < 32 ? 1 : (int)n;
+}
+
+constexpr int64_t kSlotBytes = (int64_t)8 * 32 * (kDV + 1) * sizeof(float);
+int64_t workspace_bytes_of(int levels, int64_t n_base) {
+  return levels * n_base * kSlotBytes + ((n_base * 4 + 15) & ~(int64_t)15);
 }
 
 // Head pairs per work-group: the largest of 4, 2, 1 dividing HQ / HKV; a larger
 // ratio runs as several scheduled pairs per stored one.
 int group_of(int ratio) { return ratio % 4 == 0 ? 4 : ratio % 2 == 0 ? 2 : 1; }
 
-template <int REP>
-void launch(const PrefillDiffArgs& a, int64_t n, hipStream_t st) {
-  if (a.bt)
-    hipLaunchKernelGGL((prefill_diff_kernel<REP, true>), dim3((unsigned)n),
+template <int REP, bool PAGED>
+void launch_source(const PrefillDiffArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)(a.nsplit * a.n_base));
+  if (a.nsplit > 1)
+    hipLaunchKernelGGL((prefill_diff_kernel<REP, PAGED, true>), grid,
                        dim3(512), kLds, st, a);
   else
-    hipLaunchKernelGGL((prefill_diff_kernel<REP, false>), dim3((unsigned)n),
+    hipLaunchKernelGGL((prefill_diff_kernel<REP, PAGED, false>), grid,
                        dim3(512), kLds, st, a);
+}
+
+template <int REP>
+int launch(const PrefillDiffArgs& a, hipStream_t st) {
+  if (a.bt) launch_source<REP, true>(a, st);
+  else launch_source<REP, false>(a, st);
+  const int rc = check_launch("prefill_diff");
+  if (rc || a.nsplit <= 1) return rc;
+  hipLaunchKernelGGL((prefill_diff_merge<REP>), dim3(a.n_base, 16), dim3(256),
+                     0, st, a);
+  return check_launch("prefill_diff_merge");
 }
 
 }  // namespace
@@ -504,13 +745,13 @@ using namespace tmopt;
 extern "C" size_t tmopt_attn_prefill_diff_workspace_size(
     int num_seqs, int max_seqlen_q, int HQ, int HKV, int64_t bt_stride,
     int window) {
-  (void)num_seqs;
-  (void)max_seqlen_q;
-  (void)HQ;
-  (void)HKV;
-  (void)bt_stride;
-  (void)window;
-  return 0;
+  if (num_seqs <= 0 || max_seqlen_q <= 0 || HQ <= 0 || HKV <= 0 ||
+      HKV % 2 != 0 || HQ % HKV != 0)
+    return 0;
+  const int rep = group_of(HQ / HKV), BQ = 128 / rep;
+  const int64_t n = level_wgs(HQ / 2 / rep, BQ, num_seqs, max_seqlen_q);
+  const int levels = split_levels(n, BQ, max_seqlen_q, bt_stride, window);
+  return levels > 1 ? (size_t)workspace_bytes_of(levels, n) : 0;
 }
 
 extern "C" int tmopt_attn_prefill_diff(
@@ -572,19 +813,21 @@ extern "C" int tmopt_attn_prefill_diff(
                   TMOPT_EUNSUPPORTED,
                   "prefill_diff: a run's k/v span must stay below 2 GiB");
   }
-  const size_t need = tmopt_attn_prefill_diff_workspace_size(
-      num_seqs, max_seqlen_q, HQ, HKV, paged ? bt_stride : 0, window);
-  TMOPT_REQUIRE(need == 0 || !workspace ||
-                    (workspace_bytes >= need &&
-                     (uintptr_t)workspace % 16 == 0),
-                TMOPT_EWORKSPACE,
-                "prefill_diff: workspace %zu bytes < %zu needed (or unaligned)",
-                workspace_bytes, need);
   const int rep = group_of(HQ / HKV), pairs = HQ / 2 / rep, BQ = 128 / rep;
-  const int64_t n = launch_wgs(pairs, BQ, num_seqs, max_seqlen_q);
+  const int64_t n = level_wgs(pairs, BQ, num_seqs, max_seqlen_q);
   TMOPT_REQUIRE(n < 0x7fffffff, TMOPT_EUNSUPPORTED,
                 "prefill_diff: %lld work-groups exceed the grid limit",
                 (long long)n);
+  const int levels = workspace == nullptr
+                         ? 1
+                         : split_levels(n, BQ, max_seqlen_q,
+                                        paged ? bt_stride : 0, window);
+  const int64_t need = workspace_bytes_of(levels, n);
+  TMOPT_REQUIRE(levels <= 1 || ((int64_t)workspace_bytes >= need &&
+                                (uintptr_t)workspace % 16 == 0),
+                TMOPT_EWORKSPACE,
+                "prefill_diff: workspace %zu bytes < %lld needed (or unaligned)",
+                workspace_bytes, (long long)need);
   PrefillDiffArgs a;
   a.q = (const __bf16*)q;
   a.q_st = q_stride_tok;
@@ -615,9 +858,14 @@ extern "C" int tmopt_attn_prefill_diff(
   a.lse = lse;
   a.lse_sh = lse_stride_head;
   a.reject = reject;
+  a.nsplit = levels;
+  a.n_base = (int)n;
+  a.cus = device_cus();
+  a.part_o = (float*)workspace;
+  a.part_lse = a.part_o + levels * n * 8 * 32 * kDV;
+  a.part_n = (int*)(a.part_lse + levels * n * 8 * 32);
   const hipStream_t st = (hipStream_t)stream;
-  if (rep == 4) launch<4>(a, n, st);
-  else if (rep == 2) launch<2>(a, n, st);
-  else launch<1>(a, n, st);
-  return check_launch("prefill_diff");
+  if (rep == 4) return launch<4>(a, st);
+  if (rep == 2) return launch<2>(a, st);
+  return launch<1>(a, st);
 }

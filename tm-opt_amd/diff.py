@@ -138,7 +138,7 @@ def prefill_diff_varlen(q, k, v, cu_seqlens, lam, scale, norm_weight=None,
                         norm_eps=1e-5, out_scale=1.0, window=0,
                         max_seqlen=None, prior_lens=None, k_pool=None,
                         v_pool=None, block_table=None, out=None, lse=None,
-                        return_lse=True, reject=None):
+                        return_lse=True, reject=None, max_context=None):
     """Varlen causal (optionally windowed) differential attention.
 
     q [total, HQ, 128] bf16 (head_dim contiguous, any token / head strides);
@@ -152,6 +152,14 @@ def prefill_diff_varlen(q, k, v, cu_seqlens, lam, scale, norm_weight=None,
     lam fp32 [HQ / 2] or [1]. reject: optional int32 device scalar; nonzero
     gives NaN outputs. max_seqlen bounds the run lengths (read from the
     device, with a synchronisation, if None).
+    A launch of few query blocks that may see many keys splits these over
+    work-groups and joins the pieces: a second launch, up to 3 x 257 KB of
+    scratch per compute unit, and last bits that depend on the launch's other
+    runs and the table's width. max_context: an upper bound of prior + run
+    length, where the host has one; without it the row width of the block
+    table bounds the keys, and short contexts under a wide table pay for the
+    second launch (64Q/8KV, 4,134 pages: 64 tokens without context 18.4 us
+    against 14.2). It decides about the split alone.
     Returns (out [total, HQ / 2, 256] bf16, lse [HQ, total] fp32 or None)."""
     total, HQ, D = q.shape
     dev = q.device
@@ -194,8 +202,14 @@ def prefill_diff_varlen(q, k, v, cu_seqlens, lam, scale, norm_weight=None,
         assert lse.is_contiguous() and lse.device == dev
     elif return_lse:
         lse = torch.empty((HQ, total), dtype=torch.float32, device=dev)
+    keys = bts
+    if bts and max_context is not None:
+        keys = max(1, min(bts, -(-int(max_context) // PAGE_SIZE)))
     n = _workspace_size(dev, "tmopt_attn_prefill_diff_workspace_size", S,
-                        int(max_seqlen), HQ, HKV, bts, int(window))
+                        int(max_seqlen), HQ, HKV, keys, int(window))
+    if n and keys != bts:       # (the launch sizes its scratch by the table)
+        n = _workspace_size(dev, "tmopt_attn_prefill_diff_workspace_size", S,
+                            int(max_seqlen), HQ, HKV, bts, int(window))
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     _call(dev, "tmopt_attn_prefill_diff", q.data_ptr(), q.stride(0),
           q.stride(1), _ptr(k), strides[0], strides[1], _ptr(v), strides[2],
