@@ -88,7 +88,7 @@ def decode_diff_workspace(B, HQ, HKV, device, num_workgroups=0):
 
 def decode_diff_paged(q, k_pool, v_pool, block_table, ctx_lens, lam, scale,
                       norm_weight=None, norm_eps=1e-5, out_scale=1.0,
-                      window=0, table_wrap=0, min_pages=8, num_workgroups=0,
+                      window=0, table_wrap=0, min_pages=2, num_workgroups=0,
                       out=None, lse=None, workspace=None, return_lse=True):
     """Differential attention of one new token per request, paged.
 
