@@ -636,17 +636,15 @@ __global__ __launch_bounds__(128 * H * S) void decode_diff_merge(
 #pragma unroll
     for (int i = 0; i < 4; ++i) part[grp][m][2 + i][lane] = acc[i];
   };
-  if (S > 1) {
-    if (sub > 0) put();
-    __syncthreads();
-    if (sub == 0)
-      for (int j = 1; j < min(np, S); ++j) {
-        f32x4 o;
+  if (sub > 0) put();
+  __syncthreads();
+  if (sub == 0)
+    for (int j = 1; j < min(np, S); ++j) {
+      f32x4 o;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = part[grp + j][m][2 + i][lane];
-        add(part[grp + j][m][0][lane], part[grp + j][m][1][lane], o);
-      }
-  }
+      for (int i = 0; i < 4; ++i) o[i] = part[grp + j][m][2 + i][lane];
+      add(part[grp + j][m][0][lane], part[grp + j][m][1][lane], o);
+    }
   const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
   acc = acc * inv;
   if (sub == 0 && hok && a.lse && lane == 0)
@@ -673,11 +671,16 @@ __global__ __launch_bounds__(128 * H * S) void decode_diff_merge(
       u32x2{pack_bf16x2_rn(acc[0], acc[1]), pack_bf16x2_rn(acc[2], acc[3])};
 }
 
-// The merge's shape, from the pieces of an average request.
+// The merge's shape, from the pieces of an average request (at most one more
+// than its share of the R ranges): two groups of waves per head pair, or eight.
+// Graph replays with 1 / 2 / 8 groups, us a call, 32Q/4KV: one request of
+// 50,001 tokens 49.4 / 38.0 / 32.3, 4 of 4K-8K 25.2 / 22.8 / 20.8, 9 up to 4.7K
+// 24.0 / 21.7 / 20.9, 16 up to 2K 21.2 / 20.4 / 21.0, 24 up to 4K 32.1 / 31.5 /
+// 34.5, 64 of 1K-8K 112 / 112 / 117.
 void launch_merge(const DecodeDiffArgs& a, int R, hipStream_t st) {
   const int np = 1 + R / a.B, H = a.HQ / 2;
-  if (np <= 8 || H > 65535)
-    hipLaunchKernelGGL((decode_diff_merge<4, 1>), dim3(a.B, (H + 3) / 4),
+  if (np <= 16 || H > 65535)
+    hipLaunchKernelGGL((decode_diff_merge<2, 2>), dim3(a.B, (H + 1) / 2),
                        dim3(512), 0, st, a);
   else
     hipLaunchKernelGGL((decode_diff_merge<1, 8>), dim3(a.B, H), dim3(1024), 0,
