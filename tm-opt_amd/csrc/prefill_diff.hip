@@ -36,7 +36,8 @@ constexpr int kRowB = 256;                // one key's slice of a stored head
 constexpr int kSliceB = kBN * kRowB;      // 8 KB
 constexpr int kStage = 4 * kSliceB;       // K, K', V, V'
 constexpr int kNStage = 4;
-constexpr int kLds = kNStage * kStage + 8 * 128;   // and the norms' sums
+constexpr int kLds = kNStage * kStage + 8 * 128 + kDV * 4;   // and, for the
+                                          // norm, its sums and weights
 constexpr float kLazy = 8.0f;             // lazy-rescale threshold (log2)
 constexpr int kRing = 4;                  // fragments read kRing - 1 ahead
 // a buffer offset past every resource this kernel builds (their ranges are
@@ -187,6 +188,11 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
   const bool qok = qi < len;
   const int qpos = prior + qi;
   const int kvs = 2 * (wk.kvh / a.kv_div);    // the first stored head
+  // (what the end needs is fetched here: its latency would show there)
+  const float lam = as_const(a.w.lam)[(int64_t)hp * a.w.lam_stride];
+  const uint32_t wlds =
+      (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)smem) +
+      kNStage * kStage + 8 * 128;
 
   // ---- tile loads ----------------------------------------------------------
   // Wave w moves key rows 4w..4w+3 of each of the four slices, one 1 KB
@@ -418,6 +424,8 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
     }
     issue_tile(0, 0);
     if (ntiles > 1) issue_tile(1, 1);
+    if (w == 0 && a.w.weight)
+      dma(make_rsrc(a.w.weight, kDV * 4), wlds, 16 * lane);
     wait_vm<0>();
     __syncthreads();
 #pragma unroll
@@ -501,7 +509,6 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
     a.lse[(2 * hp + map) * a.lse_sh + t0 + qi] =
         rejected ? __builtin_nanf("") :
         l_tot > 0.0f ? (m_run + fast_log2(l_tot)) * kLn2 : -INFINITY;
-  const float lam = a.w.lam[(int64_t)hp * a.w.lam_stride];
   // dims 128 map .. +127 are this wave's; the others go to its partner, lane by
   // lane (16 bytes each: 1 KB per store)
   const uint32_t mine = lds0 + (uint32_t)w * 16384 + 16 * lane;
@@ -558,8 +565,9 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
       f32x4 x = f32x4{d[db][4 * g4], d[db][4 * g4 + 1], d[db][4 * g4 + 2],
                       d[db][4 * g4 + 3]} * f;
       if (a.w.weight)
-        x *= *reinterpret_cast<const f32x4*>(a.w.weight + 128 * map + 32 * db +
-                                             8 * g4 + 4 * h2);
+        x *= __builtin_bit_cast(
+            f32x4, lds_ld128(wlds + 4 * (128 * map + 32 * db + 8 * g4 +
+                                         4 * h2)));
       const int c = 4 * db + g4;    // 16-byte chunk: dims 8c .. 8c+7
       lds_st64(ob + l32 * kRowB + 16 * (c ^ (l32 & 15)) + 8 * h2,
                u32x2{pack_bf16x2_rn(x[0], x[1]), pack_bf16x2_rn(x[2], x[3])});
