@@ -407,8 +407,11 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
     // t. Tile t + 3 goes out at the start of slot 2t into the stage of tile t -
     // 1 (last read in slot 2t - 1) and must be in LDS before slot 2t + 4; each
     // wave waits for its own part at the end of every odd slot, before the
-    // barrier that publishes it. The queries come first, through stages 2 and 3
-    // (8 KB per wave; rows past the run end arrive as zeros).
+    // barrier that publishes it. The queries come first, each wave's own 32
+    // rows through its 8 KB of stages 2 and 3 (rows past the run end arrive as
+    // zeros).
+    if (w == 0 && a.w.weight)
+      dma(make_rsrc(a.w.weight, kDV * 4), wlds, 16 * lane);
     const uint32_t qlds = lds0 + 2 * kStage + (uint32_t)w * (32 * kRowB);
     {
       const int64_t span = ((int64_t)(len - row0 - 1) * a.q_st + kD) * 2;
@@ -423,11 +426,9 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
       }
     }
     issue_tile(0, 0);
-    if (ntiles > 1) issue_tile(1, 1);
-    if (w == 0 && a.w.weight)
-      dma(make_rsrc(a.w.weight, kDV * 4), wlds, 16 * lane);
-    wait_vm<0>();
-    __syncthreads();
+    issue_tile(1, 1, ntiles > 1);
+    wait_vm<8>();   // the queries
+    asm volatile("" ::: "memory");
 #pragma unroll
     for (int kk = 0; kk < 8; ++kk) {
       u32x4 x = __builtin_bit_cast(
@@ -436,7 +437,8 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
       if (!qok) x = u32x4{0, 0, 0, 0};
       qf[kk] = __builtin_bit_cast(bf16x8, x);
     }
-    __syncthreads();
+    wait_vm<0>();
+    __syncthreads();   // tiles 0 and 1 are there, stages 2 and 3 free
     if (ntiles > 2) issue_tile(2, 2);
     auto odd_end = [&](int n) {
       if (n == 4) wait_vm<4>();
@@ -513,35 +515,27 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
   // lane (16 bytes each: 1 KB per store)
   const uint32_t mine = lds0 + (uint32_t)w * 16384 + 16 * lane;
   const uint32_t theirs = lds0 + (uint32_t)(w ^ 4) * 16384 + 16 * lane;
-  f32x16 d[4];
+  f32x4 d[16];   // chunk c: dims 8c + 4 h2 .. +3 of the half
 #pragma unroll
-  for (int db = 0; db < 4; ++db) {
-    const f32x16 give = map == 0 ? o_acc[4 + db] : o_acc[db];
-    d[db] = (map == 0 ? o_acc[db] : o_acc[4 + db]) * inv;
-#pragma unroll
-    for (int g4 = 0; g4 < 4; ++g4)
-      lds_st128(mine + (4 * db + g4) * 1024,
-                __builtin_bit_cast(
-                    u32x4, f32x4{give[4 * g4] * inv, give[4 * g4 + 1] * inv,
-                                 give[4 * g4 + 2] * inv,
-                                 give[4 * g4 + 3] * inv}));
+  for (int c = 0; c < 16; ++c) {
+    const int db = c >> 2, j = 4 * (c & 3);
+    const f32x4 lo = f32x4{o_acc[db][j], o_acc[db][j + 1], o_acc[db][j + 2],
+                           o_acc[db][j + 3]} * inv;
+    const f32x4 hi = f32x4{o_acc[4 + db][j], o_acc[4 + db][j + 1],
+                           o_acc[4 + db][j + 2], o_acc[4 + db][j + 3]} * inv;
+    d[c] = map == 0 ? lo : hi;
+    lds_st128(mine + c * 1024,
+              __builtin_bit_cast(u32x4, map == 0 ? hi : lo));
   }
   __syncthreads();
   float ss = 0.0f;
 #pragma unroll
-  for (int db = 0; db < 4; ++db)
-#pragma unroll
-    for (int g4 = 0; g4 < 4; ++g4) {
-      const f32x4 y = __builtin_bit_cast(
-          f32x4, lds_ld128(theirs + (4 * db + g4) * 1024));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float& x = reinterpret_cast<float*>(&d[db])[4 * g4 + i];
-        x = map == 0 ? x - lam * y[i] : y[i] - lam * x;
-        ss += x * x;
-      }
-    }
-  float f = a.w.out_scale;
+  for (int c = 0; c < 16; ++c) {
+    const f32x4 y = __builtin_bit_cast(f32x4, lds_ld128(theirs + c * 1024));
+    d[c] = map == 0 ? d[c] - y * lam : y - d[c] * lam;
+    ss += (d[c][0] * d[c][0] + d[c][1] * d[c][1]) +
+          (d[c][2] * d[c][2] + d[c][3] * d[c][3]);
+  }
   const uint32_t sums = lds0 + kNStage * kStage;
   if (a.w.weight) {
     ss = lane_pair(ss, 32, false);
@@ -551,37 +545,44 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
   }
   __syncthreads();   // (and both halves of the exchange have been read)
   if (a.w.weight) {
+    f32x4 wt[16];
+#pragma unroll
+    for (int c = 0; c < 16; ++c)
+      wt[c] = __builtin_bit_cast(
+          f32x4, lds_ld128(wlds + 4 * (128 * map + 8 * c + 4 * h2)));
     ss += __builtin_bit_cast(float, lds_ld32(sums + 128 * (w ^ 4) + 4 * l32));
-    f *= __builtin_amdgcn_rsqf(ss * (1.0f / kDV) + a.w.eps);
+    const float f =
+        a.w.out_scale * __builtin_amdgcn_rsqf(ss * (1.0f / kDV) + a.w.eps);
+#pragma unroll
+    for (int c = 0; c < 16; ++c) d[c] = d[c] * f * wt[c];
+  } else {
+#pragma unroll
+    for (int c = 0; c < 16; ++c) d[c] = d[c] * a.w.out_scale;
   }
   // Through LDS, so that the stores are whole rows: 32 queries x 128 dims,
   // query-major (256-byte rows, 16-byte chunks swizzled by row & 15), then 4
   // complete rows per store instruction.
   const uint32_t ob = lds0 + (uint32_t)w * 16384;
 #pragma unroll
-  for (int db = 0; db < 4; ++db)
-#pragma unroll
-    for (int g4 = 0; g4 < 4; ++g4) {
-      f32x4 x = f32x4{d[db][4 * g4], d[db][4 * g4 + 1], d[db][4 * g4 + 2],
-                      d[db][4 * g4 + 3]} * f;
-      if (a.w.weight)
-        x *= __builtin_bit_cast(
-            f32x4, lds_ld128(wlds + 4 * (128 * map + 32 * db + 8 * g4 +
-                                         4 * h2)));
-      const int c = 4 * db + g4;    // 16-byte chunk: dims 8c .. 8c+7
-      lds_st64(ob + l32 * kRowB + 16 * (c ^ (l32 & 15)) + 8 * h2,
-               u32x2{pack_bf16x2_rn(x[0], x[1]), pack_bf16x2_rn(x[2], x[3])});
-    }
+  for (int c = 0; c < 16; ++c)   // 16-byte chunk: dims 8c .. 8c+7
+    lds_st64(ob + l32 * kRowB + 16 * (c ^ (l32 & 15)) + 8 * h2,
+             u32x2{pack_bf16x2_rn(d[c][0], d[c][1]),
+                   pack_bf16x2_rn(d[c][2], d[c][3])});
   wave_lds_sync();
+  u32x4 y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = 4 * i + grp;
-    const u32x4 x = __builtin_bit_cast(
+    y[i] = __builtin_bit_cast(
         u32x4, lds_ld128(ob + r * kRowB + 16 * (slot ^ (r & 15))));
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + grp;
     if (row0 + r < len)
       *reinterpret_cast<u32x4*>(a.out + (int64_t)(t0 + row0 + r) * a.o_st +
                                 (int64_t)hp * a.o_sh + 128 * map + 8 * slot) =
-          x;
+          y[i];
   }
 }
 
