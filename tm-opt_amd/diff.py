@@ -22,6 +22,10 @@ import torch
 from . import _lib
 from .attn import HEAD_DIM, PAGE_SIZE, _check_rows, _ptr, _stream
 
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
+_DECODE_SIZE = "tmopt_attn_decode_diff_workspace_size"
+_PREFILL_SIZE = "tmopt_attn_prefill_diff_workspace_size"
+
 
 def _call(dev, name, *args):
     """A launch on the current stream of dev, with dev the current device (the
@@ -34,36 +38,39 @@ def _call(dev, name, *args):
 
 def _weights(lam, norm_weight, norm_eps, out_scale, HQ, dev):
     """The C arguments of the learned weights, checked."""
-    assert lam.dtype == torch.float32 and lam.dim() == 1
-    assert lam.device == dev, (lam.device, dev)
-    n = lam.shape[0]
+    n = lam.numel()
+    assert lam.dtype == _F32 and lam.dim() == 1 and lam.device == dev
     assert n == HQ // 2 or n == 1, (tuple(lam.shape), HQ)
-    assert n == 1 or lam.stride(0) == 1, "lam must be contiguous"
-    if norm_weight is not None:
-        assert norm_weight.dtype == torch.float32
-        assert norm_weight.shape == (2 * HEAD_DIM,)
-        assert norm_weight.is_contiguous() and norm_weight.device == dev
-    return (lam.data_ptr(), 0 if n == 1 else 1, _ptr(norm_weight),
-            float(norm_eps), float(out_scale))
+    assert lam.is_contiguous()
+    if norm_weight is None:
+        return lam.data_ptr(), n > 1, None, 0.0, float(out_scale)
+    assert norm_weight.dtype == _F32 and norm_weight.shape == (2 * HEAD_DIM,)
+    assert norm_weight.is_contiguous() and norm_weight.device == dev
+    return (lam.data_ptr(), n > 1, norm_weight.data_ptr(), float(norm_eps),
+            float(out_scale))
 
 
 def _pools(k_pool, v_pool, HQ, D, dev):
+    shape = k_pool.shape
+    P, page_size, HKV, Dk = shape
     assert k_pool.is_contiguous() and v_pool.is_contiguous()
-    assert k_pool.dtype == torch.bfloat16 and v_pool.dtype == torch.bfloat16
-    assert k_pool.shape == v_pool.shape and k_pool.dim() == 4
+    assert k_pool.dtype == _BF16 and v_pool.dtype == _BF16
+    assert v_pool.shape == shape and Dk == D, (shape, D)
     assert k_pool.device == dev and v_pool.device == dev
-    P, page_size, HKV, Dk = k_pool.shape
-    assert Dk == D and HKV % 2 == 0 and HQ % HKV == 0, (k_pool.shape, HQ)
+    assert HKV % 2 == 0 and HQ % HKV == 0, (shape, HQ)
     return P, page_size, HKV
 
 
 def _table(block_table, rows, dev):
-    assert block_table.dtype == torch.int32 and block_table.dim() == 2
-    assert block_table.device == dev
-    assert block_table.stride(1) == 1 and block_table.shape[0] >= rows
-    # the kernels bound every row read by the stride: rows must be whole
-    assert block_table.stride(0) == block_table.shape[1] or rows <= 1, \
+    """The row width of a block table (the stride: the kernels bound every
+    row read by it, so rows must be whole)."""
+    have, width = block_table.shape
+    stride = block_table.stride()
+    assert block_table.dtype == _I32 and block_table.device == dev
+    assert have >= rows and stride[1] == 1
+    assert stride[0] == width or rows <= 1, \
         "block-table rows must be whole (the row width is the stride)"
+    return stride[0]
 
 
 @functools.lru_cache(maxsize=1024)
@@ -81,9 +88,9 @@ def decode_diff_workspace(B, HQ, HKV, device, num_workgroups=0):
     device = torch.device(device)
     if device.type == "cuda" and device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
-    n = _workspace_size(device, "tmopt_attn_decode_diff_workspace_size", B,
-                        HQ, HKV, HEAD_DIM, int(num_workgroups))
-    return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
+    n = _workspace_size(device, _DECODE_SIZE, B, HQ, HKV, HEAD_DIM,
+                        int(num_workgroups))
+    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def decode_diff_paged(q, k_pool, v_pool, block_table, ctx_lens, lam, scale,
@@ -103,36 +110,37 @@ def decode_diff_paged(q, k_pool, v_pool, block_table, ctx_lens, lam, scale,
     if None; it needs no initialisation; calls that overlap need one each).
     Returns (out [B, HQ / 2, 256] bf16, lse [B, HQ] fp32 or None)."""
     B, HQ, D = q.shape
-    dev = q.device
-    assert q.dtype == torch.bfloat16 and q.is_contiguous()
+    dev, num_workgroups = q.device, int(num_workgroups)
+    assert q.dtype == _BF16 and q.is_contiguous()
     P, page_size, HKV = _pools(k_pool, v_pool, HQ, D, dev)
-    _table(block_table, B, dev)
-    assert ctx_lens.dtype == torch.int32 and ctx_lens.shape == (B,)
+    bts = _table(block_table, B, dev)
+    assert ctx_lens.dtype == _I32 and ctx_lens.shape == (B,)
     assert ctx_lens.is_contiguous() and ctx_lens.device == dev
     if table_wrap:
         assert 0 < window <= table_wrap * page_size, \
             "a ring table needs a window no wider than the ring"
     w = _weights(lam, norm_weight, norm_eps, out_scale, HQ, dev)
     if out is None:
-        out = torch.empty((B, HQ // 2, 2 * D), dtype=torch.bfloat16,
-                          device=dev)
+        out = torch.empty((B, HQ // 2, 2 * D), dtype=_BF16, device=dev)
     else:
         assert out.shape == (B, HQ // 2, 2 * D) and out.device == dev
-        assert out.dtype == torch.bfloat16 and out.is_contiguous()
+        assert out.dtype == _BF16 and out.is_contiguous()
     if lse is not None:
-        assert lse.shape == (B, HQ) and lse.dtype == torch.float32
+        assert lse.shape == (B, HQ) and lse.dtype == _F32
         assert lse.is_contiguous() and lse.device == dev
     elif return_lse:
-        lse = torch.empty((B, HQ), dtype=torch.float32, device=dev)
+        lse = torch.empty((B, HQ), dtype=_F32, device=dev)
     if workspace is None:
-        workspace = decode_diff_workspace(B, HQ, HKV, dev, num_workgroups)
-    assert workspace.device == dev
+        n = _workspace_size(dev, _DECODE_SIZE, B, HQ, HKV, D, num_workgroups)
+        workspace = torch.empty(n, dtype=torch.uint8, device=dev)
+    else:
+        assert workspace.device == dev and workspace.is_contiguous()
+        n = workspace.numel() * workspace.element_size()
     _call(dev, "tmopt_attn_decode_diff", q.data_ptr(), k_pool.data_ptr(),
-          v_pool.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-          int(table_wrap), ctx_lens.data_ptr(), B, HQ, HKV, D, page_size, P,
-          int(window), float(scale), *w, int(min_pages), int(num_workgroups),
-          out.data_ptr(), _ptr(lse), workspace.data_ptr(),
-          workspace.numel() * workspace.element_size())
+          v_pool.data_ptr(), block_table.data_ptr(), bts, int(table_wrap),
+          ctx_lens.data_ptr(), B, HQ, HKV, D, page_size, P, int(window),
+          float(scale), *w, int(min_pages), num_workgroups, out.data_ptr(),
+          _ptr(lse), workspace.data_ptr(), n)
     return out, lse
 
 
@@ -174,11 +182,11 @@ def prefill_diff_varlen(q, k, v, cu_seqlens, lam, scale, norm_weight=None,
     if block_table is not None:
         assert k is None and v is None, "keys come from k/v or from the pools"
         P, page_size, HKV = _pools(k_pool, v_pool, HQ, D, dev)
-        _table(block_table, S, dev)
+        bts = _table(block_table, S, dev)
         if prior_lens is not None:
             assert prior_lens.dtype == torch.int32 and prior_lens.shape == (S,)
             assert prior_lens.is_contiguous() and prior_lens.device == dev
-        strides, bts = (0, 0, 0, 0), block_table.stride(0)
+        strides = (0, 0, 0, 0)
     else:
         assert prior_lens is None, "prior context needs the paged source"
         assert k_pool is None and v_pool is None, "pools need a block table"
@@ -207,17 +215,17 @@ def prefill_diff_varlen(q, k, v, cu_seqlens, lam, scale, norm_weight=None,
     keys = bts
     if bts and max_context is not None:
         keys = max(1, min(bts, -(-int(max_context) // PAGE_SIZE)))
-    n = _workspace_size(dev, "tmopt_attn_prefill_diff_workspace_size", S,
-                        int(max_seqlen), HQ, HKV, keys, int(window))
+    max_seqlen, window = int(max_seqlen), int(window)
+    n = _workspace_size(dev, _PREFILL_SIZE, S, max_seqlen, HQ, HKV, keys,
+                        window)
     if n and keys != bts:       # (the launch sizes its scratch by the table)
-        n = _workspace_size(dev, "tmopt_attn_prefill_diff_workspace_size", S,
-                            int(max_seqlen), HQ, HKV, bts, int(window))
+        n = _workspace_size(dev, _PREFILL_SIZE, S, max_seqlen, HQ, HKV, bts,
+                            window)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     _call(dev, "tmopt_attn_prefill_diff", q.data_ptr(), q.stride(0),
           q.stride(1), _ptr(k), strides[0], strides[1], _ptr(v), strides[2],
-          strides[3], cu_seqlens.data_ptr(), _ptr(prior_lens), S,
-          int(max_seqlen), _ptr(k_pool), _ptr(v_pool), _ptr(block_table), bts,
-          page_size, P, HQ, HKV, D, int(window), float(scale), *w,
-          out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse), total,
-          _ptr(reject), _ptr(ws), n)
+          strides[3], cu_seqlens.data_ptr(), _ptr(prior_lens), S, max_seqlen,
+          _ptr(k_pool), _ptr(v_pool), _ptr(block_table), bts, page_size, P,
+          HQ, HKV, D, window, float(scale), *w, out.data_ptr(), out.stride(0),
+          out.stride(1), _ptr(lse), total, _ptr(reject), _ptr(ws), n)
     return out, lse
