@@ -135,6 +135,12 @@ def test_release(tm, dev, B, W):
         want = diff_ref.release(table, slots, lens, free, count)
         assert f.tolist() == want[0]
         assert [x.item() for x in got] == list(want[1:])
+        f, n = _dev(free, dev), _dev([count], dev)         # and in place
+        got = tm.release_pages(_dev(table, dev), _dev(slots, dev, torch.int64),
+                               _dev(lens, dev), f, n,
+                               out=(n, torch.empty_like(n)))
+        assert f.tolist() == want[0]
+        assert [x.item() for x in got] == list(want[1:])
     for i, (s, n) in ((1, (B + 2, 3)), (1, (slots[2 % B], 3)),
                       (1, (slots[1 % B], -1)),
                       (1, (slots[1 % B], 16 * W + 1))):
@@ -178,6 +184,38 @@ def test_plan_grows_in_a_graph(tm, dev):
                out.positions)
         assert [x.tolist() for x in got] == list(want[:6]), step
         assert count.item() == height and out.reject.item() == want[7]
+
+
+@pytest.mark.parametrize("B,W,T", [(3, 8, 40), (70, 300, 5000),
+                                   (1100, 4, 1200)])
+def test_plan_in_place(tm, dev, B, W, T):
+    """Heights and lengths that the plan writes over, both and each alone:
+    the same as into buffers of their own."""
+    rng = random.Random(B)
+    table, free = _state(B, W, B * W, rng)
+    slots = rng.sample(range(B), B)
+    new = [rng.choice([0, 1, 1, 7]) for _ in range(B)]
+    new[0] = T - sum(new[1:]) if sum(new[1:]) < T < 16 * W else 1
+    ctx = [rng.randint(0, 16 * W - n) for n in new]
+    for count in (B * W, 0):
+        want = diff_ref.plan(table, slots, ctx, new, free, count, T)
+        for over in ((1, 1), (0, 1), (1, 0)):
+            dt, dc = _dev(table, dev), _dev(ctx, dev)
+            n = _dev([count], dev)
+            tok = torch.empty((2, T), dtype=torch.int64, device=dev)
+            out = tm.PagePlan(
+                torch.empty((B, W), dtype=torch.int32, device=dev),
+                dc if over[0] else torch.empty_like(dc),
+                torch.empty(B + 1, dtype=torch.int32, device=dev), tok[0],
+                tok[1], n if over[1] else torch.empty_like(n),
+                torch.empty(1, dtype=torch.int32, device=dev))
+            got = tm.plan_pages(dt, _dev(slots, dev, torch.int64), dc,
+                                _dev(new, dev), _dev(free, dev), n, T,
+                                out=out)
+            assert got is out
+            got = [dt] + list(out)
+            for g, w in zip(got, want):
+                assert g.tolist() == ([w] if isinstance(w, int) else w)
 
 
 def test_plan_then_release_comes_back(tm, dev):

@@ -9,12 +9,17 @@
 // position p = ctx_i + t - cu[i] and goes to pool row table[p / 16] * 16 +
 // p % 16. A release pushes the pages back in order.
 //
-// One work-group checks the step and makes the sums and the new pages (the
-// checks decide about the whole step, and a few thousand lengths are a few
-// microseconds' work of one compute unit); then every element of the block
-// table, the slot map and the positions is independent, and as many work-groups
-// as there are of 1024 elements write them. Small steps stay in the first
-// work-group, one launch. Bound by latency: launches and dependent loads.
+// The checks decide about the whole step, so whoever writes an output needs the
+// sums over all requests. Up to 1024 requests every work-group makes them for
+// itself (the lengths are a few KB in the L2), holds them in LDS and writes its
+// 1024 elements at a time of the block table, the slot map and the positions:
+// one launch. A new page is read off the stack by whoever needs it, and its
+// entry of the page table written by the work-group that fills that part of
+// the block table, so no work-group waits for another. Where an output is one
+// of the inputs (a graph that steps on in place), or above 1024 requests, one
+// work-group makes the sums and the new pages, and a second launch the rest;
+// a small step in place is one work-group's. Bound by latency: launches and
+// dependent loads.
 #include "common.h"
 
 namespace tmopt {
@@ -24,6 +29,7 @@ constexpr int kPage = 16;
 constexpr int kMaxRequests = 8192;      // the sums live in LDS
 constexpr int kMaxRows = 1 << 18;       // one bit per table row in LDS
 constexpr int kMaxTokens = 1 << 24;     // sums of a wave stay below 2^31
+constexpr int kOwnSums = 1024;          // requests a fill may sum for itself
 constexpr int kPlanThreads = 1024;
 constexpr int kFillThreads = 256;
 constexpr int kChunk = 1024;            // elements per work-group of a fill
@@ -66,26 +72,28 @@ __device__ __forceinline__ int run_of(P s, int n, int x) {
   return lo;
 }
 
-// Checks and sums of a step, by one work-group: tok / page [B + 1] (LDS) get
-// the exclusive sums of the new tokens and of the pages taken (plan) or handed
-// back (release). Returns whether the step is accepted (the same in every
-// thread); leaves its totals in tot and the stack's height in n.
+// Checks and sums of a step, by one work-group of T threads: tok / page [B + 1]
+// (LDS) get the exclusive sums of the new tokens and of the pages taken (plan)
+// or handed back (release). Returns whether the step is accepted (the same in
+// every thread); leaves its totals in tot and the stack's height in n.
+template <int T>
 __device__ bool step_sums(const PlanArgs& a, bool release, int* tok, int* page,
                           uint32_t* seen, int64_t (&tot)[2], int& n) {
-  __shared__ int64_t wsum[2][kPlanThreads / 64];
+  __shared__ int64_t wsum[2][T / 64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  n = a.count_in[0];      // (read before count_out, which may be it, is written)
   const int nwords = (int)((a.S + 31) / 32);
-  for (int i = threadIdx.x; i < nwords; i += kPlanThreads) seen[i] = 0;
+  for (int i = threadIdx.x; i < nwords; i += T) seen[i] = 0;
   __syncthreads();
   int bad = 0;
   tot[0] = tot[1] = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
+  for (int b0 = 0; b0 < a.B; b0 += T) {
     const int b = b0 + threadIdx.x;
     int nt = 0, np = 0;
     if (b < a.B) {
       const int64_t slot = a.slots[b];
+      const int ctx = a.ctx[b], add = release ? 0 : a.add[b];
       if (slot >= 0) {
-        const int ctx = a.ctx[b], add = release ? 0 : a.add[b];
         const int64_t end = (int64_t)ctx + add;
         const int most = release ? a.W : min(a.W, a.width);
         bool ok = slot < a.S && ctx >= 0 && add >= 0 &&
@@ -109,7 +117,7 @@ __device__ bool step_sums(const PlanArgs& a, bool release, int* tok, int* page,
     }
     __syncthreads();
     int64_t bt = tot[0], bp = tot[1];
-    for (int j = 0; j < kPlanThreads / 64; ++j) {
+    for (int j = 0; j < T / 64; ++j) {
       if (j < w) {
         bt += wsum[0][j];
         bp += wsum[1][j];
@@ -124,11 +132,124 @@ __device__ bool step_sums(const PlanArgs& a, bool release, int* tok, int* page,
     __syncthreads();
   }
   if (threadIdx.x == 0) tok[0] = page[0] = 0;
-  n = a.count_in[0];      // (read before count_out, which may be it, is written)
   bad |= n < 0 || n > a.F || tot[0] > (release ? 0 : a.max_tokens) ||
          (release ? n + tot[1] > a.F : tot[1] > n);
   return !__syncthreads_or(bad);
 }
+
+// The sums of a refused step: no tokens, no pages.
+template <int T>
+__device__ void no_step(const PlanArgs& a, int* tok, int* page,
+                        int64_t (&tot)[2]) {
+  for (int i = threadIdx.x; i <= a.B; i += T) tok[i] = page[i] = 0;
+  tot[0] = tot[1] = 0;
+  __syncthreads();
+}
+
+// How rows of `width` entries are cut into parts of about 1024: `per` parts per
+// row, or `rows` whole rows per part.
+struct Cut {
+  int per, rows, parts;
+};
+Cut cut_rows(int B, int64_t width) {
+  Cut c;
+  c.per = (int)((width + kChunk - 1) / kChunk);
+  c.rows = width < kChunk ? (int)(kChunk / width) : 1;
+  c.parts = c.per > 1 ? B * c.per : (B + c.rows - 1) / c.rows;
+  return c;
+}
+
+// A whole step of up to kOwnSums requests: c.parts parts of the block table,
+// then 1024 tokens each.
+template <int T>
+__global__ __launch_bounds__(T) void plan_kernel(PlanArgs a, Cut c,
+                                                 int parts) {
+  extern __shared__ int lds[];
+  int* const tok = lds;
+  int* const page = tok + a.B + 1;
+  int* const ctx = page + a.B + 1;    // [B] tokens held
+  int* const row = ctx + a.B;         // [B] table row, -1: padding
+  uint32_t* const seen = (uint32_t*)(row + a.B);
+  for (int i = threadIdx.x; i < a.B; i += T) {
+    const int64_t slot = a.slots[i];
+    const bool real = slot >= 0 && slot < a.S;
+    row[i] = real ? (int)slot : -1;
+    ctx[i] = slot >= 0 ? a.ctx[i] : 0;
+  }
+  int64_t tot[2];
+  int n;
+  const bool ok = step_sums<T>(a, false, tok, page, seen, tot, n);
+  if (!ok) no_step<T>(a, tok, page, tot);
+  if (blockIdx.x == 0) {
+    for (int i = threadIdx.x; i < a.B; i += T) {
+      a.cu[i + 1] = tok[i + 1];
+      a.seq[i] = ctx[i] + (tok[i + 1] - tok[i]);
+    }
+    if (threadIdx.x == 0) {
+      a.cu[0] = 0;
+      a.count_out[0] = n - (int)tot[1];
+      a.reject[0] = !ok;
+    }
+  }
+  // page j of request i, which holds `old` already
+  auto page_at = [&](int i, int j, int old) {
+    return j < old ? a.table[(int64_t)row[i] * a.W + j]
+                   : a.free[n - 1 - (page[i] + j - old)];
+  };
+  for (int part = blockIdx.x; part < parts; part += gridDim.x) {
+    if (part < c.parts) {
+      const int i0 = c.per > 1 ? part / c.per : part * c.rows;
+      const int j0 = c.per > 1 ? (part - i0 * c.per) * kChunk : 0;
+      const int rows = min(c.rows, a.B - i0);
+      const int width = min(kChunk, a.width - j0);
+      const bool wide = ((a.width | a.W) & 3) == 0 &&
+                        (((uintptr_t)a.block | (uintptr_t)a.table) & 15) == 0;
+      const int step = wide ? 4 : 1, units = width / step;   // per row
+      for (int u = threadIdx.x; u < rows * units; u += T) {
+        const int r = u / units, i = i0 + r, j = j0 + step * (u - r * units);
+        const int old = pages_of(ctx[i]);
+        const int have = ok && row[i] >= 0 ? old + page[i + 1] - page[i] : 0;
+        int32_t* const src = a.table + (int64_t)max(row[i], 0) * a.W + j;
+        int32_t* const out = a.block + (int64_t)i * a.width + j;
+        if (wide) {     // 16 bytes at a time, except across the new pages
+          i32x4 x{-1, -1, -1, -1};
+          if (j + 4 <= min(old, have)) {
+            x = *reinterpret_cast<const i32x4*>(src);
+          } else if (j < have) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (j + e < have) {
+                x[e] = page_at(i, j + e, old);
+                if (j + e >= old) src[e] = x[e];
+              }
+          }
+          *reinterpret_cast<i32x4*>(out) = x;
+        } else {
+          const int x = j < have ? page_at(i, j, old) : -1;
+          out[0] = x;
+          if (j >= old && j < have) src[0] = x;
+        }
+      }
+    } else {
+      const int t0 = (part - c.parts) * kChunk;
+      for (int t = t0 + threadIdx.x; t < min(t0 + kChunk, a.max_tokens);
+           t += T) {
+        int64_t slot = -1, pos = 0;
+        if (t < (int)tot[0]) {
+          const int i = run_of(tok, a.B, t);
+          const int p = ctx[i] + t - tok[i];
+          const int pg = page_at(i, p / kPage, pages_of(ctx[i]));
+          pos = p;
+          slot = pg < 0 ? -1 : (int64_t)pg * kPage + p % kPage;
+        }
+        a.slot_map[t] = slot;
+        a.pos[t] = pos;
+      }
+    }
+  }
+}
+
+// ---- two launches: the sums and the new pages, then the rest ---------------
 
 // 4 entries j .. j+3 of block-table row i holding `have` pages of table row
 // `row`
@@ -168,21 +289,15 @@ __device__ __forceinline__ void fill_token(const PlanArgs& a, P cu, int total,
   a.pos[t] = pos;
 }
 
-// one work-group: the checks, the sums, the new pages; `whole`: and the rest
-__global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a,
-                                                            int whole) {
+__global__ __launch_bounds__(kPlanThreads) void plan_sums_kernel(PlanArgs a) {
   extern __shared__ int lds[];
   int* const tok = lds;
   int* const page = tok + a.B + 1;
   uint32_t* const seen = (uint32_t*)(page + a.B + 1);
   int64_t tot[2];
   int n;
-  const bool ok = step_sums(a, false, tok, page, seen, tot, n);
-  if (!ok) {
-    for (int i = threadIdx.x; i <= a.B; i += kPlanThreads) tok[i] = 0;
-    tot[0] = tot[1] = 0;
-    __syncthreads();
-  }
+  const bool ok = step_sums<kPlanThreads>(a, false, tok, page, seen, tot, n);
+  if (!ok) no_step<kPlanThreads>(a, tok, page, tot);
   for (int i = threadIdx.x; i < a.B; i += kPlanThreads) {
     const int ctx = a.slots[i] < 0 ? 0 : a.ctx[i];
     a.cu[i + 1] = tok[i + 1];
@@ -199,21 +314,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a,
     const int have = pages_of(a.seq[i]);
     a.table[a.slots[i] * a.W + have - (page[i + 1] - p)] = a.free[n - 1 - p];
   }
-  if (!whole) return;
-  __syncthreads();
-  const int per = (a.width + 3) / 4;
-  for (int x = threadIdx.x; x < a.B * per; x += kPlanThreads) {
-    const int i = x / per;
-    const int64_t slot = a.slots[i];
-    fill_table(a, i, 4 * (x - i * per), a.table + (slot < 0 ? 0 : slot) * a.W,
-               ok && slot >= 0 ? pages_of(a.seq[i]) : 0);
-  }
-  for (int t = threadIdx.x; t < a.max_tokens; t += kPlanThreads)
-    fill_token(a, (const int*)tok, (int)tot[0], t);
 }
 
-// the rest of a large step: work-groups [0, B * per) the block table, 1024
-// entries of a row each, the others 1024 tokens each
+// the rest: work-groups [0, B * per) the block table, 1024 entries of a row each, the others 1024 tokens each
 __global__ __launch_bounds__(kFillThreads) void plan_fill_kernel(PlanArgs a,
                                                                  int per) {
   extern __shared__ int cu[];
@@ -238,31 +341,50 @@ __global__ __launch_bounds__(kFillThreads) void plan_fill_kernel(PlanArgs a,
   }
 }
 
-__global__ __launch_bounds__(kPlanThreads) void release_kernel(PlanArgs a,
-                                                               int whole) {
+// A whole release of up to kOwnSums requests.
+template <int T>
+__global__ __launch_bounds__(T) void release_kernel(PlanArgs a, int per) {
   extern __shared__ int lds[];
   int* const tok = lds;
   int* const page = tok + a.B + 1;
   uint32_t* const seen = (uint32_t*)(page + a.B + 1);
   int64_t tot[2];
   int n;
-  const bool ok = step_sums(a, true, tok, page, seen, tot, n);
+  const bool ok = step_sums<T>(a, true, tok, page, seen, tot, n);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    a.count_out[0] = n + (ok ? (int)tot[1] : 0);
+    a.reject[0] = !ok;
+  }
+  if (!ok) return;
+  for (int part = blockIdx.x; part < a.B * per; part += gridDim.x) {
+    const int i = part / per, j0 = (part - i * per) * kChunk;
+    const int have = page[i + 1] - page[i];
+    const int32_t* const row = a.table + (have > 0 ? a.slots[i] : 0) * a.W;
+    int32_t* const dst = a.free + n + page[i];
+    for (int j = j0 + threadIdx.x; j < min(j0 + kChunk, have); j += T)
+      dst[j] = row[j];
+  }
+}
+
+// ---- two launches -----------------------------------------------------------
+
+__global__ __launch_bounds__(kPlanThreads) void release_sums_kernel(
+    PlanArgs a) {
+  extern __shared__ int lds[];
+  int* const tok = lds;
+  int* const page = tok + a.B + 1;
+  uint32_t* const seen = (uint32_t*)(page + a.B + 1);
+  int64_t tot[2];
+  int n;
+  const bool ok = step_sums<kPlanThreads>(a, true, tok, page, seen, tot, n);
   if (threadIdx.x == 0) {
     a.count_out[0] = n + (ok ? (int)tot[1] : 0);
     a.reject[0] = !ok;
   }
-  if (whole) {
-    for (int p = threadIdx.x; ok && p < (int)tot[1]; p += kPlanThreads) {
-      const int i = run_of(page, a.B, p);
-      a.free[n + p] = a.table[a.slots[i] * a.W + p - page[i]];
-    }
-  } else {
-    for (int i = threadIdx.x; i < a.B; i += kPlanThreads)
-      a.first[i] = n + page[i];
-  }
+  for (int i = threadIdx.x; i < a.B; i += kPlanThreads) a.first[i] = n + page[i];
 }
 
-// rows' pages of a large release: 1024 entries of a row per work-group
+// 1024 entries of a row per work-group
 __global__ __launch_bounds__(kFillThreads) void release_fill_kernel(PlanArgs a,
                                                                     int per) {
   const int i = blockIdx.x / per;
@@ -326,10 +448,10 @@ extern "C" int tmopt_plan_pages(
                     (max_tokens == 0 || (slot_mapping && positions)),
                 TMOPT_EINVAL, "plan_pages: null pointer");
   const int64_t per = (width + kChunk - 1) / kChunk;
-  const int64_t groups = B * per + (max_tokens + kChunk - 1) / kChunk;
-  TMOPT_REQUIRE(groups < 0x7fffffff, TMOPT_EUNSUPPORTED,
+  const int64_t tokens = (max_tokens + kChunk - 1) / kChunk;
+  TMOPT_REQUIRE(B * per + tokens < 0x7fffffff, TMOPT_EUNSUPPORTED,
                 "plan_pages: %lld work-groups exceed the grid limit",
-                (long long)groups);
+                (long long)(B * per + tokens));
   PlanArgs a{};
   a.table = page_table;
   a.S = table_rows;
@@ -351,11 +473,29 @@ extern "C" int tmopt_plan_pages(
   a.count_out = free_count_out;
   a.reject = reject;
   const hipStream_t st = (hipStream_t)stream;
-  const bool whole = B * width <= 16384 && max_tokens <= 4096;
-  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads),
-                     plan_lds(B, table_rows), st, a, (int)whole);
+  const bool in_place = seq_lens == ctx_lens || free_count_out == free_count;
+  // Small enough for one work-group (graph replays, us a step, by one / by two
+  // launches: 4 requests of 64 pages 4.4 / 5.6, 32 of 512 6.5 / 5.9, 2 of 2048
+  // new tokens 6.2 / 7.3, of 4096 8.2 / 7.3).
+  const bool small = B * width <= 16384 && max_tokens <= 4096;
+  if (B <= kOwnSums && (small || !in_place)) {
+    const size_t lds = plan_lds(B, table_rows) + 2 * (size_t)B * sizeof(int);
+    const Cut c = cut_rows(B, width);
+    const int parts = c.parts + (int)tokens;
+    if (in_place)
+      hipLaunchKernelGGL((plan_kernel<kPlanThreads>), dim3(1),
+                         dim3(kPlanThreads), lds, st, a, c, parts);
+    else
+      hipLaunchKernelGGL((plan_kernel<kFillThreads>),
+                         dim3((unsigned)(parts > 0 ? parts : 1)),
+                         dim3(kFillThreads), lds, st, a, c, parts);
+    return check_launch("plan_pages");
+  }
+  const int64_t groups = B * per + tokens;
+  hipLaunchKernelGGL(plan_sums_kernel, dim3(1), dim3(kPlanThreads),
+                     plan_lds(B, table_rows), st, a);
   const int rc2 = check_launch("plan_pages");
-  if (rc2 || whole) return rc2;
+  if (rc2 || groups == 0) return rc2;
   hipLaunchKernelGGL(plan_fill_kernel, dim3((unsigned)groups),
                      dim3(kFillThreads), (B + 1) * sizeof(int), st, a,
                      (int)per);
@@ -401,11 +541,26 @@ extern "C" int tmopt_release_pages(
   a.reject = reject;
   a.first = (int32_t*)workspace;
   const hipStream_t st = (hipStream_t)stream;
-  const bool whole = B * table_width <= 16384;
-  hipLaunchKernelGGL(release_kernel, dim3(1), dim3(kPlanThreads),
-                     plan_lds(B, table_rows), st, a, (int)whole);
+  const bool in_place = free_count_out == free_count;
+  // small enough for one work-group (16 rows of 1024 pages 7.5 us by one, 5.6 by
+  // two launches; 8 rows 5.2 / 5.3)
+  const bool small = B * table_width <= 8192;
+  if (B <= kOwnSums && (small || !in_place)) {
+    const int64_t groups = B * per > 0 ? B * per : 1;
+    if (in_place)
+      hipLaunchKernelGGL((release_kernel<kPlanThreads>), dim3(1),
+                         dim3(kPlanThreads), plan_lds(B, table_rows), st, a,
+                         (int)per);
+    else
+      hipLaunchKernelGGL((release_kernel<kFillThreads>),
+                         dim3((unsigned)groups), dim3(kFillThreads),
+                         plan_lds(B, table_rows), st, a, (int)per);
+    return check_launch("release_pages");
+  }
+  hipLaunchKernelGGL(release_sums_kernel, dim3(1), dim3(kPlanThreads),
+                     plan_lds(B, table_rows), st, a);
   const int rc2 = check_launch("release_pages");
-  if (rc2 || whole) return rc2;
+  if (rc2) return rc2;
   hipLaunchKernelGGL(release_fill_kernel, dim3((unsigned)(B * per)),
                      dim3(kFillThreads), 0, st, a, (int)per);
   return check_launch("release_pages");
