@@ -115,6 +115,16 @@ enum : int {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
+// Groups of waves per head pair in the merge, from the pieces of an average
+// request (at most one more than its share of the R ranges). Graph replays with
+// 1 / 2 / 8 groups, us a call, 32Q/4KV: one request of 50,001 tokens 49.4 / 38.0
+// / 32.3, 4 of 4K-8K 25.2 / 22.8 / 20.8, 9 up to 4.7K 24.0 / 21.7 / 20.9, 16 up
+// to 2K 21.2 / 20.4 / 21.0, 24 up to 4K 32.1 / 31.5 / 34.5, 64 of 1K-8K 112 /
+// 112 / 117.
+__host__ __device__ __forceinline__ int merge_groups(int B, int R) {
+  return 1 + R / B <= 16 ? 2 : 8;
+}
+
 // value of the lane eight columns on (within 16-lane rows): the other map's
 __device__ __forceinline__ float other_map(float x) {
   return __builtin_bit_cast(
@@ -173,12 +183,28 @@ void decode_diff_kernel(DecodeDiffArgs a) {
   }
   const int U = __builtin_amdgcn_readfirstlane(pref[a.B]);
   int C = max((U + R - 1) / R, a.min_pages);
+  // The merge takes a request's pieces in rounds of 64 (16 with two groups of
+  // waves, merge_groups), about 2.5 us each, a page of both waves 0.45 us: a
+  // little longer pieces where they save rounds (one request of 8000 tokens 19.8
+  // -> 17.0 us, of 50,001 as before).
+  const int cap = 8 * merge_groups(a.B, R);
+  if (most > (int64_t)C * cap) {
+    const int r0 = ((most + C - 1) / C + cap - 1) / cap;
+    int best = 11 * r0 + 2 * C;
+    for (int r = min(r0 - 1, 4); r > 0; --r) {
+      const int c = (most + cap * r - 1) / (cap * r);
+      if (11 * r + 2 * c < best) {
+        best = 11 * r + 2 * c;
+        C = c;
+      }
+    }
+  }
   // Whole requests, the same number for every range, where the longest ones are
   // no more than a sixteenth (and a page) above the even share: nothing is
   // split, nothing joined (96 requests under a window of 512, 64Q/16KV: 76 us a
   // call cut evenly, 70 whole).
   const int per = (a.B + R - 1) / R;
-  const bool whole = (int64_t)per * most <= C + C / 16 + 1;
+  const bool whole = (int64_t)per * most <= (int64_t)C + C / 16 + 1;
   // the range [r0, r1), and this wave's pages of it: [u0, u1), backward in the
   // second half
   int r0 = (int)min((int64_t)range * C, (int64_t)U);
@@ -671,15 +697,9 @@ __global__ __launch_bounds__(128 * H * S) void decode_diff_merge(
       u32x2{pack_bf16x2_rn(acc[0], acc[1]), pack_bf16x2_rn(acc[2], acc[3])};
 }
 
-// The merge's shape, from the pieces of an average request (at most one more
-// than its share of the R ranges): two groups of waves per head pair, or eight.
-// Graph replays with 1 / 2 / 8 groups, us a call, 32Q/4KV: one request of
-// 50,001 tokens 49.4 / 38.0 / 32.3, 4 of 4K-8K 25.2 / 22.8 / 20.8, 9 up to 4.7K
-// 24.0 / 21.7 / 20.9, 16 up to 2K 21.2 / 20.4 / 21.0, 24 up to 4K 32.1 / 31.5 /
-// 34.5, 64 of 1K-8K 112 / 112 / 117.
 void launch_merge(const DecodeDiffArgs& a, int R, hipStream_t st) {
-  const int np = 1 + R / a.B, H = a.HQ / 2;
-  if (np <= 16 || H > 65535)
+  const int H = a.HQ / 2;
+  if (merge_groups(a.B, R) == 2 || H > 65535)
     hipLaunchKernelGGL((decode_diff_merge<2, 2>), dim3(a.B, (H + 1) / 2),
                        dim3(512), 0, st, a);
   else
