@@ -36,7 +36,7 @@ def test_decode_refusals(tm):
                dict(wrap=9), dict(wrap=4), dict(wrap=4, window=65)):
         assert call(**kw) == e.TMOPT_EINVAL, kw
     for kw in (dict(B=8193), dict(D=64), dict(ps=32),
-               dict(HKV=1 << 20, HQ=1 << 20)):
+               dict(HKV=1 << 18, HQ=1 << 18)):
         assert call(**kw) == e.TMOPT_EUNSUPPORTED, kw
     for kw in (dict(ws=NULL), dict(ws=ctypes.c_void_p(8)),
                dict(nbytes=need - 1)):

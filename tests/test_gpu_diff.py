@@ -147,6 +147,37 @@ def test_decode_absent_pages(tm, dev):
     assert (out[2] == 0).all() and (lse[2] == -torch.inf).all()
 
 
+@pytest.mark.parametrize("window", [0, 50])
+def test_decode_lengths_past_the_table(tm, dev, window):
+    """Lengths far past the row's width, up to the largest int32, and negative
+    ones: the walk is bounded by the table, what it cannot name is absent."""
+    g = _gen(20)
+    c = Cache([96, 96, 96, 60, 60], 2, g, dev)
+    q = _rand((5, 4, D), g, dev)
+    w = _weights(4, g, dev)
+    for b, n in ((1, 2 ** 31 - 1), (2, 100), (3, -5)):
+        c.ctx[b] = n
+    out, lse = tm.decode_diff_paged(q, c.kp, c.vp, c.table, c.ctx, w["lam"],
+                                    0.1, window=window)
+    for b, n in ((0, 96), (1, 2 ** 31 - 1), (2, 100), (3, 0), (4, 60)):
+        lo = max(0, n - window) if window else 0
+        pos = torch.arange(min(lo, 96), min(n, 96), device=dev)
+        ref = diff_ref.attend(
+            q[b:b + 1], diff_ref.rows_of(c.kp, c.table[b], pos),
+            diff_ref.rows_of(c.vp, c.table[b], pos),
+            torch.tensor([n - 1], device=dev), pos, w["lam"], 0.1,
+            window=window)
+        diff_ref.check(out[b:b + 1], lse[b:b + 1].T, ref, f"row {b}")
+
+
+def test_decode_no_requests(tm, dev):
+    c = Cache([5], 2, _gen(21), dev)
+    out, lse = tm.decode_diff_paged(
+        torch.empty((0, 4, D), dtype=BF, device=dev), c.kp, c.vp, c.table,
+        c.ctx[:0], torch.ones(2, device=dev), 0.1)
+    assert out.shape == (0, 2, 256) and lse.shape == (0, 4)
+
+
 @pytest.mark.parametrize("std", [0.0, 30.0])
 def test_decode_flat_and_peaked(tm, dev, std):
     """Equal scores everywhere, and scores so far apart that each softmax is
@@ -359,6 +390,60 @@ def test_prefill_flat_and_peaked(tm, dev, std):
     _prefill(tm, _rand((T, 8, D), g, dev, std), _rand((T, 2, D), g, dev),
              _rand((T, 2, D), g, dev), _cu([T], dev), _weights(8, g, dev),
              D ** -0.5)
+
+
+def test_prefill_far_pages(tm, dev):
+    """Pages past 4 GiB of the pools."""
+    g = _gen(22)
+    P, hkv, n = 300000, 4, 100
+    kp = torch.zeros((P, PAGE, hkv, D), dtype=BF, device=dev)
+    vp = torch.zeros_like(kp)
+    c = Cache([n, n], hkv, g, dev)
+    far = torch.tensor([[P - 1 - i for i in range(7)],
+                        [P // 2 + i for i in range(7)]], device=dev)
+    kp[far], vp[far] = c.kp[c.table.long()], c.vp[c.table.long()]
+    _prefill(tm, _rand((130, 16, D), g, dev), None, None, _cu([90, 40], dev),
+             _weights(16, g, dev), k_pool=kp, v_pool=vp, table=far.int(),
+             prior=torch.tensor([10, 60], dtype=torch.int32, device=dev))
+
+
+@pytest.mark.parametrize("split", [0, 1])
+def test_prefill_pages_without_an_entry(tm, dev, split):
+    """Entries outside the pool, and positions past the row's width, read as
+    zero rows (of runs long enough to be split, and of short ones)."""
+    g = _gen(23)
+    n, prior = (40, 3000) if split else (40, 70)
+    c = Cache([n + prior], 2, g, dev)
+    w = _weights(4, g, dev)
+    kp = torch.cat([c.kp, torch.zeros_like(c.kp[:1])])
+    vp = torch.cat([c.vp, torch.zeros_like(c.vp[:1])])
+    P = c.kp.shape[0]
+    gone = [1, 4, (n + prior - 1) // PAGE]
+    zero = c.table.clone()
+    zero[0, gone] = P
+    c.table[0, gone[0]], c.table[0, gone[1]] = -1, P
+    q = _rand((n, 4, D), g, dev)
+    cu = _cu([n], dev)
+    pr = torch.tensor([prior], dtype=torch.int32, device=dev)
+    ref = diff_ref.prefill(q, None, None, cu.tolist(), w["lam"], 0.1,
+                           prior=pr, k_pool=kp, v_pool=vp, table=zero,
+                           **{x: y for x, y in w.items() if x != "lam"})
+    out, lse = tm.prefill_diff_varlen(
+        q, None, None, cu, w["lam"], 0.1, max_seqlen=n, prior_lens=pr,
+        k_pool=c.kp, v_pool=c.vp,
+        block_table=c.table[:, :gone[2]].contiguous(),
+        **{x: y for x, y in _user(w).items() if x != "lam"})
+    diff_ref.check(out, lse, ref)
+
+
+def test_prefill_without_tokens(tm, dev):
+    e = torch.empty((0, 4, D), dtype=BF, device=dev)
+    lam = torch.ones(2, device=dev)
+    for cu in ([0], [0, 0, 0]):
+        out, lse = tm.prefill_diff_varlen(
+            e, e[:, :2], e[:, :2],
+            torch.tensor(cu, dtype=torch.int32, device=dev), lam, 0.1)
+        assert out.shape == (0, 2, 256) and lse.shape == (4, 0)
 
 
 def test_prefill_many_runs(tm, dev):

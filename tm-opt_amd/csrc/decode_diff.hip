@@ -73,10 +73,12 @@ struct DecodeDiffArgs {
 __device__ __forceinline__ int vis_lo(int n, int window) {
   return (window > 0 && n > window) ? n - window : 0;
 }
-// pages of a request of n tokens that hold a visible key
-__device__ __forceinline__ int vis_pages(int n, int window) {
+// pages of a request of n tokens that hold a visible key and may have an entry
+// in a row of `width` (a ring's pages all have one)
+__device__ __forceinline__ int vis_pages(int n, int window, int width) {
   if (n <= 0) return 0;
-  return (int)(((uint32_t)n + kPage - 1) / kPage) - vis_lo(n, window) / kPage;
+  const int end = (int)(((uint32_t)n + kPage - 1) / kPage);
+  return max(0, min(end, width) - vis_lo(n, window) / kPage);
 }
 
 __device__ __forceinline__ int page_id(const DecodeDiffArgs& a, int b, int lp) {
@@ -156,6 +158,7 @@ void decode_diff_kernel(DecodeDiffArgs a) {
   int* ids = reinterpret_cast<int*>(smem + a.ids_off) + v * (ids_cap + 2);
 
   // ---- 1. prefix sums of visible pages: pref[b] = first page of request b --
+  const int width = a.table_wrap > 0 ? 0x7fffffff : a.bt_width;
   int most = 0;   // pages of the longest request
   {
     int carry = 0;
@@ -163,7 +166,7 @@ void decode_diff_kernel(DecodeDiffArgs a) {
       const int b = b0 + threadIdx.x;
       const int nb = b < a.B ? as_const(a.ctx_lens)[b] : 0;
       if (b < a.B) nlen[b] = nb;
-      const int np = vis_pages(nb, a.window);
+      const int np = vis_pages(nb, a.window, width);
       most = max(most, np);
       const int x = wave_scan(np);
       if (lane == 63) wsum[w] = x;
@@ -259,7 +262,7 @@ void decode_diff_kernel(DecodeDiffArgs a) {
   int cb = __builtin_amdgcn_readfirstlane(seq_of(max(cu, 0)));
   int seq_start = __builtin_amdgcn_readfirstlane(pref[cb]);
   int cur_n = __builtin_amdgcn_readfirstlane(nlen[cb]);
-  int seq_end = seq_start + vis_pages(cur_n, a.window);
+  int seq_end = seq_start + vis_pages(cur_n, a.window, width);
   int pg_of = vis_lo(cur_n, a.window) / kPage - seq_start;   // page of unit u
   int last_b = -1;  // request of the previous step handed out
   __syncthreads();  // the ids are there; every wave is done with the tables
@@ -277,7 +280,7 @@ void decode_diff_kernel(DecodeDiffArgs a) {
       do {
         cb += back ? -1 : 1;
         cur_n = as_const(ra->ctx_lens)[cb];
-        const int n = vis_pages(cur_n, a.window);
+        const int n = vis_pages(cur_n, a.window, width);
         seq_start = back ? seq_start - n : seq_end;
         seq_end = seq_start + n;
       } while (cu >= seq_end || cu < seq_start);

@@ -39,7 +39,7 @@ inline int check_diff(const char* what, int HQ, int HKV, int D, int window,
                 "%s: HQ=%d HKV=%d (HKV even, HQ a multiple of it)", what, HQ,
                 HKV);
   TMOPT_REQUIRE((int64_t)kPage * HKV * kD * 2 < (1ll << 31) &&
-                    HQ <= (1 << 20),
+                    HQ <= (1 << 17),
                 TMOPT_EUNSUPPORTED, "%s: HQ=%d HKV=%d too large", what, HQ,
                 HKV);
   TMOPT_REQUIRE(window >= 0, TMOPT_EINVAL, "%s: window=%d", what, window);

@@ -109,7 +109,7 @@ __device__ __forceinline__ int pieces_of(const PrefillDiffArgs& a, int BQ,
   for (int s = lane; s < a.S; s += 64) {
     const int len = a.cu[s + 1] - a.cu[s];
     const int nb = (len + BQ - 1) / BQ;
-    const int prior = a.prior != nullptr ? a.prior[s] : 0;
+    const int prior = a.prior != nullptr ? max(a.prior[s], 0) : 0;
     if (nb > 0) {
       const int t0 = item_tiles(a, BQ, prior, len, 0).n;
       const int t1 = item_tiles(a, BQ, prior, len, nb - 1).n;
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
     if (SPLIT && level == 0 && tid == 0) a.part_n[item] = 0;
     return;
   }
-  const int t0 = wk.t0, len = wk.len, prior = wk.prior;
+  const int t0 = wk.t0, len = wk.len, prior = max(wk.prior, 0);
   const int q0 = wk.qb * BQ;
   const int nk = prior + len;                 // keys of this run
   const int pos_lo = prior + q0;              // first query position

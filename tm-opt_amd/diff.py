@@ -62,15 +62,16 @@ def _pools(k_pool, v_pool, HQ, D, dev):
 
 
 def _table(block_table, rows, dev):
-    """The row width of a block table (the stride: the kernels bound every
-    row read by it, so rows must be whole)."""
+    """The row width of a block table, which is the stride that the kernels
+    bound every row read by (so rows must be whole; one row may be part of a
+    wider one)."""
     have, width = block_table.shape
     stride = block_table.stride()
     assert block_table.dtype == _I32 and block_table.device == dev
     assert have >= rows and stride[1] == 1
     assert stride[0] == width or rows <= 1, \
         "block-table rows must be whole (the row width is the stride)"
-    return stride[0]
+    return width
 
 
 @functools.lru_cache(maxsize=1024)
