@@ -150,7 +150,7 @@ def load(path=None):
 
 def call(name, *args):
     """Invoke an int-returning entry point; raise TmoptError on failure."""
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != TMOPT_OK:
         msg = lib.tmopt_last_error().decode(errors="replace")
