@@ -91,6 +91,20 @@ __device__ __forceinline__ Tiles item_tiles(const PrefillDiffArgs& a, int BQ,
   return Tiles{k_lo, (prior + min(len, q0 + BQ) - k_lo + kBN - 1) / kBN};
 }
 
+// Work item x of a launch that splits its keys, in the order that schedule()
+// takes: its items are numbered without gaps, head pairs first, so that the
+// pieces of few items spread over all XCDs (item, then level, is dealt to them
+// in turn). Without splits each pair of stored heads keeps to XCDs of its own.
+__device__ __forceinline__ int split_item(int pairs, int x) {
+  const int kvh = x % pairs, i = x / pairs;
+  if (pairs <= 8 && 8 % pairs == 0) {
+    const int r = 8 / pairs;
+    return 8 * (i / r) + kvh * r + i % r;
+  }
+  if (pairs % 8 == 0) return 8 * (i * (pairs / 8) + kvh / 8) + kvh % 8;
+  return x;
+}
+
 // Split keys: a launch of few items, or of few more than there are compute
 // units, leaves units idle while its longest items run. It cuts each item's
 // tiles into pieces, one work-group each (level s of the grid holds piece s of
@@ -100,12 +114,13 @@ __device__ __forceinline__ Tiles item_tiles(const PrefillDiffArgs& a, int BQ,
 // are quickest, others their share. The estimate, in us: items are taken as
 // evenly spread between `low` and `most` tiles, heaviest first, one work-group
 // per compute unit; a tile takes 1.05 on up to half the units and 1.4 on all
-// (power: 2.1 against 1.6 GHz); pieces cost 5 for their start and the merge,
-// and 0.115 each for what they write and the merge reads.
+// (power: 2.1 against 1.6 GHz); pieces cost 5 for their start and the merge, 0.1
+// for each of an item's that it joins, and 0.115 for each of the launch's that
+// is written and read, if all its rows are queries.
 constexpr int kMinPiece = 4;   // tiles
 __device__ __forceinline__ int pieces_of(const PrefillDiffArgs& a, int BQ,
                                          int lane, int tiles) {
-  int sum = 0, most = 0, items = 0;
+  int sum = 0, most = 0, items = 0, rows = 0;
   for (int s = lane; s < a.S; s += 64) {
     const int len = a.cu[s + 1] - a.cu[s];
     const int nb = (len + BQ - 1) / BQ;
@@ -116,6 +131,7 @@ __device__ __forceinline__ int pieces_of(const PrefillDiffArgs& a, int BQ,
       sum += nb * (t0 + t1) / 2;
       most = max(most, max(t0, t1));
       items += nb;
+      rows += len;
     }
   }
   for (int x = 1; x < 64; x <<= 1) most = max(most, __shfl_xor(most, x));
@@ -126,6 +142,8 @@ __device__ __forceinline__ int pieces_of(const PrefillDiffArgs& a, int BQ,
       (float)__builtin_amdgcn_readfirstlane(wave_sum(sum)) / count;
   const float low = fmaxf(0.0f, 2.0f * mean - most);
   const float all = (float)count * a.HKV;
+  const float full =
+      (float)__builtin_amdgcn_readfirstlane(wave_sum(rows)) / (count * BQ);
   float best = 0.0f;
   int n = 1;
   for (int x = 1; x <= a.nsplit; ++x) {
@@ -134,7 +152,7 @@ __device__ __forceinline__ int pieces_of(const PrefillDiffArgs& a, int BQ,
                        (most - low) * fmaxf(1.0f, 0.5f * load)) / x;
     const float us =
         len * (0.7f + 0.7f * fminf(fmaxf(load, 0.5f), 1.0f)) +
-        (x > 1 ? 5.0f + 0.115f * x * all : 0.0f);
+        (x > 1 ? 5.0f + 0.1f * x + 0.115f * full * x * all : 0.0f);
     if (x == 1 || us < best) {
       best = us;
       n = x;
@@ -156,7 +174,8 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
   const int h2 = lane >> 5;       // lane half
   const int level = SPLIT ? (int)blockIdx.x / a.n_base : 0;
   const int item = (int)blockIdx.x - level * a.n_base;
-  const Work wk = schedule(a, BQ, lane, item);
+  const Work wk =
+      schedule(a, BQ, lane, SPLIT ? split_item(a.HKV, item) : item);
   if (wk.seq < 0) {
     if (SPLIT && level == 0 && tid == 0) a.part_n[item] = 0;
     return;
@@ -495,12 +514,12 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
     float* const po = a.part_o + (pw * 32 * 64 + lane) * 4;
     if (qok)
 #pragma unroll
-    for (int db = 0; db < 8; ++db)
+      for (int db = 0; db < 8; ++db)
 #pragma unroll
-      for (int g4 = 0; g4 < 4; ++g4)
-        *reinterpret_cast<f32x4*>(po + (4 * db + g4) * 256) =
-            f32x4{o_acc[db][4 * g4] * inv, o_acc[db][4 * g4 + 1] * inv,
-                  o_acc[db][4 * g4 + 2] * inv, o_acc[db][4 * g4 + 3] * inv};
+        for (int g4 = 0; g4 < 4; ++g4)
+          *reinterpret_cast<f32x4*>(po + (4 * db + g4) * 256) =
+              f32x4{o_acc[db][4 * g4] * inv, o_acc[db][4 * g4 + 1] * inv,
+                    o_acc[db][4 * g4 + 2] * inv, o_acc[db][4 * g4 + 3] * inv};
     if (h2 == 0)
       a.part_lse[pw * 32 + l32] =
           rejected ? __builtin_nanf("") :
@@ -586,36 +605,51 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
   }
 }
 
-// Join the pieces of the items that were split: grid (n_base, 16), a work-group
-// per 8 query rows of both maps. Thread t has row t & 7 and dims 8 (t >> 3) ..
-// +7 of both, so the difference is its own and the norm one sum over threads;
-// four pieces' loads in flight at a time, joined in piece order.
-template <int REP>
-__global__ __launch_bounds__(256) void prefill_diff_merge(PrefillDiffArgs a) {
-  constexpr int BQ = 128 / REP, QSUB = BQ / 32;
+// Join the pieces of the items that were split, in a fixed order: grid (n_base,
+// 16), a work-group per 8 query rows of both maps. Thread t of a group of 256
+// has row t & 7 and dims 8 (t >> 3) .. +7 of both, so the difference is its own
+// and the norm one sum over threads. Group s of S takes pieces s, s + S, ...,
+// four pieces' loads in flight at a time; the groups' results then join through
+// LDS in order.
+template <int REP, int S>
+__global__ __launch_bounds__(256 * S) void prefill_diff_merge(
+    PrefillDiffArgs a) {
+  constexpr int BQ = 128 / REP, QSUB = BQ / 32, kBatch = 4;
   __shared__ float sums[4][8];
+  __shared__ float part[S > 1 ? S - 1 : 1][20][S > 1 ? 256 : 1];
   const int np = min(as_const(a.part_n)[blockIdx.x], a.nsplit);
   if (np <= 1) return;                        // no item, or written in place
   const int lane = threadIdx.x & 63;
-  const int w = threadIdx.x >> 6;
-  const Work wk = schedule(a, BQ, lane, blockIdx.x);
+  const int tid = threadIdx.x & 255, w = tid >> 6;
+  const int group = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8);
+  const Work wk =
+      schedule(a, BQ, lane, split_item(a.HKV, (int)blockIdx.x));
   const int rb = blockIdx.y >> 2;             // 32-row block of the item
-  const int l32 = 8 * (blockIdx.y & 3) + (threadIdx.x & 7);
-  const int c = threadIdx.x >> 3;             // 8-dim chunk
+  const int l32 = 8 * (blockIdx.y & 3) + (tid & 7);
+  const int c = tid >> 3;                     // 8-dim chunk
   const int row0 = wk.qb * BQ + 32 * (rb % QSUB) + 8 * (blockIdx.y & 3);
   if (row0 >= wk.len) return;
-  const int qi = row0 + (threadIdx.x & 7);
+  const int qi = row0 + (tid & 7);
   const int hp = wk.kvh * REP + rb / QSUB;
   float m[2] = {-INFINITY, -INFINITY}, sum[2] = {0, 0};
   f32x4 acc[2][2] = {};
-  constexpr int kBatch = 4;
-  for (int s0 = 0; s0 < np; s0 += kBatch) {
+  auto add = [&](int i, float l, float w1, const f32x4 (&o)[2]) {
+    const float m_new = fmaxf(m[i], l);
+    const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+    const float keep = fast_exp2((m[i] - m_use) * kLog2e);
+    const float wt = fast_exp2((l - m_use) * kLog2e);
+    sum[i] = sum[i] * keep + wt * w1;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) acc[i][x] = acc[i][x] * keep + o[x] * wt;
+    m[i] = m_new;
+  };
+  for (int s0 = group; qi < wk.len && s0 < np; s0 += kBatch * S) {
     float l[kBatch][2];
     f32x4 o[kBatch][2][2];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       const int64_t slot =
-          (int64_t)min(s0 + j, np - 1) * a.n_base + blockIdx.x;
+          (int64_t)min(s0 + j * S, np - 1) * a.n_base + blockIdx.x;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int64_t pw = slot * 8 + 4 * i + rb;
@@ -626,26 +660,40 @@ __global__ __launch_bounds__(256) void prefill_diff_merge(PrefillDiffArgs a) {
               a.part_o + ((pw * 32 + c) * 64 + 32 * x + l32) * 4);
       }
     }
+    __builtin_amdgcn_sched_barrier(0);   // (all of them, before the first use)
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      if (s0 + j >= np) break;
+      if (s0 + j * S >= np) break;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) add(i, l[j][i], 1.0f, o[j][i]);
+    }
+  }
+  if constexpr (S > 1) {
+    if (group > 0) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float m_new = fmaxf(m[i], l[j][i]);
-        const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-        const float keep = fast_exp2((m[i] - m_use) * kLog2e);
-        const float wt = fast_exp2((l[j][i] - m_use) * kLog2e);
-        sum[i] = sum[i] * keep + wt;
+        part[group - 1][10 * i][tid] = m[i];
+        part[group - 1][10 * i + 1][tid] = sum[i];
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-          acc[i][x] = acc[i][x] * keep + o[j][i][x] * wt;
-        m[i] = m_new;
+        for (int e = 0; e < 8; ++e)
+          part[group - 1][10 * i + 2 + e][tid] = acc[i][e >> 2][e & 3];
       }
     }
+    __syncthreads();
+    if (group == 0)
+      for (int g = 0; g + 1 < min(np, S); ++g)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          f32x4 o[2];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            o[e >> 2][e & 3] = part[g][10 * i + 2 + e][tid];
+          add(i, part[g][10 * i][tid], part[g][10 * i + 1][tid], o);
+        }
   }
   // (a rejected launch's pieces are NaN, and so are their sums)
   const bool rejected = a.reject != nullptr && as_const(a.reject)[0] != 0;
-  const bool qok = qi < wk.len;
+  const bool qok = group == 0 && qi < wk.len;
   if (a.lse && c < 2 && qok)
     a.lse[(2 * hp + c) * a.lse_sh + wk.t0 + qi] =
         rejected ? __builtin_nanf("") :
@@ -666,9 +714,9 @@ __global__ __launch_bounds__(256) void prefill_diff_merge(PrefillDiffArgs a) {
   if (a.w.weight) {
     ss += __shfl_xor(ss, 8);
     ss = lane_pair(lane_pair(ss, 16, false), 32, false);
-    if (lane < 8) sums[w][lane] = ss;
+    if (group == 0 && lane < 8) sums[w][lane] = ss;
     __syncthreads();
-    const int q = threadIdx.x & 7;
+    const int q = tid & 7;
     ss = (sums[0][q] + sums[1][q]) + (sums[2][q] + sums[3][q]);
     f *= __builtin_amdgcn_rsqf(ss * (1.0f / kDV) + a.w.eps);
   }
@@ -695,29 +743,37 @@ int64_t level_wgs(int pairs, int BQ, int64_t S, int max_seqlen) {
   return pairs * items;
 }
 
-// Levels of a launch (1: keys are not split), from what the host knows: the
-// longest run, and the row width of a block table or the window as bounds of
-// its keys. Up to half the compute units' worth of items, as many pieces as
-// there are units; up to one and a half, two or three pieces an item even out
-// the rounds; larger grids fill the chip by themselves. The device decides from
-// the lengths.
-int split_levels(int64_t n_base, int BQ, int max_seqlen, int64_t bt_stride,
-                 int window) {
+// How a launch is laid out: levels (1: keys are not split) of n_base
+// work-groups each, from what the host knows: the longest run, and the row
+// width of a block table or the window as bounds of its keys. Up to half the
+// compute units' worth of items, as many pieces as there are units; up to one
+// and a half, two or three pieces an item even out the rounds; larger grids
+// fill the chip by themselves. The device decides from the lengths.
+struct Layout {
+  int levels;
+  int64_t n_base;
+};
+Layout layout_of(int pairs, int BQ, int64_t S, int max_seqlen,
+                 int64_t bt_stride, int window) {
   const int64_t cus = device_cus();
+  const int64_t items = S * ((max_seqlen + BQ - 1) / BQ) * pairs;
   int64_t keys = bt_stride > 0 ? bt_stride * kPage : max_seqlen;
   if (window > 0 && keys > (int64_t)window + BQ + kBN)
     keys = (int64_t)window + BQ + kBN;
   const int64_t tiles = (keys + kBN - 1) / kBN;
-  int64_t n = (2 * n_base <= cus ? cus : 3 * cus) / n_base;
+  int64_t n = (2 * items <= cus ? cus : 3 * cus) / items;
   if (n > 64) n = 64;
-  // a piece costs kPieceUs, so the tiles it saves must be worth that
+  // a piece costs some 5 tiles' time, so it must have more than that
   if (n > tiles / 8) n = tiles / 8;
-  return n < 2 || tiles < 32 ? 1 : (int)n;
+  if (n < 2 || tiles < 32)
+    return Layout{1, level_wgs(pairs, BQ, S, max_seqlen)};
+  return Layout{(int)n, items};
 }
 
 constexpr int64_t kSlotBytes = (int64_t)8 * 32 * (kDV + 1) * sizeof(float);
-int64_t workspace_bytes_of(int levels, int64_t n_base) {
-  return levels * n_base * kSlotBytes + ((n_base * 4 + 15) & ~(int64_t)15);
+int64_t workspace_bytes_of(const Layout& x) {
+  if (x.levels <= 1) return 0;
+  return x.levels * x.n_base * kSlotBytes + ((x.n_base * 4 + 15) & ~(int64_t)15);
 }
 
 // Head pairs per work-group: the largest of 4, 2, 1 dividing HQ / HKV; a larger
@@ -741,8 +797,14 @@ int launch(const PrefillDiffArgs& a, hipStream_t st) {
   else launch_source<REP, false>(a, st);
   const int rc = check_launch("prefill_diff");
   if (rc || a.nsplit <= 1) return rc;
-  hipLaunchKernelGGL((prefill_diff_merge<REP>), dim3(a.n_base, 16), dim3(256),
-                     0, st, a);
+  // many pieces of few items: four groups (3 queries after 22,000, 16Q/2KV, 58 us
+  // a call with one and the pieces of an item on one XCD, 48 so)
+  if (a.nsplit > 8)
+    hipLaunchKernelGGL((prefill_diff_merge<REP, 4>), dim3(a.n_base, 16),
+                       dim3(1024), 0, st, a);
+  else
+    hipLaunchKernelGGL((prefill_diff_merge<REP, 1>), dim3(a.n_base, 16),
+                       dim3(256), 0, st, a);
   return check_launch("prefill_diff_merge");
 }
 
@@ -758,9 +820,8 @@ extern "C" size_t tmopt_attn_prefill_diff_workspace_size(
       HKV % 2 != 0 || HQ % HKV != 0)
     return 0;
   const int rep = group_of(HQ / HKV), BQ = 128 / rep;
-  const int64_t n = level_wgs(HQ / 2 / rep, BQ, num_seqs, max_seqlen_q);
-  const int levels = split_levels(n, BQ, max_seqlen_q, bt_stride, window);
-  return levels > 1 ? (size_t)workspace_bytes_of(levels, n) : 0;
+  return (size_t)workspace_bytes_of(
+      layout_of(HQ / 2 / rep, BQ, num_seqs, max_seqlen_q, bt_stride, window));
 }
 
 extern "C" int tmopt_attn_prefill_diff(
@@ -823,17 +884,16 @@ extern "C" int tmopt_attn_prefill_diff(
                   "prefill_diff: a run's k/v span must stay below 2 GiB");
   }
   const int rep = group_of(HQ / HKV), pairs = HQ / 2 / rep, BQ = 128 / rep;
-  const int64_t n = level_wgs(pairs, BQ, num_seqs, max_seqlen_q);
-  TMOPT_REQUIRE(n < 0x7fffffff, TMOPT_EUNSUPPORTED,
+  Layout x = layout_of(pairs, BQ, num_seqs, max_seqlen_q,
+                       paged ? bt_stride : 0, window);
+  if (workspace == nullptr)
+    x = Layout{1, level_wgs(pairs, BQ, num_seqs, max_seqlen_q)};
+  TMOPT_REQUIRE(x.n_base < 0x7fffffff, TMOPT_EUNSUPPORTED,
                 "prefill_diff: %lld work-groups exceed the grid limit",
-                (long long)n);
-  const int levels = workspace == nullptr
-                         ? 1
-                         : split_levels(n, BQ, max_seqlen_q,
-                                        paged ? bt_stride : 0, window);
-  const int64_t need = workspace_bytes_of(levels, n);
-  TMOPT_REQUIRE(levels <= 1 || ((int64_t)workspace_bytes >= need &&
-                                (uintptr_t)workspace % 16 == 0),
+                (long long)x.n_base);
+  const int64_t need = workspace_bytes_of(x);
+  TMOPT_REQUIRE(need == 0 || ((int64_t)workspace_bytes >= need &&
+                              (uintptr_t)workspace % 16 == 0),
                 TMOPT_EWORKSPACE,
                 "prefill_diff: workspace %zu bytes < %lld needed (or unaligned)",
                 workspace_bytes, (long long)need);
@@ -867,12 +927,13 @@ extern "C" int tmopt_attn_prefill_diff(
   a.lse = lse;
   a.lse_sh = lse_stride_head;
   a.reject = reject;
-  a.nsplit = levels;
-  a.n_base = (int)n;
+  a.nsplit = x.levels;
+  a.n_base = (int)x.n_base;
   a.cus = device_cus();
+  const int64_t slots = x.levels * x.n_base;
   a.part_o = (float*)workspace;
-  a.part_lse = a.part_o + levels * n * 8 * 32 * kDV;
-  a.part_n = (int*)(a.part_lse + levels * n * 8 * 32);
+  a.part_lse = a.part_o + slots * 8 * 32 * kDV;
+  a.part_n = (int*)(a.part_lse + slots * 8 * 32);
   const hipStream_t st = (hipStream_t)stream;
   if (rep == 4) return launch<4>(a, st);
   if (rep == 2) return launch<2>(a, st);
