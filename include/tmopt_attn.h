@@ -489,7 +489,7 @@ int tmopt_prefill_check_positions(const int64_t* q_positions,
  *         - lam_h softmax(scale q_2h+1 K_2g+1^T) V_g
  *   out_h = O_h / sqrt(mean(O_h^2) + norm_eps) * norm_weight * out_scale
  * (norm_weight NULL: out_h = O_h * out_scale). The caches and pools are those
- * of the other entry points; HKV is even, HQ a multiple of it.
+ * of the other entry points; HKV is even, HQ a multiple of it, at most 131072.
  * lam:          fp32, one value per pair (lam_stride 1) or one for all
  *               (lam_stride 0).
  * norm_weight:  fp32 [256], 16-byte aligned; norm_eps > 0 with it.
@@ -527,8 +527,13 @@ int tmopt_attn_decode_diff(const void* q, const void* k_pool,
  *         cu_seqlens_q (strides % 8, D contiguous); prior_lens NULL;
  *   block_table != NULL, k == v == NULL: every key from k_pool / v_pool
  *         [num_pages, page_size, HKV, D] through block_table [num_seqs,
- *         bt_stride], the runs' own rows already written. Pages past the row
- *         width or outside the pool read as zeros.
+ *         bt_stride], the runs' own rows already written; prior_lens >= 0 or
+ *         NULL (none). Pages past the row width or outside the pool read as
+ *         zeros; rows past a run's end, and pages before the first key that
+ *         some query of a block sees, are never read.
+ * A block of up to 128 consecutive queries multiplies the values of every
+ * tile of 32 keys that one of them sees, with weight zero where a query does
+ * not: those value rows must be finite. Keys need not be.
  * out: [total, HQ / 2, 2 D] with element strides (% 8, 16-byte aligned), the
  * 2 D contiguous; lse fp32 [HQ, total] rows of lse_stride_head elements, or
  * NULL. Rows past the last run are left as they were.
@@ -549,8 +554,8 @@ int tmopt_attn_prefill_diff(
     int D, int window, float scale, const float* lam, int lam_stride,
     const float* norm_weight, float norm_eps, float out_scale, void* out,
     int64_t o_stride_tok, int64_t o_stride_head, float* lse,
-    int64_t lse_stride_head, const int32_t* reject, void* workspace, size_t workspace_bytes,
-    tmopt_stream_t stream);
+    int64_t lse_stride_head, const int32_t* reject, void* workspace,
+    size_t workspace_bytes, tmopt_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
 /* Page plan of a serving step                                              */

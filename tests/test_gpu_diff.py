@@ -120,6 +120,17 @@ def test_decode_ring(tm, dev, window):
             min_pages=2)
 
 
+@pytest.mark.parametrize("window,wrap", [(40, 4), (64, 4), (1, 1)])
+def test_decode_ring_at_the_last_positions(tm, dev, window, wrap):
+    """A ring's positions may come up to what int32 holds."""
+    g = _gen(21)
+    ends = [2 ** 31 - 1, 2 ** 31 - 16, 2 ** 31 - 17, 5]
+    c = Cache(ends, 4, g, dev, first=[max(0, n - window) for n in ends],
+              wrap=wrap)
+    _decode(tm, c, _rand((4, 16, D), g, dev), 0.1, _weights(16, g, dev),
+            window=window, wrap=wrap)
+
+
 def test_decode_absent_pages(tm, dev):
     """Entries outside the pool and positions past the row's width count as
     absent; a request that has no other page gives zeros."""
@@ -555,3 +566,113 @@ def test_serving_steps_together(tm, dev, window):
     assert bad.item() == 0
     step([3, 1], [150, 1])
     step([3, 0, 1], [1, 1, 1])
+
+
+@pytest.mark.parametrize("bad", [NAN, float("inf"), -float("inf")])
+@pytest.mark.parametrize("hq,hkv", [(16, 4), (4, 4)])
+def test_prefill_keys_that_are_no_numbers(tm, dev, hq, hkv, bad):
+    """A key that a query does not see, by causality or by the window, may
+    hold anything."""
+    g = _gen(19)
+    n, at, window = 150, 40, 32
+    w = _weights(hq, g, dev)
+    kw = {k: v for k, v in w.items() if k != "lam"}
+    q = _rand((n, hq, D), g, dev)
+    k, v = _rand((n, hkv, D), g, dev), _rand((n, hkv, D), g, dev)
+    k[at] = bad
+    cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+    pos = torch.arange(n, device=dev)
+    good = k.clone()
+    good[at] = 0
+    for win in (0, window):
+        out, lse = tm.prefill_diff_varlen(
+            q, k, v, cu, w["lam"], 0.1, window=win, max_seqlen=n,
+            **{x: y for x, y in _user(w).items() if x != "lam"})
+        for rows in [slice(0, at)] + ([slice(at + win, n)] if win else []):
+            ref = diff_ref.attend(q[rows], good, v, pos[rows], pos, w["lam"],
+                                  0.1, window=win, **kw)
+            diff_ref.check(out[rows], lse[:, rows], ref, f"{win} {rows}")
+
+
+def test_decode_step_in_a_graph(tm, dev):
+    """Plan, KV write and attention of a decode step as one graph: each replay
+    goes on from where the last one was, takes pages as the requests reach
+    them, and from the first step without a page on changes nothing."""
+    g = _gen(20)
+    hq, hkv, S, W, lens = 16, 4, 5, 8, [14, 16, 45]
+    B = len(lens) + 1                       # the last row is padding
+    w = _weights(hq, g, dev)
+    kw = {k: v for k, v in _user(w).items() if k != "lam"}
+    kp = torch.full((24, PAGE, hkv, D), NAN, dtype=BF, device=dev)
+    vp = torch.full_like(kp, NAN)
+    pt = torch.full((S, W), -1, dtype=torch.int32, device=dev)
+    free = torch.randperm(11, generator=g).int().to(dev)
+    count = torch.tensor([11], dtype=torch.int32, device=dev)
+    slots = torch.tensor([4, 0, 2, -1], device=dev)
+    T = sum(lens)
+    K, V = _rand((T, hkv, D), g, dev), _rand((T, hkv, D), g, dev)
+    p = tm.plan_pages(pt, slots, torch.zeros(B, dtype=torch.int32, device=dev),
+                      torch.tensor(lens + [0], dtype=torch.int32, device=dev),
+                      free, count, T)
+    tm.kv_write_slots(K, V, p.slot_mapping, kp, vp)
+    seen = [(a, b) for a, b in zip(K.split(lens), V.split(lens))]
+    count.copy_(p.free_count)
+    ctx, one = p.seq_lens.clone(), torch.ones(B, dtype=torch.int32, device=dev)
+    q = torch.zeros((B, hq, D), dtype=BF, device=dev)
+    k = torch.zeros((B, hkv, D), dtype=BF, device=dev)
+    v = torch.zeros_like(k)
+    plan = tm.plan_pages(pt, slots, ctx, torch.zeros_like(one), free, count, B)
+    plan = plan._replace(seq_lens=ctx, free_count=count)
+
+    def step():
+        tm.plan_pages(pt, slots, ctx, one, free, count, B, out=plan)
+        tm.kv_write_slots(k, v, plan.slot_mapping, kp, vp)
+        return tm.decode_diff_paged(q, kp, vp, plan.block_table,
+                                    plan.seq_lens, w["lam"], 0.1, **kw)
+
+    def refill():
+        for x in (q, k, v):
+            x.copy_(_rand(x.shape, g, dev))
+
+    def check(res, what):
+        assert plan.reject.item() == 0 and count.item() >= 0
+        for i in range(B - 1):
+            seen[i] = tuple(torch.cat([o, x[i:i + 1]])
+                            for o, x in zip(seen[i], (k, v)))
+            n = seen[i][0].shape[0]
+            assert ctx[i].item() == n
+            pos = torch.arange(n, device=dev)
+            ref = diff_ref.attend(
+                q[i:i + 1], *seen[i], pos[n - 1:], pos, w["lam"], 0.1,
+                **{x: y for x, y in w.items() if x != "lam"})
+            diff_ref.check(res[0][i:i + 1], res[1][i:i + 1].T, ref,
+                           f"{what} {i}")
+        assert (res[0][B - 1] == 0).all()
+        assert (res[1][B - 1] == -float("inf")).all()
+
+    refill()
+    check(step(), "eager")                  # (and the warm-up)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        res = step()
+    # five of the eleven pages are taken at first, the last one at step 20; the
+    # second request's 49th token, at step 33, finds none
+    while True:
+        need = sum(s[0].shape[0] % PAGE == 0 for s in seen)
+        refill()
+        before = count.item(), ctx.tolist(), pt.tolist()
+        have = kp.clone()
+        gr.replay()
+        torch.cuda.synchronize()
+        if need > before[0]:
+            break
+        check(res, f"replay at {ctx.tolist()}")
+    assert before[0] == 0 and len(seen[1][0]) == 48
+    for _ in range(2):                      # refused: nothing has changed
+        assert plan.reject.item() == 1
+        assert (count.item(), ctx.tolist(), pt.tolist()) == before
+        assert torch.equal(kp.isnan(), have.isnan())
+        assert torch.equal(kp.nan_to_num(), have.nan_to_num())
+        assert (plan.block_table == -1).all() and (res[0] == 0).all()
+        gr.replay()
+        torch.cuda.synchronize()

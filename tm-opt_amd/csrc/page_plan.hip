@@ -19,7 +19,10 @@
 // of the inputs (a graph that steps on in place), or above 1024 requests, one
 // work-group makes the sums and the new pages, and a second launch the rest;
 // a small step in place is one work-group's. Bound by latency: launches and
-// dependent loads.
+// dependent loads. Graph replays, us a step, where an empty kernel takes 2.1: 4
+// decode rows 3.5, 64 rows 3.8, 96 rows and 2 chunks of 2048 tokens under tables
+// of 4,224 pages 6.4; a release of one row of 500 pages 2.9, of 64 rows of up to
+// 4,096 3.5.
 #include "common.h"
 
 namespace tmopt {
@@ -316,7 +319,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_sums_kernel(PlanArgs a) {
   }
 }
 
-// the rest: work-groups [0, B * per) the block table, 1024 entries of a row each, the others 1024 tokens each
+// the rest: work-groups [0, B * per) the block table, 1024 entries of a row
+// each, the others 1024 tokens each
 __global__ __launch_bounds__(kFillThreads) void plan_fill_kernel(PlanArgs a,
                                                                  int per) {
   extern __shared__ int cu[];
