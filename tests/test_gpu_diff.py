@@ -676,3 +676,24 @@ def test_decode_step_in_a_graph(tm, dev):
         assert (plan.block_table == -1).all() and (res[0] == 0).all()
         gr.replay()
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("B,hq,hkv,wgs,norm", [
+    (128, 32, 4, 0, True), (192, 8, 4, 0, True), (193, 8, 2, 0, False),
+    (700, 8, 4, 0, True), (64, 64, 16, 0, True), (63, 64, 16, 0, True),
+    (97, 64, 16, 0, False), (50, 16, 4, 7, True), (50, 16, 4, 50, True),
+    (33, 16, 8, 11, True)])
+def test_decode_short_requests(tm, dev, B, hq, hkv, wgs, norm):
+    """Batches of short requests: whole ones per range, several per range, and
+    what a range's neighbours share."""
+    g = _gen(22)
+    ends = torch.randint(0, 200, (B,), generator=g).tolist()
+    ends[B // 2] = 0
+    ends[-1] = 1
+    c = Cache(ends, hkv, g, dev)
+    _decode(tm, c, _rand((B, hq, D), g, dev), 0.1,
+            _weights(hq, g, dev, norm=norm), num_workgroups=wgs)
+    even = [199] * B                        # no request longer than another
+    c = Cache(even, hkv, g, dev)
+    _decode(tm, c, _rand((B, hq, D), g, dev), 0.1,
+            _weights(hq, g, dev, norm=norm), num_workgroups=wgs, window=150)

@@ -37,6 +37,8 @@
 // 3.1 TB/s: its walk runs at 7.3 TB/s, 5 us go to the start, 8 to the merge of
 // its 184 pieces; 4 of 128-1024 tokens 14.1 in a graph, 17.5 eagerly: two
 // launches and their chains of dependent loads.
+#include <algorithm>
+
 #include "diff.h"
 
 namespace tmopt {
@@ -48,7 +50,7 @@ constexpr int kStageB = 4 * kSliceB;       // K, K', V, V' of a page
 constexpr int kWaveLds = 2 * kStageB + 16 * kRowB;   // two stages, query rows
 constexpr int kWaves = 4;
 constexpr int kMaxB = 8192;                // prefix table lives in LDS
-constexpr int kIds = 4000;                 // page ids kept in LDS, all ranges
+constexpr int kIds = 3744;                 // page ids kept in LDS, all ranges
 
 struct DecodeDiffArgs {
   const __bf16* q;
@@ -74,7 +76,7 @@ struct DecodeDiffArgs {
   float* part_o;     // [B + R, HQ, 256] fp32, R ranges
   float* part_lse;   // [B + R, HQ]
   int* geo;          // [B + 2]: pages per range, then the page prefix
-  int ids_off;       // LDS byte offset of the page ids
+  int ids_off;       // LDS byte offset of the norm's weights, then the page ids
 };
 
 __device__ __forceinline__ int vis_lo(int n, int window) {
@@ -162,16 +164,21 @@ void decode_diff_kernel(DecodeDiffArgs a) {
   int* wsum = pref + a.B + 1;                // [4] sums, [4] maxima
   int* nlen = wsum + 2 * kWaves;             // [B]
   const int ids_cap = kIds / subs;
-  int* ids = reinterpret_cast<int*>(smem + a.ids_off) + v * (ids_cap + 2);
+  int* ids = reinterpret_cast<int*>(smem + a.ids_off) + kDV + v * (ids_cap + 2);
+  const uint32_t lds_wt =
+      (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)smem) +
+      a.ids_off;
 
   // ---- 1. prefix sums of visible pages: pref[b] = first page of request b --
   const int width = a.table_wrap > 0 ? 0x7fffffff : a.bt_width;
   int most = 0;   // pages of the longest request
   {
     int carry = 0;
+    int next = (int)threadIdx.x < a.B ? a.ctx_lens[threadIdx.x] : 0;
     for (int b0 = 0; b0 < a.B; b0 += 64 * kWaves) {
       const int b = b0 + threadIdx.x;
-      const int nb = b < a.B ? as_const(a.ctx_lens)[b] : 0;
+      const int nb = next;
+      next = b + 64 * kWaves < a.B ? a.ctx_lens[b + 64 * kWaves] : 0;
       if (b < a.B) nlen[b] = nb;
       const int np = vis_pages(nb, a.window, width);
       most = max(most, np);
@@ -191,6 +198,16 @@ void decode_diff_kernel(DecodeDiffArgs a) {
     for (int j = 0; j < kWaves; ++j) most = max(most, wsum[kWaves + j]);
     most = __builtin_amdgcn_readfirstlane(most);
   }
+  // What the end of a piece needs is here before the walk: a load there would
+  // wait for every page on its way.
+  const int col_h = r & 7;                        // head pair of the column
+  const bool col_ok = col_h < a.rep;
+  float lam = a.w.lam[(int64_t)(pair * a.rep + min(col_h, a.rep - 1)) *
+                      a.w.lam_stride];
+  const bool puts_wt = a.w.weight != nullptr && threadIdx.x < kDV / 4;
+  u32x4 wt{};
+  if (puts_wt)
+    wt = *reinterpret_cast<const u32x4*>(a.w.weight + 4 * threadIdx.x);
   const int U = __builtin_amdgcn_readfirstlane(pref[a.B]);
   int C = max((U + R - 1) / R, a.min_pages);
   // The merge takes a request's pieces in rounds of 64 (16 with two groups of
@@ -209,12 +226,30 @@ void decode_diff_kernel(DecodeDiffArgs a) {
       }
     }
   }
-  // Whole requests, the same number for every range, where the longest ones are
-  // no more than a sixteenth (and a page) above the even share: nothing is
-  // split, nothing joined (96 requests under a window of 512, 64Q/16KV: 76 us a
-  // call cut evenly, 70 whole).
+  // Whole requests, the same number for every range: nothing is split, nothing
+  // joined. Partial results and their merge cost some 1.5 us per 1000 rows (HQ of
+  // each request, of no more than there are ranges), a page above the even share
+  // 0.3 where two waves walk a range, 0.75 where one does; and up to a sixteenth
+  // more is within what an even share spreads. Graph replays, us, evenly / whole:
+  // 32Q/4KV 192 requests of 100-300 tokens 34.3 / 24.4, 128 up to 300 26.4 /
+  // 21.2, 180 of 500-800 57.8 / 50.0, 600 up to 200 61 / 45; 64Q/16KV 96 of
+  // 100-300 43.7 / 37.6, 96 under a window of 512 with contexts of 100-2000 73.8 /
+  // 64.3. What stays even would lose: 64 up to 300 19.9 / 21.9, 64 under a window
+  // of 512 27 / 32, 64Q/16KV 32 up to 300 21 / 30.
   const int per = (a.B + R - 1) / R;
-  const bool whole = (int64_t)per * most <= (int64_t)C + C / 16 + 1;
+  if (per > 1) {   // the pages of the heaviest range
+    most = 0;
+    for (int i = threadIdx.x * per; i < a.B; i += 64 * kWaves * per)
+      most = max(most, pref[min(i + per, a.B)] - pref[i]);
+    for (int x = 1; x < 64; x <<= 1) most = max(most, __shfl_xor(most, x));
+    __syncthreads();
+    if (lane == 0) wsum[w] = most;
+    __syncthreads();
+    for (int j = 0; j < kWaves; ++j) most = max(most, wsum[j]);
+    most = __builtin_amdgcn_readfirstlane(most);
+  }
+  const int slack = min(a.B, R) * a.HQ >> (halves > 1 ? 8 : 9);
+  const bool whole = most <= (int64_t)C + C / 16 + 1 + slack;
   // the range [r0, r1), and this wave's pages of it: [u0, u1), backward in the
   // second half
   int r0 = (int)min((int64_t)range * C, (int64_t)U);
@@ -234,8 +269,6 @@ void decode_diff_kernel(DecodeDiffArgs a) {
   const int u0 = half == 0 ? r0 : mid, u1 = half == 0 ? mid : r1;
   const bool back = half != 0;
   const int rep = a.rep;
-  const int col_h = r & 7;                        // head pair of the column
-  const bool col_ok = col_h < rep;
   const int hq = 2 * (pair * rep + col_h) + (r >> 3);   // query head
 
   // ---- 2. requests with no visible key: output 0, LSE -inf ---------------
@@ -272,6 +305,8 @@ void decode_diff_kernel(DecodeDiffArgs a) {
   int seq_end = seq_start + vis_pages(cur_n, a.window, width);
   int pg_of = vis_lo(cur_n, a.window) / kPage - seq_start;   // page of unit u
   int last_b = -1;  // request of the previous step handed out
+  if (puts_wt) lds_st128(lds_wt + 16 * threadIdx.x, wt);
+  asm volatile("" : "+v"(lam));   // (has arrived: no wait for it in the walk)
   __syncthreads();  // the ids are there; every wave is done with the tables
   const uint32_t ids0 =
       (uint32_t)(uintptr_t)((__attribute__((address_space(3))) int*)ids);
@@ -417,8 +452,6 @@ void decode_diff_kernel(DecodeDiffArgs a) {
     const ArgsPtr ra = rare_args();
     const int HQ = ra->HQ;
     if (flags & kWhole) {
-      const int h = pair * rep + min(col_h, rep - 1);
-      const float lam = ra->w.lam[(int64_t)h * ra->w.lam_stride];
       float ss = 0.0f;
 #pragma unroll
       for (int blk = 0; blk < 16; ++blk)
@@ -430,21 +463,28 @@ void decode_diff_kernel(DecodeDiffArgs a) {
           ss += d * d;
         }
       float f = ra->w.out_scale;
-      const float* const wt = ra->w.weight;
-      if (wt != nullptr) {
+      const bool norm = ra->w.weight != nullptr;
+      if (norm) {
         ss = lane_pair(lane_pair(ss, 16, false), 32, false);
         f *= __builtin_amdgcn_rsqf(ss * (1.0f / kDV) + ra->w.eps);
       }
-      if (col_ok && r < 8) {
-        __bf16* const o = ra->out + ((int64_t)b * (HQ / 2) + h) * kDV + 4 * g;
 #pragma unroll
-        for (int blk = 0; blk < 16; ++blk) {
-          f32x4 x = o_acc[blk] * f;
-          if (wt != nullptr)
-            x *= *reinterpret_cast<const f32x4*>(wt + 16 * blk + 4 * g);
+      for (int blk = 0; blk < 16; ++blk) o_acc[blk] = o_acc[blk] * f;
+      if (norm) {
+#pragma unroll
+        for (int blk = 0; blk < 16; ++blk)
+          o_acc[blk] *= __builtin_bit_cast(f32x4,
+                                           lds_ld128(lds_wt + 64 * blk + 16 * g));
+      }
+      if (col_ok && r < 8) {
+        __bf16* const o = ra->out +
+                          ((int64_t)b * (HQ / 2) + pair * rep + col_h) * kDV +
+                          4 * g;
+#pragma unroll
+        for (int blk = 0; blk < 16; ++blk)
           *reinterpret_cast<u32x2*>(o + 16 * blk) =
-              u32x2{pack_bf16x2_rn(x[0], x[1]), pack_bf16x2_rn(x[2], x[3])};
-        }
+              u32x2{pack_bf16x2_rn(o_acc[blk][0], o_acc[blk][1]),
+                    pack_bf16x2_rn(o_acc[blk][2], o_acc[blk][3])};
       }
       float* const lse = ra->lse;
       if (lse != nullptr && col_ok && g == 0)
@@ -581,6 +621,7 @@ void decode_diff_kernel(DecodeDiffArgs a) {
           end_flags = cur.flags;
         } else {
           finish_piece(cur.b, cur.flags);
+          asm volatile("" ::: "memory");   // (its stores come before any wait)
         }
       }
       cur = nx;
@@ -733,15 +774,24 @@ struct Shape {
   int rep, pairs, per_wg, G, R;   // R: ranges of the launch
 };
 // Three work-groups per four CUs, as the plain decode; four waves each, which
-// take 4, 2 or 1 pairs of stored heads of 1, 1 or 2 ranges.
-Shape shape_of(int HQ, int HKV, int num_workgroups) {
+// take 4, 2 or 1 pairs of stored heads of 1, 1 or 2 ranges. Four pairs where
+// there are requests for two thirds of their ranges, which then are likely
+// whole; else two, whose ranges two waves share (graph replays, us, by two / four:
+// 64Q/8KV 8 requests of 1K-8K 37.9 / 41.2, one of 50,000 46.0 / 49.8, 64 of
+// 100-1000 39.9 / 41.5; 64Q/16KV 32 up to 300 20.9 / 22.1, 96 up to 300 38.8 /
+// 37.6, 96 under a window of 512 68.5 / 64.1).
+Shape shape_of(int B, int HQ, int HKV, int num_workgroups) {
   Shape s;
   s.rep = group_of(HQ / HKV);
   s.pairs = HQ / 2 / s.rep;
-  s.per_wg = s.pairs % 4 == 0 ? 4 : s.pairs % 2 == 0 ? 2 : 1;
-  const int ny = s.pairs / s.per_wg;
-  s.G = num_workgroups > 0 ? num_workgroups : 3 * device_cus() / (4 * ny);
-  if (s.G < 1) s.G = 1;
+  auto groups = [&](int per_wg) {
+    const int ny = s.pairs / per_wg;
+    return std::max(1, num_workgroups > 0 ? num_workgroups
+                                          : 3 * device_cus() / (4 * ny));
+  };
+  s.per_wg = s.pairs % 2 == 0 ? 2 : 1;
+  if (s.pairs % 4 == 0 && B >= 2 * groups(4) / 3) s.per_wg = 4;
+  s.G = groups(s.per_wg);
   const int subs = kWaves / s.per_wg;
   s.R = s.G * (subs > 1 ? subs / 2 : 1);
   return s;
@@ -767,7 +817,7 @@ extern "C" size_t tmopt_attn_decode_diff_workspace_size(int B, int HQ, int HKV,
                                                         int num_workgroups) {
   (void)D;
   if (B <= 0 || HQ <= 0 || HKV <= 0 || HKV % 2 != 0 || HQ % HKV != 0) return 0;
-  return ws_layout(B, HQ, shape_of(HQ, HKV, num_workgroups).R, nullptr,
+  return ws_layout(B, HQ, shape_of(B, HQ, HKV, num_workgroups).R, nullptr,
                    nullptr);
 }
 
@@ -809,7 +859,7 @@ extern "C" int tmopt_attn_decode_diff(
   TMOPT_REQUIRE(((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool |
                  (uintptr_t)out) % 16 == 0,
                 TMOPT_EINVAL, "decode_diff: tensors must be 16-byte aligned");
-  const Shape s = shape_of(HQ, HKV, num_workgroups);
+  const Shape s = shape_of(B, HQ, HKV, num_workgroups);
   const int ny = s.pairs / s.per_wg;
   TMOPT_REQUIRE(ny <= 65535, TMOPT_EUNSUPPORTED,
                 "decode_diff: %d pairs of stored heads exceed the grid",
@@ -850,7 +900,7 @@ extern "C" int tmopt_attn_decode_diff(
       ((2 * (size_t)B + 1 + 2 * kWaves) * sizeof(int) + 15) & ~(size_t)15;
   const size_t tiles = (size_t)kWaves * kWaveLds;
   a.ids_off = (int)(tab > tiles ? tab : tiles);
-  const size_t lds = a.ids_off + (kIds + 2 * kWaves) * sizeof(int);
+  const size_t lds = a.ids_off + (kDV + kIds + 2 * kWaves) * sizeof(int);
   hipStream_t st = (hipStream_t)stream;
   hipLaunchKernelGGL(decode_diff_kernel, dim3(s.G, ny), dim3(64 * kWaves), lds,
                      st, a);
