@@ -636,6 +636,13 @@ __global__ __launch_bounds__(256 * S) void prefill_diff_merge(
   if (row0 >= wk.len) return;
   const int qi = row0 + (tid & 7);
   const int hp = wk.kvh * REP + rb / QSUB;
+  const float lam = a.w.lam[(int64_t)hp * a.w.lam_stride];
+  const bool norm = a.w.weight != nullptr;
+  f32x4 wt[2] = {};
+  if (norm) {
+    wt[0] = *reinterpret_cast<const f32x4*>(a.w.weight + 8 * c);
+    wt[1] = *reinterpret_cast<const f32x4*>(a.w.weight + 8 * c + 4);
+  }
   float m[2] = {-INFINITY, -INFINITY}, sum[2] = {0, 0};
   f32x4 acc[2][2] = {};
   auto add = [&](int i, float l, float w1, const f32x4 (&o)[2]) {
@@ -705,7 +712,6 @@ __global__ __launch_bounds__(256 * S) void prefill_diff_merge(
         sum[c] > 0.0f ? m[c] + fast_log2(sum[c]) * kLn2 : -INFINITY;
   const float inv0 = sum[0] > 0.0f ? 1.0f / sum[0] : 0.0f;
   const float inv1 = sum[1] > 0.0f ? 1.0f / sum[1] : 0.0f;
-  const float lam = a.w.lam[(int64_t)hp * a.w.lam_stride];
   float ss = 0.0f;
   f32x4 d[2];
 #pragma unroll
@@ -729,8 +735,7 @@ __global__ __launch_bounds__(256 * S) void prefill_diff_merge(
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     f32x4 z = d[x] * f;
-    if (a.w.weight)
-      z *= *reinterpret_cast<const f32x4*>(a.w.weight + 8 * c + 4 * x);
+    if (norm) z *= wt[x];
     y[2 * x] = pack_bf16x2_rn(z[0], z[1]);
     y[2 * x + 1] = pack_bf16x2_rn(z[2], z[3]);
   }
