@@ -19,8 +19,8 @@
 //    leaves a normalised fp32 result of both maps with their LSE;
 //    decode_diff_merge joins the pieces in order, then takes the difference and
 //    the norm. No atomics: repeated calls are bitwise equal.
-//  * A range belongs to two waves where there are fewer than four pairs of
-//    stored heads: the first walks its first half forward, the second its
+//  * A range belongs to two waves where a work-group has fewer than four pairs
+//    of stored heads: the first walks its first half forward, the second its
 //    second half backward, so that the request in the middle is the last of
 //    both, and they join it in LDS. A 256-wide fp32 row per map and piece is
 //    what the split costs, twice that of plain attention.
@@ -29,13 +29,14 @@
 //    a load is the page's rows that hold visible keys; other rows read as zeros
 //    and cost no traffic, so every step issues the same loads and the waits
 //    count exactly.
-//  * Page ids of a range are fetched before the walk into LDS.
+//  * Page ids of a range and the norm's weights are fetched into LDS before the
+//    walk: a load within it would wait for every page on its way.
 //
 // Us a call, the merge included (32Q/4KV with the norm unless said): 64 requests
-// of 1K-8K tokens 104.5, 5.8 TB/s (1.00 of the bytes fetched are the formula's);
+// of 1K-8K tokens 102.9, 5.9 TB/s (1.00 of the bytes fetched are the formula's);
 // 96 under a window of 512, 64Q/16KV, 66.0, 6.1 TB/s; one of 50,001 tokens 32.7,
 // 3.1 TB/s: its walk runs at 7.3 TB/s, 5 us go to the start, 8 to the merge of
-// its 184 pieces; 4 of 128-1024 tokens 14.1 in a graph, 17.5 eagerly: two
+// its 184 pieces; 4 of 128-1024 tokens 14.3 in a graph, 17.5 eagerly: two
 // launches and their chains of dependent loads.
 #include <algorithm>
 

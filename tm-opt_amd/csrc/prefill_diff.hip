@@ -24,7 +24,7 @@
 //    normalised O and takes the difference and the norm of the other half.
 //  * Work items are dealt to the XCDs heaviest first (prefill_sched.h).
 //
-// 4 prompts of 8,192 tokens run at 1,197 TFLOP/s, 4 of 2K-8K at 1,135 (32Q/4KV):
+// 4 prompts of 8,192 tokens run at 1,197 TFLOP/s, 4 of 2K-8K at 1,163 (32Q/4KV):
 // matrix cycles are 0.66 of all, at the 1.6 GHz that the power limit leaves a
 // full chip (a plain 8192^3 product 1,263 TFLOP/s at 1.75 GHz). There a tile is
 // 0.97 us of the matrix pipes and takes 1.4; an item's start and end cost some 9
