@@ -697,3 +697,28 @@ def test_decode_short_requests(tm, dev, B, hq, hkv, wgs, norm):
     c = Cache(even, hkv, g, dev)
     _decode(tm, c, _rand((B, hq, D), g, dev), 0.1,
             _weights(hq, g, dev, norm=norm), num_workgroups=wgs, window=150)
+
+
+@pytest.mark.parametrize("hq,hkv,window", [
+    (32, 4, 0), (32, 4, 40), (16, 8, 0), (12, 4, 70), (6, 2, 0), (24, 8, 33)])
+@pytest.mark.parametrize("paged", [False, True])
+def test_prefill_large_launches(tm, dev, hq, hkv, window, paged):
+    """More work-groups than the chip holds at once: the same edges as the
+    smaller launches."""
+    g = _gen(23)
+    lens = (RUNS[:-2] + [1, 95, 96, 97, 0, 17]) * 4 + [160]
+    S = len(lens)
+    q = _rand((sum(lens), hq, D), g, dev)
+    w = _weights(hq, g, dev, norm=window != 40)
+    call = dict(max_seqlen=300)
+    if not paged:
+        k, v = (_rand((sum(lens), hkv, D), g, dev) for _ in "kv")
+        _prefill(tm, q, k, v, _cu(lens, dev), w, window=window, call=call)
+        return
+    prior = torch.randint(0, 60, (S,), generator=g).tolist()
+    first = [max(0, p - window + 1) if window else 0 for p in prior]
+    c = Cache([a + b for a, b in zip(lens, prior)], hkv, g, dev, first=first)
+    _prefill(tm, q, None, None, _cu(lens, dev), w,
+             prior=torch.tensor(prior, dtype=torch.int32, device=dev),
+             k_pool=c.kp, v_pool=c.vp, table=c.table, window=window,
+             call=call)

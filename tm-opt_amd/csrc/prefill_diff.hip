@@ -4,8 +4,8 @@
 // Matrix bound: per visible (query, key) pair and map 128 products for the
 // score and 256 for the values.
 //
-//  * A work-group owns (run, pair of stored heads, block of 128 / REP queries)
-//    for REP head pairs: 128 rows of each map, over the same tiles of 32 keys
+//  * A work-group of eight waves owns (run, pair of stored heads, block of 128 /
+//    REP queries) for REP head pairs: 128 rows of each map, over the same tiles of 32 keys
 //    (K, K' and the 256-wide V: 32 KB) in LDS. Wave w has map w >> 2 of row
 //    block w & 3 (32 rows), so waves w and w + 4, which share a SIMD, are the
 //    two maps of the same rows. O^T of 32 rows x 256 dims takes 128 registers,
@@ -22,6 +22,14 @@
 //    the softmax of a tile.
 //  * The maps meet in LDS at the end: each wave gives its partner half of its
 //    normalised O and takes the difference and the norm of the other half.
+//  * A launch whose items fit the chip at once takes work-groups of four waves
+//    with 64 rows of each map, two per compute unit: each has two stages, K a tile
+//    ahead of V, and no phases to keep; one's start and end run beside the other's
+//    products. Graph replays, us, eight / four waves: 30 tokens 64Q/8KV 9.4 / 7.9,
+//    600 32Q/4KV 26.6 / 23.7, 777 33.0 / 29.0, 1,200 under a window of 512 32Q/8KV
+//    31.4 / 26.4. Full chips are quicker with eight, whose loads reach three tiles
+//    ahead and serve twice the rows: 64 x 512 358 / 413, 4 x 8,192 2,750 / 2,950.
+//    (Four waves with four stages, one work-group per unit, were slower on both.)
 //  * Work items are dealt to the XCDs heaviest first (prefill_sched.h).
 //
 // 4 prompts of 8,192 tokens run at 1,197 TFLOP/s, 4 of 2K-8K at 1,163 (32Q/4KV):
@@ -41,9 +49,12 @@ constexpr int kBN = 32;                   // keys per tile
 constexpr int kRowB = 256;                // one key's slice of a stored head
 constexpr int kSliceB = kBN * kRowB;      // 8 KB
 constexpr int kStage = 4 * kSliceB;       // K, K', V, V'
-constexpr int kNStage = 4;
-constexpr int kLds = kNStage * kStage + 8 * 128 + kDV * 4;   // and, for the
-                                          // norm, its sums and weights
+// Tiles in LDS of a work-group of W waves, and its bytes with the norm's sums
+// and weights.
+constexpr int stages_of(int W) { return W == 8 ? 4 : 2; }
+constexpr int lds_of(int W) {
+  return stages_of(W) * kStage + W * 128 + kDV * 4;
+}
 constexpr float kLazy = 8.0f;             // lazy-rescale threshold (log2)
 constexpr int kRing = 4;                  // fragments read kRing - 1 ahead
 // a buffer offset past every resource this kernel builds (their ranges are
@@ -168,10 +179,13 @@ __device__ __forceinline__ int pieces_of(const PrefillDiffArgs& a, int BQ,
   return __builtin_amdgcn_readfirstlane(max(1, n));
 }
 
-template <int REP, bool PAGED, bool SPLIT>
-__global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
-  constexpr int BQ = 128 / REP;   // queries per work-group
-  constexpr int QSUB = BQ / 32;   // 32-query sub-blocks per head pair
+template <int W, int REP, bool PAGED, bool SPLIT>
+__global__ __launch_bounds__(64 * W, 2) void prefill_diff_kernel(
+    PrefillDiffArgs a) {
+  constexpr int RB = W / 2;            // 32-row blocks of a map
+  constexpr int BQ = 32 * RB / REP;    // queries per work-group
+  constexpr int QSUB = BQ / 32;        // 32-query sub-blocks per head pair
+  static_assert(!SPLIT || W == 8, "pieces are eight waves'");
   extern __shared__ __align__(16) char smem[];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -206,9 +220,9 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
   }
 
   // ---- this wave's row block: map, head pair and 32-query sub-block ------
-  const int map = w >> 2;
-  const int hp = wk.kvh * REP + (w & 3) / QSUB;
-  const int row0 = q0 + 32 * ((w & 3) % QSUB);
+  const int map = w / RB;
+  const int hp = wk.kvh * REP + (w % RB) / QSUB;
+  const int row0 = q0 + 32 * ((w % RB) % QSUB);
   const int qi = row0 + l32;                  // this lane's query (column)
   const bool qok = qi < len;
   const int qpos = prior + qi;
@@ -217,14 +231,15 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
   const float lam = as_const(a.w.lam)[(int64_t)hp * a.w.lam_stride];
   const uint32_t wlds =
       (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)smem) +
-      kNStage * kStage + 8 * 128;
+      stages_of(W) * kStage + W * 128;
 
   // ---- tile loads ----------------------------------------------------------
-  // Wave w moves key rows 4w..4w+3 of each of the four slices, one 1 KB
-  // instruction each: lane l fills row l >> 4, physical 16-byte slot l & 15,
-  // and fetches the logical chunk that belongs there.
+  // Of eight waves, wave w moves key rows 4w..4w+3 of each of the four slices, one
+  // 1 KB instruction each: lane l fills row l >> 4, physical 16-byte slot l & 15,
+  // and fetches the logical chunk that belongs there. Of four, rows 8w..8w+7 by
+  // two.
   const int grp = lane >> 4, slot = lane & 15;
-  const int krow = 4 * w + grp;
+  const int krow = 32 / W * w + grp;
   const int kchunk = slot ^ (krow & 15);
   const int vchunk = ((((slot >> 2) ^ grp) & 3) << 2) | (slot & 3);
   const uint32_t lds0 =
@@ -250,7 +265,7 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
     klane = grp * kst_b + 16 * kchunk;
     vlane = grp * vst_b + 16 * vchunk;
   }
-  // tile t (index from k_lo) into LDS stage st: 4 instructions per wave. live
+  // Eight waves: tile t (index from k_lo) into LDS stage st: 4 instructions. live
   // == false issues the same ones fetching nothing: the loops issue a tile
   // every iteration, past the last one too, so that the count of loads in
   // flight is the same on every path and the waits are exact.
@@ -286,6 +301,42 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
       dma(rv[0], dst + 2 * kSliceB, vo);
       dma(rv[1], dst + 3 * kSliceB, vo);
     }
+  };
+
+  // Four waves: K (v 0) or V (v 1) of tile t into stage t & 1, nothing past the
+  // last tile: the waits of these loads are for all of them.
+  [[maybe_unused]] const int kstep = 16 * ((kchunk ^ 4) - kchunk);
+  auto issue_half = [&](int t, int v) __attribute__((always_inline)) {
+    if (t >= ntiles) return;
+    const int key0 = k_lo + t * kBN + 8 * w;   // first of the wave's rows
+    const uint32_t dst =
+        lds0 + (t & 1) * kStage + 2 * v * kSliceB + 8 * w * kRowB;
+    const int st_b = v ? vst_b : kst_b;
+    i32x4 r0, r1;
+    int o;
+    if constexpr (PAGED) {   // (as above; the second head is 256 bytes on)
+      const int lp = key0 >> 4;
+      const int pg = (unsigned)lp < (unsigned)a.bt_width ? trow[lp] : -1;
+      const int r_lo = min(kPage, max(0, kwin - kPage * lp));
+      const int r_hi = min(kPage, max(0, nk - kPage * lp));
+      const bool valid = (unsigned)pg < (unsigned)a.num_pages && r_hi > r_lo;
+      r0 = r1 = make_rsrc(
+          reinterpret_cast<const char*>(v ? a.v : a.k) +
+              (valid ? ((int64_t)pg * kPage + r_lo) * kst_b : 0),
+          valid ? (uint32_t)((r_hi - r_lo) * kst_b) : 0u);
+      o = ((key0 & (kPage - 1)) - r_lo) * kst_b;
+    } else {
+      r0 = v ? rv[0] : rk[0];
+      r1 = v ? rv[1] : rk[1];
+      o = key0 * st_b;
+    }
+    constexpr int kHead = PAGED ? kRowB : 0;
+    const int l0 = (v ? vlane : klane) + o;
+    const int l1 = l0 + 4 * st_b + (v ? 0 : kstep);
+    dma(r0, dst, l0);
+    dma(r0, dst + 4 * kRowB, l1);
+    dma(r1, dst + kSliceB, l0 + kHead);
+    dma(r1, dst + kSliceB + 4 * kRowB, l1 + kHead);
   };
 
   // ---- LDS fragment addresses -------------------------------------------
@@ -390,8 +441,8 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
     constexpr bool with_s = decltype(with_s_c)::value;
     // this wave's MFMAs first; the softmax wave fills the issue slots between
     __builtin_amdgcn_s_setprio(1);
-    const uint32_t vb = lds0 + (t & 3) * kStage;
-    const uint32_t kb = lds0 + ((t + 1) & 3) * kStage;
+    const uint32_t vb = lds0 + (t & (stages_of(W) - 1)) * kStage;
+    const uint32_t kb = lds0 + ((t + 1) & (stages_of(W) - 1)) * kStage;
     constexpr int R = kRing, RK = 3;
     bf16x8 vf[R], kf[RK];
 #pragma unroll
@@ -426,17 +477,21 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
 
   const bool rejected = a.reject != nullptr && as_const(a.reject)[0] != 0;
   if (!rejected) {
-    // Slot 2t: group 0 multiplies tile t, group 1 does the softmax of tile t;
+    // Eight waves. Slot 2t: group 0 multiplies tile t, group 1 does the softmax of tile t;
     // slot 2t + 1: group 0 the softmax of tile t + 1, group 1 multiplies tile
     // t. Tile t + 3 goes out at the start of slot 2t into the stage of tile t -
     // 1 (last read in slot 2t - 1) and must be in LDS before slot 2t + 4; each
     // wave waits for its own part at the end of every odd slot, before the
-    // barrier that publishes it. The queries come first, each wave's own 32
-    // rows through its 8 KB of stages 2 and 3 (rows past the run end arrive as
-    // zeros).
+    // barrier that publishes it.
+    // Four waves. K runs a tile ahead of V: after the products of tile t and the
+    // scores of tile t + 1, a barrier frees V(t) and K(t + 1) for V(t + 2) and K(t
+    // + 3), which have until the next one to arrive.
+    // The queries come first, each wave's own 32 rows through its 8 KB of the
+    // last stages (rows past the run end arrive as zeros).
     if (w == 0 && a.w.weight)
       dma(make_rsrc(a.w.weight, kDV * 4), wlds, 16 * lane);
-    const uint32_t qlds = lds0 + 2 * kStage + (uint32_t)w * (32 * kRowB);
+    const uint32_t qlds =
+        lds0 + stages_of(W) / 2 * kStage + (uint32_t)w * (32 * kRowB);
     {
       const int64_t span = ((int64_t)(len - row0 - 1) * a.q_st + kD) * 2;
       const i32x4 rq = make_rsrc(a.q + (int64_t)(t0 + row0) * a.q_st +
@@ -449,8 +504,13 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
         dma(rq, qlds + i * 1024, r * qst_b + 16 * (slot ^ (r & 15)));
       }
     }
-    issue_tile(0, 0);
-    issue_tile(1, 1, ntiles > 1);
+    if constexpr (W == 8) {
+      issue_tile(0, 0);
+      issue_tile(1, 1, ntiles > 1);
+    } else {
+      issue_half(0, 0);
+      issue_half(0, 1);
+    }
     wait_vm<8>();   // the queries
     asm volatile("" ::: "memory");
 #pragma unroll
@@ -462,8 +522,13 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
       qf[kk] = __builtin_bit_cast(bf16x8, x);
     }
     wait_vm<0>();
-    __syncthreads();   // tiles 0 and 1 are there, stages 2 and 3 free
-    if (ntiles > 2) issue_tile(2, 2);
+    __syncthreads();   // tile 0 (of four stages, 1 too) is there, the others free
+    if constexpr (W == 8) {
+      if (ntiles > 2) issue_tile(2, 2);
+    } else {
+      issue_half(1, 0);
+      issue_half(1, 1);
+    }
     auto odd_end = [&](int n) {
       if (n == 4) wait_vm<4>();
       else wait_vm<0>();
@@ -474,7 +539,21 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
     constexpr std::true_type kWithS{};
     constexpr std::false_type kNoS{};
     auto none = [] {};
-    if (map == 0) {
+    if constexpr (W == 4) {
+      first_scores();
+      softmax_phase(k_lo, true, none);
+      odd_end(0);   // tile 1 is there, K(0) free
+      issue_half(2, 0);
+      for (int t = 0; t + 1 < ntiles; ++t) {
+        mfma_phase(t, kWithS);
+        odd_end(0);
+        issue_half(t + 2, 1);
+        issue_half(t + 3, 0);
+        softmax_phase(k_lo + (t + 1) * kBN, false, none);
+      }
+      mfma_phase(ntiles - 1, kNoS);
+      odd_end(0);
+    } else if (map == 0) {
       first_scores();
       softmax_phase(k_lo, true, none);
       for (int t = 0; t + 1 < ntiles; ++t) {
@@ -538,7 +617,7 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
   // dims 128 map .. +127 are this wave's; the others go to its partner, lane by
   // lane (16 bytes each: 1 KB per store)
   const uint32_t mine = lds0 + (uint32_t)w * 16384 + 16 * lane;
-  const uint32_t theirs = lds0 + (uint32_t)(w ^ 4) * 16384 + 16 * lane;
+  const uint32_t theirs = lds0 + (uint32_t)(w ^ RB) * 16384 + 16 * lane;
   f32x4 d[16];   // chunk c: dims 8c + 4 h2 .. +3 of the half
 #pragma unroll
   for (int c = 0; c < 16; ++c) {
@@ -560,7 +639,7 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
     ss += (d[c][0] * d[c][0] + d[c][1] * d[c][1]) +
           (d[c][2] * d[c][2] + d[c][3] * d[c][3]);
   }
-  const uint32_t sums = lds0 + kNStage * kStage;
+  const uint32_t sums = lds0 + stages_of(W) * kStage;
   if (a.w.weight) {
     ss = lane_pair(ss, 32, false);
     if (h2 == 0)
@@ -574,7 +653,7 @@ __global__ __launch_bounds__(512) void prefill_diff_kernel(PrefillDiffArgs a) {
     for (int c = 0; c < 16; ++c)
       wt[c] = __builtin_bit_cast(
           f32x4, lds_ld128(wlds + 4 * (128 * map + 8 * c + 4 * h2)));
-    ss += __builtin_bit_cast(float, lds_ld32(sums + 128 * (w ^ 4) + 4 * l32));
+    ss += __builtin_bit_cast(float, lds_ld32(sums + 128 * (w ^ RB) + 4 * l32));
     const float f =
         a.w.out_scale * __builtin_amdgcn_rsqf(ss * (1.0f / kDV) + a.w.eps);
 #pragma unroll
@@ -786,27 +865,29 @@ int64_t workspace_bytes_of(const Layout& x) {
   return x.levels * x.n_base * kSlotBytes + ((x.n_base * 4 + 15) & ~(int64_t)15);
 }
 
-// Head pairs per work-group: the largest of 4, 2, 1 dividing HQ / HKV; a larger
-// ratio runs as several scheduled pairs per stored one.
-int group_of(int ratio) { return ratio % 4 == 0 ? 4 : ratio % 2 == 0 ? 2 : 1; }
+// Head pairs per work-group: the largest of 4 (eight waves), 2, 1 dividing HQ /
+// HKV; a larger ratio runs as several scheduled pairs per stored one.
+int group_of(int ratio, int most) {
+  return most >= 4 && ratio % 4 == 0 ? 4 : ratio % 2 == 0 ? 2 : 1;
+}
 
-template <int REP, bool PAGED>
-void launch_source(const PrefillDiffArgs& a, hipStream_t st) {
+template <int W, int REP, bool SPLIT>
+int launch_whole(const PrefillDiffArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)(a.nsplit * a.n_base));
-  if (a.nsplit > 1)
-    hipLaunchKernelGGL((prefill_diff_kernel<REP, PAGED, true>), grid,
-                       dim3(512), kLds, st, a);
+  if (a.bt)
+    hipLaunchKernelGGL((prefill_diff_kernel<W, REP, true, SPLIT>), grid,
+                       dim3(64 * W), lds_of(W), st, a);
   else
-    hipLaunchKernelGGL((prefill_diff_kernel<REP, PAGED, false>), grid,
-                       dim3(512), kLds, st, a);
+    hipLaunchKernelGGL((prefill_diff_kernel<W, REP, false, SPLIT>), grid,
+                       dim3(64 * W), lds_of(W), st, a);
+  return check_launch("prefill_diff");
 }
 
 template <int REP>
 int launch(const PrefillDiffArgs& a, hipStream_t st) {
-  if (a.bt) launch_source<REP, true>(a, st);
-  else launch_source<REP, false>(a, st);
-  const int rc = check_launch("prefill_diff");
-  if (rc || a.nsplit <= 1) return rc;
+  if (a.nsplit <= 1) return launch_whole<8, REP, false>(a, st);
+  const int rc = launch_whole<8, REP, true>(a, st);
+  if (rc) return rc;
   // many pieces of few items: four groups (3 queries after 22,000, 16Q/2KV, 58 us
   // a call with one and the pieces of an item on one XCD, 48 so)
   if (a.nsplit > 8)
@@ -829,7 +910,7 @@ extern "C" size_t tmopt_attn_prefill_diff_workspace_size(
   if (num_seqs <= 0 || max_seqlen_q <= 0 || HQ <= 0 || HKV <= 0 ||
       HKV % 2 != 0 || HQ % HKV != 0)
     return 0;
-  const int rep = group_of(HQ / HKV), BQ = 128 / rep;
+  const int rep = group_of(HQ / HKV, 4), BQ = 128 / rep;
   return (size_t)workspace_bytes_of(
       layout_of(HQ / 2 / rep, BQ, num_seqs, max_seqlen_q, bt_stride, window));
 }
@@ -893,11 +974,22 @@ extern "C" int tmopt_attn_prefill_diff(
                   TMOPT_EUNSUPPORTED,
                   "prefill_diff: a run's k/v span must stay below 2 GiB");
   }
-  const int rep = group_of(HQ / HKV), pairs = HQ / 2 / rep, BQ = 128 / rep;
+  int rep = group_of(HQ / HKV, 4), pairs = HQ / 2 / rep, BQ = 128 / rep;
   Layout x = layout_of(pairs, BQ, num_seqs, max_seqlen_q,
                        paged ? bt_stride : 0, window);
-  if (workspace == nullptr)
-    x = Layout{1, level_wgs(pairs, BQ, num_seqs, max_seqlen_q)};
+  bool small = false;   // four waves: all work-groups on the chip at once
+  if (workspace == nullptr || x.levels == 1) {
+    const int rep4 = group_of(HQ / HKV, 2), BQ4 = 64 / rep4;
+    x = Layout{1, level_wgs(HQ / 2 / rep4, BQ4, num_seqs, max_seqlen_q)};
+    small = x.n_base <= 2 * device_cus();
+    if (small) {
+      rep = rep4;
+      pairs = HQ / 2 / rep;
+      BQ = BQ4;
+    } else {
+      x.n_base = level_wgs(pairs, BQ, num_seqs, max_seqlen_q);
+    }
+  }
   TMOPT_REQUIRE(x.n_base < 0x7fffffff, TMOPT_EUNSUPPORTED,
                 "prefill_diff: %lld work-groups exceed the grid limit",
                 (long long)x.n_base);
@@ -945,6 +1037,9 @@ extern "C" int tmopt_attn_prefill_diff(
   a.part_lse = a.part_o + slots * 8 * 32 * kDV;
   a.part_n = (int*)(a.part_lse + slots * 8 * 32);
   const hipStream_t st = (hipStream_t)stream;
+  if (small)
+    return rep == 2 ? launch_whole<4, 2, false>(a, st)
+                    : launch_whole<4, 1, false>(a, st);
   if (rep == 4) return launch<4>(a, st);
   if (rep == 2) return launch<2>(a, st);
   return launch<1>(a, st);
