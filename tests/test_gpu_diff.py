@@ -722,3 +722,31 @@ def test_prefill_large_launches(tm, dev, hq, hkv, window, paged):
              prior=torch.tensor(prior, dtype=torch.int32, device=dev),
              k_pool=c.kp, v_pool=c.vp, table=c.table, window=window,
              call=call)
+
+
+@pytest.mark.parametrize("n,prior,hq,hkv,window", [
+    (16, 1000, 16, 4, 0), (16, 1000, 12, 4, 900), (40, 1500, 24, 8, 0),
+    (1, 3000, 8, 2, 0), (70, 1100, 4, 4, 0), (300, 1000, 32, 4, 0),
+    (500, 6000, 32, 8, 0)])
+def test_prefill_pieces_of_either_size(tm, dev, n, prior, hq, hkv, window):
+    """Split launches with work-groups of four and of eight waves, beside runs
+    that are not worth a split or have no tokens."""
+    g = _gen(n + hq)
+    lens, before = [n, 0, n // 3, 1], [prior, 9, 33, prior // 2]
+    first = [max(0, p - window + 1) if window else 0 for p in before]
+    c = Cache([a + b for a, b in zip(lens, before)], hkv, g, dev, first=first)
+    q = _rand((sum(lens), hq, D), g, dev)
+    pr = torch.tensor(before, dtype=torch.int32, device=dev)
+    for norm in (True, False):
+        _prefill(tm, q, None, None, _cu(lens, dev),
+                 _weights(hq, g, dev, norm=norm), prior=pr, k_pool=c.kp,
+                 v_pool=c.vp, table=c.table, window=window)
+
+
+@pytest.mark.parametrize("n,hq,hkv", [(1100, 4, 2), (1500, 8, 2), (2050, 4, 4)])
+def test_prefill_packed_pieces(tm, dev, n, hq, hkv):
+    g = _gen(n)
+    lens = [n, 3]
+    T = sum(lens)
+    _prefill(tm, _rand((T, hq, D), g, dev), _rand((T, hkv, D), g, dev),
+             _rand((T, hkv, D), g, dev), _cu(lens, dev), _weights(hq, g, dev))

@@ -133,8 +133,10 @@ __device__ __forceinline__ int split_item(int pairs, int x) {
 // per compute unit; a tile takes 1.05 on up to half the units and 1.4 on all
 // (power: 2.1 against 1.6 GHz); pieces cost 5 for their start and the merge, 0.1
 // for each of an item's that it joins, and 0.115 for each of the launch's that
-// is written and read, if all its rows are queries.
+// is written and read, if all its rows are queries. Of four waves, two per unit:
+// a tile takes 1.0 alone and 1.5 beside another, a piece is half the size.
 constexpr int kMinPiece = 4;   // tiles
+template <int W>
 __device__ __forceinline__ int pieces_of(const PrefillDiffArgs& a, int BQ,
                                          int lane, int tiles) {
   int sum = 0, most = 0, items = 0, rows = 0;
@@ -164,12 +166,13 @@ __device__ __forceinline__ int pieces_of(const PrefillDiffArgs& a, int BQ,
   float best = 0.0f;
   int n = 1;
   for (int x = 1; x <= a.nsplit; ++x) {
-    const float load = all * x / a.cus;
+    const float load = all * x / (W == 8 ? a.cus : 2 * a.cus);
     const float len = (low * fmaxf(1.0f, ceilf(load - 0.02f)) +
                        (most - low) * fmaxf(1.0f, 0.5f * load)) / x;
+    const float part = fminf(fmaxf(load, 0.5f), 1.0f);
     const float us =
-        len * (0.7f + 0.7f * fminf(fmaxf(load, 0.5f), 1.0f)) +
-        (x > 1 ? 5.0f + 0.1f * x + 0.115f * full * x * all : 0.0f);
+        len * (W == 8 ? 0.7f + 0.7f * part : 0.5f + part) +
+        (x > 1 ? 5.0f + 0.1f * x + (0.115f / 8 * W) * full * x * all : 0.0f);
     if (x == 1 || us < best) {
       best = us;
       n = x;
@@ -185,7 +188,6 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_diff_kernel(
   constexpr int RB = W / 2;            // 32-row blocks of a map
   constexpr int BQ = 32 * RB / REP;    // queries per work-group
   constexpr int QSUB = BQ / 32;        // 32-query sub-blocks per head pair
-  static_assert(!SPLIT || W == 8, "pieces are eight waves'");
   extern __shared__ __align__(16) char smem[];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -211,7 +213,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_diff_kernel(
   int k_lo = tl.k_lo, ntiles = tl.n;
   int np = 1;
   if constexpr (SPLIT) {
-    np = pieces_of(a, BQ, lane, tl.n);
+    np = pieces_of<W>(a, BQ, lane, tl.n);
     if (level == 0 && tid == 0) a.part_n[item] = np;
     if (level >= np) return;
     const int b0 = (int)((int64_t)tl.n * level / np);
@@ -594,7 +596,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_diff_kernel(
   if (SPLIT && np > 1) {
     // lane-major partial: every store writes 1 KB (of rows past the run,
     // nothing)
-    const int64_t pw = (int64_t)blockIdx.x * 8 + w;
+    const int64_t pw = (int64_t)blockIdx.x * W + w;
     float* const po = a.part_o + (pw * 32 * 64 + lane) * 4;
     if (qok)
 #pragma unroll
@@ -695,10 +697,10 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_diff_kernel(
 // and the norm one sum over threads. Group s of S takes pieces s, s + S, ...,
 // four pieces' loads in flight at a time; the groups' results then join through
 // LDS in order.
-template <int REP, int S>
+template <int W, int REP, int S>
 __global__ __launch_bounds__(256 * S) void prefill_diff_merge(
     PrefillDiffArgs a) {
-  constexpr int BQ = 128 / REP, QSUB = BQ / 32, kBatch = 4;
+  constexpr int RB = W / 2, BQ = 32 * RB / REP, QSUB = BQ / 32, kBatch = 4;
   __shared__ float sums[4][8];
   __shared__ float part[S > 1 ? S - 1 : 1][20][S > 1 ? 256 : 1];
   const int np = min(as_const(a.part_n)[blockIdx.x], a.nsplit);
@@ -743,7 +745,7 @@ __global__ __launch_bounds__(256 * S) void prefill_diff_merge(
           (int64_t)min(s0 + j * S, np - 1) * a.n_base + blockIdx.x;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int64_t pw = slot * 8 + 4 * i + rb;
+        const int64_t pw = slot * W + RB * i + rb;
         l[j][i] = a.part_lse[pw * 32 + l32];
 #pragma unroll
         for (int x = 0; x < 2; ++x)
@@ -832,43 +834,76 @@ int64_t level_wgs(int pairs, int BQ, int64_t S, int max_seqlen) {
   return pairs * items;
 }
 
-// How a launch is laid out: levels (1: keys are not split) of n_base
-// work-groups each, from what the host knows: the longest run, and the row
-// width of a block table or the window as bounds of its keys. Up to half the
-// compute units' worth of items, as many pieces as there are units; up to one
-// and a half, two or three pieces an item even out the rounds; larger grids
-// fill the chip by themselves. The device decides from the lengths.
-struct Layout {
-  int levels;
-  int64_t n_base;
-};
-Layout layout_of(int pairs, int BQ, int64_t S, int max_seqlen,
-                 int64_t bt_stride, int window) {
-  const int64_t cus = device_cus();
-  const int64_t items = S * ((max_seqlen + BQ - 1) / BQ) * pairs;
-  int64_t keys = bt_stride > 0 ? bt_stride * kPage : max_seqlen;
-  if (window > 0 && keys > (int64_t)window + BQ + kBN)
-    keys = (int64_t)window + BQ + kBN;
-  const int64_t tiles = (keys + kBN - 1) / kBN;
-  int64_t n = (2 * items <= cus ? cus : 3 * cus) / items;
-  if (n > 64) n = 64;
-  // a piece costs some 5 tiles' time, so it must have more than that
-  if (n > tiles / 8) n = tiles / 8;
-  if (n < 2 || tiles < 32)
-    return Layout{1, level_wgs(pairs, BQ, S, max_seqlen)};
-  return Layout{(int)n, items};
-}
-
-constexpr int64_t kSlotBytes = (int64_t)8 * 32 * (kDV + 1) * sizeof(float);
-int64_t workspace_bytes_of(const Layout& x) {
-  if (x.levels <= 1) return 0;
-  return x.levels * x.n_base * kSlotBytes + ((x.n_base * 4 + 15) & ~(int64_t)15);
-}
-
 // Head pairs per work-group: the largest of 4 (eight waves), 2, 1 dividing HQ /
 // HKV; a larger ratio runs as several scheduled pairs per stored one.
 int group_of(int ratio, int most) {
   return most >= 4 && ratio % 4 == 0 ? 4 : ratio % 2 == 0 ? 2 : 1;
+}
+
+// How a launch is laid out: work-groups of W waves for rep head pairs and BQ
+// queries, in levels (1: keys are not split) of n_base.
+struct Layout {
+  int W, rep, pairs, BQ;
+  int levels;
+  int64_t n_base;
+};
+Layout groups_of(int W, int HQ, int HKV) {
+  const int rep = group_of(HQ / HKV, W / 2);
+  return Layout{W, rep, HQ / 2 / rep, 16 * W / rep, 1, 0};
+}
+
+// From what the host knows: the longest run, and the row width of a block table
+// or the window as bounds of its keys. Up to half the compute units' worth of
+// items, as many pieces as there are units; up to one and a half, two or three
+// pieces an item even out the rounds where keys are many (below 128 tiles two
+// work-groups per unit do it better: a prompt of 1200, 32Q/4KV, 48.8 us a call in
+// pieces, 40.5 whole, of 3000, 16Q/2KV, 99.5 / 92.5); larger grids fill the chip by
+// themselves. The device decides from the lengths. Four waves where all whole items, or the
+// pieces at 20 tiles each or less, are on the chip at once: there an item's start
+// and end weigh most. Graph replays of split calls, us, eight / four waves: 16
+// tokens after 1000, 64Q/8KV 21.7 / 19.3, 300 after 1000, 32Q/4KV 38.7 / 35.6, 128
+// after 8000, 16Q/2KV 45 / 41.8; 64 after 30,000, 64Q/8KV 114 / 123, one after
+// 20,000 48 / 68 (keys are read for half as many rows).
+Layout layout_of(int HQ, int HKV, int64_t S, int max_seqlen,
+                 int64_t bt_stride, int window, bool split) {
+  const int64_t cus = device_cus();
+  const Layout w4 = groups_of(4, HQ, HKV), w8 = groups_of(8, HQ, HKV);
+  auto count = [&](const Layout& x) {
+    return S * ((max_seqlen + x.BQ - 1) / x.BQ) * x.pairs;
+  };
+  auto tiles_of = [&](const Layout& x) {
+    int64_t keys = bt_stride > 0 ? bt_stride * kPage : max_seqlen;
+    if (window > 0 && keys > (int64_t)window + x.BQ + kBN)
+      keys = (int64_t)window + x.BQ + kBN;
+    return (keys + kBN - 1) / kBN;
+  };
+  const int64_t few = count(w4);
+  // (packed runs see half of their keys)
+  const bool four =
+      few <= cus && few * tiles_of(w4) <= (bt_stride > 0 ? 20 : 40) * cus;
+  Layout r = four ? w4 : w8;
+  const int64_t items = count(r), tiles = tiles_of(r);
+  int64_t n = (2 * items <= cus ? cus : 3 * cus) * (four ? 2 : 1) / items;
+  if (n > 64) n = 64;
+  // a piece costs some 5 tiles' time, so it must have more than that
+  if (n > tiles / 8) n = tiles / 8;
+  if (split && n >= 2 && tiles >= (2 * items <= cus ? 32 : 128)) {
+    r.levels = (int)n;
+    r.n_base = items;
+    return r;
+  }
+  r = w4;
+  r.n_base = level_wgs(r.pairs, r.BQ, S, max_seqlen);
+  if (r.n_base <= 2 * cus) return r;
+  r = w8;
+  r.n_base = level_wgs(r.pairs, r.BQ, S, max_seqlen);
+  return r;
+}
+
+int64_t workspace_bytes_of(const Layout& x) {
+  if (x.levels <= 1) return 0;
+  return x.levels * x.n_base * x.W * 32 * (kDV + 1) * (int64_t)sizeof(float) +
+         ((x.n_base * 4 + 15) & ~(int64_t)15);
 }
 
 template <int W, int REP, bool SPLIT>
@@ -883,19 +918,20 @@ int launch_whole(const PrefillDiffArgs& a, hipStream_t st) {
   return check_launch("prefill_diff");
 }
 
-template <int REP>
+template <int W, int REP>
 int launch(const PrefillDiffArgs& a, hipStream_t st) {
-  if (a.nsplit <= 1) return launch_whole<8, REP, false>(a, st);
-  const int rc = launch_whole<8, REP, true>(a, st);
+  if (a.nsplit <= 1) return launch_whole<W, REP, false>(a, st);
+  const int rc = launch_whole<W, REP, true>(a, st);
   if (rc) return rc;
   // many pieces of few items: four groups (3 queries after 22,000, 16Q/2KV, 58 us
   // a call with one and the pieces of an item on one XCD, 48 so)
+  const dim3 grid(a.n_base, 2 * W);
   if (a.nsplit > 8)
-    hipLaunchKernelGGL((prefill_diff_merge<REP, 4>), dim3(a.n_base, 16),
-                       dim3(1024), 0, st, a);
+    hipLaunchKernelGGL((prefill_diff_merge<W, REP, 4>), grid, dim3(1024), 0, st,
+                       a);
   else
-    hipLaunchKernelGGL((prefill_diff_merge<REP, 1>), dim3(a.n_base, 16),
-                       dim3(256), 0, st, a);
+    hipLaunchKernelGGL((prefill_diff_merge<W, REP, 1>), grid, dim3(256), 0, st,
+                       a);
   return check_launch("prefill_diff_merge");
 }
 
@@ -910,9 +946,8 @@ extern "C" size_t tmopt_attn_prefill_diff_workspace_size(
   if (num_seqs <= 0 || max_seqlen_q <= 0 || HQ <= 0 || HKV <= 0 ||
       HKV % 2 != 0 || HQ % HKV != 0)
     return 0;
-  const int rep = group_of(HQ / HKV, 4), BQ = 128 / rep;
   return (size_t)workspace_bytes_of(
-      layout_of(HQ / 2 / rep, BQ, num_seqs, max_seqlen_q, bt_stride, window));
+      layout_of(HQ, HKV, num_seqs, max_seqlen_q, bt_stride, window, true));
 }
 
 extern "C" int tmopt_attn_prefill_diff(
@@ -974,22 +1009,9 @@ extern "C" int tmopt_attn_prefill_diff(
                   TMOPT_EUNSUPPORTED,
                   "prefill_diff: a run's k/v span must stay below 2 GiB");
   }
-  int rep = group_of(HQ / HKV, 4), pairs = HQ / 2 / rep, BQ = 128 / rep;
-  Layout x = layout_of(pairs, BQ, num_seqs, max_seqlen_q,
-                       paged ? bt_stride : 0, window);
-  bool small = false;   // four waves: all work-groups on the chip at once
-  if (workspace == nullptr || x.levels == 1) {
-    const int rep4 = group_of(HQ / HKV, 2), BQ4 = 64 / rep4;
-    x = Layout{1, level_wgs(HQ / 2 / rep4, BQ4, num_seqs, max_seqlen_q)};
-    small = x.n_base <= 2 * device_cus();
-    if (small) {
-      rep = rep4;
-      pairs = HQ / 2 / rep;
-      BQ = BQ4;
-    } else {
-      x.n_base = level_wgs(pairs, BQ, num_seqs, max_seqlen_q);
-    }
-  }
+  const Layout x =
+      layout_of(HQ, HKV, num_seqs, max_seqlen_q, paged ? bt_stride : 0, window,
+                workspace != nullptr);
   TMOPT_REQUIRE(x.n_base < 0x7fffffff, TMOPT_EUNSUPPORTED,
                 "prefill_diff: %lld work-groups exceed the grid limit",
                 (long long)x.n_base);
@@ -1016,10 +1038,10 @@ extern "C" int tmopt_attn_prefill_diff(
   a.bt_width = bt_stride > 0x7fffffff ? 0x7fffffff : (int)bt_stride;
   a.num_pages = num_pages > 0x7fffffff ? 0x7fffffff : (int)num_pages;
   a.HQ = HQ;
-  a.HKV = pairs;
-  a.kv_div = HQ / HKV / rep;
+  a.HKV = x.pairs;
+  a.kv_div = HQ / HKV / x.rep;
   a.S = num_seqs;
-  a.nqb_max = (max_seqlen_q + BQ - 1) / BQ;
+  a.nqb_max = (max_seqlen_q + x.BQ - 1) / x.BQ;
   a.window = window;
   a.scale_log2 = scale * kLog2e;
   a.w = DiffWeights{lam, lam_stride, norm_weight, norm_eps, out_scale};
@@ -1032,15 +1054,13 @@ extern "C" int tmopt_attn_prefill_diff(
   a.nsplit = x.levels;
   a.n_base = (int)x.n_base;
   a.cus = device_cus();
-  const int64_t slots = x.levels * x.n_base;
+  const int64_t rows = x.levels * x.n_base * x.W * 32;
   a.part_o = (float*)workspace;
-  a.part_lse = a.part_o + slots * 8 * 32 * kDV;
-  a.part_n = (int*)(a.part_lse + slots * 8 * 32);
+  a.part_lse = a.part_o + rows * kDV;
+  a.part_n = (int*)(a.part_lse + rows);
   const hipStream_t st = (hipStream_t)stream;
-  if (small)
-    return rep == 2 ? launch_whole<4, 2, false>(a, st)
-                    : launch_whole<4, 1, false>(a, st);
-  if (rep == 4) return launch<4>(a, st);
-  if (rep == 2) return launch<2>(a, st);
-  return launch<1>(a, st);
+  if (x.W == 4) return x.rep == 2 ? launch<4, 2>(a, st) : launch<4, 1>(a, st);
+  if (x.rep == 4) return launch<8, 4>(a, st);
+  if (x.rep == 2) return launch<8, 2>(a, st);
+  return launch<8, 1>(a, st);
 }
