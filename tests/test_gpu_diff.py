@@ -750,3 +750,14 @@ def test_prefill_packed_pieces(tm, dev, n, hq, hkv):
     T = sum(lens)
     _prefill(tm, _rand((T, hq, D), g, dev), _rand((T, hkv, D), g, dev),
              _rand((T, hkv, D), g, dev), _cu(lens, dev), _weights(hq, g, dev))
+
+
+@pytest.mark.parametrize("hq,hkv,window", [(32, 4, 0), (12, 4, 50), (8, 8, 0)])
+def test_prefill_many_short_runs(tm, dev, hq, hkv, window):
+    """More work-groups than the chip holds, of few keys each."""
+    g = _gen(24)
+    lens = torch.randint(0, 230, (90,), generator=g).tolist() + [230, 0]
+    T = sum(lens)
+    _prefill(tm, _rand((T, hq, D), g, dev), _rand((T, hkv, D), g, dev),
+             _rand((T, hkv, D), g, dev), _cu(lens, dev), _weights(hq, g, dev),
+             window=window)

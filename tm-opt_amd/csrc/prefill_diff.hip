@@ -863,7 +863,10 @@ Layout groups_of(int W, int HQ, int HKV) {
 // and end weigh most. Graph replays of split calls, us, eight / four waves: 16
 // tokens after 1000, 64Q/8KV 21.7 / 19.3, 300 after 1000, 32Q/4KV 38.7 / 35.6, 128
 // after 8000, 16Q/2KV 45 / 41.8; 64 after 30,000, 64Q/8KV 114 / 123, one after
-// 20,000 48 / 68 (keys are read for half as many rows).
+// 20,000 48 / 68 (keys are read for half as many rows). And where no query sees
+// more than 8 tiles: 128 prompts of 128, 32Q/4KV 124 / 113, of 200 242 / 212, 128 of
+// 500 under a window of 100 555 / 513 (64 of 256 142 / 146, 40 of 300, 64Q/8KV 234
+// / 239).
 Layout layout_of(int HQ, int HKV, int64_t S, int max_seqlen,
                  int64_t bt_stride, int window, bool split) {
   const int64_t cus = device_cus();
@@ -894,7 +897,7 @@ Layout layout_of(int HQ, int HKV, int64_t S, int max_seqlen,
   }
   r = w4;
   r.n_base = level_wgs(r.pairs, r.BQ, S, max_seqlen);
-  if (r.n_base <= 2 * cus) return r;
+  if (r.n_base <= 2 * cus || tiles_of(w4) <= 8) return r;
   r = w8;
   r.n_base = level_wgs(r.pairs, r.BQ, S, max_seqlen);
   return r;
