@@ -32,12 +32,12 @@
 //  * Page ids of a range and the norm's weights are fetched into LDS before the
 //    walk: a load within it would wait for every page on its way.
 //
-// Us a call, the merge included (32Q/4KV with the norm unless said): 64 requests
-// of 1K-8K tokens 102.9, 5.9 TB/s (1.00 of the bytes fetched are the formula's);
-// 96 under a window of 512, 64Q/16KV, 66.0, 6.1 TB/s; one of 50,001 tokens 32.7,
-// 3.1 TB/s: its walk runs at 7.3 TB/s, 5 us go to the start, 8 to the merge of
-// its 184 pieces; 4 of 128-1024 tokens 14.3 in a graph, 17.5 eagerly: two
-// launches and their chains of dependent loads.
+// Us a call, the merge included (32Q/4KV with the norm unless said): 64
+// requests of 1K-8K tokens 102.9, 5.9 TB/s (1.00 of the bytes fetched are the
+// formula's); 96 under a window of 512, 64Q/16KV, 66.0, 6.1 TB/s; one of 50,001
+// tokens 32.7, 3.1 TB/s: its walk runs at 7.3 TB/s, 5 us go to the start, 8 to
+// the merge of its 184 pieces; 4 of 128-1024 tokens 14.3 in a graph, 17.5
+// eagerly: two launches and their chains of dependent loads.
 #include <algorithm>
 
 #include "diff.h"
@@ -129,10 +129,10 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // Groups of waves per head pair in the merge, from the pieces of an average
 // request (at most one more than its share of the R ranges). Graph replays with
-// 1 / 2 / 8 groups, us a call, 32Q/4KV: one request of 50,001 tokens 49.4 / 38.0
-// / 32.3, 4 of 4K-8K 25.2 / 22.8 / 20.8, 9 up to 4.7K 24.0 / 21.7 / 20.9, 16 up
-// to 2K 21.2 / 20.4 / 21.0, 24 up to 4K 32.1 / 31.5 / 34.5, 64 of 1K-8K 112 /
-// 112 / 117.
+// 1 / 2 / 8 groups, us a call, 32Q/4KV: one request of 50,001 tokens 49.4 /
+// 38.0 / 32.3, 4 of 4K-8K 25.2 / 22.8 / 20.8, 9 up to 4.7K 24.0 / 21.7 / 20.9,
+// 16 up to 2K 21.2 / 20.4 / 21.0, 24 up to 4K 32.1 / 31.5 / 34.5, 64 of 1K-8K
+// 112 / 112 / 117.
 __host__ __device__ __forceinline__ int merge_groups(int B, int R) {
   return 1 + R / B <= 16 ? 2 : 8;
 }
@@ -213,8 +213,8 @@ void decode_diff_kernel(DecodeDiffArgs a) {
   int C = max((U + R - 1) / R, a.min_pages);
   // The merge takes a request's pieces in rounds of 64 (16 with two groups of
   // waves, merge_groups), about 2.5 us each, a page of both waves 0.45 us: a
-  // little longer pieces where they save rounds (one request of 8000 tokens 19.8
-  // -> 17.0 us, of 50,001 as before).
+  // little longer pieces where they save rounds (one request of 8000 tokens
+  // 19.8 -> 17.0 us, of 50,001 as before).
   const int cap = 8 * merge_groups(a.B, R);
   if (most > (int64_t)C * cap) {
     const int r0 = ((most + C - 1) / C + cap - 1) / cap;
@@ -228,15 +228,15 @@ void decode_diff_kernel(DecodeDiffArgs a) {
     }
   }
   // Whole requests, the same number for every range: nothing is split, nothing
-  // joined. Partial results and their merge cost some 1.5 us per 1000 rows (HQ of
-  // each request, of no more than there are ranges), a page above the even share
-  // 0.3 where two waves walk a range, 0.75 where one does; and up to a sixteenth
-  // more is within what an even share spreads. Graph replays, us, evenly / whole:
-  // 32Q/4KV 192 requests of 100-300 tokens 34.3 / 24.4, 128 up to 300 26.4 /
-  // 21.2, 180 of 500-800 57.8 / 50.0, 600 up to 200 61 / 45; 64Q/16KV 96 of
-  // 100-300 43.7 / 37.6, 96 under a window of 512 with contexts of 100-2000 73.8 /
-  // 64.3. What stays even would lose: 64 up to 300 19.9 / 21.9, 64 under a window
-  // of 512 27 / 32, 64Q/16KV 32 up to 300 21 / 30.
+  // joined. Partial results and their merge cost some 1.5 us per 1000 rows (HQ
+  // of each request, of no more than there are ranges), a page above the even
+  // share 0.3 where two waves walk a range, 0.75 where one does; and up to a
+  // sixteenth more is within what an even share spreads. Graph replays, us,
+  // evenly / whole: 32Q/4KV 192 requests of 100-300 tokens 34.3 / 24.4, 128 up
+  // to 300 26.4 / 21.2, 180 of 500-800 57.8 / 50.0, 600 up to 200 61 / 45;
+  // 64Q/16KV 96 of 100-300 43.7 / 37.6, 96 under a window of 512 with contexts
+  // of 100-2000 73.8 / 64.3. What stays even would lose: 64 up to 300 19.9 /
+  // 21.9, 64 under a window of 512 27 / 32, 64Q/16KV 32 up to 300 21 / 30.
   const int per = (a.B + R - 1) / R;
   if (per > 1) {   // the pages of the heaviest range
     most = 0;
@@ -777,10 +777,10 @@ struct Shape {
 // Three work-groups per four CUs, as the plain decode; four waves each, which
 // take 4, 2 or 1 pairs of stored heads of 1, 1 or 2 ranges. Four pairs where
 // there are requests for two thirds of their ranges, which then are likely
-// whole; else two, whose ranges two waves share (graph replays, us, by two / four:
-// 64Q/8KV 8 requests of 1K-8K 37.9 / 41.2, one of 50,000 46.0 / 49.8, 64 of
-// 100-1000 39.9 / 41.5; 64Q/16KV 32 up to 300 20.9 / 22.1, 96 up to 300 38.8 /
-// 37.6, 96 under a window of 512 68.5 / 64.1).
+// whole; else two, whose ranges two waves share (graph replays, us, by two /
+// four: 64Q/8KV 8 requests of 1K-8K 37.9 / 41.2, one of 50,000 46.0 / 49.8, 64
+// of 100-1000 39.9 / 41.5; 64Q/16KV 32 up to 300 20.9 / 22.1, 96 up to 300 38.8
+// / 37.6, 96 under a window of 512 68.5 / 64.1).
 Shape shape_of(int B, int HQ, int HKV, int num_workgroups) {
   Shape s;
   s.rep = group_of(HQ / HKV);

@@ -14,15 +14,15 @@
 // itself (the lengths are a few KB in the L2), holds them in LDS and writes its
 // 1024 elements at a time of the block table, the slot map and the positions:
 // one launch. A new page is read off the stack by whoever needs it, and its
-// entry of the page table written by the work-group that fills that part of
-// the block table, so no work-group waits for another. Where an output is one
-// of the inputs (a graph that steps on in place), or above 1024 requests, one
-// work-group makes the sums and the new pages, and a second launch the rest;
-// a small step in place is one work-group's. Bound by latency: launches and
+// entry of the page table written by the work-group that fills that part of the
+// block table, so no work-group waits for another. Where an output is one of
+// the inputs (a graph that steps on in place), or above 1024 requests, one
+// work-group makes the sums and the new pages, and a second launch the rest; a
+// small step in place is one work-group's. Bound by latency: launches and
 // dependent loads. Graph replays, us a step, where an empty kernel takes 2.1: 4
-// decode rows 3.5, 64 rows 3.8, 96 rows and 2 chunks of 2048 tokens under tables
-// of 4,224 pages 6.4; a release of one row of 500 pages 2.9, of 64 rows of up to
-// 4,096 3.5.
+// decode rows 3.5, 64 rows 3.8, 96 rows and 2 chunks of 2048 tokens under
+// tables of 4,224 pages 6.4; a release of one row of 500 pages 2.9, of 64 rows
+// of up to 4,096 3.5.
 #include "common.h"
 
 namespace tmopt {
@@ -546,8 +546,8 @@ extern "C" int tmopt_release_pages(
   a.first = (int32_t*)workspace;
   const hipStream_t st = (hipStream_t)stream;
   const bool in_place = free_count_out == free_count;
-  // small enough for one work-group (16 rows of 1024 pages 7.5 us by one, 5.6 by
-  // two launches; 8 rows 5.2 / 5.3)
+  // small enough for one work-group (16 rows of 1024 pages 7.5 us by one, 5.6
+  // by two launches; 8 rows 5.2 / 5.3)
   const bool small = B * table_width <= 8192;
   if (B <= kOwnSums && (small || !in_place)) {
     const int64_t groups = B * per > 0 ? B * per : 1;

@@ -4,13 +4,13 @@
 // Matrix bound: per visible (query, key) pair and map 128 products for the
 // score and 256 for the values.
 //
-//  * A work-group of eight waves owns (run, pair of stored heads, block of 128 /
-//    REP queries) for REP head pairs: 128 rows of each map, over the same tiles of 32 keys
-//    (K, K' and the 256-wide V: 32 KB) in LDS. Wave w has map w >> 2 of row
-//    block w & 3 (32 rows), so waves w and w + 4, which share a SIMD, are the
-//    two maps of the same rows. O^T of 32 rows x 256 dims takes 128 registers,
-//    which leaves two waves per SIMD room for 32-key tiles, not for 64-key
-//    ones.
+//  * A work-group of eight waves owns (run, pair of stored heads, block of 128
+//    / REP queries) for REP head pairs: 128 rows of each map, over the same
+//    tiles of 32 keys (K, K' and the 256-wide V: 32 KB) in LDS. Wave w has map
+//    w >> 2 of row block w & 3 (32 rows), so waves w and w + 4, which share a
+//    SIMD, are the two maps of the same rows. O^T of 32 rows x 256 dims takes
+//    128 registers, which leaves two waves per SIMD room for 32-key tiles, not
+//    for 64-key ones.
 //  * S^T = K.Q^T (v_mfma_f32_32x32x16_bf16, keys on M, queries on N) leaves one
 //    query per lane; P^T is then the B operand of O^T = V^T.P^T as it is.
 //  * Tiles go from global memory straight into LDS (buffer_load ... lds), rows
@@ -22,21 +22,24 @@
 //    the softmax of a tile.
 //  * The maps meet in LDS at the end: each wave gives its partner half of its
 //    normalised O and takes the difference and the norm of the other half.
-//  * A launch whose items fit the chip at once takes work-groups of four waves
-//    with 64 rows of each map, two per compute unit: each has two stages, K a tile
-//    ahead of V, and no phases to keep; one's start and end run beside the other's
-//    products. Graph replays, us, eight / four waves: 30 tokens 64Q/8KV 9.4 / 7.9,
-//    600 32Q/4KV 26.6 / 23.7, 777 33.0 / 29.0, 1,200 under a window of 512 32Q/8KV
-//    31.4 / 26.4. Full chips are quicker with eight, whose loads reach three tiles
-//    ahead and serve twice the rows: 64 x 512 358 / 413, 4 x 8,192 2,750 / 2,950.
-//    (Four waves with four stages, one work-group per unit, were slower on both.)
+//  * A launch whose items fit the chip at once, or see few keys each
+//    (layout_of), takes work-groups of four waves with 64 rows of each map, two
+//    per compute unit: each has two stages, K a tile ahead of V, and no phases
+//    to keep; one's start and end run beside the other's products. Graph
+//    replays, us, eight / four waves: 30 tokens 64Q/8KV 9.4 / 7.9, 600 32Q/4KV
+//    26.6 / 23.7, 777 33.0 / 29.0, 1,200 under a window of 512 32Q/8KV 31.4 /
+//    26.4. Full chips are quicker with eight, whose loads reach three tiles
+//    ahead and serve twice the rows: 64 x 512 358 / 413, 4 x 8,192 2,750 /
+//    2,950. (Four waves with four stages, one work-group per unit, were slower
+//    on both.)
 //  * Work items are dealt to the XCDs heaviest first (prefill_sched.h).
 //
-// 4 prompts of 8,192 tokens run at 1,197 TFLOP/s, 4 of 2K-8K at 1,163 (32Q/4KV):
-// matrix cycles are 0.66 of all, at the 1.6 GHz that the power limit leaves a
-// full chip (a plain 8192^3 product 1,263 TFLOP/s at 1.75 GHz). There a tile is
-// 0.97 us of the matrix pipes and takes 1.4; an item's start and end cost some 9
-// us, which no other work-group hides (one per CU by its LDS).
+// 4 prompts of 8,192 tokens run at 1,197 TFLOP/s, 4 of 2K-8K at 1,163
+// (32Q/4KV): matrix cycles are 0.66 of all, at the 1.6 GHz that the power limit
+// leaves a full chip (a plain 8192^3 product 1,263 TFLOP/s at 1.75 GHz). There
+// a tile is 0.97 us of the matrix pipes and takes 1.4; an item's start and end
+// cost some 9 us, which no other work-group hides (one per CU by its LDS and
+// registers).
 #include <type_traits>
 
 #include "diff.h"
@@ -131,10 +134,11 @@ __device__ __forceinline__ int split_item(int pairs, int x) {
 // are quickest, others their share. The estimate, in us: items are taken as
 // evenly spread between `low` and `most` tiles, heaviest first, one work-group
 // per compute unit; a tile takes 1.05 on up to half the units and 1.4 on all
-// (power: 2.1 against 1.6 GHz); pieces cost 5 for their start and the merge, 0.1
-// for each of an item's that it joins, and 0.115 for each of the launch's that
-// is written and read, if all its rows are queries. Of four waves, two per unit:
-// a tile takes 1.0 alone and 1.5 beside another, a piece is half the size.
+// (power: 2.1 against 1.6 GHz); pieces cost 5 for their start and the merge,
+// 0.1 for each of an item's that it joins, and 0.115 for each of the launch's
+// that is written and read, if all its rows are queries. Of four waves, two per
+// unit: a tile takes 1.0 alone and 1.5 beside another, a piece is half the
+// size.
 constexpr int kMinPiece = 4;   // tiles
 template <int W>
 __device__ __forceinline__ int pieces_of(const PrefillDiffArgs& a, int BQ,
@@ -267,8 +271,8 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_diff_kernel(
     klane = grp * kst_b + 16 * kchunk;
     vlane = grp * vst_b + 16 * vchunk;
   }
-  // Eight waves: tile t (index from k_lo) into LDS stage st: 4 instructions. live
-  // == false issues the same ones fetching nothing: the loops issue a tile
+  // Eight waves: tile t (index from k_lo) into LDS stage st: 4 instructions.
+  // live == false issues the same ones fetching nothing: the loops issue a tile
   // every iteration, past the last one too, so that the count of loads in
   // flight is the same on every path and the waits are exact.
   auto issue_tile = [&](int t, int st, bool live = true)
@@ -479,17 +483,17 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_diff_kernel(
 
   const bool rejected = a.reject != nullptr && as_const(a.reject)[0] != 0;
   if (!rejected) {
-    // Eight waves. Slot 2t: group 0 multiplies tile t, group 1 does the softmax of tile t;
-    // slot 2t + 1: group 0 the softmax of tile t + 1, group 1 multiplies tile
-    // t. Tile t + 3 goes out at the start of slot 2t into the stage of tile t -
-    // 1 (last read in slot 2t - 1) and must be in LDS before slot 2t + 4; each
-    // wave waits for its own part at the end of every odd slot, before the
-    // barrier that publishes it.
-    // Four waves. K runs a tile ahead of V: after the products of tile t and the
-    // scores of tile t + 1, a barrier frees V(t) and K(t + 1) for V(t + 2) and K(t
-    // + 3), which have until the next one to arrive.
-    // The queries come first, each wave's own 32 rows through its 8 KB of the
-    // last stages (rows past the run end arrive as zeros).
+    // Eight waves. Slot 2t: group 0 multiplies tile t, group 1 does the softmax
+    // of tile t; slot 2t + 1: group 0 the softmax of tile t + 1, group 1
+    // multiplies tile t. Tile t + 3 goes out at the start of slot 2t into the
+    // stage of tile t - 1 (last read in slot 2t - 1) and must be in LDS before
+    // slot 2t + 4; each wave waits for its own part at the end of every odd
+    // slot, before the barrier that publishes it. Four waves. K runs a tile
+    // ahead of V: after the products of tile t and the scores of tile t + 1, a
+    // barrier frees V(t) and K(t + 1) for V(t + 2) and K(t + 3), which have
+    // until the next one to arrive. The queries come first, each wave's own 32
+    // rows through its 8 KB of the last stages (rows past the run end arrive as
+    // zeros).
     if (w == 0 && a.w.weight)
       dma(make_rsrc(a.w.weight, kDV * 4), wlds, 16 * lane);
     const uint32_t qlds =
@@ -856,17 +860,17 @@ Layout groups_of(int W, int HQ, int HKV) {
 // or the window as bounds of its keys. Up to half the compute units' worth of
 // items, as many pieces as there are units; up to one and a half, two or three
 // pieces an item even out the rounds where keys are many (below 128 tiles two
-// work-groups per unit do it better: a prompt of 1200, 32Q/4KV, 48.8 us a call in
-// pieces, 40.5 whole, of 3000, 16Q/2KV, 99.5 / 92.5); larger grids fill the chip by
-// themselves. The device decides from the lengths. Four waves where all whole items, or the
-// pieces at 20 tiles each or less, are on the chip at once: there an item's start
-// and end weigh most. Graph replays of split calls, us, eight / four waves: 16
-// tokens after 1000, 64Q/8KV 21.7 / 19.3, 300 after 1000, 32Q/4KV 38.7 / 35.6, 128
-// after 8000, 16Q/2KV 45 / 41.8; 64 after 30,000, 64Q/8KV 114 / 123, one after
-// 20,000 48 / 68 (keys are read for half as many rows). And where no query sees
-// more than 8 tiles: 128 prompts of 128, 32Q/4KV 124 / 113, of 200 242 / 212, 128 of
-// 500 under a window of 100 555 / 513 (64 of 256 142 / 146, 40 of 300, 64Q/8KV 234
-// / 239).
+// work-groups per unit do it better: a prompt of 1200, 32Q/4KV, 48.8 us a call
+// in pieces, 40.5 whole, of 3000, 16Q/2KV, 99.5 / 92.5); larger grids fill the
+// chip by themselves. The device decides from the lengths. Four waves where all
+// whole items, or the pieces at 20 tiles each or less, are on the chip at once:
+// there an item's start and end weigh most. Graph replays of split calls, us,
+// eight / four waves: 16 tokens after 1000, 64Q/8KV 21.7 / 19.3, 300 after
+// 1000, 32Q/4KV 38.7 / 35.6, 128 after 8000, 16Q/2KV 45 / 41.8; 64 after
+// 30,000, 64Q/8KV 114 / 123, one after 20,000 48 / 68 (keys are read for half
+// as many rows). And where no query sees more than 8 tiles: 128 prompts of 128,
+// 32Q/4KV 124 / 113, of 200 242 / 212, 128 of 500 under a window of 100 555 /
+// 513 (64 of 256 142 / 146, 40 of 300, 64Q/8KV 234 / 239).
 Layout layout_of(int HQ, int HKV, int64_t S, int max_seqlen,
                  int64_t bt_stride, int window, bool split) {
   const int64_t cus = device_cus();
@@ -926,8 +930,8 @@ int launch(const PrefillDiffArgs& a, hipStream_t st) {
   if (a.nsplit <= 1) return launch_whole<W, REP, false>(a, st);
   const int rc = launch_whole<W, REP, true>(a, st);
   if (rc) return rc;
-  // many pieces of few items: four groups (3 queries after 22,000, 16Q/2KV, 58 us
-  // a call with one and the pieces of an item on one XCD, 48 so)
+  // many pieces of few items: four groups (3 queries after 22,000, 16Q/2KV, 58
+  // us a call with one and the pieces of an item on one XCD, 48 so)
   const dim3 grid(a.n_base, 2 * W);
   if (a.nsplit > 8)
     hipLaunchKernelGGL((prefill_diff_merge<W, REP, 4>), grid, dim3(1024), 0, st,
