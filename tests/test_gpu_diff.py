@@ -761,3 +761,31 @@ def test_prefill_many_short_runs(tm, dev, hq, hkv, window):
     _prefill(tm, _rand((T, hq, D), g, dev), _rand((T, hkv, D), g, dev),
              _rand((T, hkv, D), g, dev), _cu(lens, dev), _weights(hq, g, dev),
              window=window)
+
+
+@pytest.mark.parametrize("bound", [400, 200])
+def test_prefill_large_strides_outputs_and_reject(tm, dev, bound):
+    """As the smaller launches: tensors inside wider ones, outputs given, rows
+    past the last run left as they were, a refused step."""
+    g = _gen(25)
+    lens = [70, 1, 130, 0, 33] * 16
+    n = sum(lens)
+    T = n + 29
+    q = _rand((T, 3, 16, 136), g, dev)[:, 1, :, 8:]
+    kv = _rand((T, 2, 6, D), g, dev)
+    k, v = kv[:, 0, 1:5], kv[:, 1, 2:]
+    cu, w = _cu(lens, dev), _weights(16, g, dev)
+    big = torch.full((T, 9, 264), 7.0, dtype=BF, device=dev)
+    out, lse = big[:, :8, :256], torch.full((16, T), 7.0, device=dev)
+    _prefill(tm, q, k, v, cu, w, call=dict(out=out, lse=lse,
+                                           max_seqlen=bound))
+    assert (big[n:] == 7).all() and (big[:, 8] == 7).all()
+    assert (big[..., 256:] == 7).all() and (lse[:, n:] == 7).all()
+    for flag in (0, 1, 0):
+        r = torch.tensor([flag], dtype=torch.int32, device=dev)
+        o, l = tm.prefill_diff_varlen(
+            q[:n], k[:n], v[:n], cu, w["lam"], 0.1, max_seqlen=bound,
+            reject=r, **{x: y for x, y in _user(w).items() if x != "lam"})
+        assert torch.isnan(o).all() == bool(flag)
+        assert torch.isnan(l).all() == bool(flag)
+        assert flag or (torch.equal(o, out[:n]) and torch.equal(l, lse[:, :n]))
