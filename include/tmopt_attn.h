@@ -537,21 +537,25 @@ int tmopt_attn_decode_diff(const void* q, const void* k_pool,
  * out: [total, HQ / 2, 2 D] with element strides (% 8, 16-byte aligned), the
  * 2 D contiguous; lse fp32 [HQ, total] rows of lse_stride_head elements, or
  * NULL. Rows past the last run are left as they were.
+ * max_context: an upper bound of prior + run length, or 0: the row width of the
+ * block table bounds it. It decides about the launch's layout alone.
  * workspace: scratch of tmopt_attn_prefill_diff_workspace_size bytes, 16-byte
  * aligned, without initialisation; NULL: the keys of a block of queries are
  * not split over work-groups.
  */
 size_t tmopt_attn_prefill_diff_workspace_size(int num_seqs, int max_seqlen_q,
-                                              int HQ, int HKV,
-                                              int64_t bt_stride, int window);
+                                              int64_t max_context, int HQ,
+                                              int HKV, int64_t bt_stride,
+                                              int window);
 int tmopt_attn_prefill_diff(
     const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k,
     int64_t k_stride_tok, int64_t k_stride_head, const void* v,
     int64_t v_stride_tok, int64_t v_stride_head, const int32_t* cu_seqlens_q,
     const int32_t* prior_lens, int num_seqs, int max_seqlen_q,
-    const void* k_pool, const void* v_pool, const int32_t* block_table,
-    int64_t bt_stride, int page_size, int64_t num_pages, int HQ, int HKV,
-    int D, int window, float scale, const float* lam, int lam_stride,
+    int64_t max_context, const void* k_pool, const void* v_pool,
+    const int32_t* block_table, int64_t bt_stride, int page_size,
+    int64_t num_pages, int HQ, int HKV, int D, int window, float scale,
+    const float* lam, int lam_stride,
     const float* norm_weight, float norm_eps, float out_scale, void* out,
     int64_t o_stride_tok, int64_t o_stride_head, float* lse,
     int64_t lse_stride_head, const int32_t* reject, void* workspace,

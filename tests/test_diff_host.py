@@ -46,16 +46,16 @@ def test_decode_refusals(tm):
 def test_prefill_refusals(tm):
     lib, e = tm._lib.load(), tm._lib
     size = lib.tmopt_attn_prefill_diff_workspace_size
-    for bad in ((0, 64, 32, 4), (1, 0, 32, 4), (1, 64, 0, 4), (1, 64, 32, 0),
-                (-1, 64, 32, 4), (1, 64, 33, 4)):
+    for bad in ((0, 64, 0, 32, 4), (1, 0, 0, 32, 4), (1, 64, 0, 0, 4),
+                (1, 64, 0, 32, 0), (-1, 64, 0, 32, 4), (1, 64, 0, 33, 4)):
         assert size(*bad, 500, 0) == 0
 
     def call(q=P, qt=4096, k=P, kt=512, kh=128, v=P, cu=P, prior=NULL, S=2,
-             n=64, kp=NULL, vp=NULL, bt=NULL, bts=8, ps=16, pages=9, HQ=32,
+             n=64, most=0, kp=NULL, vp=NULL, bt=NULL, bts=8, ps=16, pages=9, HQ=32,
              HKV=4, D=128, window=0, scale=0.1, lam=P, out=P, ot=4096, lse=P,
              ws=NULL, nbytes=0):
         return lib.tmopt_attn_prefill_diff(
-            q, qt, 128, k, kt, kh, v, kt, kh, cu, prior, S, n, kp, vp, bt,
+            q, qt, 128, k, kt, kh, v, kt, kh, cu, prior, S, n, most, kp, vp, bt,
             bts, ps, pages, HQ, HKV, D, window, scale, lam, 1, NULL, 0.0, 1.0,
             out, ot, 256, lse, 128, NULL, ws, nbytes, NULL)
     pool = dict(k=NULL, v=NULL, kp=P, vp=P, bt=P)
@@ -66,21 +66,24 @@ def test_prefill_refusals(tm):
                dict(k=ODD), dict(kt=500), dict(kt=-512), dict(kh=100),
                dict(prior=P), dict(HQ=33), dict(HQ=3, HKV=3),
                dict(window=-1), dict(scale=0.0), dict(scale=math.nan),
-               dict(lam=NULL), dict(bt=P, kp=P, vp=P),
+               dict(most=-1), dict(lam=NULL), dict(bt=P, kp=P, vp=P),
                dict(pool, kp=NULL), dict(pool, vp=ODD), dict(pool, bts=0),
                dict(pool, pages=0)):
         assert call(**kw) == e.TMOPT_EINVAL, kw
     for kw in (dict(D=64), dict(pool, ps=32), dict(n=1 << 18),
                dict(n=1 << 17, qt=128, kt=1 << 14)):
         assert call(**kw) == e.TMOPT_EUNSUPPORTED, kw
-    need = size(2, 64, 32, 4, 500, 0)
+    need = size(2, 64, 0, 32, 4, 500, 0)
     assert 0 < need <= 256 * 3 * 258 * 1024
     for kw in (dict(ws=ctypes.c_void_p(8), nbytes=need),
                dict(ws=P, nbytes=need - 1)):
         assert call(**dict(pool, bts=500, **kw)) == e.TMOPT_EWORKSPACE, kw
     # without a block table only the run's own length counts
-    assert size(1, 200, 32, 4, 0, 0) == 0 < size(1, 4000, 4, 2, 0, 0)
-    assert size(1, 4000, 4, 2, 0, 100) == 0
+    assert size(1, 200, 0, 32, 4, 0, 0) == 0 < size(1, 4000, 0, 4, 2, 0, 0)
+    assert size(1, 4000, 0, 4, 2, 0, 100) == 0
+    # a bound of the contexts counts where it is below the table's width
+    assert size(2, 64, 900, 32, 4, 500, 0) == 0
+    assert size(2, 64, 1 << 40, 32, 4, 500, 0) == need
 
 
 def test_plan_refusals(tm):

@@ -106,13 +106,13 @@ SIGNATURES = {
         _c_i32, _c_ptr, _c_f32, _c_f32, _c_i32, _c_i32, _c_ptr, _c_ptr,
         _c_ptr, _c_size, _c_ptr]),
     "tmopt_attn_prefill_diff_workspace_size": (_c_size, [
-        _c_i32, _c_i32, _c_i32, _c_i32, _c_i64, _c_i32]),
+        _c_i32, _c_i32, _c_i64, _c_i32, _c_i32, _c_i64, _c_i32]),
     "tmopt_attn_prefill_diff": (_c_i32, [
         _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64,
-        _c_i64, _c_ptr, _c_ptr, _c_i32, _c_i32, _c_ptr, _c_ptr, _c_ptr,
-        _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_f32,
-        _c_ptr, _c_i32, _c_ptr, _c_f32, _c_f32, _c_ptr, _c_i64, _c_i64,
-        _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_size, _c_ptr]),
+        _c_i64, _c_ptr, _c_ptr, _c_i32, _c_i32, _c_i64, _c_ptr, _c_ptr,
+        _c_ptr, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,
+        _c_f32, _c_ptr, _c_i32, _c_ptr, _c_f32, _c_f32, _c_ptr, _c_i64,
+        _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_size, _c_ptr]),
     "tmopt_plan_pages": (_c_i32, [
         _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i32, _c_ptr,
         _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr,

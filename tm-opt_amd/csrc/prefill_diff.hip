@@ -40,6 +40,7 @@
 // a tile is 0.97 us of the matrix pipes and takes 1.4; an item's start and end
 // cost some 9 us, which no other work-group hides (one per CU by its LDS and
 // registers).
+#include <algorithm>
 #include <type_traits>
 
 #include "diff.h"
@@ -856,8 +857,8 @@ Layout groups_of(int W, int HQ, int HKV) {
   return Layout{W, rep, HQ / 2 / rep, 16 * W / rep, 1, 0};
 }
 
-// From what the host knows: the longest run, and the row width of a block table
-// or the window as bounds of its keys. Up to half the compute units' worth of
+// From what the host knows: the longest run, and the row width of a block
+// table, the longest context or the window as bounds of its keys. Up to half the compute units' worth of
 // items, as many pieces as there are units; up to one and a half, two or three
 // pieces an item even out the rounds where keys are many (below 128 tiles two
 // work-groups per unit do it better: a prompt of 1200, 32Q/4KV, 48.8 us a call
@@ -872,7 +873,8 @@ Layout groups_of(int W, int HQ, int HKV) {
 // 32Q/4KV 124 / 113, of 200 242 / 212, 128 of 500 under a window of 100 555 /
 // 513 (64 of 256 142 / 146, 40 of 300, 64Q/8KV 234 / 239).
 Layout layout_of(int HQ, int HKV, int64_t S, int max_seqlen,
-                 int64_t bt_stride, int window, bool split) {
+                 int64_t max_context, int64_t bt_stride, int window,
+                 bool split) {
   const int64_t cus = device_cus();
   const Layout w4 = groups_of(4, HQ, HKV), w8 = groups_of(8, HQ, HKV);
   auto count = [&](const Layout& x) {
@@ -880,6 +882,7 @@ Layout layout_of(int HQ, int HKV, int64_t S, int max_seqlen,
   };
   auto tiles_of = [&](const Layout& x) {
     int64_t keys = bt_stride > 0 ? bt_stride * kPage : max_seqlen;
+    if (max_context > 0) keys = std::min(keys, max_context);
     if (window > 0 && keys > (int64_t)window + x.BQ + kBN)
       keys = (int64_t)window + x.BQ + kBN;
     return (keys + kBN - 1) / kBN;
@@ -948,13 +951,14 @@ int launch(const PrefillDiffArgs& a, hipStream_t st) {
 using namespace tmopt;
 
 extern "C" size_t tmopt_attn_prefill_diff_workspace_size(
-    int num_seqs, int max_seqlen_q, int HQ, int HKV, int64_t bt_stride,
-    int window) {
+    int num_seqs, int max_seqlen_q, int64_t max_context, int HQ, int HKV,
+    int64_t bt_stride, int window) {
   if (num_seqs <= 0 || max_seqlen_q <= 0 || HQ <= 0 || HKV <= 0 ||
       HKV % 2 != 0 || HQ % HKV != 0)
     return 0;
   return (size_t)workspace_bytes_of(
-      layout_of(HQ, HKV, num_seqs, max_seqlen_q, bt_stride, window, true));
+      layout_of(HQ, HKV, num_seqs, max_seqlen_q, max_context, bt_stride, window,
+                true));
 }
 
 extern "C" int tmopt_attn_prefill_diff(
@@ -962,12 +966,12 @@ extern "C" int tmopt_attn_prefill_diff(
     int64_t k_stride_tok, int64_t k_stride_head, const void* v,
     int64_t v_stride_tok, int64_t v_stride_head, const int32_t* cu_seqlens_q,
     const int32_t* prior_lens, int num_seqs, int max_seqlen_q,
-    const void* k_pool, const void* v_pool, const int32_t* block_table,
-    int64_t bt_stride, int page_size, int64_t num_pages, int HQ, int HKV,
-    int D, int window, float scale, const float* lam, int lam_stride,
-    const float* norm_weight, float norm_eps, float out_scale, void* out,
-    int64_t o_stride_tok, int64_t o_stride_head, float* lse,
-    int64_t lse_stride_head, const int32_t* reject, void* workspace,
+    int64_t max_context, const void* k_pool, const void* v_pool,
+    const int32_t* block_table, int64_t bt_stride, int page_size,
+    int64_t num_pages, int HQ, int HKV, int D, int window, float scale,
+    const float* lam, int lam_stride, const float* norm_weight, float norm_eps,
+    float out_scale, void* out, int64_t o_stride_tok, int64_t o_stride_head,
+    float* lse, int64_t lse_stride_head, const int32_t* reject, void* workspace,
     size_t workspace_bytes, tmopt_stream_t stream) {
   clear_error();
   if (num_seqs == 0 || max_seqlen_q == 0) return TMOPT_OK;
@@ -976,6 +980,8 @@ extern "C" int tmopt_attn_prefill_diff(
                 num_seqs, max_seqlen_q);
   TMOPT_REQUIRE(q && out && cu_seqlens_q, TMOPT_EINVAL,
                 "prefill_diff: null q/out/cu_seqlens");
+  TMOPT_REQUIRE(max_context >= 0, TMOPT_EINVAL,
+                "prefill_diff: max_context=%lld", (long long)max_context);
   const int rc = check_diff("prefill_diff", HQ, HKV, D, window, scale, lam,
                             lam_stride, norm_weight, norm_eps);
   if (rc) return rc;
@@ -1017,8 +1023,8 @@ extern "C" int tmopt_attn_prefill_diff(
                   "prefill_diff: a run's k/v span must stay below 2 GiB");
   }
   const Layout x =
-      layout_of(HQ, HKV, num_seqs, max_seqlen_q, paged ? bt_stride : 0, window,
-                workspace != nullptr);
+      layout_of(HQ, HKV, num_seqs, max_seqlen_q, max_context,
+                paged ? bt_stride : 0, window, workspace != nullptr);
   TMOPT_REQUIRE(x.n_base < 0x7fffffff, TMOPT_EUNSUPPORTED,
                 "prefill_diff: %lld work-groups exceed the grid limit",
                 (long long)x.n_base);

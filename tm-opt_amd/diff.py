@@ -169,8 +169,9 @@ def prefill_diff_varlen(q, k, v, cu_seqlens, lam, scale, norm_weight=None,
     runs and the table's width. max_context: an upper bound of prior + run
     length, where the host has one; without it the row width of the block
     table bounds the keys, and short contexts under a wide table pay for the
-    second launch (64Q/8KV, 4,134 pages: 64 tokens without context 16.6 us
-    against 8.9). It decides about the split alone.
+    second launch (64Q/8KV, 4,134 pages: 64 tokens without context 16.8 us
+    against 9.0, 30 after 2,000 31.2 against 24.6). It decides about the
+    launch's layout alone.
     Returns (out [total, HQ / 2, 256] bf16, lse [HQ, total] fp32 or None)."""
     total, HQ, D = q.shape
     dev = q.device
@@ -213,20 +214,15 @@ def prefill_diff_varlen(q, k, v, cu_seqlens, lam, scale, norm_weight=None,
         assert lse.is_contiguous() and lse.device == dev
     elif return_lse:
         lse = torch.empty((HQ, total), dtype=torch.float32, device=dev)
-    keys = bts
-    if bts and max_context is not None:
-        keys = max(1, min(bts, -(-int(max_context) // PAGE_SIZE)))
+    most = 0 if max_context is None else max(1, int(max_context))
     max_seqlen, window = int(max_seqlen), int(window)
-    n = _workspace_size(dev, _PREFILL_SIZE, S, max_seqlen, HQ, HKV, keys,
+    n = _workspace_size(dev, _PREFILL_SIZE, S, max_seqlen, most, HQ, HKV, bts,
                         window)
-    if n and keys != bts:       # (the launch sizes its scratch by the table)
-        n = _workspace_size(dev, _PREFILL_SIZE, S, max_seqlen, HQ, HKV, bts,
-                            window)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     _call(dev, "tmopt_attn_prefill_diff", q.data_ptr(), q.stride(0),
           q.stride(1), _ptr(k), strides[0], strides[1], _ptr(v), strides[2],
           strides[3], cu_seqlens.data_ptr(), _ptr(prior_lens), S, max_seqlen,
-          _ptr(k_pool), _ptr(v_pool), _ptr(block_table), bts, page_size, P,
+          most, _ptr(k_pool), _ptr(v_pool), _ptr(block_table), bts, page_size, P,
           HQ, HKV, D, window, float(scale), *w, out.data_ptr(), out.stride(0),
           out.stride(1), _ptr(lse), total, _ptr(reject), _ptr(ws), n)
     return out, lse
