@@ -166,7 +166,8 @@ def prefill_diff_varlen(q, k, v, cu_seqlens, lam, scale, norm_weight=None,
     A launch of few query blocks that may see many keys splits these over
     work-groups and joins the pieces: a second launch, up to 3 x 257 KB of
     scratch per compute unit, and last bits that depend on the launch's other
-    runs and the table's width. max_context: an upper bound of prior + run
+    runs and the table's width. (So may those of a window's rows on how many
+    runs share a launch: small ones take blocks of other sizes.) max_context: an upper bound of prior + run
     length, where the host has one; without it the row width of the block
     table bounds the keys, and short contexts under a wide table pay for the
     second launch (64Q/8KV, 4,134 pages: 64 tokens without context 16.8 us
