@@ -476,6 +476,19 @@ int tmopt_prefill_check_positions(const int64_t* q_positions,
                                   const int64_t* kv_positions, int64_t T,
                                   int32_t* reject, tmopt_stream_t stream);
 
+/*
+ * NaN into `rows` rows of out [rows, heads, dim] bf16 (element strides % 4, dim
+ * contiguous and % 4, 8-byte aligned) and of lse [lse_heads, rows] fp32 (rows of
+ * lse_stride_head elements, or NULL) where *reject is nonzero, nothing
+ * otherwise. For steps whose refusal leaves them without runs
+ * (tmopt_plan_pages): a prefill of such bounds owns no row, so what its outputs
+ * held before would stay. Before or after the prefill, on its stream.
+ */
+int tmopt_refused_rows(const int32_t* reject, void* out, int64_t o_stride_tok,
+                       int64_t o_stride_head, int64_t rows, int heads, int dim,
+                       float* lse, int64_t lse_stride_head, int lse_heads,
+                       tmopt_stream_t stream);
+
 /* ------------------------------------------------------------------------ */
 /* Differential attention                                                   */
 /* ------------------------------------------------------------------------ */
@@ -587,7 +600,8 @@ int tmopt_attn_prefill_diff(
  *                min(table_width, width) tokens, more than max_tokens in all,
  *                or more pages than are free. A rejected step takes no page
  *                and has no tokens: block_table and slot_mapping are -1,
- *                cu_seqlens and positions 0, seq_lens the contexts.
+ *                cu_seqlens and positions 0, seq_lens the contexts (a
+ *                prefill of it owns no row: tmopt_refused_rows).
  * No other outputs may overlap inputs or each other. B <= 8192 (0: no
  * request), table_rows <= 262144, max_tokens, width and table_width <= 2^24.
  */

@@ -98,6 +98,9 @@ SIGNATURES = {
         _c_i32, _c_i32, _c_i32, _c_i32, _c_i64, _c_i32, _c_i32]),
     "tmopt_prefill_check_positions": (_c_i32, [
         _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr]),
+    "tmopt_refused_rows": (_c_i32, [
+        _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_ptr,
+        _c_i64, _c_i32, _c_ptr]),
     "tmopt_attn_decode_diff_workspace_size": (_c_size, [
         _c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
     "tmopt_attn_decode_diff": (_c_i32, [

@@ -469,8 +469,9 @@ def prefill_varlen(q, k, v, cu_seqlens, scale, window=0, max_seqlen=None,
     rel: optional fused relative bias [total, HQ, E] (last axis contiguous,
     any token/head strides): pair (q, k) of head h adds rel[q_row, h,
     pos_q - pos_k] inside 0 <= dist < E (attn_prefill.py:115-120).
-    reject: optional int32 device scalar; nonzero -> NaN outputs (device-side
-    input rejection without a host sync).
+    reject: optional int32 device scalar; nonzero -> NaN in every row of out
+    and lse, those that cu_seqlens gives no run included (device-side input
+    rejection without a host sync).
     A launch of few query blocks that may see many keys splits these over
     work-groups and merges the pieces: a second launch, up to 2 x 129 KB of
     scratch per compute unit (66 MB), and last bits of the results that depend
@@ -483,10 +484,22 @@ def prefill_varlen(q, k, v, cu_seqlens, scale, window=0, max_seqlen=None,
     decides about the split alone.
     Returns (out [total, HQ, D] bf16, lse [HQ, total] fp32 or None).
     Reference: engine/pyengine/kernels/attn_prefill.py:71-194."""
-    return _prefill_varlen(q, k, v, cu_seqlens, scale, window, max_seqlen,
-                           prior_lens, k_pool, v_pool, block_table,
-                           table_wrap, rel, out, lse, return_lse, reject,
-                           max_context)
+    out, lse = _prefill_varlen(q, k, v, cu_seqlens, scale, window, max_seqlen,
+                               prior_lens, k_pool, v_pool, block_table,
+                               table_wrap, rel, out, lse, return_lse, reject,
+                               max_context)
+    if reject is not None:
+        _lib.call("tmopt_refused_rows", *_refused_rows(reject, out, lse),
+                  _stream(q.device))
+    return out, lse
+
+
+def _refused_rows(reject, out, lse):
+    """The C arguments of the launch that a refused step's outputs need where
+    its cu_seqlens gives no run (plan_pages)."""
+    return (_ptr(reject), _ptr(out), out.stride(0), out.stride(1), *out.shape,
+            _ptr(lse), *((0, 0) if lse is None else
+                         (lse.stride(0), lse.shape[0])))
 
 
 def _prefill_varlen(q, k, v, cu_seqlens, scale, window, max_seqlen,

@@ -352,9 +352,10 @@ def attn_prefill_fused(q, k, v, rel, q_positions, kv_positions, window,
             "caches must be empty (chunked prefill: prefill_chunk_state)"
         lens = [T] * B if lens is None else [int(x) for x in lens]
         _append_rows(kr, vr, caches, lens)
-    attn.prefill_varlen(qp, kr, vr, cu, 1.0 / D, window=w, max_seqlen=T,
-                        rel=relp, out=out.view(B * T, H, D),
-                        return_lse=False, reject=reject)
+    # (every row is a run's: no launch for rows without one)
+    attn._prefill_varlen(qp, kr, vr, cu, 1.0 / D, w, T, None, None, None,
+                         None, 0, relp, out.view(B * T, H, D), None, False,
+                         reject)
     return out
 
 
@@ -460,12 +461,11 @@ def attn_prefill_chunk_global(q, k, v, rel, pool_kp, pool_vp, table_dev,
         total if cu_seqlens is None else None, reject=True)
     if cu_seqlens is not None:
         cu = cu_seqlens
-    out, _ = attn.prefill_varlen(q, k, v, cu, 1.0 / D, window=0,
-                                 max_seqlen=max_seqlen, prior_lens=start,
-                                 k_pool=pool_kp, v_pool=pool_vp,
-                                 block_table=table, rel=rel,
-                                 return_lse=False, reject=reject,
-                                 max_context=max_context)
+    # (a slot outside the table leaves the runs as they are, so the prefill
+    # itself writes every row's NaN)
+    out, _ = attn._prefill_varlen(q, k, v, cu, 1.0 / D, 0, max_seqlen, start,
+                                  pool_kp, pool_vp, table, 0, rel, None, None,
+                                  False, reject, max_context)
     attn.kv_write_paged(k, v, table, start, pool_kp, pool_vp, cu_seqlens=cu,
                         max_seqlen=max_seqlen)
     return out

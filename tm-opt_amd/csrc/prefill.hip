@@ -93,10 +93,62 @@ __global__ __launch_bounds__(1024) void positions_check_kernel(
   if (threadIdx.x == 0) reject[0] = bad ? 1 : 0;
 }
 
+// NaN over the outputs of a refused step, 8 bytes (4 dims) or one LSE a thread
+// and turn; nothing otherwise. (A launch of its own, since a step may be refused
+// with bounds that give the prefill's work-groups no row; it adds 1.6 us to a
+// call in a graph.)
+__global__ __launch_bounds__(256) void refused_rows_kernel(
+    const int32_t* reject, __bf16* out, int64_t o_st, int64_t o_sh,
+    int64_t rows, int heads, int units, float* lse, int64_t lse_sh,
+    int lse_heads) {
+  if (as_const(reject)[0] == 0) return;
+  const int64_t step = (int64_t)gridDim.x * 256;
+  const int64_t x0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row_units = (int64_t)heads * units;
+  for (int64_t x = x0; x < rows * row_units; x += step) {
+    const int64_t row = x / row_units;
+    const int i = (int)(x - row * row_units);
+    *reinterpret_cast<u32x2*>(out + row * o_st + (int64_t)(i / units) * o_sh +
+                              4 * (i % units)) =
+        u32x2{0x7fc07fc0u, 0x7fc07fc0u};
+  }
+  if (lse)
+    for (int64_t x = x0; x < rows * lse_heads; x += step)
+      lse[x / rows * lse_sh + x % rows] = __builtin_nanf("");
+}
+
 }  // namespace
 }  // namespace tmopt
 
 using namespace tmopt;
+
+extern "C" int tmopt_refused_rows(const int32_t* reject, void* out,
+                                  int64_t o_stride_tok, int64_t o_stride_head,
+                                  int64_t rows, int heads, int dim, float* lse,
+                                  int64_t lse_stride_head, int lse_heads,
+                                  tmopt_stream_t stream) {
+  clear_error();
+  if (rows == 0) return TMOPT_OK;
+  TMOPT_REQUIRE(reject && out, TMOPT_EINVAL, "refused_rows: null pointer");
+  TMOPT_REQUIRE(rows > 0 && heads > 0 && dim > 0 && dim % 4 == 0 &&
+                    (int64_t)heads * dim <= 0x7fffffff &&
+                    o_stride_tok % 4 == 0 && o_stride_head % 4 == 0 &&
+                    (uintptr_t)out % 8 == 0 &&
+                    (!lse || (lse_heads > 0 && lse_heads <= (1 << 20))),
+                TMOPT_EINVAL,
+                "refused_rows: rows=%lld heads=%d dim=%d lse_heads=%d, or "
+                "rows misaligned",
+                (long long)rows, heads, dim, lse_heads);
+  TMOPT_REQUIRE(rows <= (1ll << 31), TMOPT_EUNSUPPORTED,
+                "refused_rows: %lld rows", (long long)rows);
+  const int64_t wgs = (rows * heads * (dim / 4) + 2047) / 2048;
+  hipLaunchKernelGGL(refused_rows_kernel,
+                     dim3((unsigned)(wgs < 512 ? wgs : 512)), dim3(256), 0,
+                     (hipStream_t)stream, reject, (__bf16*)out, o_stride_tok,
+                     o_stride_head, rows, heads, dim / 4, lse, lse_stride_head,
+                     lse_heads);
+  return check_launch("refused_rows");
+}
 
 extern "C" int tmopt_prefill_check_positions(const int64_t* q_positions,
                                              const int64_t* kv_positions,

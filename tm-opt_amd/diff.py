@@ -20,7 +20,8 @@ import functools
 import torch
 
 from . import _lib
-from .attn import HEAD_DIM, PAGE_SIZE, _check_rows, _ptr, _stream
+from .attn import (HEAD_DIM, PAGE_SIZE, _check_rows, _ptr, _refused_rows,
+                   _stream)
 
 _BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 _DECODE_SIZE = "tmopt_attn_decode_diff_workspace_size"
@@ -161,7 +162,8 @@ def prefill_diff_varlen(q, k, v, cu_seqlens, lam, scale, norm_weight=None,
         context included, from k_pool/v_pool [num_pages, 16, HKV, 128]; the
         run's own keys must already be there.
     lam fp32 [HQ / 2] or [1]. reject: optional int32 device scalar; nonzero
-    gives NaN outputs. max_seqlen bounds the run lengths (read from the
+    gives NaN in every row of out and lse, those that cu_seqlens gives no run
+    included. max_seqlen bounds the run lengths (read from the
     device, with a synchronisation, if None).
     A launch of few query blocks that may see many keys splits these over
     work-groups and joins the pieces: a second launch, up to 3 x 257 KB of
@@ -226,4 +228,6 @@ def prefill_diff_varlen(q, k, v, cu_seqlens, lam, scale, norm_weight=None,
           most, _ptr(k_pool), _ptr(v_pool), _ptr(block_table), bts, page_size, P,
           HQ, HKV, D, window, float(scale), *w, out.data_ptr(), out.stride(0),
           out.stride(1), _ptr(lse), total, _ptr(reject), _ptr(ws), n)
+    if reject is not None:
+        _call(dev, "tmopt_refused_rows", *_refused_rows(reject, out, lse))
     return out, lse

@@ -62,7 +62,8 @@ def plan_pages(page_table, slots, ctx_lens, new_lens, free_pages, free_count,
     tokens, too few free pages) gives reject = 1, takes no page and has no
     tokens: block table and slot mapping -1, cu_seqlens and positions 0,
     seq_lens the contexts. prefill_varlen and prefill_diff_varlen take reject
-    as it is."""
+    as it is, and their outputs are NaN whole then; a KV write of such a plan
+    writes nothing, a decode gives zeros."""
     dev, B, T = page_table.device, slots.numel(), int(max_tokens)
     _check_state(dev, page_table, free_pages, free_count)
     _check_index(slots, torch.int64, B, dev)
