@@ -508,6 +508,8 @@ int tmopt_refused_rows(const int32_t* reject, void* out, int64_t o_stride_tok,
  * norm_weight:  fp32 [256], 16-byte aligned; norm_eps > 0 with it.
  * Sums, maxima, the difference and the norm are fp32; probabilities are
  * rounded to bf16 for their product with the values, outputs once.
+ * A visible key whose score is NaN or +infinity gives NaN in its map's LSE and in
+ * the pair's outputs of the queries that see it; one of -infinity has weight 0.
  */
 
 /*

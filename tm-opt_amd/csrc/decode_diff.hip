@@ -448,8 +448,9 @@ void decode_diff_kernel(DecodeDiffArgs a) {
   auto finish_piece = [&](int b, int flags) {
     const float l_tot = lane_pair(lane_pair(l_part, 16, false), 32, false);
     const float inv = l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
+    // (a key that is no number makes the sum none: neither is the LSE)
     const float lse_nat =
-        l_tot > 0.0f ? (m_run + fast_log2(l_tot)) * kLn2 : -INFINITY;
+        l_tot == 0.0f ? -INFINITY : (m_run + fast_log2(l_tot)) * kLn2;
     const ArgsPtr ra = rare_args();
     const int HQ = ra->HQ;
     if (flags & kWhole) {
@@ -730,7 +731,7 @@ __global__ __launch_bounds__(128 * H * S) void decode_diff_merge(
   acc = acc * inv;
   if (sub == 0 && hok && a.lse && lane == 0)
     a.lse[(int64_t)b * a.HQ + 2 * h + m] =
-        sum > 0.0f ? mx + fast_log2(sum) * kLn2 : -INFINITY;
+        sum == 0.0f ? -INFINITY : mx + fast_log2(sum) * kLn2;
   // the second map goes to the first one's wave
   if (sub == 0 && m == 1) put();
   __syncthreads();

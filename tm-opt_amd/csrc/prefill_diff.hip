@@ -598,6 +598,9 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_diff_kernel(
   const float l_tot = lane_pair(l_part, 32, false);
   const float inv = rejected ? __builtin_nanf("") :
                     l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
+  // (a key that is no number makes the sum none: neither is the LSE)
+  const float lse_nat =
+      l_tot == 0.0f ? -INFINITY : (m_run + fast_log2(l_tot)) * kLn2;
   if (SPLIT && np > 1) {
     // lane-major partial: every store writes 1 KB (of rows past the run,
     // nothing)
@@ -613,14 +616,12 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_diff_kernel(
                     o_acc[db][4 * g4 + 2] * inv, o_acc[db][4 * g4 + 3] * inv};
     if (h2 == 0)
       a.part_lse[pw * 32 + l32] =
-          rejected ? __builtin_nanf("") :
-          l_tot > 0.0f ? (m_run + fast_log2(l_tot)) * kLn2 : -INFINITY;
+          rejected ? __builtin_nanf("") : lse_nat;
     return;
   }
   if (a.lse && h2 == 0 && qok)
     a.lse[(2 * hp + map) * a.lse_sh + t0 + qi] =
-        rejected ? __builtin_nanf("") :
-        l_tot > 0.0f ? (m_run + fast_log2(l_tot)) * kLn2 : -INFINITY;
+        rejected ? __builtin_nanf("") : lse_nat;
   // dims 128 map .. +127 are this wave's; the others go to its partner, lane by
   // lane (16 bytes each: 1 KB per store)
   const uint32_t mine = lds0 + (uint32_t)w * 16384 + 16 * lane;
@@ -795,7 +796,7 @@ __global__ __launch_bounds__(256 * S) void prefill_diff_merge(
   if (a.lse && c < 2 && qok)
     a.lse[(2 * hp + c) * a.lse_sh + wk.t0 + qi] =
         rejected ? __builtin_nanf("") :
-        sum[c] > 0.0f ? m[c] + fast_log2(sum[c]) * kLn2 : -INFINITY;
+        sum[c] == 0.0f ? -INFINITY : m[c] + fast_log2(sum[c]) * kLn2;
   const float inv0 = sum[0] > 0.0f ? 1.0f / sum[0] : 0.0f;
   const float inv1 = sum[1] > 0.0f ? 1.0f / sum[1] : 0.0f;
   float ss = 0.0f;
