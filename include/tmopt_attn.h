@@ -618,10 +618,12 @@ int tmopt_plan_pages(int32_t* page_table, int64_t table_rows,
                      int32_t* reject, tmopt_stream_t stream);
 
 /*
- * Pushes the ceil(lens[i] / 16) pages of table row slots[i] onto the stack
- * free_pages (capacity free_capacity), request by request in page order, and
- * writes its new height (free_count_out may be free_count). Negative slots are
- * skipped; the rows keep their entries. reject = 1, and nothing else happens,
+ * Pushes the pages that the first ceil(lens[i] / 16) entries of table row
+ * slots[i] name onto the stack free_pages (capacity free_capacity), request by
+ * request in page order, and writes its new height (free_count_out may be
+ * free_count). Negative entries name none (pages of a window that went back
+ * before) and are left out, negative slots are skipped; the rows keep their
+ * entries. reject = 1, and nothing else happens,
  * for a slot outside the table or named twice, a length that is negative or
  * past the row, or a stack that would overflow. workspace:
  * tmopt_release_pages_workspace_size bytes, 16-byte aligned. Limits as in

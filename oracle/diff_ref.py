@@ -184,7 +184,8 @@ def release(page_table, slots, lens, free, count):
         if slots[i] >= S or not 0 <= lens[i] <= PAGE * W:
             bad = True
             continue
-        back += page_table[slots[i]][:(lens[i] + PAGE - 1) // PAGE]
+        row = page_table[slots[i]][:(lens[i] + PAGE - 1) // PAGE]
+        back += [p for p in row if p >= 0]         # (the others name no page)
     if bad or count + len(back) > len(free):
         return list(free), count, 1
     free = list(free)

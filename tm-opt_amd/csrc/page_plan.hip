@@ -7,7 +7,8 @@
 // pages as free[count - 1 - first_i - j]. Token t of the step belongs to the
 // request i with cu[i] <= t < cu[i + 1] (cu the exclusive sum of new), sits at
 // position p = ctx_i + t - cu[i] and goes to pool row table[p / 16] * 16 +
-// p % 16. A release pushes the pages back in order.
+// p % 16. A release pushes the pages back in order; entries of its rows that
+// name no page (a window's that went back before) are left out.
 //
 // The checks decide about the whole step, so whoever writes an output needs the
 // sums over all requests. Up to 1024 requests every work-group makes them for
@@ -18,11 +19,13 @@
 // block table, so no work-group waits for another. Where an output is one of
 // the inputs (a graph that steps on in place), or above 1024 requests, one
 // work-group makes the sums and the new pages, and a second launch the rest; a
-// small step in place is one work-group's. Bound by latency: launches and
+// small step in place is one work-group's. A release needs the number of pages
+// that each row names before it can place any, so it is two launches, the first
+// of which counts, above 1024 table entries. Bound by latency: launches and
 // dependent loads. Graph replays, us a step, where an empty kernel takes 2.1: 4
-// decode rows 3.5, 64 rows 3.8, 96 rows and 2 chunks of 2048 tokens under
-// tables of 4,224 pages 6.4; a release of one row of 500 pages 2.9, of 64 rows
-// of up to 4,096 3.5.
+// decode rows 4.1, 64 rows 4.5, 96 rows and 2 chunks of 2048 tokens under
+// tables of 4,224 pages 6.9; a release of one row of 500 pages 4.5, of 64 rows
+// of up to 4,096 7.2.
 #include "common.h"
 
 namespace tmopt {
@@ -33,6 +36,7 @@ constexpr int kMaxRequests = 8192;      // the sums live in LDS
 constexpr int kMaxRows = 1 << 18;       // one bit per table row in LDS
 constexpr int kMaxTokens = 1 << 24;     // sums of a wave stay below 2^31
 constexpr int kOwnSums = 1024;          // requests a fill may sum for itself
+constexpr int kOwnEntries = 1024;       // entries a release may count for itself
 constexpr int kPlanThreads = 1024;
 constexpr int kFillThreads = 256;
 constexpr int kChunk = 1024;            // elements per work-group of a fill
@@ -57,7 +61,7 @@ struct PlanArgs {
   int64_t* pos;
   int32_t* count_out;
   int32_t* reject;
-  int32_t* first;          // release: [B] stack index of each row's first page
+  int32_t* gaps;           // release: [B + 1], see release_gaps_kernel
 };
 
 __device__ __forceinline__ int pages_of(int n) {
@@ -76,12 +80,15 @@ __device__ __forceinline__ int run_of(P s, int n, int x) {
 }
 
 // Checks and sums of a step, by one work-group of T threads: tok / page [B + 1]
-// (LDS) get the exclusive sums of the new tokens and of the pages taken (plan)
-// or handed back (release). Returns whether the step is accepted (the same in
+// (LDS) get the exclusive sums of the new tokens and of the pages taken (plan),
+// or of a release's entries (modulo 2^32) and of the pages handed back (gaps[b]
+// of row b's entries name none). Returns whether the step is accepted (the same in
 // every thread); leaves its totals in tot and the stack's height in n.
 template <int T>
-__device__ bool step_sums(const PlanArgs& a, bool release, int* tok, int* page,
-                          uint32_t* seen, int64_t (&tot)[2], int& n) {
+__device__ bool step_sums(const PlanArgs& a, const int* gaps, int* tok,
+                          int* page, uint32_t* seen, int64_t (&tot)[2],
+                          int& n) {
+  const bool release = gaps != nullptr;
   __shared__ int64_t wsum[2][T / 64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   n = a.count_in[0];      // (read before count_out, which may be it, is written)
@@ -107,8 +114,9 @@ __device__ bool step_sums(const PlanArgs& a, bool release, int* tok, int* page,
           ok = !(atomicOr(&seen[slot >> 5], bit) & bit);   // once per step
         }
         if (ok) {
-          nt = add;
-          np = release ? pages_of(ctx) : pages_of((int)end) - pages_of(ctx);
+          nt = release ? pages_of(ctx) : add;
+          np = release ? pages_of(ctx) - gaps[b]
+                       : pages_of((int)end) - pages_of(ctx);
         }
         bad |= !ok;
       }
@@ -135,8 +143,9 @@ __device__ bool step_sums(const PlanArgs& a, bool release, int* tok, int* page,
     __syncthreads();
   }
   if (threadIdx.x == 0) tok[0] = page[0] = 0;
-  bad |= n < 0 || n > a.F || tot[0] > (release ? 0 : a.max_tokens) ||
-         (release ? n + tot[1] > a.F : tot[1] > n);
+  bad |= n < 0 || n > a.F ||
+         (release ? n + tot[1] > a.F
+                  : tot[0] > a.max_tokens || tot[1] > n);
   return !__syncthreads_or(bad);
 }
 
@@ -181,7 +190,7 @@ __global__ __launch_bounds__(T) void plan_kernel(PlanArgs a, Cut c,
   }
   int64_t tot[2];
   int n;
-  const bool ok = step_sums<T>(a, false, tok, page, seen, tot, n);
+  const bool ok = step_sums<T>(a, nullptr, tok, page, seen, tot, n);
   if (!ok) no_step<T>(a, tok, page, tot);
   if (blockIdx.x == 0) {
     for (int i = threadIdx.x; i < a.B; i += T) {
@@ -299,7 +308,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_sums_kernel(PlanArgs a) {
   uint32_t* const seen = (uint32_t*)(page + a.B + 1);
   int64_t tot[2];
   int n;
-  const bool ok = step_sums<kPlanThreads>(a, false, tok, page, seen, tot, n);
+  const bool ok = step_sums<kPlanThreads>(a, nullptr, tok, page, seen, tot, n);
   if (!ok) no_step<kPlanThreads>(a, tok, page, tot);
   for (int i = threadIdx.x; i < a.B; i += kPlanThreads) {
     const int ctx = a.slots[i] < 0 ? 0 : a.ctx[i];
@@ -345,16 +354,103 @@ __global__ __launch_bounds__(kFillThreads) void plan_fill_kernel(PlanArgs a,
   }
 }
 
-// A whole release of up to kOwnSums requests.
+// ---- release ----------------------------------------------------------------
+
+// entries of the page table that request b of a release names (0: none, or one
+// that refuses the step)
+__device__ __forceinline__ int named(const PlanArgs& a, int b) {
+  const int64_t slot = a.slots[b];
+  const int n = a.ctx[b];
+  return slot >= 0 && slot < a.S && n >= 0 && n <= (int64_t)a.W * kPage
+             ? pages_of(n)
+             : 0;
+}
+
+// sum over a work-group, in every thread
+__device__ __forceinline__ int group_sum(int x, int* wsum) {
+  x = wave_scan(x);
+  __syncthreads();      // (the last sum has been read)
+  if ((threadIdx.x & 63) == 63) wsum[threadIdx.x >> 6] = x;
+  __syncthreads();
+  int sum = 0;
+  for (int j = 0; j < (int)blockDim.x / 64; ++j) sum += wsum[j];
+  return sum;
+}
+
+// The first of two launches: gaps[b] = how many entries of request b's name no
+// page, by a work-group each (of 64 to 1024 threads, by the rows' width);
+// gaps[B] = the stack's height, which the second launch may write over.
+__global__ __launch_bounds__(kPlanThreads) void release_gaps_kernel(
+    PlanArgs a) {
+  __shared__ int wsum[kPlanThreads / 64];
+  const int b = blockIdx.x;
+  const int n = named(a, b);
+  const int32_t* const row = a.table + (n > 0 ? a.slots[b] : 0) * a.W;
+  int gaps = 0;
+#pragma unroll 4
+  for (int j = threadIdx.x; j < n; j += blockDim.x) gaps += row[j] < 0;
+  gaps = group_sum(gaps, wsum);
+  if (threadIdx.x == 0) {
+    a.gaps[b] = gaps;
+    if (b == 0) a.gaps[a.B] = a.count_in[0];
+  }
+}
+
+// Pushes part [j0, end) of a row with gaps: the pages before the part are
+// counted, then 'T' entries at a time go behind each other.
 template <int T>
+__device__ void push_with_gaps(const int32_t* row, int j0, int end,
+                               int32_t* dst, int* wsum) {
+  const int w = threadIdx.x >> 6;
+  int before = 0;
+  for (int j = threadIdx.x; j < j0; j += T) before += row[j] >= 0;
+  dst += group_sum(before, wsum);
+  for (int b = j0; b < end; b += T) {
+    const int j = b + threadIdx.x;
+    const int page = j < end ? row[j] : -1;
+    const int x = wave_scan(page >= 0);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) wsum[w] = x;
+    __syncthreads();
+    int at = x - 1;
+    for (int k = 0; k < T / 64; ++k) {
+      if (k < w) at += wsum[k];
+    }
+    if (page >= 0) dst[at] = page;
+    for (int k = 0; k < T / 64; ++k) dst += wsum[k];
+  }
+}
+
+// A release in parts of 1024 entries of a row. OWN: a whole one of up to
+// kOwnSums requests and kOwnEntries entries, whose work-groups each count the
+// gaps; otherwise the second of two launches.
+template <int T, bool OWN>
 __global__ __launch_bounds__(T) void release_kernel(PlanArgs a, int per) {
   extern __shared__ int lds[];
+  __shared__ int wsum[T / 64];
   int* const tok = lds;
   int* const page = tok + a.B + 1;
   uint32_t* const seen = (uint32_t*)(page + a.B + 1);
+  const int* gaps = a.gaps;
+  if constexpr (OWN) {
+    int* const own = (int*)(seen + (a.S + 31) / 32);   // [B]
+    for (int i = threadIdx.x; i < a.B; i += T) {
+      own[i] = 0;
+      tok[i] = named(a, i);
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int x = threadIdx.x; x < a.B * a.W; x += T) {
+      const int b = x / a.W, j = x - b * a.W;
+      if (j < tok[b] && a.table[a.slots[b] * a.W + j] < 0)
+        atomicAdd(own + b, 1);
+    }
+    __syncthreads();
+    gaps = own;
+  }
   int64_t tot[2];
   int n;
-  const bool ok = step_sums<T>(a, true, tok, page, seen, tot, n);
+  const bool ok = step_sums<T>(a, gaps, tok, page, seen, tot, n);
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     a.count_out[0] = n + (ok ? (int)tot[1] : 0);
     a.reject[0] = !ok;
@@ -363,45 +459,15 @@ __global__ __launch_bounds__(T) void release_kernel(PlanArgs a, int per) {
   for (int part = blockIdx.x; part < a.B * per; part += gridDim.x) {
     const int i = part / per, j0 = (part - i * per) * kChunk;
     const int have = page[i + 1] - page[i];
-    const int32_t* const row = a.table + (have > 0 ? a.slots[i] : 0) * a.W;
+    const int all = (int)((uint32_t)tok[i + 1] - (uint32_t)tok[i]);
+    const int end = min(j0 + kChunk, all);
+    if (have == 0 || j0 >= end) continue;
+    const int32_t* const row = a.table + a.slots[i] * a.W;
     int32_t* const dst = a.free + n + page[i];
-    for (int j = j0 + threadIdx.x; j < min(j0 + kChunk, have); j += T)
-      dst[j] = row[j];
-  }
-}
-
-// ---- two launches -----------------------------------------------------------
-
-__global__ __launch_bounds__(kPlanThreads) void release_sums_kernel(
-    PlanArgs a) {
-  extern __shared__ int lds[];
-  int* const tok = lds;
-  int* const page = tok + a.B + 1;
-  uint32_t* const seen = (uint32_t*)(page + a.B + 1);
-  int64_t tot[2];
-  int n;
-  const bool ok = step_sums<kPlanThreads>(a, true, tok, page, seen, tot, n);
-  if (threadIdx.x == 0) {
-    a.count_out[0] = n + (ok ? (int)tot[1] : 0);
-    a.reject[0] = !ok;
-  }
-  for (int i = threadIdx.x; i < a.B; i += kPlanThreads) a.first[i] = n + page[i];
-}
-
-// 1024 entries of a row per work-group
-__global__ __launch_bounds__(kFillThreads) void release_fill_kernel(PlanArgs a,
-                                                                    int per) {
-  const int i = blockIdx.x / per;
-  const int j0 = (blockIdx.x - i * per) * kChunk + threadIdx.x;
-  const int64_t slot = a.slots[i];
-  if (slot < 0 || a.reject[0] != 0) return;
-  const int have = pages_of(a.ctx[i]);
-  const int32_t* const row = a.table + slot * a.W;
-  int32_t* const dst = a.free + a.first[i];
-#pragma unroll
-  for (int k = 0; k < kChunk / kFillThreads; ++k) {
-    const int j = j0 + k * kFillThreads;
-    if (j < have) dst[j] = row[j];
+    if (have == all)
+      for (int j = j0 + threadIdx.x; j < end; j += T) dst[j] = row[j];
+    else
+      push_with_gaps<T>(row, j0, end, dst, wsum);
   }
 }
 
@@ -507,7 +573,7 @@ extern "C" int tmopt_plan_pages(
 }
 
 extern "C" size_t tmopt_release_pages_workspace_size(int B) {
-  return B > 0 ? ((size_t)B * sizeof(int32_t) + 15) & ~(size_t)15 : 0;
+  return B > 0 ? (((size_t)B + 1) * sizeof(int32_t) + 15) & ~(size_t)15 : 0;
 }
 
 extern "C" int tmopt_release_pages(
@@ -543,29 +609,40 @@ extern "C" int tmopt_release_pages(
   a.count_in = free_count;
   a.count_out = free_count_out;
   a.reject = reject;
-  a.first = (int32_t*)workspace;
+  a.gaps = (int32_t*)workspace;
   const hipStream_t st = (hipStream_t)stream;
-  const bool in_place = free_count_out == free_count;
-  // small enough for one work-group (16 rows of 1024 pages 7.5 us by one, 5.6
-  // by two launches; 8 rows 5.2 / 5.3)
-  const bool small = B * table_width <= 8192;
-  if (B <= kOwnSums && (small || !in_place)) {
-    const int64_t groups = B * per > 0 ? B * per : 1;
-    if (in_place)
-      hipLaunchKernelGGL((release_kernel<kPlanThreads>), dim3(1),
-                         dim3(kPlanThreads), plan_lds(B, table_rows), st, a,
-                         (int)per);
+  const int64_t parts = B * per > 0 ? B * per : 1;
+  if (B <= kOwnSums && B * table_width <= kOwnEntries) {
+    // (one work-group where the height is written over; one launch of 8 rows of
+    // 1024 pages takes 15.7 us where two take 6.6, one row of 4096 10.2 / 6.5)
+    const size_t lds = plan_lds(B, table_rows) + (size_t)B * sizeof(int);
+    if (free_count_out == free_count)
+      hipLaunchKernelGGL((release_kernel<kPlanThreads, true>), dim3(1),
+                         dim3(kPlanThreads), lds, st, a, (int)per);
     else
-      hipLaunchKernelGGL((release_kernel<kFillThreads>),
-                         dim3((unsigned)groups), dim3(kFillThreads),
-                         plan_lds(B, table_rows), st, a, (int)per);
+      hipLaunchKernelGGL((release_kernel<kFillThreads, true>),
+                         dim3((unsigned)parts), dim3(kFillThreads), lds, st, a,
+                         (int)per);
     return check_launch("release_pages");
   }
-  hipLaunchKernelGGL(release_sums_kernel, dim3(1), dim3(kPlanThreads),
-                     plan_lds(B, table_rows), st, a);
+  const int threads = table_width <= 256    ? 64
+                      : table_width <= 2048 ? kFillThreads
+                                            : kPlanThreads;
+  hipLaunchKernelGGL(release_gaps_kernel, dim3(B), dim3(threads), 0, st, a);
   const int rc2 = check_launch("release_pages");
   if (rc2) return rc2;
-  hipLaunchKernelGGL(release_fill_kernel, dim3((unsigned)(B * per)),
-                     dim3(kFillThreads), 0, st, a, (int)per);
+  a.count_in = a.gaps + B;
+  // above kOwnSums the sums weigh most: no more work-groups than there are
+  // compute units (4096 rows of up to 64 pages: 256 work-groups 19.5 us in a
+  // graph, 128 24.7, 512 26.8)
+  const int64_t most = B <= kOwnSums ? 1024 : 256;
+  const unsigned groups = (unsigned)(parts < most ? parts : most);
+  const size_t lds = plan_lds(B, table_rows);
+  if (B <= kOwnSums)
+    hipLaunchKernelGGL((release_kernel<kFillThreads, false>), dim3(groups),
+                       dim3(kFillThreads), lds, st, a, (int)per);
+  else
+    hipLaunchKernelGGL((release_kernel<kPlanThreads, false>), dim3(groups),
+                       dim3(kPlanThreads), lds, st, a, (int)per);
   return check_launch("release_pages");
 }

@@ -2,12 +2,13 @@
 (plan_pages), and the way back of finished requests' pages (release_pages).
 
 A cache keeps, on the device, a page table [S, W] int32 with one row per
-request it can hold, and a stack of free pages: free_pages [F] int32 with the
-height free_count [1] int32. plan_pages takes the pages a step's new tokens
-need off the stack into the requests' rows, and gives the index tensors that
-decode_paged, decode_diff_paged, prefill_varlen, prefill_diff_varlen,
-kv_write_slots and kv_write_paged take. Nothing is read back to the host, so a
-whole step can be captured and replayed while the requests grow.
+request it can hold, and a stack of free pages: free_pages [F] int32, of which
+the first free_count [1] int32 name pages (none negative). plan_pages takes the
+pages a step's new tokens need off the stack into the requests' rows, and gives
+the index tensors that decode_paged, decode_diff_paged, prefill_varlen,
+prefill_diff_varlen, kv_write_slots and kv_write_paged take. Nothing is read
+back to the host, so a whole step can be captured and replayed while the
+requests grow.
 """
 from typing import NamedTuple
 
@@ -102,8 +103,10 @@ def plan_pages(page_table, slots, ctx_lens, new_lens, free_pages, free_count,
 
 
 def release_pages(page_table, slots, lens, free_pages, free_count, out=None):
-    """Push the ceil(lens[i] / 16) pages of page-table row slots[i] (negative:
-    none) back onto the stack free_pages (in place), in order.
+    """Push the pages that the first ceil(lens[i] / 16) entries of page-table
+    row slots[i] (negative: none) name back onto the stack free_pages (in
+    place), in order. Entries that name none (negative: of pages a windowed
+    request gave back before) are left out.
 
     Returns (free_count [1], reject [1]) int32: the stack's height
     afterwards, and 1 where nothing was done: a slot outside the table or
@@ -116,7 +119,7 @@ def release_pages(page_table, slots, lens, free_pages, free_count, out=None):
     _check_index(lens, torch.int32, B, dev)
     S, W = page_table.shape
     # the pair and the scratch in one allocation (16-byte steps)
-    n = -(-B // 4) * 4
+    n = -(-(B + 1) // 4) * 4
     ws, count, reject = torch.empty(n + 2, dtype=torch.int32,
                                     device=dev).split_with_sizes((n, 1, 1))
     if out is None:
