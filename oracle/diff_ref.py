@@ -9,7 +9,19 @@ eps)^-1/2, whose relative change is at most r^2 mean(|O| |dO|). The output is
 rounded once more (2^-8 of it). What fp32 adds (a score of 128 products, each
 exact, is off by at most 128 x 2^-24 of the sum of their sizes; sums of n
 probabilities by n x 2^-24) is counted too, and a tenth of everything for
-products of errors."""
+products of errors.
+
+Over long contexts these bounds, which add every rounding with one sign, pass
+the outputs themselves. power_inputs() makes inputs for which they need not be
+added: scores that are whole numbers of powers of two (scale ln 2, whose
+product with log2 e is 1 in fp32, queries of two entries of 1 or -1, keys of
+-1, 0 and 1) and values of -2 to 2. Probabilities are then 2^-4 to 2^4, bf16
+holds them as they are, and all sums within a piece are multiples of 2^-4 below
+2^20: fp32 holds them too. What is left is each piece's LSE (below 22: log2 by
+2^-19, its sum with the maximum by 2^-20, the product with ln 2 by 2^-20 and
+ln 2 itself by 2^-20.5: 3.6e-6) that weighs it, and up to 64 roundings of
+2^-24 in a join, both above and below the line: 1.5e-5, below 2^-16
+(exact=True)."""
 import math
 
 import torch
@@ -19,11 +31,22 @@ HALF_BF16 = 2.0 ** -8
 HALF_F32 = 2.0 ** -24
 
 
+def power_inputs(T, N, hq, hkv, g):
+    """q [T, hq, 128], k and v [N, hkv, 128] (bf16) for exact=True, scale
+    ln 2."""
+    q = torch.zeros((T, hq, 128))
+    at = torch.rand((T, hq, 128), generator=g).topk(2, -1).indices
+    q.scatter_(-1, at, torch.randint(0, 2, at.shape, generator=g) * 2.0 - 1)
+    k = torch.randint(-1, 2, (N, hkv, 128), generator=g, dtype=torch.int8)
+    v = torch.randint(-2, 3, (N, hkv, 128), generator=g, dtype=torch.int8)
+    return q.bfloat16(), k.bfloat16(), v.bfloat16()
+
+
 def attend(q, K, V, qpos, kpos, lam, scale, weight=None, eps=1e-5,
-           out_scale=1.0, window=0):
-    """q [T, HQ, 128] at qpos [T], K and V [N, HKV, 128] at kpos [N].
-    Returns float64 (out [T, HQ/2, 256], lse [HQ, T], and the bounds of
-    both)."""
+           out_scale=1.0, window=0, exact=False):
+    """q [T, HQ, 128] at qpos [T], K and V [N, HKV, 128] at kpos [N]; exact:
+    inputs of power_inputs(). Returns float64 (out [T, HQ/2, 256], lse [HQ, T],
+    and the bounds of both)."""
     T, HQ, D = q.shape
     N, HKV = K.shape[0], K.shape[1]
     rep = HQ // HKV
@@ -53,6 +76,9 @@ def attend(q, K, V, qpos, kpos, lam, scale, weight=None, eps=1e-5,
             f = 1.0 if m == 0 else -float(f)
             out[:, h] += f * (p @ v)
             rel = HALF_BF16 + 2 * ds + (2 * N + 64) * HALF_F32
+            if exact:
+                rel = torch.full_like(rel, 2.0 ** -16)
+                lerr[2 * h + m] = 2.0 ** -16
             err[:, h] += abs(f) * rel[:, None] * (p @ v.abs())
     if weight is not None:
         r = 1.0 / torch.sqrt(out.square().mean(-1, keepdim=True) + eps)
