@@ -182,6 +182,8 @@ def prefill_diff_varlen(q, k, v, cu_seqlens, lam, scale, norm_weight=None,
     assert cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1
     assert cu_seqlens.is_contiguous() and cu_seqlens.device == dev
     S = cu_seqlens.shape[0] - 1
+    if total == 0:
+        max_seqlen = 0                   # no run, whatever the bound
     if max_seqlen is None:
         max_seqlen = int((cu_seqlens[1:] - cu_seqlens[:-1]).max()) if S else 0
     if block_table is not None:
