@@ -74,8 +74,8 @@ struct DecodeDiffArgs {
   DiffWeights w;
   __bf16* out;
   float* lse;
-  float* part_o;     // [B + R, HQ, 256] fp32, R ranges
-  float* part_lse;   // [B + R, HQ]
+  float* part_o;     // [2 R, HQ, 256] fp32, R ranges (see part_slot)
+  float* part_lse;   // [2 R, HQ]
   int* geo;          // [B + 2]: pages per range, then the page prefix
   int ids_off;       // LDS byte offset of the norm's weights, then the page ids
 };
@@ -123,7 +123,14 @@ enum : int {
   kThere = 8,   // the page is there
   kWhole = 16,  // the piece is the whole request
   kCross = 32,  // the two waves of the range share the piece
+  kStarts = 64, // the piece's request starts in this range
 };
+
+// Where a piece leaves its result: a range has two at most that are not whole
+// requests, of the one that it goes on with and of the one that it begins.
+__device__ __forceinline__ int part_slot(int range, bool starts) {
+  return 2 * range + starts;
+}
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
@@ -344,6 +351,7 @@ void decode_diff_kernel(DecodeDiffArgs a) {
                       (a.window <= 0 || past + kPage <= a.window);
     st.flags = (cb != last_b ? kFirst : 0) | (last ? kLast : 0) |
                (full ? kFull : 0) | (phys >= 0 ? kThere : 0) |
+               (seq_start >= r0 ? kStarts : 0) |
                (seq_start >= r0 && seq_end <= r1 ? kWhole : 0) |
                (mid < r1 && seq_start < mid && seq_end > mid ? kCross : 0);
     last_b = cb;
@@ -492,8 +500,8 @@ void decode_diff_kernel(DecodeDiffArgs a) {
       if (lse != nullptr && col_ok && g == 0)
         lse[(int64_t)b * HQ + hq] = lse_nat;
     } else if (col_ok) {
-      // slot b + range is unique: ranges and requests are both in order
-      const int64_t slot = (int64_t)(b + range) * HQ + hq;
+      const int64_t slot =
+          (int64_t)part_slot(range, flags & kStarts) * HQ + hq;
       float* const o = ra->part_o + slot * kDV + 4 * g;
 #pragma unroll
       for (int blk = 0; blk < 16; ++blk)
@@ -684,8 +692,7 @@ __global__ __launch_bounds__(128 * H * S) void decode_diff_merge(
   const int h = blockIdx.y * H + grp / S;
   const bool hok = h < a.HQ / 2;
   const int d0 = 4 * lane;
-  const int64_t slot0 =
-      (int64_t)(b + first) * a.HQ + 2 * (hok ? h : 0) + m;
+  const int head = 2 * (hok ? h : 0) + m;
   float mx = -INFINITY, sum = 0.0f;
   f32x4 acc = f32x4{0, 0, 0, 0};
   auto add = [&](float l, float w1, f32x4 o) {   // a piece (LSE l, weight w1)
@@ -704,7 +711,8 @@ __global__ __launch_bounds__(128 * H * S) void decode_diff_merge(
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       const bool in = k + j * S < np;
-      const int64_t slot = slot0 + (int64_t)(in ? k + j * S : 0) * a.HQ;
+      const int x = in ? k + j * S : 0;
+      const int64_t slot = (int64_t)part_slot(first + x, x == 0) * a.HQ + head;
       l[j] = in ? a.part_lse[slot] : -INFINITY;
       o[j] = *reinterpret_cast<const f32x4*>(a.part_o + slot * kDV + d0);
     }
@@ -800,7 +808,7 @@ Shape shape_of(int B, int HQ, int HKV, int num_workgroups) {
 }
 
 size_t ws_layout(int B, int HQ, int R, size_t* off_lse, size_t* off_geo) {
-  const size_t slots = (size_t)B + R;
+  const size_t slots = 2 * (size_t)R;
   const size_t o_bytes = slots * HQ * kDV * sizeof(float);
   const size_t l_bytes = (slots * HQ * sizeof(float) + 255) & ~(size_t)255;
   const size_t g_bytes = (((size_t)B + 2) * sizeof(int) + 255) & ~(size_t)255;
