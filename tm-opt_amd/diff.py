@@ -105,12 +105,12 @@ def decode_diff_paged(q, k_pool, v_pool, block_table, ctx_lens, lam, scale,
 
     q [B, HQ, 128] bf16 contiguous (request b's query at position
     ctx_lens[b] - 1); k_pool/v_pool [num_pages, 16, HKV, 128] bf16;
-    block_table [B, bt_stride] int32; ctx_lens [B] int32; lam fp32 [HQ / 2]
-    or [1]; window 0 = global; table_wrap > 0 = each table row is a ring of
-    that many pages; min_pages / num_workgroups: work-split knobs (see the C
-    header; shares of 8 / 4 / 2 pages at least, us per call, 32Q/4KV: one
-    request of 1000 tokens 15.6 / 13.8 / 13.2, 4 up to 1K 16.7 / 15.0 / 14.4,
-    16 up to 2K 18.9 each). workspace: from decode_diff_workspace() (allocated
+    block_table [B, bt_stride] int32 (keys of entries that name no page are
+    absent); ctx_lens [B] int32; lam fp32 [HQ / 2] or [1]; window 0 = global;
+    table_wrap > 0 = each table row is a ring of that many pages; min_pages /
+    num_workgroups: work-split knobs (see the C header; shares of 8 / 4 / 2
+    pages at least, us per call, 32Q/4KV: one request of 1000 tokens 15.6 /
+    13.8 / 13.2, 4 up to 1K 16.7 / 15.0 / 14.4, 16 up to 2K 18.9 each). workspace: from decode_diff_workspace() (allocated
     if None; it needs no initialisation; calls that overlap need one each).
     Returns (out [B, HQ / 2, 256] bf16, lse [B, HQ] fp32 or None)."""
     B, HQ, D = q.shape
@@ -162,21 +162,24 @@ def prefill_diff_varlen(q, k, v, cu_seqlens, lam, scale, norm_weight=None,
         packed like q, and there is no prior context;
       * block_table [S, bt_stride] int32 given, k/v None: every key, prior
         context included, from k_pool/v_pool [num_pages, 16, HKV, 128]; the
-        run's own keys must already be there.
+        run's own keys must already be there. Pages without an entry read as
+        zeros, keys of score 0 (to decode_diff_paged they are absent): a table
+        may lack pages before the window, not ones that a query sees.
     lam fp32 [HQ / 2] or [1]. reject: optional int32 device scalar; nonzero
     gives NaN in every row of out and lse, those that cu_seqlens gives no run
-    included. max_seqlen bounds the run lengths (read from the
-    device, with a synchronisation, if None).
+    included. max_seqlen bounds the run lengths (read from the device, with a
+    synchronisation, if None).
     A launch of few query blocks that may see many keys splits these over
     work-groups and joins the pieces: a second launch, up to 3 x 257 KB of
     scratch per compute unit, and last bits that depend on the launch's other
     runs and the table's width. (So may those of a window's rows on how many
-    runs share a launch: small ones take blocks of other sizes.) max_context: an upper bound of prior + run
-    length, where the host has one; without it the row width of the block
-    table bounds the keys, and short contexts under a wide table pay for the
-    second launch (64Q/8KV, 4,134 pages: 64 tokens without context 16.8 us
-    against 9.0, 30 after 2,000 31.2 against 24.6). It decides about the
-    launch's layout alone.
+    runs share a launch: small ones take blocks of other sizes.) max_context: an
+    upper bound of prior + run length, where the host has one; without it the
+    row width of the block table bounds the keys, and short contexts under a
+    wide table (plan_pages' is as wide as the cache's rows) pay for the second
+    launch (64Q/8KV, 4,134 pages: 64 tokens without context 16.8 us against
+    9.0, 30 after 2,000 31.2 against 24.6). It decides about the launch's
+    layout alone.
     Returns (out [total, HQ / 2, 256] bf16, lse [HQ, total] fp32 or None)."""
     total, HQ, D = q.shape
     dev = q.device
