@@ -243,17 +243,7 @@ void decode_kernel(DecodeArgs a) {
       const int nb = b < a.B ? seq_n<KIND>(kernel_args(false), b) : 0;
       const int v = vis_pages(nb, a.window);
       if (b < a.B) nlen[b] = nb;
-      // inclusive scan over the wave by DPP (VALU, no LDS round trips):
-      // within each 16-lane row by shifts of 1, 2, 4, 8, then row 0's
-      // total into row 1 and row 2's into row 3, then rows 0-1's total into
-      // rows 2-3
-      int x = v;
-      x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);  // shr 1
-      x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);  // shr 2
-      x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);  // shr 4
-      x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);  // shr 8
-      x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false); // bcast 15
-      x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false); // bcast 31
+      const int x = wave_scan(v);
       if (lane == 63) wsum[w] = x;
       __syncthreads();
       int before = carry;
