@@ -586,7 +586,8 @@ int tmopt_attn_prefill_diff(
  * own table: row slots[i] backs request i, its first ceil(ctx_lens[i] / 16)
  * entries name the pages the request holds. new_lens[i] tokens come to it in
  * this step (0: none), and the pages they need are taken off the stack
- * free_pages[0 .. free_count) (from its top, in request order) into the row.
+ * free_pages[0 .. free_count), none of them negative, (from its top, in request
+ * order) into the row.
  * A negative slot is padding: a request without tokens or pages.
  * Written:
  *   block_table  [B, width]: row i of the step, the request's pages up to

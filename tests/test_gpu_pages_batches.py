@@ -86,3 +86,26 @@ def test_release_batches(tm, dev, B, W):
         twice = list(slots)
         twice[i] = s
         assert _release(tm, dev, table, twice, lens, free, 0) == 1
+
+
+@pytest.mark.parametrize("B", [8192, 3])
+def test_largest_table(tm, dev, B):
+    """As many requests and table rows as one call takes, and a small step in
+    a table of as many rows."""
+    rng = random.Random(B)
+    S, W = 262144, 2
+    table = [[7 * i, 7 * i + 1] for i in range(S)]
+    slots = rng.sample(range(S), B)
+    slots[-1] = S - 1 if S - 1 not in slots else slots[-1]
+    ctx = [rng.randint(0, 31) for _ in range(B)]
+    new = [rng.randint(0, 32 - c) for c in ctx]
+    free = [10 ** 7 + i for i in range(2 * B + 9)]
+    assert _plan(tm, dev, table, slots, ctx, new, free, len(free) - 5,
+                 sum(new)) == 0
+    total = sum((c + 15) // 16 for c in ctx)
+    assert _release(tm, dev, table, slots, ctx, free, len(free) - total) == 0
+    assert _release(tm, dev, table, slots, ctx, free,
+                    len(free) - total + 1) == 1
+    slots[0] = slots[-1]
+    assert _plan(tm, dev, table, slots, ctx, new, free, len(free),
+                 sum(new)) == 1

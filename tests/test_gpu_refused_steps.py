@@ -101,3 +101,14 @@ def test_refused_rows_of_a_wider_tensor(tm, dev, diff):
         assert (big[s.T] == 7).all() and (big[:, heads] == 7).all()
         assert (big[..., dim:] == 7).all() and (out[rows:] == 7).all()
         assert torch.isnan(out[:rows]).all() == (count == 3)
+
+
+def test_refused_rows_are_those_of_q(tm, dev):
+    """prefill_varlen takes outputs longer than its queries: the rows behind
+    these stay as they are, in a refused step too."""
+    s = Serving(dev)
+    s.count.fill_(4)
+    p = s.plan(tm)
+    out = torch.full((s.T + 9, HQ, D), 7.0, dtype=BF, device=dev)
+    s.prefill(tm, False, p, s.most, out=out, return_lse=False)
+    assert torch.isnan(out[:s.T]).all() and (out[s.T:] == 7).all()

@@ -236,5 +236,6 @@ def prefill_diff_varlen(q, k, v, cu_seqlens, lam, scale, norm_weight=None,
           HQ, HKV, D, window, float(scale), *w, out.data_ptr(), out.stride(0),
           out.stride(1), _ptr(lse), total, _ptr(reject), _ptr(ws), n)
     if reject is not None:
-        _call(dev, "tmopt_refused_rows", *_refused_rows(reject, out, lse))
+        _call(dev, "tmopt_refused_rows",
+              *_refused_rows(reject, out, lse, total))
     return out, lse
