@@ -33,10 +33,10 @@
 //    walk: a load within it would wait for every page on its way.
 //
 // Us a call, the merge included (32Q/4KV with the norm unless said): 64
-// requests of 1K-8K tokens 102.9, 5.9 TB/s (1.00 of the bytes fetched are the
+// requests of 1K-8K tokens 103.2, 5.9 TB/s (1.00 of the bytes fetched are the
 // formula's); 96 under a window of 512, 64Q/16KV, 66.0, 6.1 TB/s; one of 50,001
-// tokens 32.7, 3.1 TB/s: its walk runs at 7.3 TB/s, 5 us go to the start, 8 to
-// the merge of its 184 pieces; 4 of 128-1024 tokens 14.3 in a graph, 17.5
+// tokens 33.0, 3.1 TB/s: its walk runs at 7.3 TB/s, 5 us go to the start, 8 to
+// the merge of its 184 pieces; 4 of 128-1024 tokens 14.0 in a graph, 17.9
 // eagerly: two launches and their chains of dependent loads.
 #include <algorithm>
 
@@ -614,7 +614,8 @@ void decode_diff_kernel(DecodeDiffArgs a) {
       // ---- probabilities: fp32 sum, bf16 operand -----------------------------
       // (B-operand element i is token 4g + i; rounded to what the matrix
       // instruction takes, each by half a step at most, while the sum that
-      // divides them keeps 32 bits)
+      // divides them keeps 32 bits: against 64 bits outputs are off by 1.7e-3
+      // to 1.9e-3 where fp32 probabilities give 1.7e-3)
       float p[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) p[i] = fast_exp2(x[i] - m_use);

@@ -23,9 +23,9 @@
 // that each row names before it can place any, so it is two launches, the first
 // of which counts, above 1024 table entries. Bound by latency: launches and
 // dependent loads. Graph replays, us a step, where an empty kernel takes 2.1: 4
-// decode rows 4.1, 64 rows 4.5, 96 rows and 2 chunks of 2048 tokens under
-// tables of 4,224 pages 6.9; a release of one row of 500 pages 4.5, of 64 rows
-// of up to 4,096 7.2.
+// decode rows 3.4, 64 rows 3.8, 96 rows and 2 chunks of 2048 tokens under
+// tables of 4,224 pages 6.3; a release of one row of 500 pages 3.9, of 64 rows
+// of up to 4,096 6.6.
 #include "common.h"
 
 namespace tmopt {

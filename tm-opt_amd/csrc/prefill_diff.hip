@@ -34,9 +34,10 @@
 //    on both.)
 //  * Work items are dealt to the XCDs heaviest first (prefill_sched.h).
 //
-// 4 prompts of 8,192 tokens run at 1,197 TFLOP/s, 4 of 2K-8K at 1,163
-// (32Q/4KV): matrix cycles are 0.66 of all, at the 1.6 GHz that the power limit
-// leaves a full chip (a plain 8192^3 product 1,263 TFLOP/s at 1.75 GHz). There
+// 4 prompts of 8,192 tokens run at 1,134-1,197 TFLOP/s, 4 of 2K-8K at
+// 1,092-1,158 (32Q/4KV, by the session): matrix cycles are 0.67 of all, at the 1.6
+// GHz that the power limit leaves a full chip (a plain 8192^3 product 1,263
+// TFLOP/s at 1.75 GHz). There
 // a tile is 0.97 us of the matrix pipes and takes 1.4; an item's start and end
 // cost some 9 us, which no other work-group hides (one per CU by its LDS and
 // registers).
@@ -420,7 +421,11 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_diff_kernel(
       const float p0 = fast_exp2(__builtin_fmaf(sc[2 * q], sl2, -m_use));
       const float p1 = fast_exp2(__builtin_fmaf(sc[2 * q + 1], sl2, -m_use));
       psum += p0 + p1;
-      pw[q] = pack_bf16x2_rn(p0, p1);   // (the matrix operand's type)
+      // (the matrix operand's type: each is off by half a step, 2^-8 of it, at
+      // most, the sum above keeps 32 bits; against 64 bits outputs are off by
+      // 2.0e-3 to 2.2e-3 where fp32 probabilities give 1.7e-3, which is the
+      // outputs' own rounding)
+      pw[q] = pack_bf16x2_rn(p0, p1);
     }
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk)

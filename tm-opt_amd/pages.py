@@ -64,7 +64,8 @@ def plan_pages(page_table, slots, ctx_lens, new_lens, free_pages, free_count,
     tokens: block table and slot mapping -1, cu_seqlens and positions 0,
     seq_lens the contexts. prefill_varlen and prefill_diff_varlen take reject
     as it is, and their outputs are NaN whole then; a KV write of such a plan
-    writes nothing, a decode gives zeros."""
+    writes nothing, a decode gives zeros. (Their max_context keeps a few tokens
+    under a wide block table to one launch.)"""
     dev, B, T = page_table.device, slots.numel(), int(max_tokens)
     _check_state(dev, page_table, free_pages, free_count)
     _check_index(slots, torch.int64, B, dev)
