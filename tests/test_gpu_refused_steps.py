@@ -112,3 +112,14 @@ def test_refused_rows_are_those_of_q(tm, dev):
     out = torch.full((s.T + 9, HQ, D), 7.0, dtype=BF, device=dev)
     s.prefill(tm, False, p, s.most, out=out, return_lse=False)
     assert torch.isnan(out[:s.T]).all() and (out[s.T:] == 7).all()
+
+
+def test_refused_lse_as_one_row(tm, dev):
+    """prefill_varlen asks of an LSE buffer that it holds HQ x total values:
+    one row of them, at the end of an allocation, is filled and no more."""
+    s = Serving(dev)
+    s.count.fill_(4)
+    p = s.plan(tm)
+    buf = torch.full((HQ * s.T + 4096,), 7.0, device=dev)
+    s.prefill(tm, False, p, s.most, lse=buf[:HQ * s.T])
+    assert torch.isnan(buf[:HQ * s.T]).all() and (buf[HQ * s.T:] == 7).all()

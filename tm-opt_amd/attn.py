@@ -490,17 +490,17 @@ def prefill_varlen(q, k, v, cu_seqlens, scale, window=0, max_seqlen=None,
                                max_context)
     if reject is not None:
         _lib.call("tmopt_refused_rows",
-                  *_refused_rows(reject, out, lse, q.shape[0]),
+                  *_refused_rows(reject, out, lse, *q.shape, q.shape[1]),
                   _stream(q.device))
     return out, lse
 
 
-def _refused_rows(reject, out, lse, rows):
-    """The C arguments of the launch that the outputs of a refused step of
-    `rows` queries need where its cu_seqlens gives no run (plan_pages)."""
-    return (_ptr(reject), _ptr(out), out.stride(0), out.stride(1), rows,
-            out.shape[1], out.shape[2], _ptr(lse),
-            *((0, 0) if lse is None else (lse.stride(0), lse.shape[0])))
+def _refused_rows(reject, out, lse, rows, heads, dim, lse_heads):
+    """The C arguments of the launch that the outputs of a refused step, out
+    [rows, heads, dim] and lse [lse_heads, rows] contiguous, need where its
+    cu_seqlens gives no run (plan_pages)."""
+    return (_ptr(reject), _ptr(out), out.stride(0), out.stride(1), rows, heads,
+            dim, _ptr(lse), rows, lse_heads)
 
 
 def _prefill_varlen(q, k, v, cu_seqlens, scale, window, max_seqlen,

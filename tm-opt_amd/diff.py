@@ -237,5 +237,5 @@ def prefill_diff_varlen(q, k, v, cu_seqlens, lam, scale, norm_weight=None,
           out.stride(1), _ptr(lse), total, _ptr(reject), _ptr(ws), n)
     if reject is not None:
         _call(dev, "tmopt_refused_rows",
-              *_refused_rows(reject, out, lse, total))
+              *_refused_rows(reject, out, lse, *out.shape, HQ))
     return out, lse
