@@ -577,6 +577,76 @@ int tmopt_attn_prefill_diff(
     size_t workspace_bytes, tmopt_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* A cache held in 4 bits                                                   */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * K and V of a token's head are four blocks of 32 dims each. A block keeps 32
+ * e2m1 elements (codes 0..7: 0, .5, 1, 1.5, 2, 3, 4, 6; 8..15 the negatives) and
+ * one scale byte E, 2^(E - 127). Written: the smallest scale with amax <= 7 *
+ * scale (E - 127 >= -125), elements to the nearest, ties to the even code, cut
+ * at 6. A block with a value that is no number, infinite, or above 7 * 2^125
+ * takes E = 255 and reads as NaN.
+ * The pool is [num_pages, HKV, 2176] bytes, contiguous and 16-byte aligned; a
+ * page's record of one head holds
+ *      0  K elements, 16 tokens of 64 bytes: dims 2i (low half) and 2i + 1
+ *         (high half) in byte i
+ *   1024  V elements, 16 groups c of 16 tokens of 4 bytes: dims 8c .. 8c + 7
+ *   2048  K scale bytes, 4 blocks of 16 tokens
+ *   2112  V scale bytes, 4 blocks of 16 tokens
+ * D == 128, page_size == 16 (TMOPT_EUNSUPPORTED otherwise).
+ */
+
+/*
+ * Token rows into the pool: k, v [T, HKV, D] bf16 with element strides
+ * (multiples of 8, D contiguous, 16-byte aligned), slot_mapping [T] int64 rows
+ * page * 16 + offset. Rows outside the pool (negative ones among them) are
+ * skipped. A row named twice in one call holds unspecified values. Other
+ * tokens of a page are not touched, so they may be read meanwhile.
+ */
+int tmopt_kv_write_mx4(const void* k, const void* v, int64_t k_stride_tok,
+                       int64_t k_stride_head, int64_t v_stride_tok,
+                       int64_t v_stride_head, const int64_t* slot_mapping,
+                       int64_t T, int HKV, int D, int page_size, void* pool,
+                       int64_t num_pages, tmopt_stream_t stream);
+
+/*
+ * And back: k, v [T, HKV, D] bf16 contiguous, 16-byte aligned, the values held
+ * (exact down to 2^-126); zeros for a row outside the pool.
+ */
+int tmopt_kv_read_mx4(const void* pool, int64_t num_pages,
+                      const int64_t* slot_mapping, int64_t T, int HKV, int D,
+                      int page_size, void* k, void* v, tmopt_stream_t stream);
+
+/*
+ * One new token per request over the 4-bit cache. q, block_table, table_wrap,
+ * ctx_lens, window, scale (> 0), rel, rel_extent, min_pages, num_workgroups,
+ * out and lse as in tmopt_attn_decode_paged (HQ * rel_extent < 2^29), keys
+ * without an entry included (they are absent).
+ * softcap:  > 0: scores are softcap * tanh(scale q.k / softcap).
+ * slopes:   fp32 [HQ] or NULL: the score of a key at distance d (pos_q - pos_k)
+ *           gets -slopes[h] * d, after the cap.
+ * rel goes without softcap and slopes (TMOPT_EUNSUPPORTED).
+ * A visible key whose score is NaN or +infinity gives NaN as LSE and outputs, a
+ * visible value block that is NaN gives NaN in its dims.
+ * Any HQ / HKV; each stored head is read once for up to 8 query heads (a larger
+ * ratio runs in groups of its largest divisor up to 8). B <= 8192.
+ * workspace: tmopt_attn_decode_mx4_workspace_size bytes, 16-byte aligned,
+ * without initialisation.
+ */
+size_t tmopt_attn_decode_mx4_workspace_size(int B, int HQ, int HKV, int D,
+                                            int num_workgroups);
+int tmopt_attn_decode_mx4(const void* q, const void* pool,
+                          const int32_t* block_table, int64_t bt_stride,
+                          int table_wrap, const int32_t* ctx_lens, int B,
+                          int HQ, int HKV, int D, int page_size,
+                          int64_t num_pages, int window, float scale,
+                          float softcap, const float* slopes, const void* rel,
+                          int rel_extent, int min_pages, int num_workgroups,
+                          void* out, float* lse, void* workspace,
+                          size_t workspace_bytes, tmopt_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
 /* Page plan of a serving step                                              */
 /* ------------------------------------------------------------------------ */
 

@@ -9,6 +9,8 @@ lib/libtmopt_attn.so), reached from PyTorch-ROCm through ctypes:
             decode_paged_noalloc, prefill_varlen (MFMA),
             prefill_check_positions.
   diff      differential attention: decode_diff_paged, prefill_diff_varlen.
+  mx4       a cache held in 4 bits: kv_write_mx4 / kv_read_mx4,
+            decode_mx4_paged.
   pages     the page plan of a step from its requests' lengths: plan_pages,
             release_pages.
   compat    the reference's call signatures (attn_swa, attn_global,
@@ -34,6 +36,8 @@ from .compat import (attn_global, attn_prefill_chunk_global,
                      prefill_chunk_state)
 from .diff import (decode_diff_paged, decode_diff_workspace,
                    prefill_diff_varlen)
+from .mx4 import (decode_mx4_paged, decode_mx4_workspace, kv_read_mx4,
+                  kv_write_mx4, mx4_pool)
 from .pages import PagePlan, plan_pages, release_pages
 
 __all__ = [
@@ -48,5 +52,7 @@ __all__ = [
     "attn_prefill_chunk_swa", "attn_prefill_chunk_global",
     "prefill_chunk_state",
     "decode_diff_paged", "decode_diff_workspace", "prefill_diff_varlen",
+    "decode_mx4_paged", "decode_mx4_workspace", "kv_read_mx4", "kv_write_mx4",
+    "mx4_pool",
     "PagePlan", "plan_pages", "release_pages",
 ]

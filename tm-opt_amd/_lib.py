@@ -116,6 +116,19 @@ SIGNATURES = {
         _c_ptr, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,
         _c_f32, _c_ptr, _c_i32, _c_ptr, _c_f32, _c_f32, _c_ptr, _c_i64,
         _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_size, _c_ptr]),
+    "tmopt_kv_write_mx4": (_c_i32, [
+        _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64,
+        _c_i32, _c_i32, _c_i32, _c_ptr, _c_i64, _c_ptr]),
+    "tmopt_kv_read_mx4": (_c_i32, [
+        _c_ptr, _c_i64, _c_ptr, _c_i64, _c_i32, _c_i32, _c_i32, _c_ptr,
+        _c_ptr, _c_ptr]),
+    "tmopt_attn_decode_mx4_workspace_size": (_c_size, [
+        _c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
+    "tmopt_attn_decode_mx4": (_c_i32, [
+        _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i32, _c_ptr, _c_i32, _c_i32,
+        _c_i32, _c_i32, _c_i32, _c_i64, _c_i32, _c_f32, _c_f32, _c_ptr,
+        _c_ptr, _c_i32, _c_i32, _c_i32, _c_ptr, _c_ptr, _c_ptr, _c_size,
+        _c_ptr]),
     "tmopt_plan_pages": (_c_i32, [
         _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i32, _c_ptr,
         _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
