@@ -577,6 +577,82 @@ int tmopt_attn_prefill_diff(
     size_t workspace_bytes, tmopt_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* Score functions and masks                                                */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Attention whose score of query q (position p) and key k (position j) is
+ *   z = scale q.k;  x = softcap tanh(z / softcap)  (softcap 0: x = z)
+ *   x - slopes[h] |p - j|                          (slopes: fp32 [HQ] or NULL)
+ * (the tanh off by 2^-19 at most), and whose query sees the keys of its request
+ * with
+ *   j >= first_keys, j > p - window (window > 0), j <= max(p, prefix_lens - 1).
+ * first_keys: int32, one per query token, or NULL: where the query's document
+ * begins in a request of several (any value; negative ones are 0).
+ * prefix_lens: int32, one per run, or NULL: of each run the first tokens, which
+ * all of it sees (a prefix past the run's end stops there).
+ * A query that sees no key gives zeros and LSE -infinity. A visible key whose
+ * score is NaN (or +infinity, without a cap) gives NaN as output and LSE.
+ * Sums and maxima are fp32; probabilities are rounded to bf16 for their product
+ * with the values, outputs once.
+ */
+
+/*
+ * One new token per request. q, k_pool, v_pool, block_table, table_wrap,
+ * ctx_lens, window, min_pages, num_workgroups, out and lse as in
+ * tmopt_attn_decode_paged; scale > 0; first_keys [B]. workspace:
+ * tmopt_attn_decode_workspace_size bytes, 16-byte aligned. B <= 8192.
+ */
+int tmopt_attn_decode_scored(const void* q, const void* k_pool,
+                             const void* v_pool, const int32_t* block_table,
+                             int64_t bt_stride, int table_wrap,
+                             const int32_t* ctx_lens, int B, int HQ, int HKV,
+                             int D, int page_size, int64_t num_pages,
+                             int window, float scale, float softcap,
+                             const float* slopes, const int32_t* first_keys,
+                             int min_pages, int num_workgroups, void* out,
+                             float* lse, void* workspace,
+                             size_t workspace_bytes, tmopt_stream_t stream);
+
+/*
+ * Packed runs of queries. q [total, HQ, D] with element strides, D contiguous;
+ * cu_seqlens_q, prior_lens, max_seqlen_q, window, scale, out, lse ([HQ, total])
+ * and reject as in tmopt_attn_prefill_varlen; first_keys [total], prefix_lens
+ * [num_seqs]. Keys:
+ *   block_table == NULL: k, v [total, HKV, D], the runs' own rows packed by
+ *         cu_seqlens_q (strides % 8, D contiguous); prior_lens NULL;
+ *   block_table != NULL, k == v == NULL: every key from k_pool / v_pool
+ *         [num_pages, page_size, HKV, D] through block_table [num_seqs,
+ *         bt_stride], the runs' own rows already written. Pages past the row
+ *         width or outside the pool read as zeros.
+ * A block of up to 256 consecutive queries (256 / the query heads it groups)
+ * multiplies the values of every tile of 64 keys between the first and the last
+ * key that one of them sees, with weight zero where a query does not: those
+ * value rows must be finite.
+ * max_context: an upper bound of prior + run length, or 0: the row width of the
+ * block table bounds it. It decides about the launch's layout alone.
+ * workspace: scratch of tmopt_attn_prefill_scored_workspace_size bytes (which
+ * may be 0), 16-byte aligned, without initialisation; NULL: keys are not split
+ * over work-groups.
+ */
+size_t tmopt_attn_prefill_scored_workspace_size(int num_seqs, int max_seqlen_q,
+                                                int64_t max_context, int HQ,
+                                                int HKV, int64_t bt_stride,
+                                                int window);
+int tmopt_attn_prefill_scored(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k,
+    int64_t k_stride_tok, int64_t k_stride_head, const void* v,
+    int64_t v_stride_tok, int64_t v_stride_head, const int32_t* cu_seqlens_q,
+    const int32_t* prior_lens, int num_seqs, int max_seqlen_q,
+    int64_t max_context, const void* k_pool, const void* v_pool,
+    const int32_t* block_table, int64_t bt_stride, int page_size,
+    int64_t num_pages, int HQ, int HKV, int D, int window, float scale,
+    float softcap, const float* slopes, const int32_t* first_keys,
+    const int32_t* prefix_lens, void* out, int64_t o_stride_tok,
+    int64_t o_stride_head, float* lse, const int32_t* reject, void* workspace,
+    size_t workspace_bytes, tmopt_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
 /* A cache held in 4 bits                                                   */
 /* ------------------------------------------------------------------------ */
 
@@ -645,6 +721,31 @@ int tmopt_attn_decode_mx4(const void* q, const void* pool,
                           int rel_extent, int min_pages, int num_workgroups,
                           void* out, float* lse, void* workspace,
                           size_t workspace_bytes, tmopt_stream_t stream);
+
+/*
+ * Packed runs of queries over the 4-bit cache: every key, the runs' own among
+ * them, from the pages. q, cu_seqlens_q, prior_lens, max_seqlen_q, max_context,
+ * block_table, window, out, lse, reject and workspace as in
+ * tmopt_attn_prefill_scored (its rule for values: rows between the first and
+ * the last key that a block of queries sees must hold no NaN block), softcap,
+ * slopes as in tmopt_attn_decode_mx4; rel [total, HQ, rel_extent] with element
+ * strides as in tmopt_attn_prefill_varlen.
+ */
+size_t tmopt_attn_prefill_mx4_workspace_size(int num_seqs, int max_seqlen_q,
+                                             int64_t max_context, int HQ,
+                                             int HKV, int64_t bt_stride,
+                                             int window);
+int tmopt_attn_prefill_mx4(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+    const int32_t* cu_seqlens_q, const int32_t* prior_lens, int num_seqs,
+    int max_seqlen_q, int64_t max_context, const void* pool,
+    const int32_t* block_table, int64_t bt_stride, int page_size,
+    int64_t num_pages, int HQ, int HKV, int D, int window, float scale,
+    float softcap, const float* slopes, const void* rel,
+    int64_t rel_stride_tok, int64_t rel_stride_head, int rel_extent, void* out,
+    int64_t o_stride_tok, int64_t o_stride_head, float* lse,
+    const int32_t* reject, void* workspace, size_t workspace_bytes,
+    tmopt_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
 /* Page plan of a serving step                                              */

@@ -110,6 +110,8 @@ def attend(q, K, V, qpos, kpos, scale, softcap=0.0, slopes=None, rel=None,
         seen &= dist < window
     if first is not None:
         seen &= kpos[None, :] >= first[:, None]
+    # (rows that no query sees may hold anything)
+    V = torch.where(seen.any(0)[:, None, None], V, 0.0)
     out = q.new_zeros((T, HQ, D))
     err = torch.zeros_like(out)
     lse = q.new_full((HQ, T), -math.inf)

@@ -9,8 +9,10 @@ lib/libtmopt_attn.so), reached from PyTorch-ROCm through ctypes:
             decode_paged_noalloc, prefill_varlen (MFMA),
             prefill_check_positions.
   diff      differential attention: decode_diff_paged, prefill_diff_varlen.
+  scored    attention with a tanh cap, a bias by distance, document and
+            prefix masks: decode_scored_paged, prefill_scored_varlen.
   mx4       a cache held in 4 bits: kv_write_mx4 / kv_read_mx4,
-            decode_mx4_paged.
+            decode_mx4_paged, prefill_mx4_varlen.
   pages     the page plan of a step from its requests' lengths: plan_pages,
             release_pages.
   compat    the reference's call signatures (attn_swa, attn_global,
@@ -37,8 +39,9 @@ from .compat import (attn_global, attn_prefill_chunk_global,
 from .diff import (decode_diff_paged, decode_diff_workspace,
                    prefill_diff_varlen)
 from .mx4 import (decode_mx4_paged, decode_mx4_workspace, kv_read_mx4,
-                  kv_write_mx4, mx4_pool)
+                  kv_write_mx4, mx4_pool, prefill_mx4_varlen)
 from .pages import PagePlan, plan_pages, release_pages
+from .scored import decode_scored_paged, prefill_scored_varlen
 
 __all__ = [
     "TmoptError", "TmoptLibraryMissing", "version", "HEAD_DIM", "PAGE_SIZE",
@@ -53,6 +56,7 @@ __all__ = [
     "prefill_chunk_state",
     "decode_diff_paged", "decode_diff_workspace", "prefill_diff_varlen",
     "decode_mx4_paged", "decode_mx4_workspace", "kv_read_mx4", "kv_write_mx4",
-    "mx4_pool",
+    "mx4_pool", "prefill_mx4_varlen",
+    "decode_scored_paged", "prefill_scored_varlen",
     "PagePlan", "plan_pages", "release_pages",
 ]

@@ -129,6 +129,26 @@ SIGNATURES = {
         _c_i32, _c_i32, _c_i32, _c_i64, _c_i32, _c_f32, _c_f32, _c_ptr,
         _c_ptr, _c_i32, _c_i32, _c_i32, _c_ptr, _c_ptr, _c_ptr, _c_size,
         _c_ptr]),
+    "tmopt_attn_prefill_mx4_workspace_size": (_c_size, [
+        _c_i32, _c_i32, _c_i64, _c_i32, _c_i32, _c_i64, _c_i32]),
+    "tmopt_attn_prefill_mx4": (_c_i32, [
+        _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i32, _c_i32, _c_i64,
+        _c_ptr, _c_ptr, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32,
+        _c_i32, _c_f32, _c_f32, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i32,
+        _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_size, _c_ptr]),
+    "tmopt_attn_decode_scored": (_c_i32, [
+        _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i32, _c_ptr, _c_i32,
+        _c_i32, _c_i32, _c_i32, _c_i32, _c_i64, _c_i32, _c_f32, _c_f32,
+        _c_ptr, _c_ptr, _c_i32, _c_i32, _c_ptr, _c_ptr, _c_ptr, _c_size,
+        _c_ptr]),
+    "tmopt_attn_prefill_scored_workspace_size": (_c_size, [
+        _c_i32, _c_i32, _c_i64, _c_i32, _c_i32, _c_i64, _c_i32]),
+    "tmopt_attn_prefill_scored": (_c_i32, [
+        _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64,
+        _c_i64, _c_ptr, _c_ptr, _c_i32, _c_i32, _c_i64, _c_ptr, _c_ptr,
+        _c_ptr, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,
+        _c_f32, _c_f32, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64,
+        _c_ptr, _c_ptr, _c_ptr, _c_size, _c_ptr]),
     "tmopt_plan_pages": (_c_i32, [
         _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i32, _c_ptr,
         _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr,

@@ -19,7 +19,9 @@ ARCH = os.environ.get("TMOPT_ARCH", "gfx950")
 
 SOURCES = ["capi.hip", "kv_write.hip", "decode.hip", "prefill.hip",
            "prefill_split.hip", "decode_diff.hip", "prefill_diff.hip",
-           "page_plan.hip", "kv_mx4.hip", "decode_mx4.hip"]
+           "page_plan.hip", "kv_mx4.hip", "decode_mx4.hip", "decode_scored.hip",
+           "prefill_scored.hip", "prefill_scored_split.hip",
+           "prefill_mx4.hip", "prefill_mx4_split.hip"]
 
 FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-fPIC", "-std=c++17",

@@ -6,16 +6,6 @@
 namespace tmopt {
 namespace {
 
-// Three work-groups per four CUs (one wave per SIMD where they run). 160 / 176
-// / 192 / 208 / 256 / 512 work-groups, us: 64 sequences of 1K-8K (32Q/4KV) 98.8
-// / 96.7 / 96.5 / 96.7 / 99.0 / 110.5, window 4096 at 128 sequences 168.9 /
-// 164.6 / 165.1 / 166.2 / 170.7 / 178.5.
-int default_wgs(int HKV) {
-  const int ny = HKV / waves_per_wg(HKV);
-  const int g = 3 * device_cus() / (4 * ny);
-  return g > 0 ? g : 1;
-}
-
 template <int REP, int KIND>
 void launch_kind(const DecodeArgs& a, dim3 grid, int nw, size_t lds,
                  hipStream_t st) {

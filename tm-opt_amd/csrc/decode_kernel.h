@@ -65,9 +65,18 @@
 #pragma once
 
 #include "common.h"
+#include "score.h"
 
 namespace tmopt {
 namespace {
+
+// The score functions and the first keys of score.h, in a translation unit of
+// their own: the other kernels keep the instructions they have without them.
+#ifdef TMOPT_DECODE_SCORED
+constexpr bool kScored = true;
+#else
+constexpr bool kScored = false;
+#endif
 
 constexpr int kD = 128;
 constexpr int kPS = 16;                      // tokens per page
@@ -122,6 +131,11 @@ struct DecodeArgs {
                      // is above 16 (then kv_div groups of `rep` query
                      // heads each read the stored head's pages)
   int HKV_stored;    // KV heads of a pool token row
+#ifdef TMOPT_DECODE_SCORED
+  Cap cap;
+  const float* slopes;     // [HQ] or null
+  const int32_t* first;    // [B] first visible position, or null
+#endif
 };
 
 __device__ __forceinline__ int vis_lo(int n, int window) {
@@ -152,6 +166,24 @@ __device__ __forceinline__ int seq_n(ArgsPtr a, int b) {
   return as_const(a->ctx_lens)[b];
 }
 
+// First key that sequence b of n keys sees, and its visible pages (macros: the
+// plain kernels keep their expressions, and with them their instructions).
+#ifdef TMOPT_DECODE_SCORED
+__device__ __forceinline__ int seq_lo(ArgsPtr a, int b, int n) {
+  const int lo = vis_lo(n, a->window);
+  return a->first != nullptr ? max(lo, as_const(a->first)[b]) : lo;
+}
+__device__ __forceinline__ int seq_pages(ArgsPtr a, int b, int n) {
+  const int lo = seq_lo(a, b, n);   // (n may come up to 2^31 - 1)
+  return n <= 0 || lo >= n ? 0 : (n - 1) / kPS + 1 - lo / kPS;
+}
+#define TMOPT_SEQ_LO(args, b, n) seq_lo(args, b, n)
+#define TMOPT_SEQ_PAGES(args, b, n) seq_pages(args, b, n)
+#else
+#define TMOPT_SEQ_LO(args, b, n) vis_lo(n, a.window)
+#define TMOPT_SEQ_PAGES(args, b, n) vis_pages(n, a.window)
+#endif
+
 template <int KIND>
 __device__ __forceinline__ int page_id(ArgsPtr a, int b, int lp) {
   const int idx = a->table_wrap > 0 ? lp % a->table_wrap : lp;
@@ -178,6 +210,9 @@ struct Step {
   int n;       // its context length
   int pg;      // first logical page
   int flags;
+#ifdef TMOPT_DECODE_SCORED
+  int lo;      // its first visible key
+#endif
 };
 enum : int {
   kFirst = 1,   // first step of this piece: the query rows come with it
@@ -241,7 +276,9 @@ void decode_kernel(DecodeArgs a) {
     for (int b0 = 0; b0 < a.B; b0 += blockDim.x) {
       const int b = b0 + threadIdx.x;
       const int nb = b < a.B ? seq_n<KIND>(kernel_args(false), b) : 0;
-      const int v = vis_pages(nb, a.window);
+      // (a length of 0 past the batch: no page, and nothing looked up)
+      const int v =
+          kScored && b >= a.B ? 0 : TMOPT_SEQ_PAGES(kernel_args(false), b, nb);
       if (b < a.B) nlen[b] = nb;
       const int x = wave_scan(v);
       if (lane == 63) wsum[w] = x;
@@ -319,14 +356,15 @@ void decode_kernel(DecodeArgs a) {
   for (int i = threadIdx.x; i < nids; i += blockDim.x) {
     const int b = seq_of(u0 + i);
     ids[i] = page_id<KIND>(kernel_args(false), b,
-                           vis_lo(nlen[b], a.window) / kPS +
+                           TMOPT_SEQ_LO(kernel_args(false), b, nlen[b]) / kPS +
                                (u0 + i - pref[b]));
   }
   int cb = __builtin_amdgcn_readfirstlane(seq_of(u0));
   int seq_start = __builtin_amdgcn_readfirstlane(pref[cb]);
   int cur_n = __builtin_amdgcn_readfirstlane(nlen[cb]);
-  int seq_end = seq_start + vis_pages(cur_n, a.window);
-  int pg_of = vis_lo(cur_n, a.window) / kPS - seq_start;   // page of unit u
+  int seq_end = seq_start + TMOPT_SEQ_PAGES(kernel_args(false), cb, cur_n);
+  // page of unit u
+  int pg_of = TMOPT_SEQ_LO(kernel_args(false), cb, cur_n) / kPS - seq_start;
   int cu = u0;
   int last_b = -1;  // sequence of the previous step handed out
   __syncthreads();  // the ids are there; every wave is done with the tables
@@ -349,9 +387,9 @@ void decode_kernel(DecodeArgs a) {
         ++cb;
         seq_start = seq_end;
         cur_n = seq_n<KIND>(ra, cb);
-        seq_end = seq_start + vis_pages(cur_n, a.window);
+        seq_end = seq_start + TMOPT_SEQ_PAGES(ra, cb, cur_n);
       } while (seq_end <= cu);
-      pg_of = vis_lo(cur_n, a.window) / kPS - seq_start;
+      pg_of = TMOPT_SEQ_LO(ra, cb, cur_n) / kPS - seq_start;
     }
     const int cnt = min(2, min(seq_end, u1) - cu);
     st.b = cb;
@@ -371,8 +409,14 @@ void decode_kernel(DecodeArgs a) {
     id1 = (int)lds_ld32(ids_at + 4);
     // every token visible: not before the window, not past the end
     const int past = st.n - (st.pg + 2) * kPS;
+#ifdef TMOPT_DECODE_SCORED
+    st.lo = seq_lo(kernel_args(true), cb, cur_n);
+    const bool full =
+        (phys0 | phys1) >= 0 && past >= 0 && st.pg * kPS >= st.lo;
+#else
     const bool full = (phys0 | phys1) >= 0 && past >= 0 &&
                       (a.window <= 0 || past + 2 * kPS <= a.window);
+#endif
     st.flags = (cb != last_b ? kFirst : 0) |
                (cu == min(seq_end, u1) ? kLast : 0) | (full ? kFull : 0) |
                (phys0 >= 0 ? kPage0 : 0) | (phys1 >= 0 ? kPage1 : 0) |
@@ -429,7 +473,11 @@ void decode_kernel(DecodeArgs a) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int phys = t == 0 ? phys0 : phys1;
+#ifdef TMOPT_DECODE_SCORED
+      const int r_lo = t == 0 ? max(0, st.lo - st.pg * kPS) : 0;
+#else
       const int r_lo = t == 0 && a.window > 0 ? max(0, past - a.window) : 0;
+#endif
       const int r_hi = min(kPS, past - kPS * t);
       const uint64_t base = (uint64_t)(uint32_t)max(phys, 0) *
                                 (uint32_t)(kPS * row_bytes) +
@@ -522,6 +570,10 @@ void decode_kernel(DecodeArgs a) {
   float m_run = -INFINITY;
   float l_part = 0.0f;
   bf16x8 qf[4];   // query fragments
+#ifdef TMOPT_DECODE_SCORED
+  const float slope =
+      a.slopes != nullptr && head_ok ? a.slopes[hq] * kLog2e : 0.0f;
+#endif
 
   // End of a piece of sequence b: write the result (whole sequence) or a
   // normalised partial that decode_combine_kernel merges.
@@ -529,9 +581,14 @@ void decode_kernel(DecodeArgs a) {
     const int b = st.b;
     float l_tot = l_part;
     l_tot = lane_pair(lane_pair(l_tot, 16, false), 32, false);
-    const float inv = l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
+    // (scored: no number as a sum gives no number as LSE)
+    auto some = [&]() __attribute__((always_inline)) {
+      if constexpr (kScored) return l_tot != 0.0f;
+      else return l_tot > 0.0f;
+    };
+    const float inv = some() ? 1.0f / l_tot : 0.0f;
     const float lse_nat =
-        l_tot > 0.0f ? (m_run + fast_log2(l_tot)) * kLn2 : -INFINITY;
+        some() ? (m_run + fast_log2(l_tot)) * kLn2 : -INFINITY;
     // Buffer stores with a per-row (wave-uniform) base: the lane offsets
     // stay 32-bit, and padded heads / the LSE of lanes g != 0 / a missing
     // LSE output get an out-of-range offset or an empty resource (dropped),
@@ -696,12 +753,22 @@ void decode_kernel(DecodeArgs a) {
         if constexpr (REL) bias_values(a, cur, bw[t], t, sh, g, bias);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+#ifdef TMOPT_DECODE_SCORED
+          x[t][i] = a.cap.in != 0.0f ? a.cap(sc[t][i])
+                                     : sc[t][i] * a.scale_log2;
+          x[t][i] -= slope * (float)(rel_dist(cur) - 16 * t - 4 * g - i);
+#else
           x[t][i] = sc[t][i] * a.scale_log2;
+#endif
           if constexpr (REL) x[t][i] += bias[i] * kLog2e;
         }
       }
       if (!(cur.flags & kFull)) {
+#ifdef TMOPT_DECODE_SCORED
+        const int lo = cur.lo;
+#else
         const int lo = vis_lo(cur.n, a.window);
+#endif
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const bool page_ok = cur.flags & (t == 0 ? kPage0 : kPage1);
@@ -886,6 +953,16 @@ size_t ws_layout(int B, int HQ, int G, size_t* off_lse, size_t* off_geo) {
   if (off_lse) *off_lse = o_bytes;
   if (off_geo) *off_geo = o_bytes + l_bytes;
   return o_bytes + l_bytes + g_bytes;
+}
+
+// Three work-groups per four CUs (one wave per SIMD where they run). 160 / 176
+// / 192 / 208 / 256 / 512 work-groups, us: 64 sequences of 1K-8K (32Q/4KV) 98.8
+// / 96.7 / 96.5 / 96.7 / 99.0 / 110.5, window 4096 at 128 sequences 168.9 /
+// 164.6 / 165.1 / 166.2 / 170.7 / 178.5.
+int default_wgs(int HKV) {
+  const int ny = HKV / waves_per_wg(HKV);
+  const int g = 3 * device_cus() / (4 * ny);
+  return g > 0 ? g : 1;
 }
 
 }  // namespace

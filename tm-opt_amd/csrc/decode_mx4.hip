@@ -521,7 +521,8 @@ extern "C" int tmopt_attn_decode_mx4(
                     (window > 0 && (int64_t)window <= (int64_t)table_wrap * kPS),
                 TMOPT_EINVAL, "decode_mx4: window=%d outside a ring of %d pages",
                 window, table_wrap);
-  TMOPT_REQUIRE(scale > 0.0f && softcap >= 0.0f && softcap < INFINITY,
+  TMOPT_REQUIRE(scale > 0.0f && scale < INFINITY && softcap >= 0.0f &&
+                    softcap < INFINITY,
                 TMOPT_EINVAL, "decode_mx4: scale=%g softcap=%g", scale,
                 softcap);
   TMOPT_REQUIRE(min_pages > 0 && num_workgroups >= 0 && num_workgroups <= 65535,

@@ -47,7 +47,9 @@
 
 #include <type_traits>
 
+#include "mx4.h"
 #include "prefill_sched.h"
+#include "score.h"
 
 namespace tmopt {
 
@@ -95,14 +97,37 @@ struct PrefillArgs {
   float* part_o;     // [nsplit * n_base][8 waves][16][64 lanes][4] fp32
   float* part_lse;   // [nsplit * n_base][256 rows]
   int* part_n;       // [n_base] pieces of each item (0: no such item)
+  // scored kernels (TMOPT_PREFILL_SCORED)
+  Cap cap;
+  const float* slopes;    // [HQ] or null
+  const int32_t* first;   // first position each query token sees, or null
+  const int32_t* prefix;  // [S] tokens of a run that all of it sees, or null
+  const uint8_t* pool4;   // kPaged4: the 4-bit cache
 };
 
 // prefill_split.hip: the split kernel and the merge, for `rep` query heads per
-// work-group and key source `src`
+// work-group and key source `src`; likewise the scored and the 4-bit kernels
+// (prefill_scored.hip, prefill_mx4.hip, whole items and split ones)
 void launch_prefill_split(const PrefillArgs& a, int rep, int src, size_t lds,
                           hipStream_t st);
+void launch_prefill_scored(const PrefillArgs& a, int rep, int src, size_t lds,
+                           hipStream_t st);
+void launch_prefill_scored_split(const PrefillArgs& a, int rep, int src,
+                                 size_t lds, hipStream_t st);
+void launch_prefill_mx4(const PrefillArgs& a, int rep, size_t lds,
+                        hipStream_t st);
+void launch_prefill_mx4_split(const PrefillArgs& a, int rep, size_t lds,
+                              hipStream_t st);
 
 namespace {
+
+// The score functions and masks of score.h, in translation units of their own:
+// the other kernels keep the instructions they have without them.
+#ifdef TMOPT_PREFILL_SCORED
+constexpr bool kScored = true;
+#else
+constexpr bool kScored = false;
+#endif
 
 constexpr int kD = 128;
 constexpr int kBN = 64;                   // keys per tile
@@ -129,6 +154,46 @@ __device__ __forceinline__ Tiles item_tiles(const PrefillArgs& a, int BQ,
   const int lo = a.window > 0 ? max(0, prior + q0 - a.window + 1) : 0;
   const int k_lo = (lo / kBN) * kBN;
   return Tiles{k_lo, (prior + min(len, q0 + BQ) - k_lo + kBN - 1) / kBN};
+}
+
+// The masks of a scored item: least and greatest first position of its queries
+// (0 without any), and the end of the keys that some query sees.
+struct Masks {
+  int first_lo, first_hi, k_hi, prefix;
+};
+__device__ __forceinline__ Masks item_masks(const PrefillArgs& a, int BQ,
+                                            int lane, const Work& wk) {
+  const int q0 = wk.qb * BQ;
+  const int qn = min(BQ, wk.len - q0);
+  Masks m{0, 0, wk.prior + q0 + qn, 0};
+  if (a.prefix != nullptr) {
+    m.prefix = min(as_const(a.prefix)[wk.seq], wk.prior + wk.len);
+    m.k_hi = max(m.k_hi, m.prefix);
+  }
+  if (a.first != nullptr) {
+    int lo = 0x7fffffff, hi = 0;
+    for (int i = lane; i < qn; i += 64) {
+      const int f = max(0, a.first[wk.t0 + q0 + i]);
+      lo = min(lo, f);
+      hi = max(hi, f);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      lo = min(lo, __shfl_xor(lo, d));
+      hi = max(hi, __shfl_xor(hi, d));
+    }
+    m.first_lo = __builtin_amdgcn_readfirstlane(lo);
+    m.first_hi = __builtin_amdgcn_readfirstlane(hi);
+  }
+  return m;
+}
+// and its tiles: one at least, also where no query sees a key
+__device__ __forceinline__ Tiles item_tiles(const PrefillArgs& a, int BQ,
+                                            const Work& wk, const Masks& m) {
+  const int win = a.window > 0 ? wk.prior + wk.qb * BQ - a.window + 1 : 0;
+  const int lo = min(max(0, max(win, m.first_lo)), m.k_hi - 1);
+  const int k_lo = (lo / kBN) * kBN;
+  return Tiles{k_lo, (m.k_hi - k_lo + kBN - 1) / kBN};
 }
 
 // Split keys: a launch of few items leaves most of the chip idle, and its
@@ -216,6 +281,7 @@ enum Source : int {
                 // pages), the run's own keys from packed k / v
   kPackedCM = 3,  // kPacked with channel-major k / v: tokens contiguous,
                   // head_dim strided (the sconv output), read in place
+  kPaged4 = 4,  // kPaged over the 4-bit cache
 };
 
 // Channel-major tiles in LDS are 128 dim rows of 64 keys (128 bytes, eight
@@ -250,8 +316,9 @@ template <int REP, bool REL, int SRC>
 __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
 #endif
   constexpr bool CM = SRC == kPackedCM;   // channel-major k / v tiles
+  constexpr bool Q4 = SRC == kPaged4;
   constexpr bool POOL = SRC == kPaged || SRC == kMixed;  // keys from pools
-  constexpr bool OWN = SRC != kPaged;     // the run's keys from packed k/v
+  constexpr bool OWN = SRC != kPaged && !Q4;  // the run's keys from packed k/v
   constexpr int BQ = 256 / REP;   // queries per work-group
   constexpr int QSUB = BQ / 32;   // 32-query sub-blocks per head
   extern __shared__ __align__(16) char smem[];
@@ -278,16 +345,20 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
   const int qn = min(BQ, len - q0);
   const int pos_lo = prior + q0;              // first query position
   const int pos_hi = prior + q0 + qn - 1;     // last valid query position
-  // first key any query of the block may see
-  const int kwin = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0;
+  // first key any query of the block may see, and the end of those
+  [[maybe_unused]] Masks mk{0, 0, pos_hi + 1, 0};
+  if constexpr (kScored) mk = item_masks(a, BQ, lane, wk);
+  const int kwin = max(a.window > 0 ? max(0, pos_lo - a.window + 1) : 0,
+                       kScored ? mk.first_lo : 0);
+  const int kend = kScored ? mk.k_hi : pos_hi + 1;
 #ifdef TMOPT_PREFILL_PIECES
   const int k_lo = item_k_lo + tile0 * kBN;
-  const int k_hi = min(pos_hi + 1, item_k_lo + tile1 * kBN);   // exclusive
+  const int k_hi = min(kend, item_k_lo + tile1 * kBN);   // exclusive
   const int ntiles = tile1 - tile0;
 #else
   // (tiles start at a multiple of the tile width)
-  const int k_lo = (kwin / kBN) * kBN;
-  const int k_hi = pos_hi + 1;                // exclusive
+  const int k_lo = ((kScored ? min(kwin, kend - 1) : kwin) / kBN) * kBN;
+  const int k_hi = kend;                // exclusive
   const int ntiles = (k_hi - k_lo + kBN - 1) / kBN;
 #endif
 
@@ -296,6 +367,14 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
   const int qi = q0 + 32 * (w % QSUB) + l32;  // this lane's query (column)
   const bool qok = qi < len;
   const int qpos = prior + qi;
+  // a scored query's first and last key, and its head's slope
+  [[maybe_unused]] int q_first = 0, q_last = qpos;
+  [[maybe_unused]] float slope = 0.0f;
+  if constexpr (kScored) {
+    if (a.first != nullptr && qok) q_first = a.first[t0 + qi];
+    q_last = max(qpos, mk.prefix - 1);
+    if (a.slopes != nullptr) slope = as_const(a.slopes)[head] * kLog2e;
+  }
 
   // ---- Q fragments: B operand of S^T (column = query, k = dims) --------
   bf16x8 qf[8];   // loaded through LDS in the prologue below
@@ -366,7 +445,7 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
     vlane = grp * row_b + kvs * (kD * 2) + 16 * vchunk;
   }
   [[maybe_unused]] const int32_t __attribute__((address_space(4)))* trow =
-      POOL ? as_const(a.bt) + (int64_t)seq * a.bt_stride : nullptr;
+      POOL || Q4 ? as_const(a.bt) + (int64_t)seq * a.bt_stride : nullptr;
   [[maybe_unused]] const int plim = SRC == kMixed ? prior : nk;
 
   // Four pool rows key0..key0+3 (one page: key0 % 4 == 0) into LDS. The
@@ -407,6 +486,66 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
     }
   };
 
+  // 4-bit pages go through registers: wave w holds the half w & 1 of page
+  // w >> 1 of a tile as it is stored (lane l: dims 16 (l & 7) .. +15 of token
+  // 8 (w & 1) + (l >> 3) of K; dims 8 (l & 15) .. +7 of tokens 8 (w & 1) + 2 (l
+  // >> 4), + 1 of V; and their scales), and writes it to LDS as bf16 one tile
+  // later, so that the loads have a tile's time. Rows outside [kwin, nk) take
+  // the scale 2^-127: they may never have been written, and the scale of a NaN
+  // would pass a weight of zero. (Always four loads a tile, as the direct loads
+  // of the other sources: the waits count them.)
+  [[maybe_unused]] u32x2 k4 = {}, v4 = {};
+  [[maybe_unused]] uint32_t ks4 = 0, vs4 = 0;
+  [[maybe_unused]] const int tok4k = 8 * (w & 1) + (lane >> 3);
+  [[maybe_unused]] const int tok4v = 8 * (w & 1) + 2 * (lane >> 4);
+  auto load4 = [&](int t, bool live) __attribute__((always_inline)) {
+    if constexpr (Q4) {
+      const int key0 = k_lo + t * kBN + kPage * (w >> 1);
+      const int lp = key0 >> 4;
+      const int pg =
+          live && (unsigned)lp < (unsigned)a.bt_width ? trow[lp] : -1;
+      const bool valid =
+          (unsigned)pg < (unsigned)a.num_pages && key0 < nk &&
+          key0 + kPage > kwin;
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint8_t*>(a.pool4) +
+              ((int64_t)(valid ? pg : 0) * a.HKV_stored + kvs) * kRecB,
+          (short)0, valid ? kRecB : 0, 0x00020000);
+      k4 = __builtin_amdgcn_raw_buffer_load_b64(
+          rs, 64 * tok4k + 8 * (lane & 7), 0, 0);
+      ks4 = __builtin_amdgcn_raw_buffer_load_b8(
+          rs, kRecKs + 16 * ((lane & 7) >> 1) + tok4k, 0, 0);
+      v4 = __builtin_amdgcn_raw_buffer_load_b64(
+          rs, kRecV + 64 * (lane & 15) + 4 * tok4v, 0, 0);
+      vs4 = __builtin_amdgcn_raw_buffer_load_b16(
+          rs, kRecVs + 16 * ((lane & 15) >> 2) + tok4v, 0, 0);
+    }
+  };
+  auto store4 = [&](int t, int st) __attribute__((always_inline)) {
+    if constexpr (Q4) {
+      const int key0 = k_lo + t * kBN + kPage * (w >> 1);
+      auto row_ok = [&](int tok) {
+        return key0 + tok >= kwin && key0 + tok < nk;
+      };
+      const uint32_t sb = lds0 + st * kStage + 16 * (w >> 1) * kRowB;
+      const float sk = scale_f32(row_ok(tok4k) ? ks4 & 0xff : 0u);
+      const uint32_t dk = sb + tok4k * kRowB;
+      const int c = 2 * (lane & 7);   // K chunk, slot c ^ (row & 15)
+      lds_st128(dk + 16 * (c ^ tok4k), dequantise8(k4[0], sk));
+      lds_st128(dk + 16 * ((c + 1) ^ tok4k), dequantise8(k4[1], sk));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = tok4v + i;
+        const float sv =
+            scale_f32(row_ok(row) ? vs4 >> (8 * i) & 0xff : 0u);
+        const int cv = lane & 15;     // V: 64-byte block b ^ (row & 3)
+        lds_st128(sb + kTileB + row * kRowB +
+                      16 * (((cv >> 2 ^ row) & 3) << 2 | (cv & 3)),
+                  dequantise8(v4[i], sv));
+      }
+    }
+  };
+
   // issue tile `t` (index from k_lo) into LDS stage `st`: 4 instructions
   // per wave (2 with the source split inside a 4-row block: one per source,
   // each under the exec mask of the lanes whose row it holds). live ==
@@ -417,7 +556,11 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
   auto issue_tile = [&](int t, int st, bool live = true) {
     const int kt = k_lo + t * kBN;
     const uint32_t sb = lds0 + st * kStage;
-    if constexpr (CM) {
+    if constexpr (Q4) {
+      // (the tile before it, which its loads have brought, to its stage)
+      store4(t - 1, (st - 1) & 3);
+      load4(t, live);
+    } else if constexpr (CM) {
       // dim rows 8w.. and 64+8w.. of the channel-major tile (see above)
       const bool in = live && kt + cm_key < len;
 #pragma unroll
@@ -729,8 +872,9 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
   // lane: two compares and a select per score.
   auto mask_tile = [&](f32x16 (&s)[2], int kt) {
     const int base = kt + 4 * h2;
-    const int hi = qok ? min(qpos, nk - 1) - base : -1;
-    const int lo = a.window > 0 ? qpos - a.window - base : -1;
+    const int hi = qok ? min(kScored ? q_last : qpos, nk - 1) - base : -1;
+    int lo = a.window > 0 ? qpos - a.window - base : -1;
+    if constexpr (kScored) lo = max(lo, q_first - 1 - base);
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -807,8 +951,39 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
   // never stored (masking them sent every tile of such a block down the
   // masked path, at about twice the cost per tile).
   auto full_tile = [&](int kt) {
+    if constexpr (kScored)
+      return kt + kBN - 1 <= max(pos_lo, mk.prefix - 1) && kt + kBN <= nk &&
+             (a.window == 0 || pos_hi - kt < a.window) && kt >= mk.first_hi;
     return (kt + kBN - 1 <= pos_lo) && (kt + kBN <= nk) &&
            (a.window == 0 || pos_hi - kt < a.window);
+  };
+  // Scores q.k -> the softmax's argument in units of log2(e), where there is a
+  // cap or a slope (elsewhere the scale comes with the exponent).
+  [[maybe_unused]] const bool with_fn =
+      kScored && (a.cap.in != 0.0f || a.slopes != nullptr);
+  [[maybe_unused]] auto score_tile = [&](f32x16 (&s)[2], int kt)
+      __attribute__((always_inline)) {
+    if (a.cap.in != 0.0f) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[kb][j] = a.cap(s[kb][j]);
+    } else {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[kb][j] *= a.scale_log2;
+    }
+    if (a.slopes != nullptr) {
+      // distance of element j of block kb: |d0 - c| (c as in mask_tile)
+      const float d0 = (float)(qpos - kt - 4 * h2);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          s[kb][j] -= slope * __builtin_fabsf(
+                                  d0 - (float)(32 * kb + 8 * (j >> 2) + (j & 3)));
+    }
   };
   f32x16 sc[2];        // scores of the tile after the one being multiplied
   bf16x8 pf[2][2];     // probabilities of the tile being multiplied
@@ -848,8 +1023,10 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
   auto softmax_phase = [&](f32x16 (&s)[2], int kt, bool first, auto&& hook) {
     const bool full = full_tile(kt);
     hook();
+    if constexpr (kScored)
+      if (with_fn) score_tile(s, kt);
     if (!full) mask_tile(s, kt);
-    const float sl2 = a.scale_log2;
+    const float sl2 = kScored && with_fn ? 1.0f : a.scale_log2;
     float mx = -INFINITY;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
@@ -973,8 +1150,15 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
       dma(rq, qlds + i * 1024, r * qst_b + 16 * (slot ^ (r & 15)));
     }
   }
-  issue_tile(0, 0);
-  if (ntiles > 1) issue_tile(1, 1);
+  if constexpr (Q4) {
+    load4(0, true);
+    store4(0, 0);
+    load4(1, ntiles > 1);
+    store4(1, 1);
+  } else {
+    issue_tile(0, 0);
+    if (ntiles > 1) issue_tile(1, 1);
+  }
   if constexpr (REL) {   // the first tile's bias windows and carry
     bias_dma(k_lo);
     bias_carry0();
@@ -990,7 +1174,8 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
     qf[kk] = __builtin_bit_cast(bf16x8, x);
   }
   __syncthreads();
-  if (ntiles > 2) issue_tile(2, 2);
+  if constexpr (Q4) load4(2, ntiles > 2);
+  else if (ntiles > 2) issue_tile(2, 2);
   // End of every odd slot: this wave's part of tile t+2 must be in LDS
   // before the barrier that publishes it. Loads issued after that tile's
   // may still fly: the DMA of tile t+3 and, with the fused bias, the 16
@@ -1062,8 +1247,13 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
 
   // ---- finalise: l over both lane halves, normalise, store --------------
   const float l_tot = l_part + __shfl_xor(l_part, 32);
+  // (no number as a sum: no number as LSE, for the newer entry points)
+  auto some = [&]() __attribute__((always_inline)) {
+    if constexpr (kScored || Q4) return l_tot != 0.0f;
+    else return l_tot > 0.0f;
+  };
   const float inv = rejected ? __builtin_nanf("") :
-                    l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
+                    some() ? 1.0f / l_tot : 0.0f;
 #ifdef TMOPT_PREFILL_PIECES
   if (part_slot >= 0) {
     // lane-major partial: every store writes 1 KB
@@ -1079,14 +1269,14 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
     if (h2 == 0)
       a.part_lse[pw * 32 + l32] =
           rejected ? __builtin_nanf("") :
-          l_tot > 0.0f ? (m_run + fast_log2(l_tot)) * kLn2 : -INFINITY;
+          some() ? (m_run + fast_log2(l_tot)) * kLn2 : -INFINITY;
     return;
   }
 #endif
   if (a.lse && h2 == 0 && qok)
     a.lse[(int64_t)head * wk.total + t0 + qi] =
         rejected ? __builtin_nanf("") :
-        l_tot > 0.0f ? (m_run + fast_log2(l_tot)) * kLn2 : -INFINITY;
+        some() ? (m_run + fast_log2(l_tot)) * kLn2 : -INFINITY;
   // O^T goes through LDS (free after the last barrier) so that the global
   // stores are whole rows: the wave writes its 32 x 128 block query-major
   // (256-byte rows, 16-byte chunks swizzled by row & 15, so neither the

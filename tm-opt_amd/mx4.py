@@ -20,9 +20,9 @@ Scores are scale q.k, and with
 """
 import torch
 
-from . import _lib
 from .attn import HEAD_DIM, PAGE_SIZE, _check_rows, _ptr, _refused_rows
 from .diff import _call, _table, _workspace_size
+from .scored import _index, _prefill_outputs, _runs, _slopes
 
 _BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 _DECODE_SIZE = "tmopt_attn_decode_mx4_workspace_size"
@@ -43,13 +43,6 @@ def _pool(pool, dev):
     assert pool.shape[2] == RECORD and pool.is_contiguous(), pool.shape
     assert pool.device == dev
     return pool.shape[0], pool.shape[1]
-
-
-def _slopes(slopes, HQ, dev):
-    if slopes is not None:
-        assert slopes.dtype == _F32 and slopes.shape == (HQ,)
-        assert slopes.is_contiguous() and slopes.device == dev
-    return _ptr(slopes)
 
 
 def kv_write_mx4(k, v, slot_mapping, pool):
@@ -157,4 +150,52 @@ def decode_mx4_paged(q, pool, block_table, ctx_lens, scale, softcap=0.0,
           HQ, HKV, D, PAGE_SIZE, P, int(window), float(scale), float(softcap),
           _slopes(slopes, HQ, dev), _ptr(rel), extent, int(min_pages),
           num_workgroups, out.data_ptr(), _ptr(lse), workspace.data_ptr(), n)
+    return out, lse
+
+
+def prefill_mx4_varlen(q, pool, block_table, cu_seqlens, prior_lens, scale,
+                       softcap=0.0, slopes=None, rel=None, window=0,
+                       max_seqlen=None, out=None, lse=None, return_lse=True,
+                       reject=None, max_context=None):
+    """Varlen causal (optionally windowed) attention over the 4-bit cache.
+
+    q [total, HQ, 128] bf16 (head_dim contiguous, any token / head strides);
+    block_table [S, bt_stride] int32; cu_seqlens [S + 1] int32; prior_lens [S]
+    int32 or None (no prior context): query j of run i sits at position
+    prior_lens[i] + j, and all its keys, the run's own among them, are in the
+    pages already. Pages without an entry read as zeros. softcap, slopes, rel
+    (bf16 [total, HQ, E], E contiguous) as above. reject: optional int32 device
+    scalar; nonzero gives NaN in every row of out and lse, those that cu_seqlens
+    gives no run included. max_seqlen bounds the run lengths (read from the
+    device, with a synchronisation, if None); max_context: an upper bound of
+    prior + run length, where the host has one (the row width of the block table
+    bounds it otherwise): whether keys are split over work-groups goes by it.
+    Returns (out [total, HQ, 128] bf16, lse [HQ, total] fp32 or None)."""
+    total, HQ, D = q.shape
+    dev = q.device
+    _check_rows(q, "q")
+    P, HKV = _pool(pool, dev)
+    assert HQ % HKV == 0, (pool.shape, HQ)
+    S, max_seqlen = _runs(cu_seqlens, total, max_seqlen, dev)
+    bts = _table(block_table, S, dev)
+    r_st = r_sh = extent = 0
+    if rel is not None:
+        assert rel.dtype == _BF16 and rel.stride(2) == 1
+        assert rel.shape[:2] == (total, HQ) and rel.device == dev, rel.shape
+        r_st, r_sh, extent = rel.stride(0), rel.stride(1), rel.shape[2]
+    out, lse = _prefill_outputs(q, out, lse, return_lse, reject)
+    most = 0 if max_context is None else max(1, int(max_context))
+    n = _workspace_size(dev, _PREFILL_SIZE, S, max_seqlen, most, HQ, HKV, bts,
+                        int(window))
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    _call(dev, "tmopt_attn_prefill_mx4", q.data_ptr(), q.stride(0),
+          q.stride(1), cu_seqlens.data_ptr(), _index(prior_lens, S, dev), S,
+          max_seqlen, most, pool.data_ptr(), block_table.data_ptr(), bts, PAGE_SIZE, P, HQ,
+          HKV, D, int(window), float(scale), float(softcap),
+          _slopes(slopes, HQ, dev), _ptr(rel), r_st, r_sh, extent,
+          out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse),
+          _ptr(reject), _ptr(ws), n)
+    if reject is not None:
+        _call(dev, "tmopt_refused_rows",
+              *_refused_rows(reject, out, lse, *out.shape, HQ))
     return out, lse
