@@ -37,6 +37,7 @@ namespace {
 constexpr int kMaxRep = 8;        // query heads per wave
 constexpr int kPages = 4;         // pages of a step
 constexpr int kIds4 = 1500;       // page ids of a range kept in LDS
+constexpr int kNt = 2;            // non-temporal: pages are read once
 
 struct Mx4Args {
   DecodeArgs d;   // (first: the page lookups read it in the argument segment)
@@ -54,13 +55,14 @@ struct Step4 {
 };
 enum : int { kHave = 64 };
 
+typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
+
 // What a lane loads of a step.
 template <bool REL>
 struct Buf4 {
   u32x4 k[kPages], v[kPages];
   uint32_t ks[kPages], vs[kPages];
-  u32x4 q[4];                           // of a piece's first step
-  uint32_t bias[REL ? kPages : 1][3];   // the dwords that hold rel[d - 3 .. d]
+  u32x3 bias[REL ? kPages : 1];         // the dwords that hold rel[d - 3 .. d]
 };
 
 // the value of lane n ^ 8 of each 16 lanes
@@ -211,6 +213,7 @@ void decode_mx4_kernel(Mx4Args args) {
   const int at_ks = kRecKs + 16 * g + n16;
   const int at_vs = kRecVs + 16 * (n16 >> 2) + 4 * g;
   const int at_q = (hq * kD + 32 * g) * 2;   // dims 32 g .. of the head's row
+  u32x4 q_next[4];   // query rows of a piece, with its first step
   auto load = [&](Buf4<REL>& x, const Step4& st, const int (&phys)[kPages])
       __attribute__((always_inline)) {
     const auto rq = __builtin_amdgcn_make_buffer_rsrc(
@@ -218,23 +221,26 @@ void decode_mx4_kernel(Mx4Args args) {
         st.flags & kFirst ? a.HQ * kD * 2 : 0, 0x00020000);
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk)
-      x.q[kk] = __builtin_amdgcn_raw_buffer_load_b128(rq, at_q + 16 * kk, 0, 0);
+      q_next[kk] =
+          __builtin_amdgcn_raw_buffer_load_b128(rq, at_q + 16 * kk, 0, 0);
 #pragma unroll
     for (int j = 0; j < kPages; ++j) {
       const auto rs = __builtin_amdgcn_make_buffer_rsrc(
           const_cast<uint8_t*>(args.pool) +
               ((int64_t)max(phys[j], 0) * rec_page + kvs * kRecB),
           (short)0, phys[j] >= 0 ? kRecB : 0, 0x00020000);
-      x.k[j] = __builtin_amdgcn_raw_buffer_load_b128(rs, at_k, 0, 0);
+      x.k[j] = __builtin_amdgcn_raw_buffer_load_b128(rs, at_k, 0, kNt);
       x.ks[j] = __builtin_amdgcn_raw_buffer_load_b8(rs, at_ks, 0, 0);
-      x.v[j] = __builtin_amdgcn_raw_buffer_load_b128(rs, at_k + kRecV, 0, 0);
+      x.v[j] = __builtin_amdgcn_raw_buffer_load_b128(rs, at_k + kRecV, 0, kNt);
       x.vs[j] = __builtin_amdgcn_raw_buffer_load_b32(rs, at_vs, 0, 0);
     }
     if constexpr (REL) {
       // rel[d - 3 .. d] of tokens 4g + 3 .. 4g of each page: three dwords from
-      // the one that holds rel[d - 3]; the resource starts at the dword of the
-      // sequence's first value. Dwords before it read as zeros, and what they
-      // or another head's values put into a score is masked or past the band.
+      // the one that holds rel[d - 3], in a resource that starts at the dword of
+      // the sequence's first value. (Before it there is nothing to read: a lane
+      // whose keys come up to the query itself may start there instead, see
+      // below.) What another head's values put into a score is masked or past
+      // the band.
       const char* const row = reinterpret_cast<const char*>(a.rel) +
                               (int64_t)max(st.b, 0) * a.HQ * a.rel_extent * 2;
       const int mis = (int)((uintptr_t)row & 3);
@@ -247,14 +253,7 @@ void decode_mx4_kernel(Mx4Args args) {
       for (int j = 0; j < kPages; ++j) {
         const int o = ((hq * a.rel_extent + dist - 16 * j - 4 * g - 3) * 2 +
                        mis) & ~3;
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-          // (an offset of its own: added by the instruction to a negative
-          // one, it would not come back into the range)
-          int oi = o + 4 * i;
-          asm volatile("" : "+v"(oi));
-          x.bias[j][i] = __builtin_amdgcn_raw_buffer_load_b32(rr, oi, 0, 0);
-        }
+        x.bias[j] = __builtin_amdgcn_raw_buffer_load_b96(rr, max(o, 0), 0, 0);
       }
     }
   };
@@ -265,18 +264,15 @@ void decode_mx4_kernel(Mx4Args args) {
   for (int m = 0; m < 4; ++m) o_acc[m] = f32x4{0, 0, 0, 0};
   float m_run = -INFINITY, l_part = 0.0f;
   bf16x8 qf[4];
-  const uint32_t p_mask = odd ? 0xffff0000u : 0x0000ffffu;
+  // (v_perm: bytes 4..7 are the two probabilities, 0x0c a zero)
+  const uint32_t p_sel0 = odd ? 0x05040c0cu : 0x0c0c0504u;
+  const uint32_t p_sel1 = odd ? 0x07060c0cu : 0x0c0c0706u;
   [[maybe_unused]] float slope = 0.0f;
   if constexpr (SCORE)
     if (args.slopes) slope = args.slopes[hq] * kLog2e;
 
   auto compute = [&](const Buf4<REL>& x, const Step4& st)
       __attribute__((always_inline)) {
-    if (st.flags & kFirst) {
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        qf[kk] = __builtin_bit_cast(bf16x8, x.q[kk]);
-    }
     // ---- scores -------------------------------------------------------------
     float s[kPages][4];
 #pragma unroll
@@ -290,8 +286,10 @@ void decode_mx4_kernel(Mx4Args args) {
             0, 0, 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        s[j][i] = SCORE && args.cap.in != 0.0f ? args.cap(c[i])
-                                               : c[i] * a.scale_log2;
+        if constexpr (SCORE)
+          s[j][i] = args.cap.in != 0.0f ? args.cap(c[i]) : c[i] * a.scale_log2;
+        else
+          s[j][i] = c[i];   // (the scale comes with the exponent)
       }
     }
     // distance of token 4g of the step's first page
@@ -306,25 +304,41 @@ void decode_mx4_kernel(Mx4Args args) {
       }
     }
     if constexpr (REL) {
+      // the bias as part of q.k, divided by the scale that follows
       if (left - 64 < a.rel_extent) {
-        const uintptr_t row = (uintptr_t)a.rel +
-                              (int64_t)st.b * a.HQ * a.rel_extent * 2;
+        const float inv_scale = kLog2e / a.scale_log2;
+        const int mis = (int)(((uintptr_t)a.rel +
+                               (int64_t)st.b * a.HQ * a.rel_extent * 2) & 3);
+        // o is even; the lane's bytes within the first dword: 0 or 2
+        const int o0 = (hq * a.rel_extent + left - 1 - 4 * g - 3) * 2 + mis;
+        const int sh = o0 & 2;
 #pragma unroll
         for (int j = 0; j < kPages; ++j) {
-          const int d0 = left - 1 - 16 * j - 4 * g;
-          const int sh = (int)((2 * (hq * a.rel_extent + d0 - 3) +
-                                (int)(row & 3)) & 2);
-          const uint32_t z0 =
-              __builtin_amdgcn_alignbyte(x.bias[j][1], x.bias[j][0], sh);
-          const uint32_t z1 =
-              __builtin_amdgcn_alignbyte(x.bias[j][2], x.bias[j][1], sh);
+          u32x3 y = x.bias[j];
+          if (left <= 64) {
+            // loaded from the resource's start instead of 1 or 2 dwords
+            // before it (which hold no value of a key that is there)
+            const int o = (o0 - 32 * j) & ~3;
+            const uint32_t y0 = y[0], y1 = y[1];
+            y[2] = o == -4 ? y1 : o == -8 ? y0 : y[2];
+            y[1] = o == -4 ? y0 : y1;
+          }
+          const uint32_t z0 = __builtin_amdgcn_alignbyte(y[1], y[0], sh);
+          const uint32_t z1 = __builtin_amdgcn_alignbyte(y[2], y[1], sh);
           const uint32_t b[4] = {z1 & 0xffff0000u, z1 << 16, z0 & 0xffff0000u,
                                  z0 << 16};
+          const int d0 = left - 1 - 16 * j - 4 * g;
+          if (left - 1 < a.rel_extent) {   // every key inside the band
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            s[j][i] += d0 - i < a.rel_extent
-                           ? __builtin_bit_cast(float, b[i]) * kLog2e
-                           : 0.0f;
+            for (int i = 0; i < 4; ++i)
+              s[j][i] += __builtin_bit_cast(float, b[i]) * inv_scale;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              s[j][i] += d0 - i < a.rel_extent
+                             ? __builtin_bit_cast(float, b[i]) * inv_scale
+                             : 0.0f;
+          }
         }
       }
     }
@@ -356,6 +370,8 @@ void decode_mx4_kernel(Mx4Args args) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[j][i]);
     mx = lane_pair(lane_pair(mx, 16, true), 32, true);
+    const float to_log2 = SCORE ? 1.0f : a.scale_log2;
+    if constexpr (!SCORE) mx *= to_log2;
     const bool move = mx > m_run;
     if (__builtin_amdgcn_ballot_w64(move)) {
       const float m_new = move ? mx : m_run;
@@ -368,12 +384,20 @@ void decode_mx4_kernel(Mx4Args args) {
     const float m_use = m_run == -INFINITY ? 0.0f : m_run;
 #pragma unroll
     for (int j = 0; j < kPages; ++j) {
-      uint32_t pw[4];
+      float p[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float p = fast_exp2(s[j][i] - m_use);
-        l_part += p;
-        pw[i] = pack_bf16x2_rn(p, p) & p_mask;
+        p[i] = fast_exp2(SCORE ? s[j][i] - m_use
+                               : __builtin_fmaf(s[j][i], to_log2, -m_use));
+        l_part += p[i];
+      }
+      // each probability in the low or the high half of its dword
+      uint32_t pw[4];
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        const uint32_t two = pack_bf16x2_rn(p[i], p[i + 1]);
+        pw[i] = __builtin_amdgcn_perm(two, 0u, p_sel0);
+        pw[i + 1] = __builtin_amdgcn_perm(two, 0u, p_sel1);
       }
       const bf16x8 pf =
           __builtin_bit_cast(bf16x8, u32x4{pw[0], pw[1], pw[2], pw[3]});
@@ -450,6 +474,11 @@ void decode_mx4_kernel(Mx4Args args) {
   // the next step's loads, then this step; false: that was the last one
   auto turn = [&](Buf4<REL>& now, Buf4<REL>& then)
       __attribute__((always_inline)) {
+    if (cur.flags & kFirst) {
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        qf[kk] = __builtin_bit_cast(bf16x8, q_next[kk]);
+    }
     next_step(nx, phys);
     load(then, nx, phys);
     compute(now, cur);
@@ -461,9 +490,9 @@ void decode_mx4_kernel(Mx4Args args) {
   }
 }
 
-// Ranges of the grid by default: eight waves per compute unit.
+// Ranges of the grid by default: four waves per compute unit, one per SIMD.
 int default_wgs4(int hkv) {
-  const int g = 8 * device_cus() / hkv;
+  const int g = 4 * device_cus() / hkv;
   return g > 0 ? g : 1;
 }
 
