@@ -707,6 +707,8 @@ int tmopt_kv_read_mx4(const void* pool, int64_t num_pages,
  * visible value block that is NaN gives NaN in its dims.
  * Any HQ / HKV; each stored head is read once for up to 8 query heads (a larger
  * ratio runs in groups of its largest divisor up to 8). B <= 8192.
+ * (Work is dealt out in steps of four pages of one request; min_pages is
+ * rounded up to them.)
  * workspace: tmopt_attn_decode_mx4_workspace_size bytes, 16-byte aligned,
  * without initialisation.
  */

@@ -216,8 +216,8 @@ def test_decode_without_functions_is_decode_paged(tm, dev):
     g = _gen(9)
     c = Cache(EDGES, 4, g, dev)
     q = _rand((len(EDGES), 32, D), g, dev)
-    a = tm.decode_scored_paged(q, c.kp, c.vp, c.table, c.ctx, 0.1)
-    b = tm.decode_paged(q, c.kp, c.vp, c.table, c.ctx, 0.1)
+    a = tm.decode_scored_paged(q, c.kp, c.vp, c.table, c.ctx, 0.1, min_pages=8)
+    b = tm.decode_paged(q, c.kp, c.vp, c.table, c.ctx, 0.1, min_pages=8)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 

@@ -36,7 +36,7 @@ namespace {
 
 constexpr int kMaxRep = 8;        // query heads per wave
 constexpr int kPages = 4;         // pages of a step
-constexpr int kIds4 = 1500;       // page ids of a range kept in LDS
+constexpr int kIds4 = 400;        // steps of a range whose page ids LDS keeps
 constexpr int kNt = 2;            // non-temporal: pages are read once
 
 struct Mx4Args {
@@ -88,21 +88,26 @@ void decode_mx4_kernel(Mx4Args args) {
   int* pref = reinterpret_cast<int*>(smem);  // [B + 1]
   int* wsum = pref + a.B + 1;                // [4]
   int* nlen = wsum + 4;                      // [B]
-  int* ids = reinterpret_cast<int*>(smem + a.ids_off);   // [kIds4 + 4]
+  int* ids = reinterpret_cast<int*>(smem + a.ids_off);   // [kIds4 * kPages]
 
-  // ---- visible pages: prefix sums, this work-group's range ----------------
+  // ---- the steps of the batch: prefix sums, this work-group's range --------
+  // A sequence has one step for every four of its visible pages, and a range is
+  // C steps of the batch: a step of one page costs what one of four does, so
+  // ranges of as many steps end together (ranges of pages gave eight requests of
+  // a few tokens to one work-group: 64 of 16 tokens took 22.8 us, now 8.2).
   // (n - 1) / 16 + 1 pages: lengths may come up to 2^31 - 1
   auto first_page = [&](int n) { return vis_lo(n, a.window) / kPS; };
   auto pages_of = [&](int n) {
     return n <= 0 ? 0 : (n - 1) / kPS + 1 - first_page(n);
   };
+  auto steps_of = [&](int n) { return (pages_of(n) + kPages - 1) / kPages; };
   {
     int carry = 0;
     for (int b0 = 0; b0 < a.B; b0 += blockDim.x) {
       const int b = b0 + threadIdx.x;
       const int nb = b < a.B ? a.ctx_lens[b] : 0;
       if (b < a.B) nlen[b] = nb;
-      const int x = wave_scan(pages_of(nb));
+      const int x = wave_scan(steps_of(nb));
       if (lane == 63) wsum[w] = x;
       __syncthreads();
       int before = carry;
@@ -115,7 +120,7 @@ void decode_mx4_kernel(Mx4Args args) {
     __syncthreads();
   }
   const int U = __builtin_amdgcn_readfirstlane(pref[a.B]);
-  const int C = max((U + G - 1) / G, a.min_pages);
+  const int C = max((U + G - 1) / G, (a.min_pages + kPages - 1) / kPages);
   if (wg == 0 && blockIdx.y == 0) {   // for the merge
     for (int i = threadIdx.x; i <= a.B; i += blockDim.x) a.geo[1 + i] = pref[i];
     if (threadIdx.x == 0) a.geo[0] = C;
@@ -146,16 +151,19 @@ void decode_mx4_kernel(Mx4Args args) {
     }
     return lo;
   };
-  const int nids = min(u1 - u0, kIds4);
+  const int nids = min(u1 - u0, kIds4) * kPages;
   for (int i = threadIdx.x; i < nids; i += blockDim.x) {
-    const int b = seq_of(u0 + i);
-    ids[i] = page_id<0>(kernel_args(false), b,
-                        first_page(nlen[b]) + (u0 + i - pref[b]));
+    const int u = u0 + i / kPages;
+    const int b = seq_of(u);
+    const int pg = (u - pref[b]) * kPages + i % kPages;
+    ids[i] = pg < pages_of(nlen[b])
+                 ? page_id<0>(kernel_args(false), b, first_page(nlen[b]) + pg)
+                 : -1;
   }
   int cb = __builtin_amdgcn_readfirstlane(seq_of(u0));
   int seq_start = __builtin_amdgcn_readfirstlane(pref[cb]);
   int cur_n = __builtin_amdgcn_readfirstlane(nlen[cb]);
-  int seq_end = seq_start + pages_of(cur_n);
+  int seq_end = seq_start + steps_of(cur_n);
   int cu = u0;
   int last_b = -1;
   __syncthreads();
@@ -170,29 +178,28 @@ void decode_mx4_kernel(Mx4Args args) {
       ++cb;
       seq_start = seq_end;
       cur_n = as_const(a.ctx_lens)[cb];
-      seq_end = seq_start + pages_of(cur_n);
+      seq_end = seq_start + steps_of(cur_n);
     }
-    const int cnt = min(kPages, min(seq_end, u1) - cu);
     st.b = cb;
     st.n = cur_n;
-    st.pg = cu - seq_start + first_page(cur_n);
+    st.pg = (cu - seq_start) * kPages + first_page(cur_n);
     const int at = cu - u0;
     int have = 0;
-    if (at + kPages <= kIds4) {
+    if (at < kIds4) {
+      const i32x4 id = reinterpret_cast<const i32x4*>(ids)[at];
 #pragma unroll
       for (int j = 0; j < kPages; ++j)
-        phys[j] = __builtin_amdgcn_readfirstlane(ids[at + j]);
+        phys[j] = __builtin_amdgcn_readfirstlane(id[j]);
     } else {
+      const int last = first_page(cur_n) + pages_of(cur_n);
 #pragma unroll
       for (int j = 0; j < kPages; ++j)
-        if (j < cnt) phys[j] = page_id<0>(kernel_args(true), cb, st.pg + j);
+        if (st.pg + j < last)
+          phys[j] = page_id<0>(kernel_args(true), cb, st.pg + j);
     }
 #pragma unroll
-    for (int j = 0; j < kPages; ++j) {
-      if (j >= cnt) phys[j] = -1;
-      have |= phys[j] >= 0 ? kHave << j : 0;
-    }
-    cu += cnt;
+    for (int j = 0; j < kPages; ++j) have |= phys[j] >= 0 ? kHave << j : 0;
+    ++cu;
     const int lo = vis_lo(cur_n, a.window);
     // (a full step has its 64 keys below n, so st.pg * 16 + 64 is in range)
     const bool full = have == 15 * kHave && cur_n - st.pg * kPS >= 64 &&
@@ -604,7 +611,7 @@ extern "C" int tmopt_attn_decode_mx4(
   x.slopes = slopes;
   const int nw = waves_per_wg(hkv);
   a.ids_off = (int)(((2 * (size_t)B + 1 + 4) * sizeof(int) + 15) & ~(size_t)15);
-  const size_t lds = a.ids_off + (kIds4 + 4) * sizeof(int);
+  const size_t lds = a.ids_off + kIds4 * kPages * sizeof(int);
   const dim3 grid(G, hkv / nw);
   hipStream_t st = (hipStream_t)stream;
   if (rel)

@@ -282,6 +282,7 @@ enum Source : int {
   kPackedCM = 3,  // kPacked with channel-major k / v: tokens contiguous,
                   // head_dim strided (the sconv output), read in place
   kPaged4 = 4,  // kPaged over the 4-bit cache
+  kBounded = 8,  // (a flag beside the source) scored: a cap alone, see Cap
 };
 
 // Channel-major tiles in LDS are 128 dim rows of 64 keys (128 bytes, eight
@@ -306,15 +307,17 @@ __device__ __forceinline__ int cm_sig(int r) {
 // out in another order, and eight prompts of 512-8192 tokens (32Q/4KV) took
 // 1037 us against 1030.
 #ifdef TMOPT_PREFILL_PIECES
-template <int REP, bool REL, int SRC>
+template <int REP, bool REL, int SRCF>
 __device__ __forceinline__ void prefill_item(const PrefillArgs& a,
                                              const Work& wk, int item_k_lo,
                                              int tile0, int tile1,
                                              int part_slot) {
 #else
-template <int REP, bool REL, int SRC>
+template <int REP, bool REL, int SRCF>
 __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
 #endif
+  constexpr int SRC = SRCF & 7;
+  constexpr bool BOUNDED = kScored && (SRCF & kBounded) != 0;
   constexpr bool CM = SRC == kPackedCM;   // channel-major k / v tiles
   constexpr bool Q4 = SRC == kPaged4;
   constexpr bool POOL = SRC == kPaged || SRC == kMixed;  // keys from pools
@@ -961,6 +964,7 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
   // cap or a slope (elsewhere the scale comes with the exponent).
   [[maybe_unused]] const bool with_fn =
       kScored && (a.cap.in != 0.0f || a.slopes != nullptr);
+  if constexpr (BOUNDED) m_run = 0.0f;
   [[maybe_unused]] auto score_tile = [&](f32x16 (&s)[2], int kt)
       __attribute__((always_inline)) {
     if (a.cap.in != 0.0f) {
@@ -1023,6 +1027,41 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
   auto softmax_phase = [&](f32x16 (&s)[2], int kt, bool first, auto&& hook) {
     const bool full = full_tile(kt);
     hook();
+    if constexpr (BOUNDED) {
+      // a cap alone: sums of 2^x, without a maximum
+      float mx = 0.0f;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int j = 0; j < 16; j += 2)
+          mx = fmaxf(fmaxf(mx, __builtin_fabsf(s[kb][j])),
+                     __builtin_fabsf(s[kb][j + 1]));
+      if (__builtin_amdgcn_ballot_w64(mx > a.cap.lim)) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) s[kb][j] = a.cap(s[kb][j]);
+      } else {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) s[kb][j] = a.cap.small(s[kb][j]);
+      }
+      if (!full) mask_tile(s, kt);
+      float psum = 0.0f;
+      uint32_t pw[16];
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        const int kb = q >> 3, kk = (q >> 2) & 1, e = q & 3;
+        const float p0 = fast_exp2(s[kb][8 * kk + 2 * e]);
+        const float p1 = fast_exp2(s[kb][8 * kk + 2 * e + 1]);
+        psum += p0 + p1;
+        pw[q] = pack_bf16x2_rn(p0, p1);
+      }
+      pack_p(pw, pf);
+      l_part += psum;
+      return;
+    }
     if constexpr (kScored)
       if (with_fn) score_tile(s, kt);
     if (!full) mask_tile(s, kt);

@@ -8,15 +8,22 @@ namespace {
 template <int REP>
 void launch(const PrefillArgs& a, int src, size_t lds, hipStream_t st) {
   const dim3 grid((unsigned)(a.n_base * a.nsplit));
-  if (src == kPacked)
-    hipLaunchKernelGGL((prefill_split_kernel<REP, false, kPacked>), grid,
-                       dim3(512), lds, st, a);
-  else if (src == kPaged)
-    hipLaunchKernelGGL((prefill_split_kernel<REP, false, kPaged>), grid,
-                       dim3(512), lds, st, a);
-  else
-    hipLaunchKernelGGL((prefill_split_kernel<REP, false, kPaged4>), grid,
-                       dim3(512), lds, st, a);
+  // a cap alone has kernels of its own
+  const int kind = src | (a.cap.bounded() && !a.slopes ? kBounded : 0);
+#define TMOPT_LAUNCH(K)                                                     \
+  case K:                                                                   \
+    hipLaunchKernelGGL((prefill_split_kernel<REP, false, K>), grid, dim3(512), \
+                       lds, st, a);                                         \
+    break
+  switch (kind) {
+    TMOPT_LAUNCH(kPacked);
+    TMOPT_LAUNCH(kPaged);
+    TMOPT_LAUNCH(kPaged4);
+    TMOPT_LAUNCH(kPacked | kBounded);
+    TMOPT_LAUNCH(kPaged | kBounded);
+    TMOPT_LAUNCH(kPaged4 | kBounded);
+  }
+#undef TMOPT_LAUNCH
   hipLaunchKernelGGL((prefill_merge_kernel<REP, true>), dim3(a.n_base, 8),
                      dim3(256), 0, st, a);
 }

@@ -14,7 +14,7 @@ namespace {
 // or not, 64 + 256 queries after 7,936 and 7,680 keys give 12 or 13 pieces),
 // and the merge must read exactly the slots that were written. Every work-group
 // of this kernel runs the same instructions on the same lengths.
-template <int REP, bool REL, int SRC>
+template <int REP, bool REL, int SRCF>
 __global__ __launch_bounds__(512) void prefill_split_kernel(PrefillArgs a) {
   constexpr int BQ = 256 / REP;
   const int lane = threadIdx.x & 63;
@@ -35,11 +35,11 @@ __global__ __launch_bounds__(512) void prefill_split_kernel(PrefillArgs a) {
   const int slot = pc.nall > 1 ? (int)blockIdx.x : -1;
   if constexpr (REL) {
     if (level < pc.np && pc.nall > 1) {
-      prefill_item<REP, false, SRC>(a, wk, tl.k_lo, t0, t1, slot);
+      prefill_item<REP, false, SRCF>(a, wk, tl.k_lo, t0, t1, slot);
       return;
     }
   }
-  prefill_item<REP, REL, SRC>(a, wk, tl.k_lo, t0, t1, slot);
+  prefill_item<REP, REL, SRCF>(a, wk, tl.k_lo, t0, t1, slot);
 }
 
 // A 32-row block of outputs on its way through LDS, query-major: 256-byte

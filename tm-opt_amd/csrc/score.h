@@ -10,23 +10,50 @@
 namespace tmopt {
 namespace {
 
-// tanh(z / cap) cap, in units of log2(e), of s = q.k: with t = exp(2 z / cap) it
+// cap tanh(z / cap), in units of log2(e), of s = q.k. With t = exp(2 z / cap) it
 // is cap (1 - 2 / (1 + t)), whatever the sign; t = 0 and infinity give -cap and
-// cap. fp32 throughout: near zero, where 1 - 2 / (1 + t) cancels, the result is
-// off by 2^-23 cap, less than a probability's rounding to bf16 for caps to 2^14.
+// cap. fp32 throughout: 1 - 2 / (1 + t) is off by 5.5 x 2^-23 at most (t by
+// 2^-23 of itself, the sum, the reciprocal and the difference by a rounding
+// each), less than a probability's rounding to bf16 for caps to 2^12.
 struct Cap {
   float in;    // 2 log2(e) scale / cap; 0: no cap
   float out;   // cap log2(e)
+  // up to |z| = cap / 2 also s (c0 + c1 s^2 + c2 s^4 + c3 s^6): five instructions
+  // of one issue slot instead of eight slots
+  float lim;   // the |s| up to which that holds
+  float c0, c1, c2, c3;
   __device__ __forceinline__ float operator()(float s) const {
     return out - 2.0f * out *
                      __builtin_amdgcn_rcpf(1.0f + fast_exp2(s * in));
   }
+  __device__ __forceinline__ float small(float s) const {
+    const float u = s * s;
+    return s * __builtin_fmaf(
+                   __builtin_fmaf(__builtin_fmaf(c3, u, c2), u, c1), u, c0);
+  }
+  // Scores within the cap need no running maximum where 2^+-cap is far inside
+  // fp32 and bf16: sums are of 2^x, x between -90 and 90.
+  __host__ __device__ bool bounded() const {
+    return in != 0.0f && out <= 90.0f;
+  }
 };
 
 inline Cap make_cap(float softcap, float scale) {
-  return softcap > 0.0f ? Cap{2.0f * kLog2e * scale / softcap,
-                              softcap * kLog2e}
-                        : Cap{0.0f, 0.0f};
+  Cap c{};
+  if (!(softcap > 0.0f)) return c;
+  c.in = 2.0f * kLog2e * scale / softcap;
+  c.out = softcap * kLog2e;
+  // Minimax in s^2 of tanh(y) / y weighted by y over |y| <= 1/2: tanh is off by
+  // 2^-22.9, 2^-21 with the roundings. (Outside these k its powers, or those of
+  // s, leave fp32.)
+  const double k = (double)scale / softcap;
+  c.lim = k > 1e-4 && k < 1e2 ? (float)(0.5 / k) : -1.0f;
+  const double a[4] = {0.999997676192731, -0.33320655218286016,
+                       0.13145145657253834, -0.04337248369819732};
+  double p = k * softcap * 1.4426950408889634;
+  float* const to[4] = {&c.c0, &c.c1, &c.c2, &c.c3};
+  for (int i = 0; i < 4; ++i, p *= k * k) *to[i] = (float)(a[i] * p);
+  return c;
 }
 
 }  // namespace
