@@ -328,3 +328,47 @@ def test_decode_large_pool(tm, dev):
         q, pool, table, torch.tensor([60], dtype=torch.int32, device=dev), 0.1)
     r = ref.attend(q, K, V, torch.tensor([59], device=dev), pos, 0.1)
     ref.check(out, lse, (r[0], r[1].T, r[2], r[3].T))
+
+
+def test_decode_largest_batch(tm, dev):
+    """8192 requests of 0 to 40 tokens; and work-split knobs at their ends."""
+    g = _gen(10)
+    ends = [int(x) for x in torch.randint(0, 41, (8192,), generator=g)]
+    c = Cache4(tm, ends, 1, g, dev)
+    q = _rand((8192, 2, D), g).to(dev)
+    out, lse = tm.decode_mx4_paged(q, c.pool, c.table, c.ctx, 0.1)
+    pick = [0, 1, 4095, 4096, 8190, 8191] + list(range(100, 8000, 97))
+    r = ref.decode(q[pick], c.kp, c.vp, c.table[pick], c.ctx[pick], 0.1)
+    ref.check(out[pick], lse[pick], r)
+    for kw in (dict(min_pages=2 ** 31 - 1), dict(num_workgroups=65535),
+               dict(num_workgroups=1, min_pages=1)):
+        o, l = tm.decode_mx4_paged(q, c.pool, c.table, c.ctx, 0.1, **kw)
+        ref.check(o[pick], l[pick], r, str(kw))
+
+
+def test_decode_lengths_past_the_table(tm, dev):
+    """Lengths far past what the table's rows hold: those keys are absent."""
+    g = _gen(11)
+    c = Cache4(tm, [64] * 100, 1, g, dev)
+    q = _rand((100, 4, D), g).to(dev)
+    c.ctx.fill_(2 ** 31 - 1)
+    out, lse = tm.decode_mx4_paged(q, c.pool, c.table, c.ctx, 0.1)
+    pos = torch.arange(64, device=dev)
+    for b in (0, 1, 57, 99):
+        r = ref.attend(q[b:b + 1], ref.rows_of(c.kp, c.table[b], pos),
+                       ref.rows_of(c.vp, c.table[b], pos),
+                       torch.tensor([2 ** 31 - 2], device=dev), pos, 0.1)
+        ref.check(out[b:b + 1], lse[b:b + 1], (r[0], r[1].T, r[2], r[3].T))
+    # a window that begins past the table: no key at all
+    out, lse = tm.decode_mx4_paged(q, c.pool, c.table, c.ctx, 0.1, window=500)
+    assert (out == 0).all() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("cap", [0.01, 1.0, 62.0, 63.0, 4000.0])
+def test_decode_caps(tm, dev, cap):
+    """Caps from far below the scores to far above them."""
+    g = _gen(12)
+    c = Cache4(tm, [33, 500], 1, g, dev)
+    q = _rand((2, 8, D), g, 4.0).to(dev)
+    _decode(tm, c, q, 0.1, softcap=cap)
+    _decode(tm, c, q * 0.01, 0.1, softcap=cap)

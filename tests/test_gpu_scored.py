@@ -221,6 +221,61 @@ def test_decode_without_functions_is_decode_paged(tm, dev):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+def test_decode_largest_batch(tm, dev):
+    """8192 requests of 0 to 40 tokens; and work-split knobs at their ends."""
+    g = _gen(10)
+    ends = [int(x) for x in torch.randint(0, 41, (8192,), generator=g)]
+    rows = torch.cumsum(torch.tensor([0] + [-(-n // PAGE) for n in ends]), 0)
+    table = torch.full((8192, 3), -1, dtype=torch.int32)
+    for i, n in enumerate(ends):
+        k = -(-n // PAGE)
+        table[i, :k] = torch.arange(int(rows[i]), int(rows[i]) + k)
+    table = table.to(dev)
+    kp, vp = (_rand((int(rows[-1]), PAGE, 1, D), g, dev) for _ in range(2))
+    ctx = _i32(ends, dev)
+    first = torch.randint(-3, 20, (8192,), generator=g).int().to(dev)
+    q = _rand((8192, 2, D), g, dev)
+    pick = [0, 1, 4095, 4096, 8190, 8191] + list(range(100, 8000, 97))
+    r = ref.decode(q[pick], kp, vp, table[pick], ctx[pick], 0.1,
+                   first=first[pick], softcap=3.0)
+    for kw in (dict(), dict(min_pages=2 ** 31 - 1),
+               dict(num_workgroups=65535), dict(num_workgroups=1)):
+        o, l = tm.decode_scored_paged(q, kp, vp, table, ctx, 0.1, softcap=3.0,
+                                      first_keys=first, **kw)
+        ref.check(o[pick], l[pick], r, str(kw))
+
+
+def test_decode_lengths_past_the_table(tm, dev):
+    g = _gen(11)
+    c = Cache([64] * 100, 1, g, dev)
+    q = _rand((100, 4, D), g, dev)
+    c.ctx.fill_(2 ** 31 - 1)
+    out, lse = tm.decode_scored_paged(q, c.kp, c.vp, c.table, c.ctx, 0.1)
+    pos = torch.arange(64, device=dev)
+    for b in (0, 1, 57, 99):
+        r = ref.attend(q[b:b + 1], ref.rows_of(c.kp, c.table[b], pos),
+                       ref.rows_of(c.vp, c.table[b], pos),
+                       torch.tensor([2 ** 31 - 2], device=dev), pos, 0.1)
+        ref.check(out[b:b + 1], lse[b:b + 1], (r[0], r[1].T, r[2], r[3].T))
+    out, lse = tm.decode_scored_paged(q, c.kp, c.vp, c.table, c.ctx, 0.1,
+                                      window=500)
+    assert (out == 0).all() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("cap", [0.01, 1.0, 62.0, 63.0, 4000.0])
+def test_caps(tm, dev, cap):
+    """Caps from far below the scores to far above them, scores that the
+    polynomial takes and that it does not."""
+    g = _gen(12)
+    c = Cache([33, 500], 1, g, dev)
+    q = _rand((2, 8, D), g, dev, 4.0)
+    _decode(tm, c, q, 0.1, softcap=cap)
+    _decode(tm, c, q * 0.01, 0.1, softcap=cap)
+    q, k, v, cu = _packed([300, 70], 8, 1, g, dev)
+    for gain in (8.0, 1.0, 0.02):
+        _prefill(tm, q * gain, k, v, cu, 0.1, f"gain {gain}", softcap=cap)
+
+
 # --------------------------------------------------------------------------
 # prefill: packed prompts
 # --------------------------------------------------------------------------

@@ -72,7 +72,7 @@ def test_decode_refusals(tm):
                    dict(HQ=0), dict(bts=0), dict(pages=0), dict(window=-1),
                    dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan),
                    dict(scale=math.inf), dict(cap=-1.0), dict(cap=math.nan),
-                   dict(cap=math.inf), dict(mp=0), dict(wgs=-1),
+                   dict(cap=math.inf), dict(cap=1e-39), dict(cap=3e38), dict(mp=0), dict(wgs=-1),
                    dict(wgs=65536), dict(wrap=-1), dict(wrap=9), dict(wrap=4),
                    dict(wrap=4, window=65)):
             assert call(**kw) == e.TMOPT_EINVAL, kw
@@ -117,7 +117,7 @@ def test_prefill_refusals(tm):
                    dict(out=ctypes.c_void_p(20)), dict(qt=4092),
                    dict(qt=-4096), dict(ot=4098), dict(HQ=33),
                    dict(HQ=4, HKV=0), dict(window=-1), dict(scale=0.0),
-                   dict(scale=math.nan), dict(cap=-2.0), dict(cap=math.inf),
+                   dict(scale=math.nan), dict(cap=-2.0), dict(cap=math.inf), dict(cap=1e-39),
                    dict(most=-1), dict(pool, kp=NULL), dict(pool, kp=ODD),
                    dict(pool, bts=0), dict(pool, pages=0)):
             assert call(**kw) == e.TMOPT_EINVAL, (call, kw)

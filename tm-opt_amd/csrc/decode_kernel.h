@@ -174,8 +174,12 @@ __device__ __forceinline__ int seq_lo(ArgsPtr a, int b, int n) {
   return a->first != nullptr ? max(lo, as_const(a->first)[b]) : lo;
 }
 __device__ __forceinline__ int seq_pages(ArgsPtr a, int b, int n) {
-  const int lo = seq_lo(a, b, n);   // (n may come up to 2^31 - 1)
-  return n <= 0 || lo >= n ? 0 : (n - 1) / kPS + 1 - lo / kPS;
+  // (n may come up to 2^31 - 1; pages past the table's width have no entry and
+  // are not walked)
+  const int lo = seq_lo(a, b, n);
+  if (n <= 0 || lo >= n) return 0;
+  const int last = (n - 1) / kPS + 1;
+  return max(0, (a->table_wrap > 0 ? last : min(last, a->bt_width)) - lo / kPS);
 }
 #define TMOPT_SEQ_LO(args, b, n) seq_lo(args, b, n)
 #define TMOPT_SEQ_PAGES(args, b, n) seq_pages(args, b, n)

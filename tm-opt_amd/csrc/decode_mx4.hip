@@ -95,10 +95,13 @@ void decode_mx4_kernel(Mx4Args args) {
   // C steps of the batch: a step of one page costs what one of four does, so
   // ranges of as many steps end together (ranges of pages gave eight requests of
   // a few tokens to one work-group: 64 of 16 tokens took 22.8 us, now 8.2).
-  // (n - 1) / 16 + 1 pages: lengths may come up to 2^31 - 1
+  // (n - 1) / 16 + 1 pages: lengths may come up to 2^31 - 1. Pages past the
+  // table's width have no entry and are not walked.
   auto first_page = [&](int n) { return vis_lo(n, a.window) / kPS; };
   auto pages_of = [&](int n) {
-    return n <= 0 ? 0 : (n - 1) / kPS + 1 - first_page(n);
+    int last = n <= 0 ? 0 : (n - 1) / kPS + 1;
+    if (a.table_wrap == 0) last = min(last, a.bt_width);
+    return max(0, last - first_page(n));
   };
   auto steps_of = [&](int n) { return (pages_of(n) + kPages - 1) / kPages; };
   {
@@ -120,7 +123,7 @@ void decode_mx4_kernel(Mx4Args args) {
     __syncthreads();
   }
   const int U = __builtin_amdgcn_readfirstlane(pref[a.B]);
-  const int C = max((U + G - 1) / G, (a.min_pages + kPages - 1) / kPages);
+  const int C = max((U + G - 1) / G, (a.min_pages - 1) / kPages + 1);
   if (wg == 0 && blockIdx.y == 0) {   // for the merge
     for (int i = threadIdx.x; i <= a.B; i += blockDim.x) a.geo[1 + i] = pref[i];
     if (threadIdx.x == 0) a.geo[0] = C;
@@ -281,7 +284,7 @@ void decode_mx4_kernel(Mx4Args args) {
   auto compute = [&](const Buf4<REL>& x, const Step4& st)
       __attribute__((always_inline)) {
     // ---- scores -------------------------------------------------------------
-    float s[kPages][4];
+    float s[kPages][4];   // (without a cap the scale comes with the exponent)
 #pragma unroll
     for (int j = 0; j < kPages; ++j) {
       f32x4 c = f32x4{0, 0, 0, 0};
@@ -292,11 +295,31 @@ void decode_mx4_kernel(Mx4Args args) {
             __builtin_bit_cast(bf16x8, dequantise8(x.k[j][kk], ks)), qf[kk], c,
             0, 0, 0);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (SCORE)
-          s[j][i] = args.cap.in != 0.0f ? args.cap(c[i]) : c[i] * a.scale_log2;
-        else
-          s[j][i] = c[i];   // (the scale comes with the exponent)
+      for (int i = 0; i < 4; ++i) s[j][i] = c[i];
+    }
+    if constexpr (SCORE) {
+      if (args.cap.in != 0.0f) {
+        float big = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kPages; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) big = fmaxf(big, __builtin_fabsf(s[j][i]));
+        if (__builtin_amdgcn_ballot_w64(big > args.cap.lim)) {
+#pragma unroll
+          for (int j = 0; j < kPages; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[j][i] = args.cap(s[j][i]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kPages; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[j][i] = args.cap.small(s[j][i]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kPages; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[j][i] *= a.scale_log2;
       }
     }
     // distance of token 4g of the step's first page
@@ -557,8 +580,7 @@ extern "C" int tmopt_attn_decode_mx4(
                     (window > 0 && (int64_t)window <= (int64_t)table_wrap * kPS),
                 TMOPT_EINVAL, "decode_mx4: window=%d outside a ring of %d pages",
                 window, table_wrap);
-  TMOPT_REQUIRE(scale > 0.0f && scale < INFINITY && softcap >= 0.0f &&
-                    softcap < INFINITY,
+  TMOPT_REQUIRE(scale > 0.0f && scale < INFINITY && good_cap(softcap, scale),
                 TMOPT_EINVAL, "decode_mx4: scale=%g softcap=%g", scale,
                 softcap);
   TMOPT_REQUIRE(min_pages > 0 && num_workgroups >= 0 && num_workgroups <= 65535,

@@ -59,8 +59,7 @@ extern "C" int tmopt_attn_decode_scored(
                 TMOPT_EINVAL,
                 "decode_scored: window=%d outside a ring of %d pages", window,
                 table_wrap);
-  TMOPT_REQUIRE(scale > 0.0f && scale < INFINITY && softcap >= 0.0f &&
-                    softcap < INFINITY,
+  TMOPT_REQUIRE(scale > 0.0f && scale < INFINITY && good_cap(softcap, scale),
                 TMOPT_EINVAL, "decode_scored: scale=%g softcap=%g", scale,
                 softcap);
   TMOPT_REQUIRE(min_pages > 0 && num_workgroups >= 0 && num_workgroups <= 65535,
@@ -96,7 +95,8 @@ extern "C" int tmopt_attn_decode_scored(
   a.num_pages = num_pages > 0x7fffffff ? 0x7fffffff : (int)num_pages;
   a.window = window;
   a.scale_log2 = scale * kLog2e;
-  a.min_pages = min_pages;
+  // (a work-group's first page, its index times this, stays within int32)
+  a.min_pages = min_pages < 32768 ? min_pages : 32768;
   a.out = (__bf16*)out;
   a.lse = lse;
   a.part_o = (float*)workspace;

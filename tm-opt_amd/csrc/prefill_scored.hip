@@ -78,7 +78,7 @@ int run(const char* what, PrefillArgs& a, int src, const void* q,
   TMOPT_REQUIRE(HQ / rep <= 65535, TMOPT_EUNSUPPORTED,
                 "%s: %d query-head groups exceed 65535", what, HQ / rep);
   TMOPT_REQUIRE(window >= 0 && scale > 0.0f && scale < INFINITY &&
-                    softcap >= 0.0f && softcap < INFINITY,
+                    good_cap(softcap, scale),
                 TMOPT_EINVAL, "%s: window=%d scale=%g softcap=%g", what, window,
                 scale, softcap);
   TMOPT_REQUIRE((int64_t)(HQ / rep) * num_seqs *

@@ -38,6 +38,12 @@ struct Cap {
   }
 };
 
+// A cap that fp32 can work with: 0, or 2 log2(e) scale / softcap in its range.
+inline bool good_cap(float softcap, float scale) {
+  return softcap == 0.0f || (softcap > 0.0f && softcap < INFINITY &&
+                             scale / softcap < 1e37f && scale / softcap > 1e-37f);
+}
+
 inline Cap make_cap(float softcap, float scale) {
   Cap c{};
   if (!(softcap > 0.0f)) return c;

@@ -132,7 +132,7 @@ def decode_mx4_paged(q, pool, block_table, ctx_lens, scale, softcap=0.0,
         assert 0 < window <= table_wrap * PAGE_SIZE, \
             "a ring table needs a window no wider than the ring"
     if out is None:
-        out = torch.empty((B, HQ, D), dtype=_BF16, device=dev)
+        out = torch.empty_like(q)
     else:
         assert out.shape == q.shape and out.device == dev
         assert out.dtype == _BF16 and out.is_contiguous()
