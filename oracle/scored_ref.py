@@ -11,7 +11,9 @@ is off by dx, the sum of
     rounding add up to 5.5 x 2^-23 < 2^-20), and so may its argument: 4 x 2^-24
     of y sech^2(y) is less than 2^-22;
   * a bias of size w: 4 x 2^-24 (w + |x|) for its product and the sum, and
-    bf16 biases are exact.
+    bf16 biases are exact. Slopes may also join q.k as the first term of its
+    sum: then each of the eight sums of 16 products rounds at their size, by
+    2^-23 w at most, 16 x 2^-24 w in all.
 Then p changes by p dx relative to the rest, so LSE = log sum exp is off by at
 most sum p dx (and n x 2^-24 for a sum of n terms, 16 x 2^-24 for exp2, log2 and
 the last products, and 8 x 2^-24 of |LSE| and of the maximum). Outputs: p is
@@ -128,7 +130,7 @@ def attend(q, K, V, qpos, kpos, scale, softcap=0.0, slopes=None, rel=None,
         if slopes is not None:
             w = slopes[h].double() * dist.abs()
             x = x - w
-            dx = dx + 4 * HALF_F32 * (w.abs() + x.abs())
+            dx = dx + HALF_F32 * (20 * w.abs() + 4 * x.abs())
         if rel is not None:
             E = rel.shape[2]
             b = rel[:, h].double().gather(1, dist.clamp(0, E - 1))

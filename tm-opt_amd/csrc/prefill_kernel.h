@@ -282,7 +282,9 @@ enum Source : int {
   kPackedCM = 3,  // kPacked with channel-major k / v: tokens contiguous,
                   // head_dim strided (the sconv output), read in place
   kPaged4 = 4,  // kPaged over the 4-bit cache
-  kBounded = 8,  // (a flag beside the source) scored: a cap alone, see Cap
+  // flags beside the source of a scored kernel
+  kBounded = 8,  // a cap alone (see Cap::bounded)
+  kSloped = 16,  // slopes without a cap
 };
 
 // Channel-major tiles in LDS are 128 dim rows of 64 keys (128 bytes, eight
@@ -318,6 +320,7 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
 #endif
   constexpr int SRC = SRCF & 7;
   constexpr bool BOUNDED = kScored && (SRCF & kBounded) != 0;
+  constexpr bool SLOPED = kScored && (SRCF & kSloped) != 0;
   constexpr bool CM = SRC == kPackedCM;   // channel-major k / v tiles
   constexpr bool Q4 = SRC == kPaged4;
   constexpr bool POOL = SRC == kPaged || SRC == kMixed;  // keys from pools
@@ -652,7 +655,7 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
   // (with the fused bias, s already holds the tile's bias / scale)
   auto scores = [&](int stage, f32x16 (&s)[2]) {
     const uint32_t kt_b = lds0 + stage * kStage;
-    if constexpr (!REL) {
+    if constexpr (!REL && !SLOPED) {
       s[0] = f32x16{};
       s[1] = f32x16{};
     }
@@ -960,10 +963,36 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
     return (kt + kBN - 1 <= pos_lo) && (kt + kBN <= nk) &&
            (a.window == 0 || pos_hi - kt < a.window);
   };
+  // The bias by distance of a key tile as the initial value of its score
+  // accumulators, -slope |distance| / scale: one instruction a score where all
+  // distances have one sign (masked ones may be wrong), and no scaling later.
+  [[maybe_unused]] const float slope_s =
+      SLOPED ? slope / a.scale_log2 : 0.0f;
+  [[maybe_unused]] auto slope_init = [&](f32x16 (&s)[2], int kt)
+      __attribute__((always_inline)) {
+    // element j of block kb is at distance d0 - c (c as in mask_tile)
+    const float d0 = (float)(qpos - kt - 4 * h2);
+    if (mk.prefix > pos_lo && kt + kBN - 1 > pos_lo) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          s[kb][j] = -slope_s * __builtin_fabsf(
+                         d0 - (float)(32 * kb + 8 * (j >> 2) + (j & 3)));
+    } else {
+      const float base = -slope_s * d0;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          s[kb][j] = __builtin_fmaf(
+              slope_s, (float)(32 * kb + 8 * (j >> 2) + (j & 3)), base);
+    }
+  };
   // Scores q.k -> the softmax's argument in units of log2(e), where there is a
-  // cap or a slope (elsewhere the scale comes with the exponent).
+  // cap (elsewhere the scale comes with the exponent).
   [[maybe_unused]] const bool with_fn =
-      kScored && (a.cap.in != 0.0f || a.slopes != nullptr);
+      kScored && !SLOPED && (a.cap.in != 0.0f || a.slopes != nullptr);
   if constexpr (BOUNDED) m_run = 0.0f;
   [[maybe_unused]] auto score_tile = [&](f32x16 (&s)[2], int kt)
       __attribute__((always_inline)) {
@@ -1119,6 +1148,7 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
       bias_tile(sc, k_lo + (t + 1) * kBN);
       b2 = bias_dma_base(k_lo + (t + 2) * kBN);
     }
+    if constexpr (with_s && SLOPED) slope_init(sc, k_lo + (t + 1) * kBN);
     const uint32_t vt_b = lds0 + (t & 3) * kStage + kTileB;
     const uint32_t kt_b = lds0 + ((t + 1) & 3) * kStage;
     auto vf_n = [&](int n) {
@@ -1145,8 +1175,8 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
       if (with_s) {
         const int skb = n & 1, skk = n >> 1;
         sc[skb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            kf[n % R], qf[skk], (!REL && n < 2) ? f32x16{} : sc[skb], 0, 0,
-            0);
+            kf[n % R], qf[skk],
+            (!REL && !SLOPED && n < 2) ? f32x16{} : sc[skb], 0, 0, 0);
       }
       if constexpr (with_s && REL) {
         if (n < 8) {
@@ -1248,6 +1278,7 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
       bias_tile(sc, k_lo);
       bias_dma(k_lo + kBN);
     }
+    if constexpr (SLOPED) slope_init(sc, k_lo);
   };
   if (grp_id == 0) {
     bias_first();
