@@ -53,7 +53,7 @@ struct Step4 {
   int pg;      // first logical page
   int flags;   // kFirst, kLast, kFull, kWhole; page j is there: kHave << j
 };
-enum : int { kHave = 64 };
+enum : int { kHave = 64 };   // (bit 6)
 
 typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
 
@@ -163,12 +163,20 @@ void decode_mx4_kernel(Mx4Args args) {
                  ? page_id<0>(kernel_args(false), b, first_page(nlen[b]) + pg)
                  : -1;
   }
+  // the sequence of the next step, from step seq_start of the batch on
   int cb = __builtin_amdgcn_readfirstlane(seq_of(u0));
   int seq_start = __builtin_amdgcn_readfirstlane(pref[cb]);
-  int cur_n = __builtin_amdgcn_readfirstlane(nlen[cb]);
-  int seq_end = seq_start + steps_of(cur_n);
+  int cur_n, cur_lo, seq_end, piece_end, seq_flags;
+  auto enter = [&](int n) __attribute__((always_inline)) {
+    cur_n = n;
+    cur_lo = vis_lo(n, a.window);
+    seq_end = seq_start + steps_of(n);
+    piece_end = min(seq_end, u1);
+    seq_flags = kFirst | (seq_start >= u0 && seq_end <= u1 ? kWhole : 0);
+  };
+  enter(__builtin_amdgcn_readfirstlane(nlen[cb]));
   int cu = u0;
-  int last_b = -1;
+  int cur_pg = first_page(cur_n) + (u0 - seq_start) * kPages;
   __syncthreads();
   auto next_step = [&](Step4& st, int (&phys)[kPages])
       __attribute__((always_inline)) {
@@ -177,17 +185,18 @@ void decode_mx4_kernel(Mx4Args args) {
 #pragma unroll
     for (int j = 0; j < kPages; ++j) phys[j] = -1;
     if (cu >= u1) return;
-    while (seq_end <= cu) {
-      ++cb;
-      seq_start = seq_end;
-      cur_n = as_const(a.ctx_lens)[cb];
-      seq_end = seq_start + steps_of(cur_n);
+    if (cu >= seq_end) {
+      do {
+        ++cb;
+        seq_start = seq_end;
+        enter(as_const(a.ctx_lens)[cb]);
+      } while (seq_end <= cu);
+      cur_pg = first_page(cur_n);
     }
     st.b = cb;
     st.n = cur_n;
-    st.pg = (cu - seq_start) * kPages + first_page(cur_n);
+    st.pg = cur_pg;
     const int at = cu - u0;
-    int have = 0;
     if (at < kIds4) {
       const i32x4 id = reinterpret_cast<const i32x4*>(ids)[at];
 #pragma unroll
@@ -197,26 +206,26 @@ void decode_mx4_kernel(Mx4Args args) {
       const int last = first_page(cur_n) + pages_of(cur_n);
 #pragma unroll
       for (int j = 0; j < kPages; ++j)
-        if (st.pg + j < last)
-          phys[j] = page_id<0>(kernel_args(true), cb, st.pg + j);
+        if (cur_pg + j < last)
+          phys[j] = page_id<0>(kernel_args(true), cb, cur_pg + j);
     }
-#pragma unroll
-    for (int j = 0; j < kPages; ++j) have |= phys[j] >= 0 ? kHave << j : 0;
     ++cu;
-    const int lo = vis_lo(cur_n, a.window);
-    // (a full step has its 64 keys below n, so st.pg * 16 + 64 is in range)
-    const bool full = have == 15 * kHave && cur_n - st.pg * kPS >= 64 &&
-                      st.pg * kPS >= lo;
-    st.flags = (cb != last_b ? kFirst : 0) |
-               (cu == min(seq_end, u1) ? kLast : 0) | (full ? kFull : 0) |
-               (seq_start >= u0 && seq_end <= u1 ? kWhole : 0) | have;
-    last_b = cb;
+    // (a full step has its 64 keys below n, so cur_pg * 16 + 64 is in range)
+    const bool full = (phys[0] | phys[1] | phys[2] | phys[3]) >= 0 &&
+                      cur_n - cur_pg * kPS >= 64 && cur_pg * kPS >= cur_lo;
+    st.flags = seq_flags | (cu == piece_end ? kLast : 0) | (full ? kFull : 0);
+#pragma unroll
+    for (int j = 0; j < kPages; ++j)
+      st.flags |= (int)((uint32_t)~phys[j] >> 31) << (6 + j);
+    seq_flags &= ~kFirst;
+    cur_pg += kPages;
   };
 
   // ---- loads ----------------------------------------------------------------
   // A page's record is one buffer resource (an absent page: an empty one,
   // whose loads give zeros and fetch nothing), so every step issues the same
-  // loads and the waits for them need no branch.
+  // loads of pages and the waits for them need no branch. A piece's query rows
+  // come before the pages of its first step.
   const int kvs = kvh / a.kv_div;
   const int rec_page = a.HKV_stored * kRecB;
   const int at_k = 64 * n16 + 16 * g;
@@ -226,13 +235,15 @@ void decode_mx4_kernel(Mx4Args args) {
   u32x4 q_next[4];   // query rows of a piece, with its first step
   auto load = [&](Buf4<REL>& x, const Step4& st, const int (&phys)[kPages])
       __attribute__((always_inline)) {
-    const auto rq = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<__bf16*>(a.q + (int64_t)max(st.b, 0) * a.HQ * kD), (short)0,
-        st.flags & kFirst ? a.HQ * kD * 2 : 0, 0x00020000);
+    if (st.flags & kFirst) {
+      const auto rq = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<__bf16*>(a.q + (int64_t)st.b * a.HQ * kD), (short)0,
+          a.HQ * kD * 2, 0x00020000);
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk)
-      q_next[kk] =
-          __builtin_amdgcn_raw_buffer_load_b128(rq, at_q + 16 * kk, 0, 0);
+      for (int kk = 0; kk < 4; ++kk)
+        q_next[kk] =
+            __builtin_amdgcn_raw_buffer_load_b128(rq, at_q + 16 * kk, 0, 0);
+    }
 #pragma unroll
     for (int j = 0; j < kPages; ++j) {
       const auto rs = __builtin_amdgcn_make_buffer_rsrc(
