@@ -104,7 +104,16 @@ void decode_mx4_kernel(Mx4Args args) {
     return max(0, last - first_page(n));
   };
   auto steps_of = [&](int n) { return (pages_of(n) + kPages - 1) / kPages; };
-  {
+  if (a.B <= 64) {   // one wave's scan, one barrier
+    const int nb = lane < a.B ? a.ctx_lens[lane] : 0;
+    const int x = wave_scan(steps_of(nb));
+    if (w == 0 && lane < a.B) {
+      nlen[lane] = nb;
+      pref[lane + 1] = x;
+      if (lane == 0) pref[0] = 0;
+    }
+    __syncthreads();
+  } else {
     int carry = 0;
     for (int b0 = 0; b0 < a.B; b0 += blockDim.x) {
       const int b = b0 + threadIdx.x;
@@ -162,9 +171,11 @@ void decode_mx4_kernel(Mx4Args args) {
     ids[i] = pg < pages_of(nlen[b])
                  ? page_id<0>(kernel_args(false), b, first_page(nlen[b]) + pg)
                  : -1;
+    if (i == 0) wsum[0] = b;
   }
+  __syncthreads();
   // the sequence of the next step, from step seq_start of the batch on
-  int cb = __builtin_amdgcn_readfirstlane(seq_of(u0));
+  int cb = __builtin_amdgcn_readfirstlane(wsum[0]);
   int seq_start = __builtin_amdgcn_readfirstlane(pref[cb]);
   int cur_n, cur_lo, seq_end, piece_end, seq_flags;
   auto enter = [&](int n) __attribute__((always_inline)) {
@@ -177,7 +188,7 @@ void decode_mx4_kernel(Mx4Args args) {
   enter(__builtin_amdgcn_readfirstlane(nlen[cb]));
   int cu = u0;
   int cur_pg = first_page(cur_n) + (u0 - seq_start) * kPages;
-  __syncthreads();
+  i32x4 id_next = reinterpret_cast<const i32x4*>(ids)[0];   // a step ahead
   auto next_step = [&](Step4& st, int (&phys)[kPages])
       __attribute__((always_inline)) {
     st.b = -1;
@@ -198,10 +209,10 @@ void decode_mx4_kernel(Mx4Args args) {
     st.pg = cur_pg;
     const int at = cu - u0;
     if (at < kIds4) {
-      const i32x4 id = reinterpret_cast<const i32x4*>(ids)[at];
 #pragma unroll
       for (int j = 0; j < kPages; ++j)
-        phys[j] = __builtin_amdgcn_readfirstlane(id[j]);
+        phys[j] = __builtin_amdgcn_readfirstlane(id_next[j]);
+      id_next = reinterpret_cast<const i32x4*>(ids)[min(at + 1, kIds4 - 1)];
     } else {
       const int last = first_page(cur_n) + pages_of(cur_n);
 #pragma unroll
