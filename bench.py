@@ -314,7 +314,9 @@ def source_digest(paths):
     return h.hexdigest()
 
 
-DECODE_SOURCES = ("tm-opt_amd/csrc/decode.hip", "tm-opt_amd/csrc/common.h")
+DECODE_SOURCES = ("tm-opt_amd/csrc/decode.hip",
+                  "tm-opt_amd/csrc/decode_kernel.h",
+                  "tm-opt_amd/csrc/score.h", "tm-opt_amd/csrc/common.h")
 
 
 def measured_traffic():

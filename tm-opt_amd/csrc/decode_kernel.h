@@ -892,7 +892,30 @@ __global__ __launch_bounds__(32 * H * S) void decode_combine_kernel(
     for (int j = 0; j < kBatch; ++j)     // (0 x infinity: weight 0 won't do)
       add(l4[j], 1.0f, k + j * S < np ? o4[j] : f32x4{0, 0, 0, 0});
   }
-  if constexpr (S > 1) {
+  if constexpr (NANS && S > 4) {
+    // pairs of groups, then pairs of those: the upper half leaves (m, sum, acc)
+    // for the lower one, five rounds for 32 groups (one group joining the other
+    // 31 in a row waits 31 times on LDS: 196 pieces of one sequence 6.0 us)
+    __shared__ float part[H * S][6][32];
+    const int l = threadIdx.x & 31;
+#pragma unroll
+    for (int w = S / 2; w > 0; w /= 2) {
+      if (sub >= w && sub < 2 * w) {
+        part[grp][0][l] = m;
+        part[grp][1][l] = sum;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[grp][2 + i][l] = acc[i];
+      }
+      __syncthreads();
+      if (sub < w) {
+        f32x4 o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = part[grp + w][2 + i][l];
+        add(part[grp + w][0][l], part[grp + w][1][l], o);
+      }
+    }
+    if (sub > 0) return;
+  } else if constexpr (S > 1) {
     // (m, sum, acc) of every group but the head's first, then merged by it
     __shared__ float part[H * S][6][32];
     const int l = threadIdx.x & 31;
@@ -913,16 +936,19 @@ __global__ __launch_bounds__(32 * H * S) void decode_combine_kernel(
     }
   }
   if (!hok) return;
-  const bool none = NANS ? sum == 0.0f : !(sum > 0.0f);
-  const float inv = !none ? 1.0f / sum : 0.0f;
+  auto some = [&]() __attribute__((always_inline)) {
+    if constexpr (NANS) return sum != 0.0f;
+    else return sum > 0.0f;
+  };
+  const float inv = some() ? 1.0f / sum : 0.0f;
   __bf16* o = a.out + ((int64_t)b * a.HQ + h) * kD + d0;
   *reinterpret_cast<u32x2*>(o) =
       u32x2{pack_bf16x2_rn(acc[0] * inv, acc[1] * inv),
             pack_bf16x2_rn(acc[2] * inv, acc[3] * inv)};
   if (a.lse && d0 == 0)
     a.lse[(int64_t)b * a.HQ + h] =
-        !none ? (m == -INFINITY ? 0.0f : m) + fast_log2(sum) * kLn2
-              : -INFINITY;
+        some() ? (m == -INFINITY ? 0.0f : m) + fast_log2(sum) * kLn2
+               : -INFINITY;
 }
 
 // The merge's shape, from the number of pieces of an average sequence (at most

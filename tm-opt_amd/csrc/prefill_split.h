@@ -129,13 +129,16 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillArgs a) {
   }
   // (a rejected launch's pieces are NaN, and so is their sum)
   const bool rejected = a.reject != nullptr && as_const(a.reject)[0] != 0;
-  const bool none = NANS ? sum == 0.0f : !(sum > 0.0f);
-  const float inv = !none ? 1.0f / sum : 0.0f;
+  auto some = [&]() __attribute__((always_inline)) {
+    if constexpr (NANS) return sum != 0.0f;
+    else return sum > 0.0f;
+  };
+  const float inv = some() ? 1.0f / sum : 0.0f;
   const int qi = qrow0 + l32;
   if (a.lse && db == 0 && lane < 32 && qi < wk.len)
     a.lse[(int64_t)head * wk.total + wk.t0 + qi] =
         rejected ? __builtin_nanf("")
-        : !none ? m + fast_log2(sum) * kLn2 : -INFINITY;
+        : some() ? m + fast_log2(sum) * kLn2 : -INFINITY;
   const uint32_t ob =
       (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)rows);
 #pragma unroll
