@@ -146,7 +146,7 @@ def test_prefill_refusals(tm):
         for kw in (dict(ws=EIGHT, nbytes=need), dict(ws=P, nbytes=need - 1)):
             assert call(**dict(pool, bts=500, **kw)) == e.TMOPT_EWORKSPACE, kw
         # a bound of the contexts counts where it is below the table's width
-        assert size(2, 64, 900, 32, 4, 500, 0) == 0
+        assert size(2, 64, 512, 32, 4, 500, 0) == 0
         assert size(2, 64, 1 << 40, 32, 4, 500, 0) == need
     size = lib.tmopt_attn_prefill_scored_workspace_size
     assert size(1, 200, 0, 32, 4, 0, 0) == 0 < size(1, 4000, 0, 4, 1, 0, 0)

@@ -204,9 +204,10 @@ __device__ __forceinline__ Tiles item_tiles(const PrefillArgs& a, int BQ,
 // in piece order. An item gets as many pieces as compute units by its share of
 // the launch's tiles (rounded down, so that the pieces run in one wave; a
 // share a little short of a whole one counts as one: the tiles of the launch
-// are an estimate from the first and last block of each run), each of kMinPiece tiles at least, and stays whole where the pieces'
-// cost (~6 us for their start and the merge, 0.065 us for the 129 KB that each
-// piece of the launch writes and reads back) is above the tiles saved, 1.7 us
+// are an estimate from the first and last block of each run), each of kMinPiece
+// tiles at least, and stays whole where the pieces' cost (~6 us for their start
+// and the merge, 0.065 us for the 129 KB that each piece of the launch writes
+// and reads back) is above the tiles saved, 1.7 us
 // each.
 // With a bias, the tiles wholly past its band (the first `plain` ones) are
 // pieces of their own, which run without one (1.7 us per tile against
@@ -216,8 +217,20 @@ __device__ __forceinline__ Tiles item_tiles(const PrefillArgs& a, int BQ,
 // Measured (per call of the chunk adapter, 64Q/8KV, bias extent 1024): 64
 // tokens after 30,000 958 -> 96 us, 500 after 15,000 531 -> 277 us, 200 + 200
 // after 8,000 276 -> 158 us, 64 after 1,500 105 -> 43 us.
+// The scored and the 4-bit prefill (TMOPT_PREFILL_SHORT_PIECES) take pieces from
+// half that on, and count less for them: ~5 us and 0.03 us a piece. Us a call,
+// pieces of 8 / 4 tiles at least, 64Q/8KV over the 4-bit cache: 1 query after
+// 1,000 24.6 / 21.0, 64 after 1,000 27.4 / 21.6, 64 after 2,000 28.1 / 23.6, 128
+// after 600 26.4 / 23.7; 4 and 2 after 5,639 and 3,901 (16Q/2KV, cap) 37.6 / 24.6.
+#ifdef TMOPT_PREFILL_SHORT_PIECES
+constexpr int kMinPiece = 4;
+constexpr int kMinSplit = 9;
+constexpr float kSplitCost = 5.0f, kPieceCost = 0.03f;
+#else
 constexpr int kMinPiece = 8;
 constexpr int kMinSplit = 16;   // tiles: two pieces
+constexpr float kSplitCost = 6.0f, kPieceCost = 0.065f;
+#endif
 struct Pieces {
   int plain;       // tiles before the bias band (all of them without a bias)
   int np, nall;    // pieces of those, pieces in all
@@ -249,7 +262,8 @@ __device__ __forceinline__ Pieces key_pieces(const PrefillArgs& a, int BQ,
   };
   const Pieces whole{tl.n, 1, 1, 0};
   const int n = pieces(share, tl.n, a.nsplit);
-  if (1.7f * tl.n * (n - 1) <= n * (6.0f + 0.065f * min(a.split_wgs, n * a.n_base)))
+  if (1.7f * tl.n * (n - 1) <=
+      n * (kSplitCost + kPieceCost * min(a.split_wgs, n * a.n_base)))
     return whole;
   if (a.rel == nullptr) return Pieces{tl.n, n, n, 0};
   // tile t is past the band if its last key is E or more before every query

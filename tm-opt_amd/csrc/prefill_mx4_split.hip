@@ -1,6 +1,7 @@
 // Launches of the prefill over the 4-bit cache with split
 // keys (prefill_split.h), without score functions
 // (those: prefill_scored_split.hip), with and without the relative bias.
+#define TMOPT_PREFILL_SHORT_PIECES
 #include "prefill_split.h"
 
 namespace tmopt {

@@ -1,6 +1,7 @@
 // C entry points of the scored prefill and of the prefill over the 4-bit cache,
 // and the scored kernels of whole items (kernels: prefill_kernel.h; split keys:
 // prefill_scored_split.hip, prefill_mx4_split.hip).
+#define TMOPT_PREFILL_SHORT_PIECES
 #define TMOPT_PREFILL_SCORED
 #include "prefill_host.h"
 

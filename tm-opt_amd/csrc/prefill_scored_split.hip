@@ -1,4 +1,5 @@
 // Launches of the scored prefill with split keys (kernels: prefill_split.h).
+#define TMOPT_PREFILL_SHORT_PIECES
 #define TMOPT_PREFILL_SCORED
 #include "prefill_split.h"
 
