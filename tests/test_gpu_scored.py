@@ -262,7 +262,7 @@ def test_decode_lengths_past_the_table(tm, dev):
     assert (out == 0).all() and (lse == -math.inf).all()
 
 
-@pytest.mark.parametrize("cap", [0.01, 1.0, 62.0, 63.0, 4000.0])
+@pytest.mark.parametrize("cap", [0.01, 1.0, 53.0, 54.0, 62.0, 63.0, 4000.0])
 def test_caps(tm, dev, cap):
     """Caps from far below the scores to far above them, scores that the
     polynomial takes and that it does not."""
@@ -325,6 +325,47 @@ def _prefill(tm, q, k, v, cu, scale, what="", prefix=None, first=None, **kw):
     ref.check(out, lse, ref.prefill(q, k, v, cu, scale, first=first,
                                     prefix=prefix, **kw), what)
     return out, lse
+
+
+@pytest.mark.parametrize("cap", [30.0, 53.0])
+def test_prefill_cap_one_key(tm, dev, cap):
+    """Queries that see themselves only: their value as it is (its probability is
+    1, which bf16 holds); the others' keys hold no number."""
+    g = _gen(31)
+    lens = [1, 70, 200]
+    q, k, v, cu = _packed(lens, 8, 2, g, dev)
+    own = torch.cat([torch.arange(n) for n in lens]).to(torch.int32).to(dev)
+    out, lse = tm.prefill_scored_varlen(q, k, v, cu, 0.1, softcap=cap,
+                                        first_keys=own)
+    assert torch.equal(out, v.repeat_interleave(4, 1))
+    z = 0.1 * (q.double() * k.repeat_interleave(4, 1).double()).sum(2)
+    x = cap * torch.tanh(z / cap)
+    # the cap 2^-19 of itself; the score's products and sums, the LSE's own
+    far = cap * 2.0 ** -19 + 132 * 2.0 ** -24 * 0.1 * (
+        q.double() * k.repeat_interleave(4, 1).double()).abs().sum(2) + \
+        24 * 2.0 ** -24 * (1 + x.abs())
+    assert ((lse.T.double() - x).abs() <= far).all()
+
+
+@pytest.mark.parametrize("cap", [30.0, 53.0])
+@pytest.mark.parametrize("order", ["up", "down", "low"])
+def test_prefill_cap_far_first_tile(tm, dev, cap, order):
+    """A first tile at one end of the cap and the rest at the other: what is
+    taken as the reference of a query is far from what its keys come to."""
+    g = _gen(32)
+    n = 400
+    base = _rand((1, 1, D), g, dev, 2.0)
+    q = base.expand(n, 8, D).contiguous()
+    sign = torch.ones(n, 1, 1, dtype=BF, device=dev)
+    sign[:70] = {"up": -1.0, "down": 1.0, "low": -1.0}[order]
+    if order != "up":
+        sign[70:] = -1.0
+    k = (base * sign * 3.0).expand(n, 2, D).contiguous()
+    v = _rand((n, 2, D), g, dev, 100.0)
+    _prefill(tm, q, k, v, _i32([0, n], dev), 0.1, order, softcap=cap)
+    first = torch.arange(n, dtype=torch.int32, device=dev) // 3 * 2
+    _prefill(tm, q, k, v, _i32([0, n], dev), 0.1, order, softcap=cap,
+             first=first)
 
 
 RUNS = [1, 0, 33, 64, 65, 200, 31, 7]
@@ -541,6 +582,42 @@ def test_chunk_split_keys(tm, dev, four, lens, prior):
         _chunk(tm, c, q, cu, p, 0.1, "masks", prefix=_i32(
             [x - 20 for x in prior], dev), first=_firsts(lens, prior, g, dev))
         _chunk(tm, c, q, cu, p, 0.1, "one launch", most=1, softcap=9.0)
+
+
+@pytest.mark.parametrize("four", [0, 1])
+def test_pages_far_into_the_pool(tm, dev, four):
+    """Rows past 2^32 bytes of the pools, by decode and prefill."""
+    g = _gen(33)
+    hkv = 16
+    P = 2 ** 32 // (hkv * (ref.RECORD if four else PAGE * D * 2)) + 40
+    ids = [P - 1, 3, P - 7, P - 2]
+    c = Cache([60], hkv, g, dev)
+    far = _i32([ids], dev)
+    pos = torch.arange(60, device=dev)
+    near = c.table[0][pos // PAGE].long(), pos % PAGE
+    q = _rand((9, 32, D), g, dev)
+    cu, prior = _i32([0, 9], dev), _i32([51], dev)
+    kw = dict(softcap=3.0)
+    if four:
+        pool = torch.empty((P, hkv, ref.RECORD), dtype=torch.uint8, device=dev)
+        rows = far[0][pos // PAGE].long() * PAGE + pos % PAGE
+        tm.kv_write_mx4(c.kp[near], c.vp[near], rows, pool)
+        c.kp[near], c.vp[near] = tm.kv_read_mx4(pool, rows)
+        got = tm.decode_mx4_paged(q[8:], pool, far, c.ctx, 0.1, **kw)
+        chunk = tm.prefill_mx4_varlen(q, pool, far, cu, prior, 0.1, **kw)
+    else:
+        kp, vp = (torch.empty((P, PAGE, hkv, D), dtype=BF, device=dev)
+                  for _ in range(2))
+        for i, page in enumerate(ids):
+            kp[page], vp[page] = c.kp[c.table[0, i]], c.vp[c.table[0, i]]
+        got = tm.decode_scored_paged(q[8:], kp, vp, far, c.ctx, 0.1, **kw)
+        chunk = tm.prefill_scored_varlen(
+            q, None, None, cu, 0.1, prior_lens=prior, k_pool=kp, v_pool=vp,
+            block_table=far, **kw)
+    ref.check(*got, ref.decode(q[8:], c.kp, c.vp, c.table, c.ctx, 0.1, **kw))
+    ref.check(*chunk, ref.prefill(q, None, None, cu, 0.1, prior=prior,
+                                  k_pool=c.kp, v_pool=c.vp, table=c.table,
+                                  **kw))
 
 
 @pytest.mark.parametrize("four", [0, 1])

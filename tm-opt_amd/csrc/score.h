@@ -31,10 +31,24 @@ struct Cap {
     return s * __builtin_fmaf(
                    __builtin_fmaf(__builtin_fmaf(c3, u, c2), u, c1), u, c0);
   }
+  // the same less m
+  __device__ __forceinline__ float less(float s, float m) const {
+    return (out - m) - 2.0f * out *
+                           __builtin_amdgcn_rcpf(1.0f + fast_exp2(s * in));
+  }
+  __device__ __forceinline__ float small_less(float s, float m) const {
+    const float u = s * s;
+    return __builtin_fmaf(
+        s,
+        __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(c3, u, c2), u, c1), u, c0),
+        -m);
+  }
   // Scores within the cap need no running maximum where 2^+-cap is far inside
-  // fp32 and bf16: sums are of 2^x, x between -90 and 90.
+  // fp32 and bf16: sums are of 2^(x - m), m the largest x of the first tile that
+  // the query sees, or kLeast where that is more: x - m is 90 at most.
+  static constexpr float kLeast = -13.0f;
   __host__ __device__ bool bounded() const {
-    return in != 0.0f && out <= 90.0f;
+    return in != 0.0f && out <= 90.0f + kLeast;
   }
 };
 
