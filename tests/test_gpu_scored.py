@@ -766,3 +766,167 @@ def test_scored_prefill_then_decode(tm, dev):
                        torch.tensor([i], device=dev),
                        torch.arange(i + 1, device=dev), 0.1, prefix=40, **kw)
         ref.check(out, lse.T, r)
+
+
+def test_captured_step_over_the_4_bit_cache(tm, dev):
+    """Plan, write and decode of a step in one graph, replayed while the requests
+    grow over page borders, with eager work between the replays."""
+    g = _gen(53)
+    B, hq, hkv, P = 3, 16, 2, 12
+    pool = tm.mx4_pool(P, hkv, dev)
+    pages = torch.full((B, 5), -1, dtype=torch.int32, device=dev)
+    free = torch.randperm(P, generator=g).to(torch.int32).to(dev)
+    slots = torch.arange(B, device=dev)
+    q, k, v = (torch.empty((B, h, D), dtype=BF, device=dev)
+               for h in (hq, hkv, hkv))
+    ctx, count, new = _i32([0, 0, 0], dev), _i32([P], dev), _i32([1] * B, dev)
+    plan = tm.plan_pages(pages, slots, ctx, new, free, count, B)
+    plan = plan._replace(seq_lens=ctx, free_count=count)
+    ws = tm.decode_mx4_workspace(B, hq, hkv, dev)
+    out = torch.empty_like(q)
+    lse = torch.empty((B, hq), device=dev)
+
+    def step():
+        tm.plan_pages(pages, slots, ctx, new, free, count, B, out=plan)
+        tm.kv_write_mx4(k, v, plan.slot_mapping, pool)
+        tm.decode_mx4_paged(q, pool, plan.block_table, plan.seq_lens, 0.1,
+                            softcap=9.0, out=out, lse=lse, workspace=ws)
+
+    for x in (q, k, v):
+        x.copy_(_rand(x.shape, g, dev))
+    step()
+    pages.fill_(-1)
+    count.fill_(P)
+    ctx.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    held = []
+    for i in range(40):
+        for x in (q, k, v):
+            x.copy_(_rand(x.shape, g, dev))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(plan.reject) == 0 and ctx.tolist() == [i + 1] * B
+        held.append((ref.held(k.cpu()), ref.held(v.cpu())))
+        if i % 8 and i not in (15, 17):
+            continue
+        for b in range(B):
+            K, V = (torch.stack([x[j][b] for x in held]).to(dev)
+                    for j in (0, 1))
+            r = ref.attend(q[b:b + 1], K, V, torch.tensor([i], device=dev),
+                           torch.arange(i + 1, device=dev), 0.1, softcap=9.0)
+            ref.check(out[b:b + 1], lse[b:b + 1].T, r, f"step {i}")
+
+
+# --------------------------------------------------------------------------
+# what else the documentation allows
+# --------------------------------------------------------------------------
+
+def test_calls_of_nothing(tm, dev):
+    g = _gen(54)
+    c, c4 = Cache([20], 2, g, dev), Cache4(tm, [20], 2, g, dev)
+    q = _rand((4, 8, D), g, dev)
+    none, cu0 = q[:0], _i32([0], dev)
+    t0, n0 = c.table[:0], c.ctx[:0]
+    for out, lse in (
+            tm.decode_scored_paged(none, c.kp, c.vp, t0, n0, 0.1),
+            tm.decode_mx4_paged(none, c4.pool, t0, n0, 0.1)):
+        assert out.shape == (0, 8, D) and lse.shape == (0, 8)
+    kept = torch.full_like(q, 3.0)
+    paged = dict(k_pool=c.kp, v_pool=c.vp, block_table=t0)
+    for run in (
+            lambda **kw: tm.prefill_scored_varlen(q, None, None, cu0, 0.1,
+                                                  **paged, **kw),
+            lambda **kw: tm.prefill_mx4_varlen(q, c4.pool, t0, cu0, None, 0.1,
+                                               **kw)):
+        run(out=kept)                    # no run: every row as it was
+        assert (kept == 3.0).all()
+    for cu in ([0, 0], [0, 0, 0]):       # runs without a query
+        tm.prefill_scored_varlen(q, q[:, :2], q[:, :2], _i32(cu, dev), 0.1,
+                                 out=kept)
+        assert (kept == 3.0).all()
+    out, lse = tm.prefill_scored_varlen(none, none[:, :2], none[:, :2],
+                                        _i32([0, 0], dev), 0.1, max_seqlen=64)
+    assert out.shape == (0, 8, D) and lse.shape == (8, 0)
+
+
+@pytest.mark.parametrize("extent", [1, 2, 5, 16, 63, 900])
+def test_bias_views(tm, dev, extent):
+    """A bias whose rows begin at any two bytes."""
+    g = _gen(55 + extent)
+    ends = [1, 5, 17, 64, 100, 700]
+    c = Cache4(tm, ends, 2, g, dev)
+    B, hq = len(ends), 8
+    q = _rand((B, hq, D), g, dev)
+    store = _rand((B * hq * extent + 3,), g, dev)
+    for off in (0, 1, 3):
+        rel = store[off:off + B * hq * extent].view(B, hq, extent)
+        out, lse = tm.decode_mx4_paged(q, c.pool, c.table, c.ctx, 0.1, rel=rel)
+        ref.check(out, lse, ref.decode(q, c.kp, c.vp, c.table, c.ctx, 0.1,
+                                       rel=rel), f"offset {off}")
+    lens = [1, 4, 16, 30, 77, 600]
+    q, _, _, cu = _packed(lens, hq, 1, g, dev)
+    wide = _rand((q.shape[0], hq, extent + 5), g, dev)
+    for off in (0, 1, 4):
+        _chunk(tm, c, q, cu, _i32([n - m for n, m in zip(ends, lens)], dev),
+               0.1, f"offset {off}", 1, rel=wide[..., off:off + extent])
+
+
+@pytest.mark.parametrize("four", [0, 1])
+def test_many_short_runs(tm, dev, four):
+    g = _gen(56)
+    n = 3000
+    lens = torch.randint(0, 4, (n,), generator=g).tolist()
+    prior = torch.randint(0, 20, (n,), generator=g).tolist()
+    ends = [a + b for a, b in zip(lens, prior)]
+    c = Cache4(tm, ends, 1, g, dev) if four else Cache(ends, 1, g, dev)
+    q, _, _, cu = _packed(lens, 4, 1, g, dev)
+    kw = dict(softcap=9.0)
+    if four:
+        got = tm.prefill_mx4_varlen(q, c.pool, c.table, cu, _i32(prior, dev),
+                                    0.1, **kw)
+    else:
+        got = tm.prefill_scored_varlen(
+            q, None, None, cu, 0.1, prior_lens=_i32(prior, dev), k_pool=c.kp,
+            v_pool=c.vp, block_table=c.table, **kw)
+    assert torch.isfinite(got[0]).all()
+    for i in list(range(0, n, 61)) + [n - 1]:
+        a, b = int(cu[i]), int(cu[i + 1])
+        if a == b:
+            continue
+        pos = torch.arange(ends[i], device=dev)
+        rows = c.table[i][pos // PAGE].long(), pos % PAGE
+        r = ref.attend(q[a:b], c.kp[rows], c.vp[rows],
+                       torch.arange(prior[i], ends[i], device=dev), pos, 0.1,
+                       **kw)
+        ref.check(got[0][a:b], got[1][:, a:b], r, f"run {i}")
+
+
+def test_prefills_at_once_on_two_streams(tm, dev):
+    """Calls that split their keys, each with scratch of its own."""
+    g = _gen(57)
+    c = Cache([5200], 2, g, dev)
+    c4 = Cache4(tm, [5200], 2, g, dev)
+    q, _, _, cu = _packed([200], 16, 1, g, dev)
+    p = _i32([5000], dev)
+
+    def calls():
+        return (tm.prefill_scored_varlen(
+                    q, None, None, cu, 0.1, softcap=30.0, prior_lens=p,
+                    k_pool=c.kp, v_pool=c.vp, block_table=c.table,
+                    max_seqlen=200),
+                tm.prefill_mx4_varlen(q, c4.pool, c4.table, cu, p, 0.1,
+                                      max_seqlen=200))
+    want = calls()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(calls())
+    torch.cuda.synchronize()
+    for a in got:
+        for x, y in zip(a, want):
+            assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])
