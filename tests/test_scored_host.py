@@ -205,6 +205,28 @@ def test_python_checks(tm):
                                          v_pool=kp),
         lambda: tm.prefill_scored_varlen(q, one, one[:1], cu, 0.1),
     ]
+    # numbers whose low 32 bits alone would be another call
+    for kw in (dict(window=(1 << 32) + 5), dict(window=1 << 31)):
+        calls += [
+            lambda kw=kw: tm.decode_mx4_paged(q, pool, table, ctx, 0.1, **kw),
+            lambda kw=kw: tm.decode_scored_paged(q, kp, kp, table, ctx, 0.1,
+                                                 **kw),
+            lambda kw=kw: tm.prefill_mx4_varlen(q, pool, table, cu, ctx, 0.1,
+                                                max_seqlen=1, **kw),
+            lambda kw=kw: tm.prefill_scored_varlen(q, one, one, cu, 0.1,
+                                                   max_seqlen=1, **kw)]
+    for kw in (dict(min_pages=(1 << 32) + 1),
+               dict(num_workgroups=(1 << 32) + 1),
+               dict(window=16, table_wrap=(1 << 32) + 1)):
+        calls += [
+            lambda kw=kw: tm.decode_mx4_paged(q, pool, table, ctx, 0.1, **kw),
+            lambda kw=kw: tm.decode_scored_paged(q, kp, kp, table, ctx, 0.1,
+                                                 **kw)]
+    calls += [
+        lambda: tm.prefill_mx4_varlen(q, pool, table, cu, ctx, 0.1,
+                                      max_seqlen=(1 << 32) + 1),
+        lambda: tm.prefill_scored_varlen(q, one, one, cu, 0.1,
+                                         max_seqlen=(1 << 32) + 1)]
     for i, call in enumerate(calls):
         with pytest.raises(AssertionError):
             call()

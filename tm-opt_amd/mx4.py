@@ -22,7 +22,7 @@ import torch
 
 from .attn import HEAD_DIM, PAGE_SIZE, _check_rows, _ptr, _refused_rows
 from .diff import _call, _table, _workspace_size
-from .scored import _index, _prefill_outputs, _runs, _slopes
+from .scored import _index, _int32, _prefill_outputs, _runs, _slopes
 
 _BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 _DECODE_SIZE = "tmopt_attn_decode_mx4_workspace_size"
@@ -94,7 +94,7 @@ def decode_mx4_workspace(B, HQ, HKV, device, num_workgroups=0):
     if device.type == "cuda" and device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
     n = _workspace_size(device, _DECODE_SIZE, B, HQ, HKV, HEAD_DIM,
-                        int(num_workgroups))
+                        _int32(num_workgroups))
     return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
 
 
@@ -116,7 +116,7 @@ def decode_mx4_paged(q, pool, block_table, ctx_lens, scale, softcap=0.0,
     initialisation; calls that overlap need one each).
     Returns (out [B, HQ, 128] bf16, lse [B, HQ] fp32 or None)."""
     B, HQ, D = q.shape
-    dev, num_workgroups = q.device, int(num_workgroups)
+    dev, num_workgroups = q.device, _int32(num_workgroups)
     assert q.dtype == _BF16 and q.is_contiguous()
     P, HKV = _pool(pool, dev)
     assert HQ % HKV == 0, (pool.shape, HQ)
@@ -148,10 +148,11 @@ def decode_mx4_paged(q, pool, block_table, ctx_lens, scale, softcap=0.0,
         assert workspace.device == dev and workspace.is_contiguous()
         n = workspace.numel() * workspace.element_size()
     _call(dev, "tmopt_attn_decode_mx4", q.data_ptr(), pool.data_ptr(),
-          block_table.data_ptr(), bts, int(table_wrap), ctx_lens.data_ptr(), B,
-          HQ, HKV, D, PAGE_SIZE, P, int(window), float(scale), float(softcap),
-          _slopes(slopes, HQ, dev), _ptr(rel), extent, int(min_pages),
-          num_workgroups, out.data_ptr(), _ptr(lse), workspace.data_ptr(), n)
+          block_table.data_ptr(), bts, _int32(table_wrap),
+          ctx_lens.data_ptr(), B, HQ, HKV, D, PAGE_SIZE, P, _int32(window),
+          float(scale), float(softcap), _slopes(slopes, HQ, dev), _ptr(rel),
+          extent, _int32(min_pages), num_workgroups, out.data_ptr(), _ptr(lse),
+          workspace.data_ptr(), n)
     return out, lse
 
 
@@ -188,12 +189,12 @@ def prefill_mx4_varlen(q, pool, block_table, cu_seqlens, prior_lens, scale,
     out, lse = _prefill_outputs(q, out, lse, return_lse, reject)
     most = 0 if max_context is None else max(1, int(max_context))
     n = _workspace_size(dev, _PREFILL_SIZE, S, max_seqlen, most, HQ, HKV, bts,
-                        int(window))
+                        _int32(window))
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     _call(dev, "tmopt_attn_prefill_mx4", q.data_ptr(), q.stride(0),
           q.stride(1), cu_seqlens.data_ptr(), _index(prior_lens, S, dev), S,
-          max_seqlen, most, pool.data_ptr(), block_table.data_ptr(), bts, PAGE_SIZE, P, HQ,
-          HKV, D, int(window), float(scale), float(softcap),
+          max_seqlen, most, pool.data_ptr(), block_table.data_ptr(), bts,
+          PAGE_SIZE, P, HQ, HKV, D, _int32(window), float(scale), float(softcap),
           _slopes(slopes, HQ, dev), _ptr(rel), r_st, r_sh, extent,
           out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse),
           _ptr(reject), _ptr(ws), n)

@@ -37,6 +37,13 @@ def _slopes(slopes, HQ, dev):
     return _ptr(slopes)
 
 
+def _int32(x):
+    """x as the C entry points take it: ctypes would drop what is above."""
+    x = int(x)
+    assert -1 << 31 <= x < 1 << 31, x
+    return x
+
+
 def _index(t, n, dev):
     """The pointer of an optional int32 tensor [n], checked."""
     if t is not None:
@@ -65,7 +72,7 @@ def _runs(cu_seqlens, total, max_seqlen, dev):
         max_seqlen = 0                   # no run, whatever the bound
     if max_seqlen is None:
         max_seqlen = int((cu_seqlens[1:] - cu_seqlens[:-1]).max()) if S else 0
-    return S, int(max_seqlen)
+    return S, _int32(max_seqlen)
 
 
 def _prefill_outputs(q, out, lse, return_lse, reject):
@@ -106,7 +113,7 @@ def decode_scored_paged(q, k_pool, v_pool, block_table, ctx_lens, scale,
     initialisation; calls that overlap need one each).
     Returns (out [B, HQ, 128] bf16, lse [B, HQ] fp32 or None)."""
     B, HQ, D = q.shape
-    dev, num_workgroups = q.device, int(num_workgroups)
+    dev, num_workgroups = q.device, _int32(num_workgroups)
     assert q.dtype == _BF16 and q.is_contiguous()
     P, page_size, HKV = _pools(k_pool, v_pool, HQ, D, dev)
     bts = _table(block_table, B, dev)
@@ -132,10 +139,10 @@ def decode_scored_paged(q, k_pool, v_pool, block_table, ctx_lens, scale,
         assert workspace.device == dev and workspace.is_contiguous()
         n = workspace.numel() * workspace.element_size()
     _call(dev, "tmopt_attn_decode_scored", q.data_ptr(), k_pool.data_ptr(),
-          v_pool.data_ptr(), block_table.data_ptr(), bts, int(table_wrap),
-          ctx_lens.data_ptr(), B, HQ, HKV, D, page_size, P, int(window),
+          v_pool.data_ptr(), block_table.data_ptr(), bts, _int32(table_wrap),
+          ctx_lens.data_ptr(), B, HQ, HKV, D, page_size, P, _int32(window),
           float(scale), float(softcap), _slopes(slopes, HQ, dev),
-          _index(first_keys, B, dev), int(min_pages), num_workgroups,
+          _index(first_keys, B, dev), _int32(min_pages), num_workgroups,
           out.data_ptr(), _ptr(lse), workspace.data_ptr(), n)
     return out, lse
 
@@ -186,13 +193,13 @@ def prefill_scored_varlen(q, k, v, cu_seqlens, scale, softcap=0.0, slopes=None,
     out, lse = _prefill_outputs(q, out, lse, return_lse, reject)
     most = 0 if max_context is None else max(1, int(max_context))
     n = _workspace_size(dev, _PREFILL_SIZE, S, max_seqlen, most, HQ, HKV, bts,
-                        int(window))
+                        _int32(window))
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     _call(dev, "tmopt_attn_prefill_scored", q.data_ptr(), q.stride(0),
           q.stride(1), _ptr(k), strides[0], strides[1], _ptr(v), strides[2],
           strides[3], cu_seqlens.data_ptr(), _index(prior_lens, S, dev), S,
           max_seqlen, most, _ptr(k_pool), _ptr(v_pool), _ptr(block_table), bts,
-          page_size, P, HQ, HKV, D, int(window), float(scale), float(softcap),
+          page_size, P, HQ, HKV, D, _int32(window), float(scale), float(softcap),
           _slopes(slopes, HQ, dev), _index(first_keys, total, dev),
           _index(prefix_lens, S, dev), out.data_ptr(), out.stride(0),
           out.stride(1), _ptr(lse), _ptr(reject), _ptr(ws), n)
