@@ -617,8 +617,8 @@ int tmopt_attn_decode_scored(const void* q, const void* k_pool,
 
 /*
  * Packed runs of queries. q [total, HQ, D] with element strides, D contiguous;
- * cu_seqlens_q, prior_lens, max_seqlen_q, window, scale, out, lse ([HQ, total])
- * and reject as in tmopt_attn_prefill_varlen; first_keys [total], prefix_lens
+ * cu_seqlens_q, prior_lens, max_seqlen_q, window, scale, out, lse ([HQ,
+ * cu_seqlens_q[num_seqs]]) and reject as in tmopt_attn_prefill_varlen; first_keys [total], prefix_lens
  * [num_seqs]. Keys:
  *   block_table == NULL: k, v [total, HKV, D], the runs' own rows packed by
  *         cu_seqlens_q (strides % 8, D contiguous); prior_lens NULL;
@@ -652,6 +652,25 @@ int tmopt_attn_prefill_scored(
     const int32_t* prefix_lens, void* out, int64_t o_stride_tok,
     int64_t o_stride_head, float* lse, const int32_t* reject, void* workspace,
     size_t workspace_bytes, tmopt_stream_t stream);
+
+/*
+ * The same with LSE rows of lse_stride_head elements (0: cu_seqlens_q[num_seqs],
+ * as above): for outputs of more rows than the runs have tokens, whose LSE
+ * columns behind the last run stay as they were.
+ */
+int tmopt_attn_prefill_scored_strided(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k,
+    int64_t k_stride_tok, int64_t k_stride_head, const void* v,
+    int64_t v_stride_tok, int64_t v_stride_head, const int32_t* cu_seqlens_q,
+    const int32_t* prior_lens, int num_seqs, int max_seqlen_q,
+    int64_t max_context, const void* k_pool, const void* v_pool,
+    const int32_t* block_table, int64_t bt_stride, int page_size,
+    int64_t num_pages, int HQ, int HKV, int D, int window, float scale,
+    float softcap, const float* slopes, const int32_t* first_keys,
+    const int32_t* prefix_lens, void* out, int64_t o_stride_tok,
+    int64_t o_stride_head, float* lse, int64_t lse_stride_head,
+    const int32_t* reject, void* workspace, size_t workspace_bytes,
+    tmopt_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
 /* A cache held in 4 bits                                                   */
@@ -749,6 +768,19 @@ int tmopt_attn_prefill_mx4(
     int64_t o_stride_tok, int64_t o_stride_head, float* lse,
     const int32_t* reject, void* workspace, size_t workspace_bytes,
     tmopt_stream_t stream);
+
+/* The same with LSE rows of lse_stride_head elements, as for the scored one. */
+int tmopt_attn_prefill_mx4_strided(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+    const int32_t* cu_seqlens_q, const int32_t* prior_lens, int num_seqs,
+    int max_seqlen_q, int64_t max_context, const void* pool,
+    const int32_t* block_table, int64_t bt_stride, int page_size,
+    int64_t num_pages, int HQ, int HKV, int D, int window, float scale,
+    float softcap, const float* slopes, const void* rel,
+    int64_t rel_stride_tok, int64_t rel_stride_head, int rel_extent, void* out,
+    int64_t o_stride_tok, int64_t o_stride_head, float* lse,
+    int64_t lse_stride_head, const int32_t* reject, void* workspace,
+    size_t workspace_bytes, tmopt_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
 /* Page plan of a serving step                                              */

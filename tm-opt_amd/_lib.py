@@ -136,6 +136,12 @@ SIGNATURES = {
         _c_ptr, _c_ptr, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32,
         _c_i32, _c_f32, _c_f32, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i32,
         _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_size, _c_ptr]),
+    "tmopt_attn_prefill_mx4_strided": (_c_i32, [
+        _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i32, _c_i32, _c_i64,
+        _c_ptr, _c_ptr, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32,
+        _c_i32, _c_f32, _c_f32, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i32,
+        _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_size,
+        _c_ptr]),
     "tmopt_attn_decode_scored": (_c_i32, [
         _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i32, _c_ptr, _c_i32,
         _c_i32, _c_i32, _c_i32, _c_i32, _c_i64, _c_i32, _c_f32, _c_f32,
@@ -149,6 +155,12 @@ SIGNATURES = {
         _c_ptr, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,
         _c_f32, _c_f32, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64,
         _c_ptr, _c_ptr, _c_ptr, _c_size, _c_ptr]),
+    "tmopt_attn_prefill_scored_strided": (_c_i32, [
+        _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64,
+        _c_i64, _c_ptr, _c_ptr, _c_i32, _c_i32, _c_i64, _c_ptr, _c_ptr,
+        _c_ptr, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,
+        _c_f32, _c_f32, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64,
+        _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_size, _c_ptr]),
     "tmopt_plan_pages": (_c_i32, [
         _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i32, _c_ptr,
         _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr,

@@ -306,6 +306,7 @@ static int prefill_impl(
   a.o_st = o_stride_tok;
   a.o_sh = o_stride_head;
   a.lse = lse;
+  a.lse_sh = 0;
   a.S = num_seqs;
   a.rel = (const __bf16*)rel;
   a.r_st = rel_stride_tok;

@@ -83,7 +83,8 @@ struct PrefillArgs {
   float scale_log2;
   __bf16* out;
   int64_t o_st, o_sh;
-  float* lse;        // [HQ, cu[S]]
+  float* lse;        // [HQ] rows, the runs' tokens in the first cu[S] columns
+  int64_t lse_sh;    // elements from row to row; 0: cu[S]
   int S;
   int nqb_max;       // query blocks of the longest run
   const __bf16* rel; // optional fused relative bias, rows like q
@@ -142,6 +143,11 @@ constexpr int kRing = 4;                  // MFMA-phase fragment ring
 // a buffer offset past every resource this kernel builds (their ranges are
 // checked below 2^31 - 16 on the host): the load returns zeros
 constexpr int kOob = 0x7ffffff0;
+
+__device__ __forceinline__ int64_t lse_stride(const PrefillArgs& a,
+                                              const Work& wk) {
+  return a.lse_sh != 0 ? a.lse_sh : wk.total;
+}
 
 // First key a work item reads (a multiple of the tile width at or below the
 // first key a query of the block may see) and its tiles from there.
@@ -1388,7 +1394,7 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
   }
 #endif
   if (a.lse && h2 == 0 && qok)
-    a.lse[(int64_t)head * wk.total + t0 + qi] =
+    a.lse[head * lse_stride(a, wk) + t0 + qi] =
         rejected ? __builtin_nanf("") :
         some() ? (m_run + fast_log2(l_tot)) * kLn2 : -INFINITY;
   // O^T goes through LDS (free after the last barrier) so that the global

@@ -43,7 +43,7 @@ __device__ __forceinline__ int items_before(const A& a, int z, int BQ,
 struct Work {
   int kvh, seq, qb;    // seq < 0: nothing to do
   int t0, len, prior;  // the run's first row, length and prior context
-  int total;           // cu[S]: rows of the launch (the LSE row length)
+  int total;           // cu[S]: rows of the launch
 };
 
 // Work item of this work-group (computed by every wave, identically).

@@ -67,8 +67,8 @@ int run(const char* what, PrefillArgs& a, int src, const void* q,
         int page_size, int64_t num_pages, int HQ, int HKV, int D, int window,
         float scale, float softcap, const float* slopes, void* out,
         int64_t o_stride_tok, int64_t o_stride_head, float* lse,
-        const int32_t* reject, void* workspace, size_t workspace_bytes,
-        hipStream_t st) {
+        int64_t lse_stride_head, const int32_t* reject, void* workspace,
+        size_t workspace_bytes, hipStream_t st) {
   TMOPT_REQUIRE(num_seqs > 0 && num_seqs <= 65535 && max_seqlen_q > 0 &&
                     max_context >= 0,
                 TMOPT_EINVAL, "%s: num_seqs=%d max_seqlen_q=%d max_context=%lld",
@@ -131,6 +131,7 @@ int run(const char* what, PrefillArgs& a, int src, const void* q,
   a.o_st = o_stride_tok;
   a.o_sh = o_stride_head;
   a.lse = lse;
+  a.lse_sh = lse_stride_head;
   a.S = num_seqs;
   a.reject = reject;
   a.n_base = (int)level_wgs(a.HKV, bq, num_seqs, max_seqlen_q);
@@ -189,7 +190,7 @@ extern "C" size_t tmopt_attn_prefill_scored_workspace_size(
                       window);
 }
 
-extern "C" int tmopt_attn_prefill_scored(
+extern "C" int tmopt_attn_prefill_scored_strided(
     const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k,
     int64_t k_stride_tok, int64_t k_stride_head, const void* v,
     int64_t v_stride_tok, int64_t v_stride_head, const int32_t* cu_seqlens_q,
@@ -199,8 +200,9 @@ extern "C" int tmopt_attn_prefill_scored(
     int64_t num_pages, int HQ, int HKV, int D, int window, float scale,
     float softcap, const float* slopes, const int32_t* first_keys,
     const int32_t* prefix_lens, void* out, int64_t o_stride_tok,
-    int64_t o_stride_head, float* lse, const int32_t* reject, void* workspace,
-    size_t workspace_bytes, tmopt_stream_t stream) {
+    int64_t o_stride_head, float* lse, int64_t lse_stride_head,
+    const int32_t* reject, void* workspace, size_t workspace_bytes,
+    tmopt_stream_t stream) {
   clear_error();
   if (num_seqs == 0 || max_seqlen_q == 0) return TMOPT_OK;
   PrefillArgs a{};
@@ -241,8 +243,29 @@ extern "C" int tmopt_attn_prefill_scored(
              q_stride_head, cu_seqlens_q, prior_lens, num_seqs, max_seqlen_q,
              max_context, block_table, bt_stride, page_size, num_pages, HQ,
              HKV, D, window, scale, softcap, slopes, out, o_stride_tok,
-             o_stride_head, lse, reject, workspace, workspace_bytes,
-             (hipStream_t)stream);
+             o_stride_head, lse, lse_stride_head, reject, workspace,
+             workspace_bytes, (hipStream_t)stream);
+}
+
+extern "C" int tmopt_attn_prefill_scored(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k,
+    int64_t k_stride_tok, int64_t k_stride_head, const void* v,
+    int64_t v_stride_tok, int64_t v_stride_head, const int32_t* cu_seqlens_q,
+    const int32_t* prior_lens, int num_seqs, int max_seqlen_q,
+    int64_t max_context, const void* k_pool, const void* v_pool,
+    const int32_t* block_table, int64_t bt_stride, int page_size,
+    int64_t num_pages, int HQ, int HKV, int D, int window, float scale,
+    float softcap, const float* slopes, const int32_t* first_keys,
+    const int32_t* prefix_lens, void* out, int64_t o_stride_tok,
+    int64_t o_stride_head, float* lse, const int32_t* reject, void* workspace,
+    size_t workspace_bytes, tmopt_stream_t stream) {
+  return tmopt_attn_prefill_scored_strided(
+      q, q_stride_tok, q_stride_head, k, k_stride_tok, k_stride_head, v,
+      v_stride_tok, v_stride_head, cu_seqlens_q, prior_lens, num_seqs,
+      max_seqlen_q, max_context, k_pool, v_pool, block_table, bt_stride,
+      page_size, num_pages, HQ, HKV, D, window, scale, softcap, slopes,
+      first_keys, prefix_lens, out, o_stride_tok, o_stride_head, lse, 0, reject,
+      workspace, workspace_bytes, stream);
 }
 
 extern "C" size_t tmopt_attn_prefill_mx4_workspace_size(
@@ -253,7 +276,7 @@ extern "C" size_t tmopt_attn_prefill_mx4_workspace_size(
                                        HKV, bt_stride, window);
 }
 
-extern "C" int tmopt_attn_prefill_mx4(
+extern "C" int tmopt_attn_prefill_mx4_strided(
     const void* q, int64_t q_stride_tok, int64_t q_stride_head,
     const int32_t* cu_seqlens_q, const int32_t* prior_lens, int num_seqs,
     int max_seqlen_q, int64_t max_context, const void* pool,
@@ -262,8 +285,8 @@ extern "C" int tmopt_attn_prefill_mx4(
     float softcap, const float* slopes, const void* rel,
     int64_t rel_stride_tok, int64_t rel_stride_head, int rel_extent, void* out,
     int64_t o_stride_tok, int64_t o_stride_head, float* lse,
-    const int32_t* reject, void* workspace, size_t workspace_bytes,
-    tmopt_stream_t stream) {
+    int64_t lse_stride_head, const int32_t* reject, void* workspace,
+    size_t workspace_bytes, tmopt_stream_t stream) {
   clear_error();
   if (num_seqs == 0 || max_seqlen_q == 0) return TMOPT_OK;
   TMOPT_REQUIRE(pool && (uintptr_t)pool % 16 == 0, TMOPT_EINVAL,
@@ -290,5 +313,25 @@ extern "C" int tmopt_attn_prefill_mx4(
              cu_seqlens_q, prior_lens, num_seqs, max_seqlen_q, max_context,
              block_table, bt_stride, page_size, num_pages, HQ, HKV, D, window,
              scale, softcap, slopes, out, o_stride_tok, o_stride_head, lse,
-             reject, workspace, workspace_bytes, (hipStream_t)stream);
+             lse_stride_head, reject, workspace, workspace_bytes,
+             (hipStream_t)stream);
+}
+
+extern "C" int tmopt_attn_prefill_mx4(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+    const int32_t* cu_seqlens_q, const int32_t* prior_lens, int num_seqs,
+    int max_seqlen_q, int64_t max_context, const void* pool,
+    const int32_t* block_table, int64_t bt_stride, int page_size,
+    int64_t num_pages, int HQ, int HKV, int D, int window, float scale,
+    float softcap, const float* slopes, const void* rel,
+    int64_t rel_stride_tok, int64_t rel_stride_head, int rel_extent, void* out,
+    int64_t o_stride_tok, int64_t o_stride_head, float* lse,
+    const int32_t* reject, void* workspace, size_t workspace_bytes,
+    tmopt_stream_t stream) {
+  return tmopt_attn_prefill_mx4_strided(
+      q, q_stride_tok, q_stride_head, cu_seqlens_q, prior_lens, num_seqs,
+      max_seqlen_q, max_context, pool, block_table, bt_stride, page_size,
+      num_pages, HQ, HKV, D, window, scale, softcap, slopes, rel,
+      rel_stride_tok, rel_stride_head, rel_extent, out, o_stride_tok,
+      o_stride_head, lse, 0, reject, workspace, workspace_bytes, stream);
 }

@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillArgs a) {
   const float inv = some() ? 1.0f / sum : 0.0f;
   const int qi = qrow0 + l32;
   if (a.lse && db == 0 && lane < 32 && qi < wk.len)
-    a.lse[(int64_t)head * wk.total + wk.t0 + qi] =
+    a.lse[head * lse_stride(a, wk) + wk.t0 + qi] =
         rejected ? __builtin_nanf("")
         : some() ? m + fast_log2(sum) * kLn2 : -INFINITY;
   const uint32_t ob =

@@ -173,7 +173,8 @@ def prefill_mx4_varlen(q, pool, block_table, cu_seqlens, prior_lens, scale,
     device, with a synchronisation, if None); max_context: an upper bound of
     prior + run length, where the host has one (the row width of the block table
     bounds it otherwise): whether keys are split over work-groups goes by it.
-    Returns (out [total, HQ, 128] bf16, lse [HQ, total] fp32 or None)."""
+    Returns (out [total, HQ, 128] bf16, lse [HQ, total] fp32 or None); rows behind
+    the last run keep what they held."""
     total, HQ, D = q.shape
     dev = q.device
     _check_rows(q, "q")
@@ -191,12 +192,12 @@ def prefill_mx4_varlen(q, pool, block_table, cu_seqlens, prior_lens, scale,
     n = _workspace_size(dev, _PREFILL_SIZE, S, max_seqlen, most, HQ, HKV, bts,
                         _int32(window))
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    _call(dev, "tmopt_attn_prefill_mx4", q.data_ptr(), q.stride(0),
+    _call(dev, "tmopt_attn_prefill_mx4_strided", q.data_ptr(), q.stride(0),
           q.stride(1), cu_seqlens.data_ptr(), _index(prior_lens, S, dev), S,
           max_seqlen, most, pool.data_ptr(), block_table.data_ptr(), bts,
           PAGE_SIZE, P, HQ, HKV, D, _int32(window), float(scale), float(softcap),
           _slopes(slopes, HQ, dev), _ptr(rel), r_st, r_sh, extent,
-          out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse),
+          out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse), total,
           _ptr(reject), _ptr(ws), n)
     if reject is not None:
         _call(dev, "tmopt_refused_rows",

@@ -170,7 +170,8 @@ def prefill_scored_varlen(q, k, v, cu_seqlens, scale, softcap=0.0, slopes=None,
     synchronisation, if None); max_context: an upper bound of prior + run
     length, where the host has one (the row width of the block table bounds it
     otherwise): whether keys are split over work-groups goes by it.
-    Returns (out [total, HQ, 128] bf16, lse [HQ, total] fp32 or None)."""
+    Returns (out [total, HQ, 128] bf16, lse [HQ, total] fp32 or None); rows behind
+    the last run keep what they held."""
     total, HQ, D = q.shape
     dev = q.device
     _check_rows(q, "q")
@@ -195,14 +196,14 @@ def prefill_scored_varlen(q, k, v, cu_seqlens, scale, softcap=0.0, slopes=None,
     n = _workspace_size(dev, _PREFILL_SIZE, S, max_seqlen, most, HQ, HKV, bts,
                         _int32(window))
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    _call(dev, "tmopt_attn_prefill_scored", q.data_ptr(), q.stride(0),
+    _call(dev, "tmopt_attn_prefill_scored_strided", q.data_ptr(), q.stride(0),
           q.stride(1), _ptr(k), strides[0], strides[1], _ptr(v), strides[2],
           strides[3], cu_seqlens.data_ptr(), _index(prior_lens, S, dev), S,
           max_seqlen, most, _ptr(k_pool), _ptr(v_pool), _ptr(block_table), bts,
           page_size, P, HQ, HKV, D, _int32(window), float(scale), float(softcap),
           _slopes(slopes, HQ, dev), _index(first_keys, total, dev),
           _index(prefix_lens, S, dev), out.data_ptr(), out.stride(0),
-          out.stride(1), _ptr(lse), _ptr(reject), _ptr(ws), n)
+          out.stride(1), _ptr(lse), total, _ptr(reject), _ptr(ws), n)
     if reject is not None:
         _call(dev, "tmopt_refused_rows",
               *_refused_rows(reject, out, lse, *out.shape, HQ))
