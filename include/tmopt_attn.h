@@ -407,8 +407,8 @@ int tmopt_attn_decode_paged_noalloc(const void* q, const void* k_pool,
  * max_seqlen_q bounds every len_i (it sizes the grid).
  * out:    [total_q, HQ, D] with element strides (o_stride_tok,
  *         o_stride_head), D contiguous.
- * lse:    [HQ, total_q] fp32 natural-log sum-exp of the scaled scores, or
- *         NULL.
+ * lse:    [HQ, cu_seqlens_q[num_seqs]] fp32 natural-log sum-exp of the scaled
+ *         scores, or NULL.
  * reject: optional device int32 (NULL = none). When it holds a nonzero
  *         value at launch, every output row and LSE entry the launch owns
  *         is written as NaN and no key is read: a caller that validated its
@@ -452,6 +452,26 @@ int tmopt_attn_prefill_varlen_split(
     void* out, int64_t o_stride_tok, int64_t o_stride_head, float* lse,
     const int32_t* reject, void* workspace, size_t workspace_bytes,
     tmopt_stream_t stream);
+
+/*
+ * The same with LSE rows of lse_stride_head elements (0: cu_seqlens_q[num_seqs],
+ * as above): for outputs of more rows than the runs have tokens, whose LSE
+ * columns behind the last run stay as they were.
+ */
+int tmopt_attn_prefill_varlen_strided_split(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k,
+    int64_t k_stride_run, int64_t k_stride_tok, int64_t k_stride_head,
+    int64_t k_stride_dim, const void* v, int64_t v_stride_run,
+    int64_t v_stride_tok, int64_t v_stride_head, int64_t v_stride_dim,
+    const int32_t* cu_seqlens_q,
+    const int32_t* prior_lens, int num_seqs, int max_seqlen_q,
+    const void* k_pool, const void* v_pool, const int32_t* block_table,
+    int64_t bt_stride, int table_wrap, int page_size, int64_t num_pages,
+    int HQ, int HKV, int D, int window, float scale, const void* rel,
+    int64_t rel_stride_tok, int64_t rel_stride_head, int rel_extent,
+    void* out, int64_t o_stride_tok, int64_t o_stride_head, float* lse,
+    int64_t lse_stride_head, const int32_t* reject, void* workspace,
+    size_t workspace_bytes, tmopt_stream_t stream);
 
 /*
  * Bytes of workspace tmopt_attn_prefill_varlen_split needs for a launch shape

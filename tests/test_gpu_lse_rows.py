@@ -82,3 +82,55 @@ def test_scored_and_mx4(tm, dev, source, split, name):
     out, lse = _rows_behind(call, n, total, hq, dev)
     ref.check(out[:n], lse[:, :n], ref.prefill(x[:n], cu=cu, scale=0.1, **args,
                                                **kw), name)
+
+
+@pytest.mark.parametrize("source", ["packed", "padded", "paged", "mixed"])
+@pytest.mark.parametrize("split", [0, 1])
+@pytest.mark.parametrize("E", [0, 200])
+def test_prefill_varlen(tm, dev, source, split, E):
+    g = torch.Generator().manual_seed(61 + split)
+    r = lambda *s: torch.randn(s, generator=g).to(torch.bfloat16)  # noqa: E731
+    own_only = source in ("packed", "padded")
+    if split:
+        lens, prior, hq, hkv = (([3300], [0], 4, 1) if own_only else
+                                ([64], [3000], 16, 2))
+    else:
+        lens, prior, hq, hkv = [50, 0, 70], [0, 3, 30], 8, 2
+    n, S = sum(lens), len(lens)
+    total = n + 57
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32)
+    q, rel = r(total, hq, D), r(total, hq, E) if E else None
+    a = dict(cu_seqlens=cu, scale=D ** -0.5, k=None, v=None)
+    if source == "padded":
+        a.update(k=r(S, max(lens), hkv, D), v=r(S, max(lens), hkv, D))
+    elif source != "paged":
+        a.update(k=r(total, hkv, D), v=r(total, hkv, D))
+    if not own_only:
+        wl = import_module("tm-opt_amd.workloads")
+        table, P = wl.paged_layout(lens, g, prior=prior)
+        a.update(prior_lens=torch.tensor(prior, dtype=torch.int32),
+                 k_pool=r(P, 16, hkv, D), v_pool=r(P, 16, hkv, D),
+                 block_table=table)
+    size = tm._lib.load().tmopt_attn_prefill_workspace_size
+    assert (size(S, max(lens), hq, hkv, 0 if own_only else table.shape[1], 0,
+                 0) > 0) == split
+
+    def rows(x, m):
+        return x[:m] if source in ("packed", "mixed") else x
+
+    def call(m, **more):
+        d = {k: x.to(dev) if torch.is_tensor(x) else x for k, x in a.items()}
+        if d["k"] is not None:
+            d.update(k=rows(d["k"], m), v=rows(d["v"], m))
+        return tm.prefill_varlen(q[:m].to(dev), **d, **more,
+                                 rel=rel[:m].to(dev) if E else None)
+    out, lse = _rows_behind(call, n, total, hq, dev)
+    if source == "padded":
+        a.update({x: torch.cat([a[x][i, :m] for i, m in enumerate(lens)])
+                  for x in ("k", "v")})
+    elif source != "paged":
+        a.update(k=a["k"][:n], v=a["v"][:n])
+    ref_o, ref_l = attn_ref.prefill_varlen(q[:n], rel=rel[:n] if E else None,
+                                           **a)
+    assert_out_close(out[:n], ref_o, source)
+    assert_lse_close(lse[:, :n], ref_l, source)

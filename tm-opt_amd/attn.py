@@ -482,7 +482,8 @@ def prefill_varlen(q, k, v, cu_seqlens, scale, window=0, max_seqlen=None,
     the launch that merges nothing (graph replays, 64Q/8KV, 4,096 pages: 64
     tokens without context 10.0 us against 7.5, 500 23.4 against 20.8). It
     decides about the split alone.
-    Returns (out [total, HQ, D] bf16, lse [HQ, total] fp32 or None).
+    Returns (out [total, HQ, D] bf16, lse [HQ, total] fp32 or None); rows behind
+    the last run keep what they held.
     Reference: engine/pyengine/kernels/attn_prefill.py:71-194."""
     out, lse = _prefill_varlen(q, k, v, cu_seqlens, scale, window, max_seqlen,
                                prior_lens, k_pool, v_pool, block_table,
@@ -573,7 +574,10 @@ def _prefill_varlen(q, k, v, cu_seqlens, scale, window, max_seqlen,
     dev = q.device
     if out is None:
         out = torch.empty((total, HQ, D), dtype=torch.bfloat16, device=dev)
-    if lse is None and return_lse:
+    if lse is not None:      # (the kernel writes rows of `total` values)
+        assert lse.dtype == torch.float32 and lse.is_contiguous()
+        assert lse.numel() >= HQ * total, (lse.shape, HQ, total)
+    elif return_lse:
         lse = torch.empty((HQ, total), dtype=torch.float32, device=dev)
     # scratch for the pieces of a launch too small for the device (0 bytes
     # for any other): the kernel splits its keys
@@ -586,8 +590,8 @@ def _prefill_varlen(q, k, v, cu_seqlens, scale, window, max_seqlen,
         ws = workspace if workspace is not None else torch.empty(
             n, dtype=torch.uint8, device=dev)
         n = ws.numel()
-    _lib.call("tmopt_attn_prefill_varlen_split", _ptr(q), q.stride(0),
-              q.stride(1),
+    _lib.call("tmopt_attn_prefill_varlen_strided_split", _ptr(q),
+              q.stride(0), q.stride(1),
               _ptr(k) if own else None, *ks,
               _ptr(v) if own else None, *vs, _ptr(cu_seqlens),
               _ptr(prior_lens), S, int(max_seqlen),
@@ -598,6 +602,6 @@ def _prefill_varlen(q, k, v, cu_seqlens, scale, window, max_seqlen,
               0 if rel is None else rel.stride(0),
               0 if rel is None else rel.stride(1),
               0 if rel is None else rel.shape[2], _ptr(out), out.stride(0),
-              out.stride(1), _ptr(lse), _ptr(reject), _ptr(ws), n,
+              out.stride(1), _ptr(lse), total, _ptr(reject), _ptr(ws), n,
               _stream(dev))
     return out, lse

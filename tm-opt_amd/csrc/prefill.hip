@@ -147,8 +147,8 @@ static int prefill_impl(
     int HQ, int HKV, int D, int window, float scale, const void* rel,
     int64_t rel_stride_tok, int64_t rel_stride_head, int rel_extent,
     void* out, int64_t o_stride_tok, int64_t o_stride_head, float* lse,
-    const int32_t* reject, void* workspace, size_t workspace_bytes,
-    tmopt_stream_t stream) {
+    int64_t lse_stride_head, const int32_t* reject, void* workspace,
+    size_t workspace_bytes, tmopt_stream_t stream) {
   clear_error();
   if (num_seqs == 0 || max_seqlen_q == 0) return TMOPT_OK;
   TMOPT_REQUIRE(num_seqs > 0 && num_seqs <= 65535 && max_seqlen_q > 0,
@@ -306,7 +306,7 @@ static int prefill_impl(
   a.o_st = o_stride_tok;
   a.o_sh = o_stride_head;
   a.lse = lse;
-  a.lse_sh = 0;
+  a.lse_sh = lse_stride_head;
   a.S = num_seqs;
   a.rel = (const __bf16*)rel;
   a.r_st = rel_stride_tok;
@@ -364,7 +364,7 @@ extern "C" int tmopt_attn_prefill_varlen(
       v_stride_head, v_stride_dim, cu_seqlens_q, prior_lens, num_seqs,
       max_seqlen_q, k_pool, v_pool, block_table, bt_stride, table_wrap,
       page_size, num_pages, HQ, HKV, D, window, scale, rel, rel_stride_tok,
-      rel_stride_head, rel_extent, out, o_stride_tok, o_stride_head, lse,
+      rel_stride_head, rel_extent, out, o_stride_tok, o_stride_head, lse, 0,
       reject, nullptr, 0, stream);
 }
 
@@ -388,6 +388,30 @@ extern "C" int tmopt_attn_prefill_varlen_split(
       v_stride_head, v_stride_dim, cu_seqlens_q, prior_lens, num_seqs,
       max_seqlen_q, k_pool, v_pool, block_table, bt_stride, table_wrap,
       page_size, num_pages, HQ, HKV, D, window, scale, rel, rel_stride_tok,
-      rel_stride_head, rel_extent, out, o_stride_tok, o_stride_head, lse,
+      rel_stride_head, rel_extent, out, o_stride_tok, o_stride_head, lse, 0,
       reject, workspace, workspace_bytes, stream);
+}
+
+extern "C" int tmopt_attn_prefill_varlen_strided_split(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k,
+    int64_t k_stride_run, int64_t k_stride_tok, int64_t k_stride_head,
+    int64_t k_stride_dim, const void* v, int64_t v_stride_run,
+    int64_t v_stride_tok, int64_t v_stride_head, int64_t v_stride_dim,
+    const int32_t* cu_seqlens_q,
+    const int32_t* prior_lens, int num_seqs, int max_seqlen_q,
+    const void* k_pool, const void* v_pool, const int32_t* block_table,
+    int64_t bt_stride, int table_wrap, int page_size, int64_t num_pages,
+    int HQ, int HKV, int D, int window, float scale, const void* rel,
+    int64_t rel_stride_tok, int64_t rel_stride_head, int rel_extent,
+    void* out, int64_t o_stride_tok, int64_t o_stride_head, float* lse,
+    int64_t lse_stride_head, const int32_t* reject, void* workspace,
+    size_t workspace_bytes, tmopt_stream_t stream) {
+  return prefill_impl(
+      q, q_stride_tok, q_stride_head, k, k_stride_run, k_stride_tok,
+      k_stride_head, k_stride_dim, v, v_stride_run, v_stride_tok,
+      v_stride_head, v_stride_dim, cu_seqlens_q, prior_lens, num_seqs,
+      max_seqlen_q, k_pool, v_pool, block_table, bt_stride, table_wrap,
+      page_size, num_pages, HQ, HKV, D, window, scale, rel, rel_stride_tok,
+      rel_stride_head, rel_extent, out, o_stride_tok, o_stride_head, lse,
+      lse_stride_head, reject, workspace, workspace_bytes, stream);
 }
