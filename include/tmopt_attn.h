@@ -611,7 +611,8 @@ int tmopt_attn_prefill_diff(
  * first_keys: int32, one per query token, or NULL: where the query's document
  * begins in a request of several (any value; negative ones are 0).
  * prefix_lens: int32, one per run, or NULL: of each run the first tokens, which
- * all of it sees (a prefix past the run's end stops there).
+ * all of it sees (any value; a prefix past the run's end stops there, a negative
+ * one is 0).
  * A query that sees no key gives zeros and LSE -infinity. A visible key whose
  * score is NaN (or +infinity, without a cap) gives NaN as output and LSE.
  * Sums and maxima are fp32; probabilities are rounded to bf16 for their product

@@ -173,7 +173,7 @@ __device__ __forceinline__ Masks item_masks(const PrefillArgs& a, int BQ,
   const int qn = min(BQ, wk.len - q0);
   Masks m{0, 0, wk.prior + q0 + qn, 0};
   if (a.prefix != nullptr) {
-    m.prefix = min(as_const(a.prefix)[wk.seq], wk.prior + wk.len);
+    m.prefix = max(0, min(as_const(a.prefix)[wk.seq], wk.prior + wk.len));
     m.k_hi = max(m.k_hi, m.prefix);
   }
   if (a.first != nullptr) {
@@ -397,7 +397,7 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
   [[maybe_unused]] int q_first = 0, q_last = qpos;
   [[maybe_unused]] float slope = 0.0f;
   if constexpr (kScored) {
-    if (a.first != nullptr && qok) q_first = a.first[t0 + qi];
+    if (a.first != nullptr && qok) q_first = max(0, a.first[t0 + qi]);
     q_last = max(qpos, mk.prefix - 1);
     if (a.slopes != nullptr) slope = as_const(a.slopes)[head] * kLog2e;
   }
@@ -903,7 +903,11 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
     const int base = kt + 4 * h2;
     const int hi = qok ? min(kScored ? q_last : qpos, nk - 1) - base : -1;
     int lo = a.window > 0 ? qpos - a.window - base : -1;
-    if constexpr (kScored) lo = max(lo, q_first - 1 - base);
+    if constexpr (kScored) {
+      // (keys of a prefix may lie ahead of the query, base past qpos, and the
+      // window be as wide as int32: the bound before the base comes off)
+      lo = max(a.window > 0 ? qpos - a.window : -1, q_first - 1) - base;
+    }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
