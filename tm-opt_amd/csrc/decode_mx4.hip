@@ -334,6 +334,21 @@ void decode_mx4_kernel(Mx4Args args) {
     }
     if constexpr (SCORE) {
       if (args.cap.in != 0.0f) {
+        if (!(st.flags & kFull)) {
+          // (the bytes of a key that is not there are nobody's: they do not
+          // choose the form of the cap)
+          const int lo = vis_lo(st.n, a.window) - st.pg * kPS;
+          const int hi = st.n - st.pg * kPS;
+#pragma unroll
+          for (int j = 0; j < kPages; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int at = 16 * j + 4 * g + i;
+              const bool ok =
+                  (st.flags & (kHave << j)) && at >= lo && at < hi;
+              s[j][i] = ok ? s[j][i] : 0.0f;
+            }
+        }
         float big = 0.0f;
 #pragma unroll
         for (int j = 0; j < kPages; ++j)
