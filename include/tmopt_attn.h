@@ -616,7 +616,8 @@ int tmopt_attn_prefill_diff(
  * A query that sees no key gives zeros and LSE -infinity. A visible key whose
  * score is NaN (or +infinity, without a cap) gives NaN as output and LSE.
  * Sums and maxima are fp32; probabilities are rounded to bf16 for their product
- * with the values, outputs once.
+ * with the values, outputs once. The sums are of up to 2^8 times each value, in
+ * fp32: finite while 2^8 times the sum of the visible values' magnitudes is.
  */
 
 /*

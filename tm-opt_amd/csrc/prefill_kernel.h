@@ -149,6 +149,16 @@ __device__ __forceinline__ int64_t lse_stride(const PrefillArgs& a,
   return a.lse_sh != 0 ? a.lse_sh : wk.total;
 }
 
+// The kernel's arguments read again in the argument segment (the pointer is
+// opaque to the compiler): those that the end of a scored kernel needs, which as
+// scalar registers over its loop took the places of ones that the loop reads.
+typedef const __attribute__((address_space(4))) PrefillArgs* LateArgs;
+__device__ __forceinline__ LateArgs late_args() {
+  auto p = (LateArgs)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
+
 // First key a work item reads (a multiple of the tile width at or below the
 // first key a query of the block may see) and its tiles from there.
 struct Tiles {
@@ -1020,10 +1030,12 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
   // cap (elsewhere the scale comes with the exponent).
   [[maybe_unused]] const bool with_fn =
       kScored && !SLOPED && (a.cap.in != 0.0f || a.slopes != nullptr);
-  [[maybe_unused]] uint64_t no_ref = 0;   // queries without a reference point
+  // A cap alone: |s| up to which x - m_run is kLazy at most (negative: a query
+  // without a reference point yet)
+  [[maybe_unused]] float reach = -1.0f;
   if constexpr (BOUNDED) {
     m_run = 0.0f;
-    no_ref = __builtin_amdgcn_ballot_w64(qok);
+    if (!qok) reach = INFINITY;   // (no row of the run: s = 0)
   }
   [[maybe_unused]] auto score_tile = [&](f32x16 (&s)[2], int kt)
       __attribute__((always_inline)) {
@@ -1081,6 +1093,20 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
     }
   };
 
+  // O^T times alpha (in place, each product tied to its accumulator register: a
+  // plain multiply under a branch leaves the compiler a merge of two copies of
+  // O^T, which it resolves with 32 register-pair moves on every tile)
+  auto scale_o = [&](float alpha) __attribute__((always_inline)) {
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        float x = o_acc[db][j];
+        asm volatile("v_mul_f32 %0, %1, %0" : "+v"(x) : "v"(alpha));
+        o_acc[db][j] = x;
+      }
+  };
+
   // softmax of scores `s` of the tile at kt (masking when needed): P^T
   // fragments, running max / sum update, O^T rescale when the max moved.
   // `hook` runs first (group 1 issues its tile DMA there).
@@ -1088,12 +1114,17 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
     const bool full = full_tile(kt);
     hook();
     if constexpr (BOUNDED) {
-      // A cap alone: sums of 2^(x - m) without a running maximum. m is the
-      // largest x of the first tile that the query sees: any m gives the same
-      // result up to the probabilities' rounding, but with this one the largest
-      // of a few keys, or the only one, has probability 1, which bf16 holds
-      // (error of 3 queries after 28 keys, cap 50, two documents: 1.8-2.1e-3
-      // with m = 0, 1.2-1.4e-3 so, 1.2e-3 that of the output's own rounding).
+      // A cap alone. The largest |s| of a tile, which the choice of the cap's form
+      // needs anyway, bounds its x: where that leaves x - m_run at kLazy at most, as
+      // nearly everywhere, no maximum of x is taken and nothing rescaled. Elsewhere
+      // (a query's first tile, scores that left the reference behind) the reference
+      // becomes the tile's maximum and kLead more, if that is above it by kLazy:
+      // probabilities are 2^kLazy at most, as with a running maximum, and moves are
+      // rare (without the lead a reference 16 below what is allowed moved on 12% of
+      // the tiles of heads whose scores spread over 8-16, and all eight waves wait
+      // for one that does: 4 prompts of 2K-8K 1,098 us against 1,070). kLead is
+      // whole, so the largest of a few keys, or the only one, has a probability that
+      // bf16 holds.
       float mx = 0.0f;
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
@@ -1114,7 +1145,7 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
             s[kb][j] = a.cap.small_less(s[kb][j], m_run);
       }
       if (!full) mask_tile(s, kt);
-      if (no_ref) {
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx > reach) != 0, 0)) {
         float top = -INFINITY;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -1122,14 +1153,20 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
           for (int j = 0; j < 16; j += 2)
             top = fmaxf(fmaxf(top, s[kb][j]), s[kb][j + 1]);
         top = lane_pair(top, 32, true);
-        const bool now = (no_ref >> lane & 1) && top > -INFINITY;
-        const float m = now ? fmaxf(top, Cap::kLeast) : 0.0f;
-        m_run += m;
+        const bool none = reach < 0.0f;
+        const bool move = top > (none ? -INFINITY : kLazy);
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(move) != 0, 0)) {
+          const float up = move ? top + Cap::kLead : 0.0f;
+          const float alpha = none ? 1.0f : fast_exp2(-up);
+          m_run += up;
+          if (move) reach = a.cap.reach(m_run + kLazy);
+          l_part *= alpha;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+          for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int j = 0; j < 16; ++j) s[kb][j] -= m;
-        no_ref &= ~__builtin_amdgcn_ballot_w64(now);
+            for (int j = 0; j < 16; ++j) s[kb][j] -= up;
+          if (!first) scale_o(alpha);
+        }
       }
       float psum = 0.0f;
       uint32_t pw[16];
@@ -1165,19 +1202,7 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
     pack_p(pw, pf);
     l_part = l_part * alpha + psum;
     // O^T holds the tiles before this one: rescale it to the new reference
-    // (in place, each product tied to its accumulator register: a plain
-    // multiply under the branch leaves the compiler a merge of two copies
-    // of O^T, which it resolves with 32 register-pair moves on every tile)
-    if (!first && __builtin_amdgcn_ballot_w64(move)) {
-#pragma unroll
-      for (int db = 0; db < 4; ++db)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          float x = o_acc[db][j];
-          asm volatile("v_mul_f32 %0, %1, %0" : "+v"(x) : "v"(alpha));
-          o_acc[db][j] = x;
-        }
-    }
+    if (!first && __builtin_amdgcn_ballot_w64(move)) scale_o(alpha);
   };
 
   // MFMA phase of tile t: O^T += V^T.P^T for tile t (four accumulators in
@@ -1370,6 +1395,10 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
   }  // !rejected
 
   // ---- finalise: l over both lane halves, normalise, store --------------
+  const auto end = [&]() __attribute__((always_inline)) {
+    if constexpr (kScored) return late_args();
+    else return &a;
+  }();
   const float l_tot = l_part + __shfl_xor(l_part, 32);
   // (no number as a sum: no number as LSE, for the newer entry points)
   auto some = [&]() __attribute__((always_inline)) {
@@ -1382,7 +1411,7 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
   if (part_slot >= 0) {
     // lane-major partial: every store writes 1 KB
     const int64_t pw = (int64_t)part_slot * 8 + w;
-    float* const po = a.part_o + (pw * 16 * 64 + lane) * 4;
+    float* const po = end->part_o + (pw * 16 * 64 + lane) * 4;
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -1391,16 +1420,20 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
             f32x4{o_acc[db][4 * g4] * inv, o_acc[db][4 * g4 + 1] * inv,
                   o_acc[db][4 * g4 + 2] * inv, o_acc[db][4 * g4 + 3] * inv};
     if (h2 == 0)
-      a.part_lse[pw * 32 + l32] =
+      end->part_lse[pw * 32 + l32] =
           rejected ? __builtin_nanf("") :
           some() ? (m_run + fast_log2(l_tot)) * kLn2 : -INFINITY;
     return;
   }
 #endif
-  if (a.lse && h2 == 0 && qok)
-    a.lse[head * lse_stride(a, wk) + t0 + qi] =
+  if (end->lse && h2 == 0 && qok) {
+    const int64_t row = end->lse_sh != 0 ? end->lse_sh
+                        : kScored ? (int64_t)as_const(end->cu)[end->S]
+                                  : (int64_t)wk.total;
+    end->lse[head * row + t0 + qi] =
         rejected ? __builtin_nanf("") :
         some() ? (m_run + fast_log2(l_tot)) * kLn2 : -INFINITY;
+  }
   // O^T goes through LDS (free after the last barrier) so that the global
   // stores are whole rows: the wave writes its 32 x 128 block query-major
   // (256-byte rows, 16-byte chunks swizzled by row & 15, so neither the
@@ -1423,16 +1456,16 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
   wave_lds_sync();
   const int qrow0 = q0 + 32 * (w % QSUB);   // query of the block's row 0
   const int c16 = lane & 15;
-  const bool al16 = ((a.o_st | a.o_sh) & 7) == 0 &&
-                    ((uintptr_t)a.out & 15) == 0;
+  const bool al16 = ((end->o_st | end->o_sh) & 7) == 0 &&
+                    ((uintptr_t)end->out & 15) == 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = 4 * i + (lane >> 4);
     const u32x4 x = __builtin_bit_cast(
         u32x4, lds_ld128(ob + r * kRowB + 16 * (c16 ^ (r & 15))));
     if (qrow0 + r < len) {
-      __bf16* const dst = a.out + (int64_t)(t0 + qrow0 + r) * a.o_st +
-                          (int64_t)head * a.o_sh + 8 * c16;
+      __bf16* const dst = end->out + (int64_t)(t0 + qrow0 + r) * end->o_st +
+                          (int64_t)head * end->o_sh + 8 * c16;
       if (al16) {
         *reinterpret_cast<u32x4*>(dst) = x;
       } else {

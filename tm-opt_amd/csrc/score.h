@@ -43,12 +43,18 @@ struct Cap {
         __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(c3, u, c2), u, c1), u, c0),
         -m);
   }
-  // Scores within the cap need no running maximum where 2^+-cap is far inside
-  // fp32 and bf16: sums are of 2^(x - m), m the largest x of the first tile that
-  // the query sees, or kLeast where that is more: x - m is 90 at most.
-  static constexpr float kLeast = -13.0f;
+  // The |s| up to which the score stays below x (0 if no |s| does, infinity if
+  // every one): 2^(in s) = (1 + r) / (1 - r), r = x / out.
+  __device__ __forceinline__ float reach(float x) const {
+    if (x >= out) return INFINITY;
+    return x <= 0.0f ? 0.0f : fast_log2((out + x) / (out - x)) / in;
+  }
+  // How far (in log2) the prefill sets a query's reference point above the largest
+  // score it has seen: keys below 2^-102 of the sum may count as nothing.
+  static constexpr float kLead = 24.0f;
+  // caps that have a kernel of their own
   __host__ __device__ bool bounded() const {
-    return in != 0.0f && out <= 90.0f + kLeast;
+    return in != 0.0f && out <= 77.0f;
   }
 };
 
