@@ -604,8 +604,8 @@ int tmopt_attn_prefill_diff(
  * Attention whose score of query q (position p) and key k (position j) is
  *   z = scale q.k;  x = softcap tanh(z / softcap)  (softcap 0: x = z)
  *   x - slopes[h] |p - j|                          (slopes: fp32 [HQ] or NULL)
- * (the tanh off by 2^-19 at most; scale / softcap between 1e-37 and 1e37, else
- * TMOPT_EINVAL), and whose query sees the keys of its request
+ * (softcap tanh() off by 2^-19 of the cap at most, and for caps above 256 by 2^-18
+ * of z at most; scale / softcap between 1e-37 and 1e37, else TMOPT_EINVAL), and whose query sees the keys of its request
  * with
  *   j >= first_keys, j > p - window (window > 0), j <= max(p, prefix_lens - 1).
  * first_keys: int32, one per query token, or NULL: where the query's document

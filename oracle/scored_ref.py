@@ -9,7 +9,11 @@ is off by dx, the sum of
     moves; the tanh itself may be off by 2^-20 (in fp32 a t = exp(2 y) off by
     2 x 2^-23 of itself, 1 + t rounded, its reciprocal off by 2^-23 and a last
     rounding add up to 5.5 x 2^-23 < 2^-20), and so may its argument: 4 x 2^-24
-    of y sech^2(y) is less than 2^-22;
+    of y sech^2(y) is less than 2^-22. Of a cap above 256 that would be more than
+    2^-11, so there it is 2^-18 of z at most: up to |z| = cap / 2 a polynomial in y
+    takes the tanh's place, off by 2^-18.7 of y (y -> 0, where its error is the
+    largest share of it) and by some roundings of 2^-24, and beyond 2^-20 of the
+    cap is 2^-19 of z;
   * a bias of size w: 4 x 2^-24 (w + |x|) for its product and the sum, and
     bf16 biases are exact. Slopes may also join q.k as the first term of its
     sum: then each of the eight sums of 16 products rounds at their size, by
@@ -128,8 +132,11 @@ def attend(q, K, V, qpos, kpos, scale, softcap=0.0, slopes=None, rel=None,
         x = q[:, h] @ K[:, g].T * scale
         dx = (128 + 4) * HALF_F32 * (q[:, h].abs() @ K[:, g].abs().T * scale)
         if softcap:
+            share = softcap * 2.0 ** -19
+            if softcap > 256:
+                share = torch.clamp(2.0 ** -18 * x.abs(), max=share)
             x = softcap * torch.tanh(x / softcap)
-            dx = dx + softcap * 2.0 ** -19
+            dx = dx + share
         if slopes is not None:
             w = slopes[h].double() * dist.abs()
             x = x - w

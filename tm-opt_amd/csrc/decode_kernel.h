@@ -758,8 +758,9 @@ void decode_kernel(DecodeArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #ifdef TMOPT_DECODE_SCORED
-          x[t][i] = a.cap.in != 0.0f ? a.cap(sc[t][i])
-                                     : sc[t][i] * a.scale_log2;
+          x[t][i] = a.cap.k != 0.0f    ? a.cap.far(sc[t][i])
+                    : a.cap.in != 0.0f ? a.cap(sc[t][i])
+                                       : sc[t][i] * a.scale_log2;
           x[t][i] -= slope * (float)(rel_dist(cur) - 16 * t - 4 * g - i);
 #else
           x[t][i] = sc[t][i] * a.scale_log2;

@@ -354,7 +354,12 @@ void decode_mx4_kernel(Mx4Args args) {
         for (int j = 0; j < kPages; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) big = fmaxf(big, __builtin_fabsf(s[j][i]));
-        if (__builtin_amdgcn_ballot_w64(big > args.cap.lim)) {
+        if (args.cap.k != 0.0f) {
+#pragma unroll
+          for (int j = 0; j < kPages; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[j][i] = args.cap.far(s[j][i]);
+        } else if (__builtin_amdgcn_ballot_w64(big > args.cap.lim)) {
 #pragma unroll
           for (int j = 0; j < kPages; ++j)
 #pragma unroll

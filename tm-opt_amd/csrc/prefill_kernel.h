@@ -313,7 +313,7 @@ enum Source : int {
                   // head_dim strided (the sconv output), read in place
   kPaged4 = 4,  // kPaged over the 4-bit cache
   // flags beside the source of a scored kernel
-  kBounded = 8,  // a cap alone (see Cap::bounded)
+  kCapped = 8,   // a cap alone (see Cap::near)
   kSloped = 16,  // slopes without a cap
 };
 
@@ -349,7 +349,7 @@ template <int REP, bool REL, int SRCF>
 __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
 #endif
   constexpr int SRC = SRCF & 7;
-  constexpr bool BOUNDED = kScored && (SRCF & kBounded) != 0;
+  constexpr bool CAPPED = kScored && (SRCF & kCapped) != 0;
   constexpr bool SLOPED = kScored && (SRCF & kSloped) != 0;
   constexpr bool CM = SRC == kPackedCM;   // channel-major k / v tiles
   constexpr bool Q4 = SRC == kPaged4;
@@ -1033,13 +1033,18 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
   // A cap alone: |s| up to which x - m_run is kLazy at most (negative: a query
   // without a reference point yet)
   [[maybe_unused]] float reach = -1.0f;
-  if constexpr (BOUNDED) {
+  if constexpr (CAPPED) {
     m_run = 0.0f;
     if (!qok) reach = INFINITY;   // (no row of the run: s = 0)
   }
   [[maybe_unused]] auto score_tile = [&](f32x16 (&s)[2], int kt)
       __attribute__((always_inline)) {
-    if (a.cap.in != 0.0f) {
+    if (a.cap.k != 0.0f) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[kb][j] = a.cap.far(s[kb][j]);
+    } else if (a.cap.in != 0.0f) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -1113,7 +1118,7 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
   auto softmax_phase = [&](f32x16 (&s)[2], int kt, bool first, auto&& hook) {
     const bool full = full_tile(kt);
     hook();
-    if constexpr (BOUNDED) {
+    if constexpr (CAPPED) {
       // A cap alone. The largest |s| of a tile, which the choice of the cap's form
       // needs anyway, bounds its x: where that leaves x - m_run at kLazy at most, as
       // nearly everywhere, no maximum of x is taken and nothing rescaled. Elsewhere

@@ -13,7 +13,7 @@ void launch(const PrefillArgs& a, int src, size_t lds, hipStream_t st) {
   const dim3 grid((unsigned)a.n_base);
   // a cap alone and slopes alone have kernels of their own
   const int kind = src | (a.cap.in == 0.0f ? (a.slopes ? kSloped : 0)
-                          : a.cap.bounded() && !a.slopes ? kBounded : 0);
+                          : a.cap.near() && !a.slopes ? kCapped : 0);
 #define TMOPT_LAUNCH(K)                                                     \
   case K:                                                                   \
     hipLaunchKernelGGL((prefill_kernel<REP, false, K>), grid, dim3(512), \
@@ -23,9 +23,9 @@ void launch(const PrefillArgs& a, int src, size_t lds, hipStream_t st) {
     TMOPT_LAUNCH(kPacked);
     TMOPT_LAUNCH(kPaged);
     TMOPT_LAUNCH(kPaged4);
-    TMOPT_LAUNCH(kPacked | kBounded);
-    TMOPT_LAUNCH(kPaged | kBounded);
-    TMOPT_LAUNCH(kPaged4 | kBounded);
+    TMOPT_LAUNCH(kPacked | kCapped);
+    TMOPT_LAUNCH(kPaged | kCapped);
+    TMOPT_LAUNCH(kPaged4 | kCapped);
     TMOPT_LAUNCH(kPacked | kSloped);
     TMOPT_LAUNCH(kPaged | kSloped);
     TMOPT_LAUNCH(kPaged4 | kSloped);

@@ -16,8 +16,8 @@ and the query sees the keys j of its request with
   j <= max(p, prefix_lens - 1)          (int32, one per run: its first tokens,
                                          read in both directions)
 
-A query that sees no key gives zeros, LSE -inf. The cap's tanh is off by 2^-19 of
-the cap at most. K and V rows, pools and block tables are those of the other
+A query that sees no key gives zeros, LSE -inf. A capped score is off by 2^-19 of
+the cap at most, with caps above 256 by 2^-18 of z at most. K and V rows, pools and block tables are those of the other
 entry points.
 """
 import torch
