@@ -271,6 +271,8 @@ static int prefill_impl(
                     o_stride_tok % 4 == 0 && o_stride_head % 4 == 0 &&
                     (uintptr_t)q % 16 == 0 && (uintptr_t)out % 8 == 0,
                 TMOPT_EINVAL, "prefill: q/out rows misaligned");
+  TMOPT_REQUIRE(lse_stride_head >= 0, TMOPT_EINVAL,
+                "prefill: lse_stride_head=%lld", (long long)lse_stride_head);
   PrefillArgs a;
   a.q = (const __bf16*)q;
   a.q_st = q_stride_tok;
