@@ -107,6 +107,8 @@ int run(const char* what, PrefillArgs& a, int src, const void* q,
                     o_stride_head % 4 == 0 && (uintptr_t)q % 16 == 0 &&
                     (uintptr_t)out % 8 == 0,
                 TMOPT_EINVAL, "%s: q/out rows misaligned", what);
+  TMOPT_REQUIRE(lse_stride_head >= 0, TMOPT_EINVAL, "%s: lse_stride_head=%lld",
+                what, (long long)lse_stride_head);
   a.q = (const __bf16*)q;
   a.q_st = q_stride_tok;
   a.q_sh = q_stride_head;
