@@ -613,6 +613,7 @@ int tmopt_attn_prefill_diff(
  * prefix_lens: int32, one per run, or NULL: of each run the first tokens, which
  * all of it sees (any value; a prefix past the run's end stops there, a negative
  * one is 0).
+ * In the prefill, scores without a cap at scales up to 256 stay below 2^30.
  * A query that sees no key gives zeros and LSE -infinity. A visible key whose
  * score is NaN (or +infinity, without a cap) gives NaN as output and LSE.
  * Sums and maxima are fp32; probabilities are rounded to bf16 for their product
@@ -744,7 +745,8 @@ int tmopt_kv_read_mx4(const void* pool, int64_t num_pages,
  * softcap:  > 0: scores are softcap * tanh(scale q.k / softcap).
  * slopes:   fp32 [HQ] or NULL: the score of a key at distance d (pos_q - pos_k)
  *           gets -slopes[h] * d, after the cap.
- * rel goes without softcap and slopes (TMOPT_EUNSUPPORTED).
+ * rel goes without softcap and slopes (TMOPT_EUNSUPPORTED), and with scales from
+ * 2^-60 on (else TMOPT_EINVAL); scores with it stay below 2^30.
  * A visible key whose score is NaN or +infinity gives NaN as LSE and outputs, a
  * visible value block that is NaN gives NaN in its dims.
  * Any HQ / HKV; each stored head is read once for up to 8 query heads (a larger

@@ -642,8 +642,10 @@ extern "C" int tmopt_attn_decode_mx4(
                 TMOPT_EINVAL, "decode_mx4: min_pages=%d num_workgroups=%d",
                 min_pages, num_workgroups);
   TMOPT_REQUIRE(rel == nullptr ||
-                    (rel_extent > 0 && (int64_t)HQ * rel_extent < (1 << 29)),
-                TMOPT_EINVAL, "decode_mx4: rel_extent=%d", rel_extent);
+                    (rel_extent > 0 && (int64_t)HQ * rel_extent < (1 << 29) &&
+                     scale >= kMinRaw),
+                TMOPT_EINVAL, "decode_mx4: rel_extent=%d scale=%g", rel_extent,
+                scale);
   TMOPT_REQUIRE(rel == nullptr || (softcap == 0.0f && slopes == nullptr),
                 TMOPT_EUNSUPPORTED,
                 "decode_mx4: a relative bias goes without softcap and slopes");
@@ -694,7 +696,7 @@ extern "C" int tmopt_attn_decode_mx4(
   if (rel)
     hipLaunchKernelGGL((decode_mx4_kernel<true, false>), grid, dim3(64 * nw),
                        lds, st, x);
-  else if (softcap > 0.0f || slopes)
+  else if (softcap > 0.0f || slopes || scale > kMaxRaw)
     hipLaunchKernelGGL((decode_mx4_kernel<false, true>), grid, dim3(64 * nw),
                        lds, st, x);
   else

@@ -1029,7 +1029,8 @@ __global__ __launch_bounds__(512) void prefill_kernel(PrefillArgs a) {
   // Scores q.k -> the softmax's argument in units of log2(e), where there is a
   // cap (elsewhere the scale comes with the exponent).
   [[maybe_unused]] const bool with_fn =
-      kScored && !SLOPED && (a.cap.in != 0.0f || a.slopes != nullptr);
+      kScored && !SLOPED &&
+      (a.cap.in != 0.0f || a.slopes != nullptr || a.scale > kMaxRaw);
   // A cap alone: |s| up to which x - m_run is kLazy at most (negative: a query
   // without a reference point yet)
   [[maybe_unused]] float reach = -1.0f;

@@ -12,7 +12,8 @@ template <int REP>
 void launch(const PrefillArgs& a, int src, size_t lds, hipStream_t st) {
   const dim3 grid((unsigned)a.n_base);
   // a cap alone and slopes alone have kernels of their own
-  const int kind = src | (a.cap.in == 0.0f ? (a.slopes ? kSloped : 0)
+  const bool raw = a.scale >= kMinRaw && a.scale <= kMaxRaw;
+  const int kind = src | (a.cap.in == 0.0f ? (a.slopes && raw ? kSloped : 0)
                           : a.cap.near() && !a.slopes ? kCapped : 0);
 #define TMOPT_LAUNCH(K)                                                     \
   case K:                                                                   \
@@ -154,7 +155,8 @@ int run(const char* what, PrefillArgs& a, int src, const void* q,
   a.part_n = (int*)(a.part_lse + slots * 256);
   a.nqb_max = (max_seqlen_q + bq - 1) / bq;
   const size_t lds = kNStage * kStage + (a.rel ? 8 * kBiasB : 0);
-  const bool scored = src != kPaged4 || softcap > 0.0f || slopes;
+  const bool scored = src != kPaged4 || softcap > 0.0f || slopes ||
+                      (scale > kMaxRaw && !a.rel);
   if (scored && a.nsplit > 1) {
     launch_prefill_scored_split(a, rep, src, lds, st);
   } else if (scored) {
@@ -296,8 +298,10 @@ extern "C" int tmopt_attn_prefill_mx4_strided(
   TMOPT_REQUIRE(rel == nullptr || (softcap == 0.0f && slopes == nullptr),
                 TMOPT_EUNSUPPORTED,
                 "prefill_mx4: a relative bias goes without softcap and slopes");
-  TMOPT_REQUIRE(rel == nullptr || (rel_extent > 0 && (uintptr_t)rel % 2 == 0),
-                TMOPT_EINVAL, "prefill_mx4: rel_extent=%d", rel_extent);
+  TMOPT_REQUIRE(rel == nullptr || (rel_extent > 0 && (uintptr_t)rel % 2 == 0 &&
+                                   !(scale < kMinRaw)),
+                TMOPT_EINVAL, "prefill_mx4: rel_extent=%d scale=%g", rel_extent,
+                scale);
   TMOPT_REQUIRE(rel == nullptr ||
                     (rel_stride_tok >= rel_extent && rel_stride_head >= 0 &&
                      64 * rel_stride_tok + 2 * (int64_t)rel_extent < kOob),

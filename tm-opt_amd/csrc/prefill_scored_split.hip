@@ -10,7 +10,8 @@ template <int REP>
 void launch(const PrefillArgs& a, int src, size_t lds, hipStream_t st) {
   const dim3 grid((unsigned)(a.n_base * a.nsplit));
   // a cap alone and slopes alone have kernels of their own
-  const int kind = src | (a.cap.in == 0.0f ? (a.slopes ? kSloped : 0)
+  const bool raw = a.scale >= kMinRaw && a.scale <= kMaxRaw;
+  const int kind = src | (a.cap.in == 0.0f ? (a.slopes && raw ? kSloped : 0)
                           : a.cap.near() && !a.slopes ? kCapped : 0);
 #define TMOPT_LAUNCH(K)                                                     \
   case K:                                                                   \

@@ -82,6 +82,12 @@ struct Cap {
   __host__ __device__ bool near() const { return in != 0.0f && k == 0.0f; }
 };
 
+// Scales for which a score may stay q.k up to the exponent, whose argument is then
+// one fma of it and the rounded maximum: off by half a step of |x|, which passes
+// fp32's exponents from |x| = 2^31 on. Above kMaxRaw scores are scaled first. A bias
+// that joins q.k divided by the scale would leave fp32 below kMinRaw.
+constexpr float kMinRaw = 0x1p-60f, kMaxRaw = 256.0f;
+
 // A cap that fp32 can work with: 0, or 2 log2(e) scale / softcap in its range.
 inline bool good_cap(float softcap, float scale) {
   return softcap == 0.0f || (softcap > 0.0f && softcap < INFINITY &&
