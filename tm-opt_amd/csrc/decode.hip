@@ -192,7 +192,8 @@ static int decode_impl(
   a.scale_log2 = scale * kLog2e;
   a.rel = (const __bf16*)rel;
   a.rel_extent = rel ? rel_extent : 0;
-  a.min_pages = min_pages;
+  // (a work-group's first page, its index times this, stays within int32)
+  a.min_pages = min_pages < 32768 ? min_pages : 32768;
   a.seqs_per_wg = seqs_per_wg;
   a.out = (__bf16*)out;
   a.lse = lse;
