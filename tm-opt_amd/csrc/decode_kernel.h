@@ -751,6 +751,19 @@ void decode_kernel(DecodeArgs a) {
       [[maybe_unused]] int sh = 0;
       if constexpr (REL)
         sh = (rel_row(rr) + 2 * (rel_dist(cur) - 31) + rel_mis(cur)) & 2;
+#ifdef TMOPT_DECODE_SCORED
+      // (one branch a step: a choice at each score becomes a branch at each)
+      float capped[2][4];
+      auto each = [&](auto fn) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) capped[t][i] = fn(sc[t][i]);
+      };
+      if (a.cap.k != 0.0f) each([&](float s) { return a.cap.far(s); });
+      else if (a.cap.in != 0.0f) each([&](float s) { return a.cap(s); });
+      else each([&](float s) { return s * a.scale_log2; });
+#endif
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         float bias[4];
@@ -758,10 +771,8 @@ void decode_kernel(DecodeArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #ifdef TMOPT_DECODE_SCORED
-          x[t][i] = a.cap.k != 0.0f    ? a.cap.far(sc[t][i])
-                    : a.cap.in != 0.0f ? a.cap(sc[t][i])
-                                       : sc[t][i] * a.scale_log2;
-          x[t][i] -= slope * (float)(rel_dist(cur) - 16 * t - 4 * g - i);
+          x[t][i] = capped[t][i] -
+                    slope * (float)(rel_dist(cur) - 16 * t - 4 * g - i);
 #else
           x[t][i] = sc[t][i] * a.scale_log2;
 #endif

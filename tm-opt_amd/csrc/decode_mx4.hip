@@ -85,7 +85,9 @@ __device__ __forceinline__ float other_half(float x) {
                                          0xF, 0xF, true));   // row_ror 8
 }
 
-template <bool REL, bool SCORE>
+// SCORE: 1 with a score function, 2 with a cap above Cap::kNear (a kernel of its
+// own: as a branch of the other's steps it cost these 1-2%)
+template <bool REL, int SCORE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void decode_mx4_kernel(Mx4Args args) {
   const DecodeArgs& a = args.d;
@@ -313,7 +315,7 @@ void decode_mx4_kernel(Mx4Args args) {
   const uint32_t p_sel0 = odd ? 0x05040c0cu : 0x0c0c0504u;
   const uint32_t p_sel1 = odd ? 0x07060c0cu : 0x0c0c0706u;
   [[maybe_unused]] float slope = 0.0f;
-  if constexpr (SCORE)
+  if constexpr (SCORE != 0)
     if (args.slopes) slope = args.slopes[hq] * kLog2e;
 
   auto compute = [&](const Buf4<REL>& x, const Step4& st)
@@ -332,9 +334,14 @@ void decode_mx4_kernel(Mx4Args args) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[j][i] = c[i];
     }
-    if constexpr (SCORE) {
+    if constexpr (SCORE == 2) {
+#pragma unroll
+      for (int j = 0; j < kPages; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[j][i] = args.cap.far(s[j][i]);
+    } else if constexpr (SCORE == 1) {
       if (args.cap.in != 0.0f) {
-        if (!(st.flags & kFull)) {
+        if (__builtin_expect(!(st.flags & kFull), 0)) {
           // (the bytes of a key that is not there are nobody's: they do not
           // choose the form of the cap)
           const int lo = vis_lo(st.n, a.window) - st.pg * kPS;
@@ -354,12 +361,7 @@ void decode_mx4_kernel(Mx4Args args) {
         for (int j = 0; j < kPages; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) big = fmaxf(big, __builtin_fabsf(s[j][i]));
-        if (args.cap.k != 0.0f) {
-#pragma unroll
-          for (int j = 0; j < kPages; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[j][i] = args.cap.far(s[j][i]);
-        } else if (__builtin_amdgcn_ballot_w64(big > args.cap.lim)) {
+        if (__builtin_amdgcn_ballot_w64(big > args.cap.lim)) {
 #pragma unroll
           for (int j = 0; j < kPages; ++j)
 #pragma unroll
@@ -379,7 +381,7 @@ void decode_mx4_kernel(Mx4Args args) {
     }
     // distance of token 4g of the step's first page
     const int left = st.n - st.pg * kPS;   // keys from the step's first on
-    if constexpr (SCORE) {
+    if constexpr (SCORE != 0) {
       if (args.slopes) {
 #pragma unroll
         for (int j = 0; j < kPages; ++j)
@@ -456,7 +458,7 @@ void decode_mx4_kernel(Mx4Args args) {
       for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[j][i]);
     mx = lane_pair(lane_pair(mx, 16, true), 32, true);
     const float to_log2 = SCORE ? 1.0f : a.scale_log2;
-    if constexpr (!SCORE) mx *= to_log2;
+    if constexpr (SCORE == 0) mx *= to_log2;
     const bool move = mx > m_run;
     if (__builtin_amdgcn_ballot_w64(move)) {
       const float m_new = move ? mx : m_run;
@@ -694,13 +696,16 @@ extern "C" int tmopt_attn_decode_mx4(
   const dim3 grid(G, hkv / nw);
   hipStream_t st = (hipStream_t)stream;
   if (rel)
-    hipLaunchKernelGGL((decode_mx4_kernel<true, false>), grid, dim3(64 * nw),
+    hipLaunchKernelGGL((decode_mx4_kernel<true, 0>), grid, dim3(64 * nw),
                        lds, st, x);
+  else if (x.cap.k != 0.0f)
+    hipLaunchKernelGGL((decode_mx4_kernel<false, 2>), grid, dim3(64 * nw), lds,
+                       st, x);
   else if (softcap > 0.0f || slopes || scale > kMaxRaw)
-    hipLaunchKernelGGL((decode_mx4_kernel<false, true>), grid, dim3(64 * nw),
+    hipLaunchKernelGGL((decode_mx4_kernel<false, 1>), grid, dim3(64 * nw),
                        lds, st, x);
   else
-    hipLaunchKernelGGL((decode_mx4_kernel<false, false>), grid, dim3(64 * nw),
+    hipLaunchKernelGGL((decode_mx4_kernel<false, 0>), grid, dim3(64 * nw),
                        lds, st, x);
   const int rc = check_launch("decode_mx4");
   if (rc) return rc;
