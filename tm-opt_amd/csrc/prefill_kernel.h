@@ -317,6 +317,20 @@ enum Source : int {
   kSloped = 16,  // slopes without a cap
 };
 
+#ifdef TMOPT_PREFILL_SCORED
+// The scored kernel of a launch: a cap alone and slopes alone have kernels of their
+// own. TMOPT_SCORED_KINDS(X): X(kind) for each that scored_kind gives.
+inline int scored_kind(const PrefillArgs& a, int src) {
+  if (a.cap.in != 0.0f) return src | (a.cap.near() && !a.slopes ? kCapped : 0);
+  const bool raw = a.scale >= kMinRaw && a.scale <= kMaxRaw;
+  return src | (a.slopes && raw ? kSloped : 0);
+}
+#define TMOPT_SCORED_KINDS(X)                                   \
+  X(kPacked) X(kPaged) X(kPaged4)                               \
+  X(kPacked | kCapped) X(kPaged | kCapped) X(kPaged4 | kCapped) \
+  X(kPacked | kSloped) X(kPaged | kSloped) X(kPaged4 | kSloped)
+#endif
+
 // Channel-major tiles in LDS are 128 dim rows of 64 keys (128 bytes, eight
 // 16-byte chunks of 8 keys). Row r keeps logical chunk c in physical slot
 // c ^ cm_sig(r). cm_sig is a bijection of (r >> 1) & 7 that flips bit 2

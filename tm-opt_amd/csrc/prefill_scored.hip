@@ -11,26 +11,12 @@ namespace {
 template <int REP>
 void launch(const PrefillArgs& a, int src, size_t lds, hipStream_t st) {
   const dim3 grid((unsigned)a.n_base);
-  // a cap alone and slopes alone have kernels of their own
-  const bool raw = a.scale >= kMinRaw && a.scale <= kMaxRaw;
-  const int kind = src | (a.cap.in == 0.0f ? (a.slopes && raw ? kSloped : 0)
-                          : a.cap.near() && !a.slopes ? kCapped : 0);
-#define TMOPT_LAUNCH(K)                                                     \
-  case K:                                                                   \
+#define TMOPT_LAUNCH(K)                                                  \
+  case K:                                                                \
     hipLaunchKernelGGL((prefill_kernel<REP, false, K>), grid, dim3(512), \
-                       lds, st, a);                                         \
-    break
-  switch (kind) {
-    TMOPT_LAUNCH(kPacked);
-    TMOPT_LAUNCH(kPaged);
-    TMOPT_LAUNCH(kPaged4);
-    TMOPT_LAUNCH(kPacked | kCapped);
-    TMOPT_LAUNCH(kPaged | kCapped);
-    TMOPT_LAUNCH(kPaged4 | kCapped);
-    TMOPT_LAUNCH(kPacked | kSloped);
-    TMOPT_LAUNCH(kPaged | kSloped);
-    TMOPT_LAUNCH(kPaged4 | kSloped);
-  }
+                       lds, st, a);                                      \
+    break;
+  switch (scored_kind(a, src)) { TMOPT_SCORED_KINDS(TMOPT_LAUNCH) }
 #undef TMOPT_LAUNCH
 }
 
