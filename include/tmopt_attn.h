@@ -454,8 +454,8 @@ int tmopt_attn_prefill_varlen_split(
     tmopt_stream_t stream);
 
 /*
- * The same with LSE rows of lse_stride_head elements (0: cu_seqlens_q[num_seqs],
- * as above): for outputs of more rows than the runs have tokens, whose LSE
+ * The same with LSE rows of lse_stride_head elements (at least
+ * cu_seqlens_q[num_seqs]; 0: that many, as above): for outputs of more rows than the runs have tokens, whose LSE
  * columns behind the last run stay as they were.
  */
 int tmopt_attn_prefill_varlen_strided_split(
@@ -677,8 +677,8 @@ int tmopt_attn_prefill_scored(
     size_t workspace_bytes, tmopt_stream_t stream);
 
 /*
- * The same with LSE rows of lse_stride_head elements (0: cu_seqlens_q[num_seqs],
- * as above): for outputs of more rows than the runs have tokens, whose LSE
+ * The same with LSE rows of lse_stride_head elements (at least
+ * cu_seqlens_q[num_seqs]; 0: that many, as above): for outputs of more rows than the runs have tokens, whose LSE
  * columns behind the last run stay as they were.
  */
 int tmopt_attn_prefill_scored_strided(
