@@ -619,6 +619,7 @@ int tmopt_attn_prefill_diff(
  * Sums and maxima are fp32; probabilities are rounded to bf16 for their product
  * with the values, outputs once. The sums are of up to 2^8 times each value, in
  * fp32: finite while 2^8 times the sum of the visible values' magnitudes is.
+ * (Prefills with a cap: values below 2^-80 may count as nothing.)
  */
 
 /*

@@ -25,7 +25,7 @@ rounded to bf16 for its product with the values, half a step is 2^-8 of it, so O
 is off by sum p (2^-8 + dx + dLSE + (2 n + 64) 2^-24) |v|, and rounded once more
 (2^-8 of it). A probability below 2^-126 of its reference point is no normal fp32
 number and may count as zero, once in its key's walk, where the reference may be
-2^24 above the largest, and once when pieces join: 2^-101 of sum |v|. A tenth is
+2^40 above the largest, and once when pieces join: 2^-85 of sum |v|. A tenth is
 added for products of errors.
 """
 import math
@@ -160,7 +160,7 @@ def attend(q, K, V, qpos, kpos, scale, softcap=0.0, slopes=None, rel=None,
         each = HALF_BF16 + dx + dl[:, None] + (2 * n[:, None] + 64) * HALF_F32
         out[:, h] = p @ V[:, g]
         err[:, h] = (p * torch.where(seen, each, 0.0)) @ V[:, g].abs()
-        err[:, h] += 2.0 ** -101 * (seen.double() @ V[:, g].abs())
+        err[:, h] += 2.0 ** -85 * (seen.double() @ V[:, g].abs())
         lse[h], lerr[h] = l, torch.where(some, dl, 0.0)
     return out, lse, 1.1 * (err + HALF_BF16 * out.abs()) + 1e-30, 1.1 * lerr
 

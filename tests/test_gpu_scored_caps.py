@@ -57,7 +57,7 @@ def _prefill_of(tm, source, q, k, v, scale, g, dev, **kw):
 
 @pytest.mark.parametrize("source", ["packed", "paged", "four"])
 @pytest.mark.parametrize("cap", [30.0, 50.0, 53.0, 60.0])
-@pytest.mark.parametrize("size", [1.0, 1e10, 1e20, 1e28])
+@pytest.mark.parametrize("size", [1e-20, 1.0, 1e10, 1e20, 1e28])
 def test_large_values_behind_low_scores(tm, dev, source, cap, size):
     """A first tile at the cap's low end and the others at its top; scores that
     rise from one key to the next."""

@@ -74,8 +74,11 @@ struct Cap {
     return x <= 0.0f ? 0.0f : fast_log2((out + x) / (out - x)) / in;
   }
   // How far (in log2) the prefill sets a query's reference point above the largest
-  // score it has seen: keys below 2^-102 of the sum may count as nothing.
-  static constexpr float kLead = 24.0f;
+  // score it has seen: keys below 2^-86 of the sum may count as nothing, and so may
+  // products with values below 2^-86. (24 / 32 / 40 / 48, us: a chunk of 1,500 in
+  // documents 94.6 / 92.0 / 91.0 / 91.0, where a query's first tile may show it a few
+  // keys only; 4 prompts of 2K-8K 1,103 / 1,095 / 1,096 / 1,096.)
+  static constexpr float kLead = 40.0f;
   // The prefill has kernels of its own for a cap up to kNear without slopes (4
   // prompts of 2K-8K with a cap of 60: 1,066 us there, 1,194 with the running
   // maximum and the exponential form that caps with slopes take).
