@@ -13,13 +13,13 @@ from test_gpu_scored import Cache, PAGE, _function, _gen, _i32, _packed
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("name", ["plain", "soft", "slopes", "cap slopes",
-                                  "rel"])
-@pytest.mark.parametrize("four", [0, 1])
+NAMES = ["plain", "soft", "slopes", "cap slopes"]
+
+
+@pytest.mark.parametrize("name,four", [(x, 0) for x in NAMES] +
+                         [(x, 1) for x in NAMES + ["rel"]])
 @pytest.mark.parametrize("at", [4000, 8999])
 def test_no_number_in_one_piece(tm, dev, name, four, at):
-    if name == "rel" and not four:
-        pytest.skip("the scored prefill takes no relative bias")
     g = _gen(95)
     n, prior, window = 64, 9000, 9000 + 32 - at   # queries below 32 see it
     c = (Cache4(tm, [n + prior], 2, g, dev) if four else

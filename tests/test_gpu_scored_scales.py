@@ -9,12 +9,11 @@ from test_gpu_scored import Cache, _gen, _i32, _packed, _rand
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("scale", [1e-38, 1e-37, 1e-20, 1e-9, 1e9])
-@pytest.mark.parametrize("cap", [0.0, 3.0])
+@pytest.mark.parametrize("scale,cap", [(1e-38, 0.0), (1e-37, 0.0), (1e-20, 0.0),
+                                       (1e-9, 0.0), (1e9, 0.0), (1e-20, 3.0),
+                                       (1e-9, 3.0), (1e9, 3.0)])
 @pytest.mark.parametrize("bias", [1, 0])
 def test_scales(tm, dev, scale, cap, bias):
-    if cap and not 1e-37 < scale / cap < 1e37:
-        pytest.skip("refused")
     g = _gen(97)
     kw = dict(softcap=cap)
     if bias:
